@@ -26,6 +26,7 @@ pub const RT_F16: rt_dtype = 1;
 pub const RT_Q8_0F: rt_dtype = 2;
 pub const RT_Q8_0H: rt_dtype = 3;
 pub const RT_Q4_K: rt_dtype = 4;
+pub const RT_Q4_0: rt_dtype = 5;
 
 pub type rt_activation = i32;
 pub const RT_ACT_NONE: rt_activation = 0;
@@ -139,6 +140,7 @@ extern "C" {
     pub fn rt_matmul_spec(d: *const rt_matmul_desc, spec: *mut rt_gemm_spec) -> rt_status;
     pub fn rt_tensor_nbytes(dtype: i32, numel: u64, nbytes: *mut u64) -> rt_status;
     pub fn rt_q8_0_scale_offset(numel: u64) -> u64;
+    pub fn rt_q4_0_scale_offset(numel: u64) -> u64;
     pub fn rt_status_string(s: rt_status) -> *const c_char;
     pub fn rt_kernel_string(kind: i32) -> *const c_char;
     // device context and buffers
@@ -172,6 +174,7 @@ extern "C" {
     pub fn rt_dequantize(ctx: *mut rt_ctx, dtype: i32, src: *const c_void, numel: u64, dst_f32: *mut c_void, stream: *mut c_void) -> rt_status;
     pub fn rt_transcode_gguf_q8_0(ctx: *mut rt_ctx, blocks: *const c_void, n_blocks: u64, dst_dtype: i32, dst: *mut c_void,
                                   stream: *mut c_void) -> rt_status;
+    pub fn rt_transcode_gguf_q4_0(ctx: *mut rt_ctx, blocks: *const c_void, n_blocks: u64, dst: *mut c_void, stream: *mut c_void) -> rt_status;
     // operators around the products
     pub fn rt_unary_enqueue(ctx: *mut rt_ctx, activation: i32, dtype: i32, src: *const c_void, dst: *mut c_void, numel: u64,
                             stream: *mut c_void) -> rt_status;

@@ -20,7 +20,11 @@
  *  - `stream` is a hipStream_t passed as void* (NULL = the default stream);
  *  - a quantized tensor is ONE buffer in the reference's segment layout
  *    (crates/ratchet-core/src/dtype/blocks.rs:61-74): int8 values, padded to
- *    256 bytes, then the per-32 scales, padded to 256 bytes.  A Q4_K tensor is
+ *    256 bytes, then the per-32 scales, padded to 256 bytes.  A Q4_0 tensor is
+ *    the same with 4-bit codes: dwords of eight, nibbles 0..3 the codes of the
+ *    values 0, 2, 4, 6 and nibbles 4..7 those of the values 1, 3, 5, 7, padded to
+ *    256 bytes, then one f16 scale d per 32 values, padded to 256 bytes; a value
+ *    is d * (code - 8).  A Q4_K tensor is
  *    the raw GGUF 144-byte super-blocks (crates/ratchet-loader/src/k_quants.rs:94-103),
  *    row-major over [rows, K/256].
  */
@@ -63,15 +67,16 @@ typedef enum rt_status {
 } rt_status;
 
 /* Replaces: enum DType (crates/ratchet-core/src/dtype/mod.rs:10-20), the
- * subset the Matmul guards admit, plus Q4_K (GgmlDType::Q4K,
- * crates/ratchet-loader/src/lib.rs:40) which the reference can name but not
+ * subset the Matmul guards admit, plus Q4_K and Q4_0 (GgmlDType::{Q4K, Q4_0},
+ * crates/ratchet-loader/src/lib.rs:35-101) which the reference can name but not
  * load. */
 typedef enum rt_dtype {
     RT_F32 = 0,
     RT_F16 = 1,
     RT_Q8_0F = 2, /* int8 blocks of 32 with f32 scales */
     RT_Q8_0H = 3, /* int8 blocks of 32 with f16 scales */
-    RT_Q4_K = 4   /* GGUF Q4_K super-blocks of 256     */
+    RT_Q4_K = 4,  /* GGUF Q4_K super-blocks of 256     */
+    RT_Q4_0 = 5   /* 4-bit blocks of 32 with f16 scales */
 } rt_dtype;
 
 /* Replaces: struct Matmul {lhs, rhs, bias, trans_lhs, trans_rhs, trans_out}
@@ -117,7 +122,7 @@ typedef enum rt_kernel_kind {
     RT_KERNEL_GEMV_Q8 = 1,   /* streaming Q8_0 weight rows x up to 8 activation vectors     */
     RT_KERNEL_GEMV_Q4K = 2,  /* streaming Q4_K weight rows x up to 16 activation vectors    */
     RT_KERNEL_GEMV_FLOAT = 3,/* streaming f16/f32 weight rows x up to 8 activation vectors  */
-    RT_KERNEL_GEMM_F16 = 4,  /* LDS-tiled MFMA GEMM, f16 operands (Q8_0H / Q4_K dequantized) */
+    RT_KERNEL_GEMM_F16 = 4,  /* LDS-tiled MFMA GEMM, f16 operands (Q8_0H / Q4_K / Q4_0 dequantized) */
     RT_KERNEL_GEMM_F32 = 5   /* LDS-tiled MFMA GEMM, f32 operands (Q8_0F dequantized)        */
 } rt_kernel_kind;
 
@@ -168,6 +173,8 @@ RT_API rt_status rt_tensor_nbytes(int32_t dtype, uint64_t numel, uint64_t *nbyte
 /* Replaces: the second BufferSegment's offset of Q8_0<T>::segments
  * (dtype/blocks.rs:61-74): byte offset of the scale stream. */
 RT_API uint64_t rt_q8_0_scale_offset(uint64_t numel);
+/* The same of a Q4_0 tensor of `numel` values: numel / 2 bytes of codes, padded to 256. */
+RT_API uint64_t rt_q4_0_scale_offset(uint64_t numel);
 
 RT_API const char *rt_status_string(rt_status s);
 RT_API const char *rt_kernel_string(int32_t kernel_kind);
@@ -222,8 +229,8 @@ RT_API rt_status rt_quantize_q8_0(rt_ctx *ctx, const void *src_f32, uint64_t num
 
 /* Replaces: Quantizer::sint8_dequantize (quant.rs:81-124) for Q8_0F, the same
  * rule with f16 scales for Q8_0H, and ggml's dequantize_row_q4_K for Q4_K
- * (the reference holds only the block struct, k_quants.rs:94-103).
- * `dst_f32` receives numel floats. */
+ * (the reference holds only the block struct, k_quants.rs:94-103); d * (code - 8)
+ * for Q4_0.  `dst_f32` receives numel floats. */
 RT_API rt_status rt_dequantize(rt_ctx *ctx, int32_t dtype, const void *src, uint64_t numel, void *dst_f32,
                         void *stream);
 
@@ -233,6 +240,11 @@ RT_API rt_status rt_dequantize(rt_ctx *ctx, int32_t dtype, const void *src, uint
  * segment layout for dst_dtype (RT_Q8_0F widens the scales to f32). */
 RT_API rt_status rt_transcode_gguf_q8_0(rt_ctx *ctx, const void *blocks, uint64_t n_blocks, int32_t dst_dtype,
                                  void *dst, void *stream);
+
+/* The same for Q4_0: `blocks` are n_blocks GGUF blocks of 18 bytes {f16 d; uint8 qs[16]} (qs[j]: value j in the
+ * low nibble, value j + 16 in the high one) in device memory, 2-byte aligned; `dst` receives RT_Q4_0's segment
+ * layout, rt_tensor_nbytes(RT_Q4_0, 32 * n_blocks) bytes, padding zeroed. */
+RT_API rt_status rt_transcode_gguf_q4_0(rt_ctx *ctx, const void *blocks, uint64_t n_blocks, void *dst, void *stream);
 
 /* ------------------------------------------------------------------------
  * GGUF container (the format the weights arrive in).
@@ -302,8 +314,8 @@ RT_API uint64_t rt_ggml_block_numel(int32_t ggml_dtype);
 /* TensorInfo::read + ratchet_from_gguf (gguf.rs:63-84,118-142): copies tensor `index` of the image to
  * the device and brings it into this library's layout for `dst_dtype`:
  *   F32 -> RT_F32, F16 -> RT_F16 (plain copies); Q8_0 -> RT_Q8_0H or RT_Q8_0F (segment layout, through
- *   the device transcoder; `staging` must hold size_in_bytes); Q4_K -> RT_Q4_K (raw super-blocks; this
- *   library's extension).  Any other pairing is RT_ERR_UNSUPPORTED (the reference bails on it).
+ *   the device transcoder; `staging` must hold size_in_bytes); Q4_0 -> RT_Q4_0 (likewise) and Q4_K ->
+ *   RT_Q4_K (raw super-blocks), this library's extensions.  Any other pairing is RT_ERR_UNSUPPORTED (the reference bails on it).
  * `dst` must hold rt_tensor_nbytes(dst_dtype, numel).  Copies are asynchronous on `stream`; the image
  * must stay valid until the stream is synchronized. */
 RT_API rt_status rt_gguf_load_tensor(rt_ctx *ctx, const rt_gguf *g, const void *image, uint64_t size, uint64_t index,

@@ -17,7 +17,7 @@ RT_MAX_RANK = 8
 RT_OK, RT_ERR_INVALID_ARG, RT_ERR_INVALID_SHAPE, RT_ERR_DTYPE_MISMATCH = 0, 1, 2, 3
 RT_ERR_UNSUPPORTED, RT_ERR_NO_DEVICE, RT_ERR_HIP, RT_ERR_OOM = 4, 5, 6, 7
 # rt_dtype
-RT_F32, RT_F16, RT_Q8_0F, RT_Q8_0H, RT_Q4_K = 0, 1, 2, 3, 4
+RT_F32, RT_F16, RT_Q8_0F, RT_Q8_0H, RT_Q4_K, RT_Q4_0 = 0, 1, 2, 3, 4, 5
 # rt_kernel_kind
 RT_KERNEL_NONE, RT_KERNEL_GEMV_Q8, RT_KERNEL_GEMV_Q4K, RT_KERNEL_GEMV_FLOAT = 0, 1, 2, 3
 RT_KERNEL_GEMM_F16, RT_KERNEL_GEMM_F32 = 4, 5
@@ -87,6 +87,7 @@ SIGNATURES = {
     "rt_matmul_spec": (_i32, [_P(MatmulDesc), _P(GemmSpec)]),
     "rt_tensor_nbytes": (_i32, [_i32, _u64, _P(_u64)]),
     "rt_q8_0_scale_offset": (_u64, [_u64]),
+    "rt_q4_0_scale_offset": (_u64, [_u64]),
     "rt_status_string": (ctypes.c_char_p, [_i32]),
     "rt_kernel_string": (ctypes.c_char_p, [_i32]),
     "rt_ctx_create": (_i32, [_i32, _P(_vp)]),
@@ -111,6 +112,7 @@ SIGNATURES = {
     "rt_quantize_q8_0": (_i32, [_vp, _vp, _u64, _vp, _vp]),
     "rt_dequantize": (_i32, [_vp, _i32, _vp, _u64, _vp, _vp]),
     "rt_transcode_gguf_q8_0": (_i32, [_vp, _vp, _u64, _i32, _vp, _vp]),
+    "rt_transcode_gguf_q4_0": (_i32, [_vp, _vp, _u64, _vp, _vp]),
     "rt_softmax_validate": (_i32, [_i32, _i32, _P(ctypes.c_int64), _i32]),
     "rt_softmax_enqueue": (_i32, [_vp, _i32, _vp, _i32, _P(ctypes.c_int64), _i32, _vp]),
     "rt_attention_validate": (_i32, [_P(AttentionDesc)]),

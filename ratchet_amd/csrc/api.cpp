@@ -264,6 +264,7 @@ rt_status rt_matmul_spec(const rt_matmul_desc *desc, rt_gemm_spec *spec) {
     RT_GUARD_END(nullptr)
 }
 
+uint64_t rt_q4_0_scale_offset(uint64_t numel) { return rt::q40_scale_offset(numel); }
 uint64_t rt_q8_0_scale_offset(uint64_t numel) { return (numel + 255u) & ~(uint64_t)255u; }
 
 rt_status rt_tensor_nbytes(int32_t dtype, uint64_t numel, uint64_t *nbytes) {
@@ -280,6 +281,10 @@ rt_status rt_tensor_nbytes(int32_t dtype, uint64_t numel, uint64_t *nbytes) {
     case RT_Q4_K:
         if (numel % 256) return RT_ERR_UNSUPPORTED;
         *nbytes = (numel / 256) * 144;
+        return RT_OK;
+    case RT_Q4_0:
+        if (numel % 32) return RT_ERR_UNSUPPORTED;
+        *nbytes = a256(numel / 2) + a256(numel / 32 * 2);
         return RT_OK;
     }
     return RT_ERR_INVALID_ARG;
@@ -491,6 +496,16 @@ rt_status rt_transcode_gguf_q8_0(rt_ctx *ctx, const void *blocks, uint64_t n_blo
     if (((uintptr_t)blocks & 1u) || ((uintptr_t)dst & 15u)) return fail(ctx, RT_ERR_INVALID_ARG, "misaligned buffer");
     DeviceGuard dg(ctx->dev.ordinal);
     hipError_t e = rt::launch_transcode_gguf_q8_0(blocks, n_blocks, dst_dtype, dst, (hipStream_t)stream);
+    if (e != hipSuccess) return hip_fail(ctx, "transcode launch", e);
+    return RT_OK;
+}
+
+rt_status rt_transcode_gguf_q4_0(rt_ctx *ctx, const void *blocks, uint64_t n_blocks, void *dst, void *stream) {
+    if (!ctx || (n_blocks && (!blocks || !dst))) return RT_ERR_INVALID_ARG;
+    if (((uintptr_t)blocks & 1u) || ((uintptr_t)dst & 15u)) return fail(ctx, RT_ERR_INVALID_ARG, "misaligned buffer");
+    DeviceGuard dg(ctx->dev.ordinal);
+    if (!dg.ok) return fail(ctx, RT_ERR_NO_DEVICE, "hipSetDevice failed");
+    hipError_t e = rt::launch_transcode_gguf_q4_0(blocks, n_blocks, dst, (hipStream_t)stream);
     if (e != hipSuccess) return hip_fail(ctx, "transcode launch", e);
     return RT_OK;
 }

@@ -143,6 +143,22 @@ __device__ __forceinline__ void q4k_scale_min(int j, const uint8_t *s, int &sc, 
     }
 }
 
+// Q4_0 codes: a dword holds eight values, nibbles 0..3 the values 0, 2, 4, 6 and nibbles 4..7 the values 1, 3, 5, 7, so that nibble i of
+// both halfwords is the pair (2 i, 2 i + 1).  A nibble in the low bits of an f16 of exponent 2^10 is 1024 + q, in the next four 1024 + 16 q:
+// one subtraction, or one fused multiply-add by 1/16, leaves q - 8.  All of it is exact; nine instructions for eight values.
+__device__ __forceinline__ half8_t q40_codes(uint32_t w) {
+    constexpr uint32_t kLow = 0x000F000Fu, kHigh = 0x00F000F0u, kBias = 0x64006400u;
+    const half2_t off = {(half_t)1032.f, (half_t)1032.f}, mul = {(half_t)0.0625f, (half_t)0.0625f}, add = {(half_t)-72.f, (half_t)-72.f};
+    const uint32_t v = w >> 8;
+    const half2_t a = __builtin_bit_cast(half2_t, (w & kLow) | kBias) - off;
+    const half2_t b = __builtin_elementwise_fma(__builtin_bit_cast(half2_t, (w & kHigh) | kBias), mul, add);
+    const half2_t c = __builtin_bit_cast(half2_t, (v & kLow) | kBias) - off;
+    const half2_t d = __builtin_elementwise_fma(__builtin_bit_cast(half2_t, (v & kHigh) | kBias), mul, add);
+    return half8_t{a[0], a[1], b[0], b[1], c[0], c[1], d[0], d[1]};
+}
+// byte offset of the scales of a Q4_0 tensor: its codes, half a byte each, fill whole 256 bytes
+inline uint64_t q40_scale_offset(uint64_t numel) { return (numel / 2 + 255u) & ~(uint64_t)255u; }
+
 // Launchers (one per kernel family).  All pointers are device pointers.
 hipError_t launch_gemv(const Problem &p, const void *A, const void *B, const void *bias, void *out,
                        hipStream_t stream, const DeviceInfo &dev);
@@ -204,5 +220,6 @@ hipError_t launch_quantize_q8_0(const float *src, uint64_t numel, void *dst, hip
 hipError_t launch_dequantize(int dtype, const void *src, uint64_t numel, float *dst, hipStream_t stream);
 hipError_t launch_transcode_gguf_q8_0(const void *blocks, uint64_t n_blocks, int dst_dtype, void *dst,
                                       hipStream_t stream);
+hipError_t launch_transcode_gguf_q4_0(const void *blocks, uint64_t n_blocks, void *dst, hipStream_t stream);
 
 } // namespace rt

@@ -355,6 +355,14 @@ rt_status gguf_load_tensor(const rt_gguf *g, const void *image, uint64_t size, u
         herr = launch_transcode_gguf_q8_0(staging, numel / 32, dst_dtype, dst, stream);
         return herr == hipSuccess ? RT_OK : (why = "transcode launch", RT_ERR_HIP);
     }
+    if (ti.ggml_dtype == RT_GGML_Q4_0 && dst_dtype == RT_Q4_0) {
+        if (!staging) return why = "Q4_0 tensors need a staging buffer of size_in_bytes", RT_ERR_INVALID_ARG;
+        if (((uintptr_t)staging & 1u) || ((uintptr_t)dst & 15u)) return why = "misaligned buffer", RT_ERR_INVALID_ARG;
+        herr = hipMemcpyAsync(staging, src, ti.size_in_bytes, hipMemcpyHostToDevice, stream);
+        if (herr != hipSuccess) return why = "tensor upload", RT_ERR_HIP;
+        herr = launch_transcode_gguf_q4_0(staging, numel / 32, dst, stream);
+        return herr == hipSuccess ? RT_OK : (why = "transcode launch", RT_ERR_HIP);
+    }
     return why = "unsupported ggml dtype " + std::to_string(ti.ggml_dtype) + " for destination dtype " + std::to_string(dst_dtype), // gguf.rs:140
            RT_ERR_UNSUPPORTED;
 }

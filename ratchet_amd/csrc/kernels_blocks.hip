@@ -1,5 +1,5 @@
-// Block-format kernels: Q8_0 quantize / dequantize, GGUF Q8_0 transcode and
-// Q4_K dequantize.  All are one-pass, HBM-bound maps over the tensor.
+// Block-format kernels: Q8_0 quantize / dequantize, GGUF Q8_0 and Q4_0 transcode,
+// Q4_K and Q4_0 dequantize.  All are one-pass, HBM-bound maps over the tensor.
 #include "device_common.h"
 
 namespace rt {
@@ -126,6 +126,48 @@ __global__ __launch_bounds__(256) void transcode_q8_0_kernel(const uint16_t *__r
     }
 }
 
+// Q4_0 dequantize: one lane per dword, eight values.
+__global__ __launch_bounds__(256) void dequantize_q40_kernel(const uint32_t *__restrict__ codes, const half_t *__restrict__ scales, uint64_t ndwords,
+                                                             float *__restrict__ dst) {
+    const uint64_t t = (uint64_t)blockIdx.x * blockDim.x + threadIdx.x;
+    if (t >= ndwords) return;
+    const half8_t q = q40_codes(codes[t]);
+    const float d = (float)scales[t >> 2];
+    float4_t *o = (float4_t *)(dst + 8 * t);
+#pragma unroll
+    for (int v = 0; v < 2; v++) {
+        float4_t r;
+#pragma unroll
+        for (int i = 0; i < 4; i++) r[i] = (float)q[4 * v + i] * d;
+        o[v] = r;
+    }
+}
+
+// GGUF Q4_0 (block_q4_0 of ggml, named but not loaded by the reference: crates/ratchet-loader/src/lib.rs:35-101): 18 bytes {f16 d; u8 qs[16]},
+// qs[j] = value j in its low nibble, value j + 16 in its high one.  One lane per block: the nibbles of eight values into one dword, even
+// values first (q40_codes).
+__device__ __forceinline__ uint32_t q40_gather(uint32_t n) { // bytes 0x0v of values 0..3 -> nibbles 0, 4, 1, 5
+    return (n & 0xFu) | ((n >> 12) & 0xF0u) | ((n << 8) & 0xF0000u) | ((n >> 4) & 0xF00000u);
+}
+__global__ __launch_bounds__(256) void transcode_q40_kernel(const uint16_t *__restrict__ blocks, uint64_t nblocks, uint8_t *__restrict__ codes,
+                                                            uint16_t *__restrict__ scales) {
+    const uint64_t b = (uint64_t)blockIdx.x * blockDim.x + threadIdx.x;
+    if (b >= nblocks) return;
+    const uint16_t *src = blocks + b * 9;
+    uint32_t w[4];
+#pragma unroll
+    for (int i = 0; i < 4; i++) w[i] = (uint32_t)src[1 + 2 * i] | ((uint32_t)src[2 + 2 * i] << 16);
+    uint4_t o;
+#pragma unroll
+    for (int u = 0; u < 4; u++) { // values 8 u .. + 7: bytes 8 (u % 2) .. + 7, low nibbles for u < 2
+        const uint32_t a = (u < 2 ? w[2 * (u & 1)] : w[2 * (u & 1)] >> 4) & 0x0F0F0F0Fu;
+        const uint32_t c = (u < 2 ? w[2 * (u & 1) + 1] : w[2 * (u & 1) + 1] >> 4) & 0x0F0F0F0Fu;
+        o[u] = q40_gather(a) | (q40_gather(c) << 8);
+    }
+    *(uint4_t *)(codes + b * 16) = o;
+    scales[b] = src[0];
+}
+
 static inline unsigned blocks_for(uint64_t n, unsigned threads) { return (unsigned)((n + threads - 1) / threads); }
 
 static void zero_padding(uint8_t *base, uint64_t from, uint64_t to, hipStream_t stream) {
@@ -157,6 +199,9 @@ hipError_t launch_dequantize(int dtype, const void *src, uint64_t numel, float *
     } else if (dtype == RT_Q4_K) {
         const uint64_t nch = numel / 64;
         hipLaunchKernelGGL(dequantize_q4k_kernel, dim3(blocks_for(nch, 256)), dim3(256), 0, stream, s, nch, dst);
+    } else if (dtype == RT_Q4_0) {
+        hipLaunchKernelGGL(dequantize_q40_kernel, dim3(blocks_for(numel / 8, 256)), dim3(256), 0, stream, (const uint32_t *)s,
+                           (const half_t *)(s + q40_scale_offset(numel)), numel / 8, dst);
     } else {
         return hipErrorInvalidValue;
     }
@@ -179,6 +224,17 @@ hipError_t launch_transcode_gguf_q8_0(const void *blocks, uint64_t n_blocks, int
         return hipErrorInvalidValue;
     zero_padding(d, numel, soff, stream);
     zero_padding(d, soff + n_blocks * ssz, soff + align256(n_blocks * ssz), stream);
+    return hipGetLastError();
+}
+
+hipError_t launch_transcode_gguf_q4_0(const void *blocks, uint64_t n_blocks, void *dst, hipStream_t stream) {
+    if (n_blocks == 0) return hipSuccess;
+    const uint64_t nb = n_blocks * 16, soff = q40_scale_offset(n_blocks * 32);
+    uint8_t *d = (uint8_t *)dst;
+    hipLaunchKernelGGL(transcode_q40_kernel, dim3(blocks_for(n_blocks, 256)), dim3(256), 0, stream, (const uint16_t *)blocks, n_blocks, d,
+                       (uint16_t *)(d + soff));
+    zero_padding(d, nb, soff, stream);
+    zero_padding(d, soff + n_blocks * 2, soff + align256(n_blocks * 2), stream);
     return hipGetLastError();
 }
 

@@ -5,11 +5,12 @@
 // cores (v_mfma_f32_32x32x16_f16 for f16 operands, v_mfma_f32_32x32x2_f32 for
 // f32).
 //
-// A may also be a quantized weight (Q8_0 segments, Q4_K super-blocks).  Its
+// A may also be a quantized weight (Q8_0 or Q4_0 segments, Q4_K super-blocks).  Its
 // integer codes are written to LDS unscaled (an int8 or a nibble is exact in
 // f16), one K tile is exactly one quantization block, and the block's scale is
 // applied in f32 to the tile's partial sums:
 //   Q8_0:  acc += d * sum_k q x
+//   Q4_0:  acc += d * sum_k (q - 8) x
 //   Q4_K:  acc += (d*sc) * sum_k q x  -  (dmin*mn) * sum_k x
 // so no weight is ever rounded to f16.  For these modes the MFMA operands are
 // exchanged so that a lane owns one weight row and needs one scale per tile.
@@ -31,11 +32,11 @@ namespace rt {
 constexpr int BK = 32;
 constexpr int kGemmThreads = 256;
 
-enum LoadMode { LM_GEN = 0, LM_VECK = 1, LM_VECR = 2, LM_Q8 = 3, LM_Q4K = 4 };
+enum LoadMode { LM_GEN = 0, LM_VECK = 1, LM_VECR = 2, LM_Q8 = 3, LM_Q4K = 4, LM_Q40 = 5 };
 
 struct GemmArgs {
     const void *A;
-    const void *scales; // Q8_0 scale stream of A
+    const void *scales; // Q8_0 or Q4_0 scale stream of A
     const void *B;
     const void *bias;
     void *out;
@@ -68,6 +69,10 @@ template <typename T, int MODE, int E> struct TileRegs {
 template <typename T, int E> struct TileRegs<T, LM_Q8, E> {
     uint4_t q;
     T d; // the block's scale as stored (f16 for Q8_0H, f32 for Q8_0F): widened when stored to LDS
+};
+template <typename T, int E> struct TileRegs<T, LM_Q40, E> {
+    uint2_t q;
+    half_t d;
 };
 template <typename T, int E> struct TileRegs<T, LM_Q4K, E> {
     uint4_t q, hdr; // raw nibbles and the super-block's header: decoded when stored, not when loaded,
@@ -141,6 +146,14 @@ template <typename T, int MODE, int ROWS> struct Loader {
             const int64_t el = stack_el + gr * rs + k0; // flat element index of the block start
             r.q = *(const uint4_t *)((const uint8_t *)base_v + el + 16 * hf);
             r.d = ((const T *)scales_v)[el >> 5];
+        } else if constexpr (MODE == LM_Q40) {
+            // one block of 32 per row per k tile: two threads per row, 8 bytes each
+            const int rr = (t >> 1) % ROWS, hf = t & 1;
+            int64_t gr = r0 + rr;
+            if (gr >= rows) gr = rows - 1;
+            const int64_t el = stack_el + gr * rs + k0;
+            r.q = *(const uint2_t *)((const uint8_t *)base_v + (el >> 1) + 8 * hf);
+            r.d = ((const half_t *)scales_v)[el >> 5];
         } else { // LM_Q4K: one sub-block of 32 weights per row per k tile
             const int rr = (t >> 1) % ROWS, hf = t & 1;
             int64_t gr = r0 + rr;
@@ -199,6 +212,11 @@ template <typename T, int MODE, int ROWS> struct Loader {
                 *(typename Tile<T>::Vec *)&S[rr][16 * hf + v * VEC] = x;
             }
             if (hf == 0) sd[rr] = (float)r.d;
+        } else if constexpr (MODE == LM_Q40) {
+            const int rr = (t >> 1) % ROWS, hf = t & 1;
+#pragma unroll
+            for (int v = 0; v < 2; v++) *(half8_t *)&S[rr][16 * hf + 8 * v] = q40_codes(r.q[v]); // exact
+            if (hf == 0) sd[rr] = (float)r.d;
         } else {
             const int rr = (t >> 1) % ROWS, hf = t & 1;
             const uint4_t hdr = r.hdr;
@@ -245,7 +263,7 @@ __global__ __launch_bounds__(kGemmThreads) void gemm_kernel(GemmArgs g) {
     constexpr int LDK = BK + Tile<T>::PAD;
     constexpr int WM = BM / 2, WN = BN / 2; // a wavefront's share of the tile
     constexpr int TA = WM / 32, TB = WN / 32; // in 32 x 32 MFMA tiles
-    constexpr bool QUANT = AMODE == LM_Q8 || AMODE == LM_Q4K;
+    constexpr bool QUANT = AMODE == LM_Q8 || AMODE == LM_Q4K || AMODE == LM_Q40;
     // quantized weights: two LDS stages (the next tile is stored while this one is multiplied)
     constexpr int NST = QUANT ? 2 : 1;
     __shared__ __attribute__((aligned(16))) T As[NST][BM][LDK];
@@ -467,6 +485,9 @@ static void launch_a(int amode, int bmode, dim3 grid, hipStream_t st, const Gemm
     case LM_Q4K:
         if constexpr (sizeof(T) == 2) launch_b<T, LM_Q4K, TS>(bmode, grid, st, g);
         break;
+    case LM_Q40:
+        if constexpr (sizeof(T) == 2) launch_b<T, LM_Q40, TS>(bmode, grid, st, g);
+        break;
     default: launch_b<T, LM_GEN, TS>(bmode, grid, st, g); break;
     }
 }
@@ -515,6 +536,10 @@ hipError_t launch_gemm(const Problem &p, const void *A, const void *B, const voi
         if (!aligned16(A)) return hipErrorNotSupported;
         amode = LM_Q8;
         g.scales = (const uint8_t *)A + rt_q8_0_scale_offset((uint64_t)p.a_stack * p.M * p.K);
+    } else if (p.a_dt == RT_Q4_0) {
+        if (!aligned16(A)) return hipErrorNotSupported;
+        amode = LM_Q40;
+        g.scales = (const uint8_t *)A + q40_scale_offset((uint64_t)p.a_stack * p.M * p.K);
     } else if (p.a_dt == RT_Q4_K) {
         if (!aligned16(A)) return hipErrorNotSupported;
         amode = LM_Q4K;

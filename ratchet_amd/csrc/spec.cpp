@@ -115,7 +115,7 @@ static rt_status read_desc(const rt_matmul_desc &d, Shape &a, Shape &b, Shape &b
 }
 
 // Allowed (lhs, rhs) pairs.  The first four are the reference's
-// (ops/matmul.rs:454-467).  (Q4_K, F16) is this library's extension, and so
+// (ops/matmul.rs:454-467).  (Q4_K, F16) and (Q4_0, F16) are this library's extension, and so
 // is each mirrored pair, where the activations are the lhs and the quantized
 // weight is the rhs read with trans_rhs ("x . W^T" spelled directly).
 static bool pair_allowed(int lhs, int rhs) {
@@ -225,6 +225,7 @@ static int pick_kernel(const Problem &p) {
     case RT_Q4_K:
         if (p.N <= kGemvQ4kMaxCols && b_kcontig) return RT_KERNEL_GEMV_Q4K;
         return RT_KERNEL_GEMM_F16;
+    case RT_Q4_0: return RT_KERNEL_GEMM_F16;
     default:
         if (p.N <= kGemvMaxCols && b_kcontig && (p.a_ks == 1 || p.K == 1)) return RT_KERNEL_GEMV_FLOAT;
         return p.a_dt == RT_F16 ? RT_KERNEL_GEMM_F16 : RT_KERNEL_GEMM_F32;

@@ -12,15 +12,16 @@ namespace rt {
 
 using Shape = std::vector<int64_t>;
 
-inline bool is_quantized(int dt) { return dt == RT_Q8_0F || dt == RT_Q8_0H || dt == RT_Q4_K; }
+inline bool is_quantized(int dt) { return dt == RT_Q8_0F || dt == RT_Q8_0H || dt == RT_Q4_K || dt == RT_Q4_0; }
 inline bool is_float(int dt) { return dt == RT_F32 || dt == RT_F16; }
-inline bool valid_dtype(int dt) { return dt >= RT_F32 && dt <= RT_Q4_K; }
-// DType::activation_dt (crates/ratchet-core/src/dtype/mod.rs:77-83); Q4_K pairs with f16.
+inline bool valid_dtype(int dt) { return dt >= RT_F32 && dt <= RT_Q4_0; }
+// DType::activation_dt (crates/ratchet-core/src/dtype/mod.rs:77-83); Q4_K and Q4_0 pair with f16.
 inline int activation_dt(int dt) {
     switch (dt) {
     case RT_Q8_0F: return RT_F32;
     case RT_Q8_0H: return RT_F16;
-    case RT_Q4_K: return RT_F16;
+    case RT_Q4_K:
+    case RT_Q4_0: return RT_F16;
     default: return dt;
     }
 }

@@ -136,7 +136,7 @@ class Header:
             raise OperationError(_ffi.RT_ERR_NO_DEVICE, "tensors are loaded to a GPU device")
         ti = self.tensor_infos[name]
         dst_dt = {GgmlDType.F32: DType.F32, GgmlDType.F16: DType.F16, GgmlDType.Q8_0: q8_dtype,
-                  GgmlDType.Q4K: DType.Q4_K}.get(ti.ggml_dtype)
+                  GgmlDType.Q4K: DType.Q4_K, GgmlDType.Q4_0: DType.Q4_0}.get(ti.ggml_dtype)
         if dst_dt is None:
             raise OperationError(_ffi.RT_ERR_UNSUPPORTED, f"unsupported ggml dtype {ti.ggml_dtype.name}")
         numel = int(np.prod(ti.shape, dtype=np.int64)) if ti.shape else 1
@@ -144,7 +144,7 @@ class Header:
         dev = f"cuda:{device.ordinal}"
         dst = torch.empty(max(tensor_nbytes(dst_dt, numel), 16), dtype=torch.uint8, device=dev)
         staging = torch.empty(max(ti.size_in_bytes(), 16), dtype=torch.uint8, device=dev) \
-            if ti.ggml_dtype == GgmlDType.Q8_0 else None
+            if ti.ggml_dtype in (GgmlDType.Q8_0, GgmlDType.Q4_0) else None
         st = _ffi.lib().rt_gguf_load_tensor(device.ctx, self._h, self._buf, len(self._image), ti.index, int(dst_dt),
                                             None if staging is None else ctypes.c_void_p(staging.data_ptr()),
                                             ctypes.c_void_p(dst.data_ptr()), _stream_ptr())

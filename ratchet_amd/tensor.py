@@ -28,18 +28,19 @@ from . import _ffi
 
 
 class DType(enum.IntEnum):
-    """crates/ratchet-core/src/dtype/mod.rs:10-20 (Matmul subset) + Q4_K."""
+    """crates/ratchet-core/src/dtype/mod.rs:10-20 (Matmul subset) + Q4_K and Q4_0."""
     F32 = _ffi.RT_F32
     F16 = _ffi.RT_F16
     Q8_0F = _ffi.RT_Q8_0F
     Q8_0H = _ffi.RT_Q8_0H
     Q4_K = _ffi.RT_Q4_K
+    Q4_0 = _ffi.RT_Q4_0
 
     def is_quantized(self) -> bool:
-        return self in (DType.Q8_0F, DType.Q8_0H, DType.Q4_K)
+        return self in (DType.Q8_0F, DType.Q8_0H, DType.Q4_K, DType.Q4_0)
 
     def activation_dt(self) -> "DType":
-        return {DType.Q8_0F: DType.F32, DType.Q8_0H: DType.F16, DType.Q4_K: DType.F16}.get(self, self)
+        return {DType.Q8_0F: DType.F32, DType.Q8_0H: DType.F16, DType.Q4_K: DType.F16, DType.Q4_0: DType.F16}.get(self, self)
 
     def numpy(self):
         return {DType.F32: np.float32, DType.F16: np.float16}[self]
@@ -714,3 +715,17 @@ def transcode_gguf_q8_0(blocks, shape: Sequence[int], dt: DType, device: Device)
                                              ctypes.c_void_p(out.data_ptr()), _stream_ptr()), device)
     _check(_ffi.lib().rt_sync(device.ctx, _stream_ptr()), device)
     return Tensor(shape, dt, device, out)
+
+
+def transcode_gguf_q4_0(blocks, shape: Sequence[int], device: Device) -> Tensor:
+    """The same for raw GGUF Q4_0 blocks -> Q4_0 tensor on `device`."""
+    torch = _torch()
+    raw = np.frombuffer(np.ascontiguousarray(blocks).tobytes(), dtype=np.uint8)
+    numel = int(np.prod(shape, dtype=np.int64))
+    assert numel % 32 == 0 and raw.size == (numel // 32) * 18
+    src = torch.from_numpy(raw.copy()).to(f"cuda:{device.ordinal}")
+    out = torch.empty(max(tensor_nbytes(DType.Q4_0, numel), 16), dtype=torch.uint8, device=f"cuda:{device.ordinal}")
+    _check(_ffi.lib().rt_transcode_gguf_q4_0(device.ctx, ctypes.c_void_p(src.data_ptr()), numel // 32,
+                                             ctypes.c_void_p(out.data_ptr()), _stream_ptr()), device)
+    _check(_ffi.lib().rt_sync(device.ctx, _stream_ptr()), device)
+    return Tensor(shape, DType.Q4_0, device, out)
