@@ -40,6 +40,7 @@ pub const RT_KERNEL_GEMV_Q4K: rt_kernel_kind = 2;
 pub const RT_KERNEL_GEMV_FLOAT: rt_kernel_kind = 3;
 pub const RT_KERNEL_GEMM_F16: rt_kernel_kind = 4;
 pub const RT_KERNEL_GEMM_F32: rt_kernel_kind = 5;
+pub const RT_KERNEL_GEMV_Q40: rt_kernel_kind = 6;
 
 #[repr(C)]
 #[derive(Clone, Copy, Default)]

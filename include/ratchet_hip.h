@@ -123,7 +123,8 @@ typedef enum rt_kernel_kind {
     RT_KERNEL_GEMV_Q4K = 2,  /* streaming Q4_K weight rows x up to 16 activation vectors    */
     RT_KERNEL_GEMV_FLOAT = 3,/* streaming f16/f32 weight rows x up to 8 activation vectors  */
     RT_KERNEL_GEMM_F16 = 4,  /* LDS-tiled MFMA GEMM, f16 operands (Q8_0H / Q4_K / Q4_0 dequantized) */
-    RT_KERNEL_GEMM_F32 = 5   /* LDS-tiled MFMA GEMM, f32 operands (Q8_0F dequantized)        */
+    RT_KERNEL_GEMM_F32 = 5,  /* LDS-tiled MFMA GEMM, f32 operands (Q8_0F dequantized)        */
+    RT_KERNEL_GEMV_Q40 = 6   /* streaming Q4_0 weight rows x up to 64 activation rows        */
 } rt_kernel_kind;
 
 /* Replaces: struct GEMMSpec and its accessors (ops/matmul.rs:32-245). */

@@ -20,7 +20,7 @@ RT_ERR_UNSUPPORTED, RT_ERR_NO_DEVICE, RT_ERR_HIP, RT_ERR_OOM = 4, 5, 6, 7
 RT_F32, RT_F16, RT_Q8_0F, RT_Q8_0H, RT_Q4_K, RT_Q4_0 = 0, 1, 2, 3, 4, 5
 # rt_kernel_kind
 RT_KERNEL_NONE, RT_KERNEL_GEMV_Q8, RT_KERNEL_GEMV_Q4K, RT_KERNEL_GEMV_FLOAT = 0, 1, 2, 3
-RT_KERNEL_GEMM_F16, RT_KERNEL_GEMM_F32 = 4, 5
+RT_KERNEL_GEMM_F16, RT_KERNEL_GEMM_F32, RT_KERNEL_GEMV_Q40 = 4, 5, 6
 
 _Shape = Shape = ctypes.c_int64 * RT_MAX_RANK
 

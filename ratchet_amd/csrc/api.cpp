@@ -136,11 +136,12 @@ rt_status lower_matmul(rt_ctx *ctx, const rt_matmul_desc &desc, int32_t activati
 }
 
 // The kernel families in the order they are offered a problem; each declines (hipErrorNotSupported) what it
-// does not take.  The first two see the streaming kernel kinds make_spec chose; from the third on the problem is
+// does not take.  The first three see the streaming kernel kinds make_spec chose; from the fourth on the problem is
 // a tiled one.
 using Launcher = hipError_t (*)(const rt::Problem &, const void *, const void *, const void *, void *, hipStream_t,
                                 const rt::DeviceInfo &);
 constexpr Launcher kLaunchers[] = {rt::launch_gemv,          // streaming kernels
+                                   rt::launch_gemv_q40,      // Q4_0 weights against up to 64 activation rows
                                    rt::launch_gemv_chunked,  // quantized weights against a few vectors more than one streaming launch takes
                                    rt::launch_gemm_stream,   // f16 / Q8_0H weights against a few dozen activation rows: one pass over the weight
                                    rt::launch_gemm_nt,       // K-contiguous f16 / Q8_0H problems: the large-tile kernel
@@ -150,7 +151,7 @@ constexpr Launcher kLaunchers[] = {rt::launch_gemv,          // streaming kernel
                                    rt::launch_gemm_f32,      // f32 products whose operands each have a contiguous axis
                                    rt::launch_gemm_q4k,      // Q4_K weights against many activation rows, and against few where K is too long for the streaming kernels
                                    rt::launch_gemm};         // anything
-constexpr int kNumLaunchers = (int)(sizeof(kLaunchers) / sizeof(kLaunchers[0])), kFirstTiled = 2;
+constexpr int kNumLaunchers = (int)(sizeof(kLaunchers) / sizeof(kLaunchers[0])), kFirstTiled = 3;
 
 // `hint` (a plan's memory): the family that took this problem last time is offered it first.
 rt_status run_matmul(rt_ctx *ctx, const Lowered &low, const void *lhs, const void *rhs, const void *bias, void *out,
@@ -181,7 +182,7 @@ rt_status run_matmul(rt_ctx *ctx, const Lowered &low, const void *lhs, const voi
         e = kLaunchers[first](p, A, B, bp, out, (hipStream_t)stream, ctx->dev);
         if (e == hipErrorNotSupported) p.kernel = low.p.kernel; // other pointers than last time: ask everyone again
     }
-    for (int i = streaming ? 0 : 1; i < kNumLaunchers && e == hipErrorNotSupported; i++) {
+    for (int i = streaming ? 0 : p.kernel == RT_KERNEL_GEMV_Q40 ? 1 : 2; i < kNumLaunchers && e == hipErrorNotSupported; i++) {
         if (i == first) continue;
         // operands that miss the streaming kernels' alignment take the tiled kernels
         if (i >= kFirstTiled) p.kernel = tiled_kind;
@@ -230,6 +231,7 @@ const char *rt_kernel_string(int32_t k) {
     case RT_KERNEL_GEMV_FLOAT: return "gemv_float";
     case RT_KERNEL_GEMM_F16: return "gemm_f16";
     case RT_KERNEL_GEMM_F32: return "gemm_f32";
+    case RT_KERNEL_GEMV_Q40: return "gemv_q40";
     }
     return "unknown";
 }

@@ -225,7 +225,7 @@ static int pick_kernel(const Problem &p) {
     case RT_Q4_K:
         if (p.N <= kGemvQ4kMaxCols && b_kcontig) return RT_KERNEL_GEMV_Q4K;
         return RT_KERNEL_GEMM_F16;
-    case RT_Q4_0: return RT_KERNEL_GEMM_F16;
+    case RT_Q4_0: return p.N <= kGemvQ40MaxCols && b_kcontig ? RT_KERNEL_GEMV_Q40 : RT_KERNEL_GEMM_F16;
     default:
         if (p.N <= kGemvMaxCols && b_kcontig && (p.a_ks == 1 || p.K == 1)) return RT_KERNEL_GEMV_FLOAT;
         return p.a_dt == RT_F16 ? RT_KERNEL_GEMM_F16 : RT_KERNEL_GEMM_F32;

@@ -69,6 +69,7 @@ struct Problem {
 constexpr int kGemvMaxCols = 8;      // VALU kernels (f16/f32/Q8_0F weights)
 constexpr int kGemvQ8hMaxCols = 16;  // matrix-core kernel (Q8_0H weights)
 constexpr int kGemvQ4kMaxCols = 16;  // matrix-core kernel (Q4_K weights); the VALU one takes up to kGemvMaxCols
+constexpr int kGemvQ40MaxCols = 64;  // matrix-core kernel (Q4_0 weights)
 
 rt_status validate(const rt_matmul_desc &d, std::string *why = nullptr);
 rt_status infer(const rt_matmul_desc &d, Shape &out, int &out_dt, std::string *why = nullptr);
