@@ -98,6 +98,24 @@ pub struct rt_attention_desc {
 }
 
 #[repr(C)]
+#[derive(Clone, Copy, Default)]
+pub struct rt_attention_q4_desc {
+    pub batch: i32,
+    pub heads: i32,
+    pub kv_heads: i32,
+    pub q_len: i32,
+    pub kv_len: i32,
+    pub head_dim: i32,
+    pub capacity: i32,
+    pub causal: i32,
+    pub q_strides: [i64; 3], // batch, head, row; in elements
+    pub o_strides: [i64; 3],
+    pub mask_strides: [i64; 2], // sequence, row
+    pub scale: f32,
+    pub mask_dtype: i32,
+}
+
+#[repr(C)]
 #[derive(Clone, Copy)]
 pub struct rt_gguf_tensor_info {
     pub name: *const c_char, // NUL-terminated, owned by the rt_gguf
@@ -196,6 +214,17 @@ extern "C" {
                                      v_cache: *mut c_void, v_src: *const c_void, src_strides: *const i64, batch: i32,
                                      heads: i32, capacity: i32, offset: i32, len: i32, head_dim: i32,
                                      stream: *mut c_void) -> rt_status;
+    // key/value cache held in 4-bit blocks
+    pub fn rt_cache_q4_nbytes(batch: i32, heads: i32, capacity: i32, head_dim: i32, nbytes: *mut u64, scale_offset: *mut u64) -> rt_status;
+    pub fn rt_cache_write_q4_enqueue(ctx: *mut rt_ctx, src_dtype: i32, k_cache: *mut c_void, k_src: *const c_void,
+                                     v_cache: *mut c_void, v_src: *const c_void, src_strides: *const i64, k_values: *mut c_void,
+                                     v_values: *mut c_void, offsets: *const i32, batch: i32, heads: i32, capacity: i32, offset: i32,
+                                     len: i32, head_dim: i32, stream: *mut c_void) -> rt_status;
+    pub fn rt_attention_q4_validate(desc: *const rt_attention_q4_desc) -> rt_status;
+    pub fn rt_attention_q4_workspace_bytes(desc: *const rt_attention_q4_desc, bytes: *mut u64) -> rt_status;
+    pub fn rt_attention_q4_enqueue(ctx: *mut rt_ctx, desc: *const rt_attention_q4_desc, q: *const c_void, k_cache: *const c_void,
+                                   v_cache: *const c_void, mask: *const c_void, kv_lens: *const i32, out: *mut c_void,
+                                   workspace: *mut c_void, workspace_bytes: u64, stream: *mut c_void) -> rt_status;
     // GGUF container (host-side parse; load = upload + layout conversion on `stream`)
     pub fn rt_gguf_parse(image: *const c_void, size: u64, out: *mut *mut rt_gguf) -> rt_status;
     pub fn rt_gguf_free(g: *mut rt_gguf);

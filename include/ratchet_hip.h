@@ -489,6 +489,66 @@ RT_API rt_status rt_cache_write_kv_enqueue(rt_ctx *ctx, int32_t dtype, void *k_c
                                            const void *v_src, const int64_t *src_strides, int32_t batch, int32_t heads,
                                            int32_t capacity, int32_t offset, int32_t len, int32_t head_dim, void *stream);
 
+/* ------------------------------------------------------------------------
+ * A key/value cache held in 4 bits (no counterpart in the reference, whose Cache keeps the tensors'
+ * dtype, ops/cache.rs:20-140): 4.5 bits a value instead of 16.
+ *   cache  [batch, heads, capacity, head_dim], one buffer of rt_cache_q4_nbytes bytes: rows of
+ *          head_dim / 2 bytes of codes (RT_Q4_0's dwords), the whole padded to 256 bytes, then from
+ *          `scale_offset` on the scales, f16, one per block of 32 values of a row; a head_dim that is no
+ *          multiple of 32 ends in a block of 16; a row takes 1, 2 or 4 scales (head_dim up to 32, 64,
+ *          128; where that is one more than its blocks it is written 0).  head_dim: a multiple of 16, 16 .. 128.
+ * A value held is d * (code - 8).  Of a block with m, its value of largest magnitude (the first of
+ * equals): d = -m / 8 rounded to eight significant bits (to multiples of 2^-24 where that is coarser;
+ * at most 8160 in magnitude), code = floor(x / d + 8.5) between 0 and 15 (8 where d is 0).  Every value held is an f16
+ * number.  A block with a NaN or an infinity: d is NaN, and what reads it is NaN.
+ * ------------------------------------------------------------------------ */
+RT_API rt_status rt_cache_q4_nbytes(int32_t batch, int32_t heads, int32_t capacity, int32_t head_dim, uint64_t *nbytes,
+                                    uint64_t *scale_offset);
+
+/* The cache writes of an attention module (rt_cache_write_kv_enqueue) into such caches, one launch:
+ *   src     [batch, heads, len, head_dim], F16, or F32 (rounded to f16 first), strided (elements: batch, head, row)
+ *   rows offset .. offset + len - 1 of every head of the cache <- src; with `offsets` (batch int32 in device memory,
+ *   or NULL) rows offset + offsets[b] .. of sequence b: those outside 0 .. capacity - 1 are not written
+ *   values  NULL, or f16 [batch, heads, len, head_dim], contiguous: receives the new rows as the cache holds them
+ *           (a prompt's attention can then run on rt_attention_enqueue and see what later steps will see)
+ * v_cache and v_src may both be NULL: one tensor.  Guards as rt_cache_write_enqueue; rows that no call names keep their bytes. */
+RT_API rt_status rt_cache_write_q4_enqueue(rt_ctx *ctx, int32_t src_dtype, void *k_cache, const void *k_src, void *v_cache, const void *v_src,
+                                           const int64_t *src_strides, void *k_values, void *v_values, const int32_t *offsets, int32_t batch,
+                                           int32_t heads, int32_t capacity, int32_t offset, int32_t len, int32_t head_dim, void *stream);
+
+/* Attention over such caches: out = softmax(scale * q k^T + mask) v, k and v the values held
+ * (rt_attention_enqueue's operator with another cache, heads that share keys, and sequences of their own lengths).
+ * q and out are f16 [batch, heads, q_len, head_dim], head_dim contiguous, the other dimensions strided (elements), so
+ * both may be [batch, q_len, heads * head_dim].  Head h reads the cache's head h / (heads / kv_heads).
+ *   kv_len    rows of the caches that are in use; with `kv_lens` (batch int32 in device memory, or NULL) sequence b has
+ *             kv_lens[b] of them, taken between 0 and kv_len
+ *   causal    key j is visible to query i iff j <= i + (the sequence's length - q_len)
+ *   mask      NULL, or additive, [q_len, kv_len] per sequence (mask_strides: sequence, 0 for one that all share, and row),
+ *             F32 or F16; a key whose mask is -inf is not seen, whatever its score or value
+ * A row that sees no key is NaN, as in rt_attention_enqueue.  Rows of the caches past a sequence's length are not used.
+ * Sums, maxima and scores are f32; the probabilities enter the second product as f16; a scale of the cache with more
+ * than eight significant bits makes values that round to f16. */
+typedef struct rt_attention_q4_desc {
+    int32_t batch, heads, kv_heads;
+    int32_t q_len, kv_len;
+    int32_t head_dim;           /* a multiple of 16, 16 .. 128 */
+    int32_t capacity;           /* rows per head of the caches */
+    int32_t causal;             /* 0 / 1 */
+    int64_t q_strides[3];       /* batch, head, row; multiples of 8 */
+    int64_t o_strides[3];
+    int64_t mask_strides[2];    /* sequence, row */
+    float scale;
+    int32_t mask_dtype;         /* RT_F32 or RT_F16; ignored when mask is NULL */
+} rt_attention_q4_desc;
+
+RT_API rt_status rt_attention_q4_validate(const rt_attention_q4_desc *desc);
+/* Bytes of workspace with which rt_attention_q4_enqueue shares the keys of a head among workgroups; as
+ * rt_attention_workspace_bytes.  Launches that share a workspace must not overlap. */
+RT_API rt_status rt_attention_q4_workspace_bytes(const rt_attention_q4_desc *desc, uint64_t *bytes);
+RT_API rt_status rt_attention_q4_enqueue(rt_ctx *ctx, const rt_attention_q4_desc *desc, const void *q, const void *k_cache,
+                                         const void *v_cache, const void *mask, const int32_t *kv_lens, void *out, void *workspace,
+                                         uint64_t workspace_bytes, void *stream);
+
 #ifdef __cplusplus
 }
 #endif

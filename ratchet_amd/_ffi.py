@@ -78,6 +78,19 @@ class AttentionDesc(ctypes.Structure):
     ]
 
 
+class AttentionQ4Desc(ctypes.Structure):
+    """rt_attention_q4_desc."""
+    _fields_ = [
+        ("batch", ctypes.c_int32), ("heads", ctypes.c_int32), ("kv_heads", ctypes.c_int32),
+        ("q_len", ctypes.c_int32), ("kv_len", ctypes.c_int32),
+        ("head_dim", ctypes.c_int32), ("capacity", ctypes.c_int32),
+        ("causal", ctypes.c_int32),
+        ("q_strides", ctypes.c_int64 * 3), ("o_strides", ctypes.c_int64 * 3), ("mask_strides", ctypes.c_int64 * 2),
+        ("scale", ctypes.c_float),
+        ("mask_dtype", ctypes.c_int32),
+    ]
+
+
 # name -> (restype, argtypes); the single source the symbol test walks too
 _vp, _u64, _i32 = ctypes.c_void_p, ctypes.c_uint64, ctypes.c_int32
 _P = ctypes.POINTER
@@ -120,6 +133,11 @@ SIGNATURES = {
     "rt_attention_enqueue": (_i32, [_vp, _P(AttentionDesc), _vp, _vp, _vp, _vp, _vp, _vp, _u64, _vp]),
     "rt_cache_write_enqueue": (_i32, [_vp, _i32, _vp, _vp, _P(ctypes.c_int64), _vp, _i32, _i32, _i32, _i32, _i32, _i32, _vp]),
     "rt_cache_write_kv_enqueue": (_i32, [_vp, _i32, _vp, _vp, _vp, _vp, _P(ctypes.c_int64), _i32, _i32, _i32, _i32, _i32, _i32, _vp]),
+    "rt_cache_q4_nbytes": (_i32, [_i32, _i32, _i32, _i32, _P(_u64), _P(_u64)]),
+    "rt_cache_write_q4_enqueue": (_i32, [_vp, _i32, _vp, _vp, _vp, _vp, _P(ctypes.c_int64), _vp, _vp, _vp, _i32, _i32, _i32, _i32, _i32, _i32, _vp]),
+    "rt_attention_q4_validate": (_i32, [_P(AttentionQ4Desc)]),
+    "rt_attention_q4_workspace_bytes": (_i32, [_P(AttentionQ4Desc), _P(_u64)]),
+    "rt_attention_q4_enqueue": (_i32, [_vp, _P(AttentionQ4Desc), _vp, _vp, _vp, _vp, _vp, _vp, _vp, _u64, _vp]),
     "rt_gguf_parse": (_i32, [_vp, _u64, _P(_vp)]),
     "rt_gguf_free": (None, [_vp]),
     "rt_gguf_error": (ctypes.c_char_p, [_vp]),

@@ -669,6 +669,96 @@ rt_status rt_cache_write_kv_enqueue(rt_ctx *ctx, int32_t dtype, void *k_cache, c
                        head_dim, true, stream);
 }
 
+rt_status rt_cache_q4_nbytes(int32_t batch, int32_t heads, int32_t capacity, int32_t head_dim, uint64_t *nbytes, uint64_t *scale_offset) {
+    if (!nbytes && !scale_offset) return RT_ERR_INVALID_ARG;
+    if (batch < 0 || heads < 0 || capacity < 0 || head_dim < 16 || head_dim > 128 || head_dim % 16) return RT_ERR_INVALID_SHAPE;
+    if ((int64_t)batch * heads > (int64_t(1) << 24)) return RT_ERR_INVALID_SHAPE; // rows below 2^55
+    const uint64_t soff = rt::cache_q4_scale_offset(batch, heads, capacity, head_dim);
+    const uint64_t sb = (uint64_t)batch * heads * capacity * rt::cache_q4_scales(head_dim) * 2;
+    if (scale_offset) *scale_offset = soff;
+    if (nbytes) *nbytes = soff + ((sb + 255u) & ~(uint64_t)255u);
+    return RT_OK;
+}
+
+rt_status rt_cache_write_q4_enqueue(rt_ctx *ctx, int32_t src_dtype, void *k_cache, const void *k_src, void *v_cache, const void *v_src,
+                                    const int64_t *src_strides, void *k_values, void *v_values, const int32_t *offsets, int32_t batch, int32_t heads,
+                                    int32_t capacity, int32_t offset, int32_t len, int32_t head_dim, void *stream) {
+    if (!ctx || !src_strides) return RT_ERR_INVALID_ARG;
+    RT_GUARD_BEGIN
+    if (src_dtype != RT_F32 && src_dtype != RT_F16) return fail(ctx, RT_ERR_DTYPE_MISMATCH, "cache: the source is F32 or F16");
+    if (batch < 0 || heads < 0 || capacity < 0 || offset < 0 || len < 0) return fail(ctx, RT_ERR_INVALID_SHAPE, "cache: negative size");
+    if (head_dim < 16 || head_dim > 128 || head_dim % 16) return fail(ctx, RT_ERR_INVALID_SHAPE, "cache: head_dim is a multiple of 16 up to 128");
+    if (len > capacity || offset > capacity || (!offsets && (int64_t)offset + len > capacity))
+        return fail(ctx, RT_ERR_INVALID_SHAPE, "cache: offset + len exceeds the capacity");
+    const int64_t esz = src_dtype == RT_F32 ? 4 : 2;
+    for (int i = 0; i < 3; i++)
+        if (src_strides[i] < 0 || (src_strides[i] * esz) % 16) return fail(ctx, RT_ERR_UNSUPPORTED, "cache: source strides must keep rows 16-byte aligned");
+    if ((int64_t)batch * heads == 0 || len == 0) return RT_OK;
+    if (!k_cache || !k_src || (!v_cache != !v_src) || (v_values && !v_cache)) return fail(ctx, RT_ERR_INVALID_ARG, "null device pointer");
+    if (((uintptr_t)k_cache | (uintptr_t)k_src | (uintptr_t)v_cache | (uintptr_t)v_src | (uintptr_t)k_values | (uintptr_t)v_values) & 15u)
+        return fail(ctx, RT_ERR_INVALID_ARG, "cache: buffers must be 16-byte aligned");
+    if ((uintptr_t)offsets & 3u) return fail(ctx, RT_ERR_INVALID_ARG, "cache: offsets must be 4-byte aligned");
+    if ((int64_t)batch * heads > 65535) return fail(ctx, RT_ERR_UNSUPPORTED, "cache: batch * heads above 65535");
+    if ((int64_t)len * ((head_dim + 31) / 32) * 4 > (int64_t(1) << 31)) return fail(ctx, RT_ERR_UNSUPPORTED, "cache: more than 2^31 / 16 rows at once");
+    DeviceGuard dg(ctx->dev.ordinal);
+    if (!dg.ok) return fail(ctx, RT_ERR_NO_DEVICE, "hipSetDevice failed");
+    hipError_t e = rt::launch_cache_write_q4(src_dtype, k_cache, k_src, v_cache, v_src, src_strides, k_values, v_values, offsets, batch, heads, capacity,
+                                             offset, len, head_dim, (hipStream_t)stream);
+    if (e != hipSuccess) return hip_fail(ctx, "cache write launch", e);
+    return RT_OK;
+    RT_GUARD_END(ctx)
+}
+
+rt_status rt_attention_q4_validate(const rt_attention_q4_desc *d) {
+    if (!d) return RT_ERR_INVALID_ARG;
+    if (d->batch < 0 || d->heads < 0 || d->kv_heads < 0 || d->q_len < 0 || d->kv_len < 0 || d->capacity < 0) return RT_ERR_INVALID_SHAPE;
+    if (d->kv_len > d->capacity) return RT_ERR_INVALID_SHAPE;
+    if (d->heads > 0 && (d->kv_heads == 0 || d->heads % d->kv_heads)) return RT_ERR_INVALID_SHAPE;
+    if (d->head_dim < 16 || d->head_dim > 128 || d->head_dim % 16) return RT_ERR_INVALID_SHAPE;
+    for (int j = 0; j < 3; j++) {
+        if (d->q_strides[j] < 0 || d->o_strides[j] < 0) return RT_ERR_INVALID_SHAPE;
+        if (d->q_strides[j] % 8) return RT_ERR_UNSUPPORTED; // q rows are read as 16-byte vectors
+    }
+    if (d->mask_strides[0] < 0 || d->mask_strides[1] < 0) return RT_ERR_INVALID_SHAPE;
+    if (d->causal != 0 && d->causal != 1) return RT_ERR_INVALID_ARG;
+    if (!(d->scale == d->scale)) return RT_ERR_INVALID_ARG;
+    if ((int64_t)d->batch * d->kv_heads > 65535 || d->kv_len > (1 << 30)) return RT_ERR_UNSUPPORTED;
+    if (d->heads > 0 && (int64_t)d->q_len * (d->heads / d->kv_heads) > 32 * 65535) return RT_ERR_UNSUPPORTED;
+    return RT_OK;
+}
+
+rt_status rt_attention_q4_workspace_bytes(const rt_attention_q4_desc *desc, uint64_t *bytes) {
+    if (!desc || !bytes) return RT_ERR_INVALID_ARG;
+    const rt_status st = rt_attention_q4_validate(desc);
+    if (st != RT_OK) return st;
+    *bytes = rt::attention_q4_workspace_bytes(*desc);
+    return RT_OK;
+}
+
+rt_status rt_attention_q4_enqueue(rt_ctx *ctx, const rt_attention_q4_desc *desc, const void *q, const void *k_cache, const void *v_cache,
+                                  const void *mask, const int32_t *kv_lens, void *out, void *workspace, uint64_t workspace_bytes, void *stream) {
+    if (!ctx || !desc) return RT_ERR_INVALID_ARG;
+    RT_GUARD_BEGIN
+    const rt_status st = rt_attention_q4_validate(desc);
+    if (st != RT_OK) return fail(ctx, st, "attention: invalid descriptor");
+    if (mask && desc->mask_dtype != RT_F32 && desc->mask_dtype != RT_F16)
+        return fail(ctx, RT_ERR_DTYPE_MISMATCH, "attention: the mask is F32 or F16");
+    if (mask && desc->mask_strides[1] < desc->kv_len) return fail(ctx, RT_ERR_INVALID_SHAPE, "attention: mask rows overlap");
+    if ((int64_t)desc->batch * desc->heads == 0 || desc->q_len == 0) return RT_OK; // empty output
+    if (!q || !out || (desc->kv_len > 0 && (!k_cache || !v_cache))) return fail(ctx, RT_ERR_INVALID_ARG, "null device pointer");
+    if (((uintptr_t)q | (uintptr_t)k_cache | (uintptr_t)v_cache) & 15u)
+        return fail(ctx, RT_ERR_INVALID_ARG, "attention: q and the caches must be 16-byte aligned");
+    if (((uintptr_t)out & 1u) || ((uintptr_t)kv_lens & 3u) || (mask && ((uintptr_t)mask & (desc->mask_dtype == RT_F32 ? 3u : 1u))))
+        return fail(ctx, RT_ERR_INVALID_ARG, "attention: out, mask and kv_lens must be aligned to their types");
+    DeviceGuard dg(ctx->dev.ordinal);
+    if (!dg.ok) return fail(ctx, RT_ERR_NO_DEVICE, "hipSetDevice failed");
+    hipError_t e = rt::launch_attention_q4(*desc, q, k_cache, v_cache, mask, kv_lens, out, workspace, workspace_bytes, (hipStream_t)stream, ctx->dev);
+    if (e == hipErrorNotSupported) return fail(ctx, RT_ERR_UNSUPPORTED, "attention: too many rows");
+    if (e != hipSuccess) return hip_fail(ctx, "attention launch", e);
+    return RT_OK;
+    RT_GUARD_END(ctx)
+}
+
 rt_status rt_gguf_load_tensor(rt_ctx *ctx, const rt_gguf *g, const void *image, uint64_t size, uint64_t index,
                               int32_t dst_dtype, void *staging, void *dst, void *stream) {
     if (!ctx || !g || !image) return RT_ERR_INVALID_ARG;

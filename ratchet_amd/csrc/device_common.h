@@ -159,6 +159,13 @@ __device__ __forceinline__ half8_t q40_codes(uint32_t w) {
 // byte offset of the scales of a Q4_0 tensor: its codes, half a byte each, fill whole 256 bytes
 inline uint64_t q40_scale_offset(uint64_t numel) { return (numel / 2 + 255u) & ~(uint64_t)255u; }
 
+// A 4-bit key/value cache [batch, heads, capacity, head_dim] in one buffer: codes, head_dim / 2 bytes a row, to whole 256 bytes, then a row's
+// scales, one f16 per 32 values (the last block may have 16), as many as the next of 1, 2 and 4.
+inline int cache_q4_scales(int head_dim) { return head_dim <= 32 ? 1 : head_dim <= 64 ? 2 : 4; }
+inline uint64_t cache_q4_scale_offset(int batch, int heads, int capacity, int head_dim) {
+    return ((uint64_t)batch * heads * capacity * (head_dim / 2) + 255u) & ~(uint64_t)255u;
+}
+
 // Launchers (one per kernel family).  All pointers are device pointers.
 hipError_t launch_gemv(const Problem &p, const void *A, const void *B, const void *bias, void *out,
                        hipStream_t stream, const DeviceInfo &dev);
@@ -213,6 +220,12 @@ hipError_t launch_cast(int src_dtype, int dst_dtype, const void *src, void *dst,
 hipError_t launch_cache_write(void *cache, const void *src, void *cache2, const void *src2, void *dst, int64_t cache_bs,
                               int64_t cache_hs, int64_t src_bs, int64_t src_hs, int64_t src_rs, int batch, int heads, int offset,
                               int len, int64_t row_bytes, hipStream_t stream);
+hipError_t launch_cache_write_q4(int src_dtype, void *k_cache, const void *k_src, void *v_cache, const void *v_src, const int64_t *strides, void *k_values,
+                                 void *v_values, const int32_t *offsets, int batch, int heads, int capacity, int offset, int len, int head_dim,
+                                 hipStream_t stream);
+uint64_t attention_q4_workspace_bytes(const rt_attention_q4_desc &d);
+hipError_t launch_attention_q4(const rt_attention_q4_desc &d, const void *q, const void *k_cache, const void *v_cache, const void *mask,
+                               const int32_t *kv_lens, void *out, void *workspace, uint64_t workspace_bytes, hipStream_t stream, const DeviceInfo &dev);
 hipError_t launch_softmax(int dtype, void *x, int64_t rows, int64_t n, hipStream_t stream);
 hipError_t launch_attention(const rt_attention_desc &d, const void *q, const void *k, const void *v, const void *mask,
                             void *out, void *workspace, uint64_t workspace_bytes, hipStream_t stream, const DeviceInfo &dev);

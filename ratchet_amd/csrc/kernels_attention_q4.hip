@@ -1,0 +1,488 @@
+// Attention over a key/value cache held in 4-bit blocks (kernels_cache_q4.hip has the format), for one or a few query rows per head of keys:
+//
+//   out[m] = softmax_j(scale * sum_b dk[j, b] sum_{c in b} q[m, c] (qk[j, c] - 8) + mask[m, j]) . (dv[j, b] (qv[j, c] - 8))
+//
+// The rows m are the query rows of the heads that share a head of keys: m = query row * group + head of the group.
+//
+// A wavefront takes 64 keys at a time.  Scores: v_mfma_f32_16x16x32_f16 contracts a block of 32 for 16 rows and 16 keys, codes unscaled (exact), the
+// block's sum scaled by dk in f32.  A load is 16 bytes a lane of consecutive pieces of consecutive keys, and a 4 x 4 transposition among lane
+// groups puts dword g of a block into lane group g, as the operand wants it (kernels_gemv_q40.hip has the same step).  Rows up to 4 (8) are put at
+// MFMA rows 4 m (4 m, 4 m + 1), where one result register (two) holds them all.
+// Softmax: running maximum and sum in f32, base 2; a row's keys are spread over 16 lanes, which four DPP rotations join for the maximum, and only at
+// the end for the sum.
+// Values: the operand of the second product holds, for one dimension, eight keys in a lane.  Codes of one key are neighbours along the dimensions, so
+// lane c (of 16) reads a dword (half, byte, nibble for what is left of head_dim) of each key's row, and a byte permutation of two keys' puts the same
+// nibble of both into the two halves of a register: the unpacking of q40_codes with pairs of keys in place of pairs of dimensions.  The
+// order of keys in that product is free: 4 r + s is key 16 s + r, so that a lane's four probabilities are neighbours.  dv (q - 8) is exact in f16 for
+// scales of eight significant bits, which is what the cache's write makes (others round here); dv = 0 past the last key.  The probabilities enter as
+// f16, as in kernels_attention.hip.
+//
+// Wavefronts of a workgroup take 64 keys in turn and are merged through LDS; where there are few heads several workgroups share the keys and a second
+// kernel merges them, in a fixed order.
+#include "device_common.h"
+
+#include <algorithm>
+#include <cmath>
+
+namespace rt {
+
+constexpr float kLog2eQ4 = 1.4426950408889634f;
+
+struct AttnQ4Args {
+    const half_t *Q;
+    const uint8_t *Kc, *Vc;
+    const half_t *Ks, *Vs;
+    const void *mask;
+    const int32_t *lens;
+    half_t *O;
+    float *part_o, *part_ml; // [row][split][D], [row][split][2]
+    int64_t q_bs, q_hs, q_rs, o_bs, o_hs, o_rs, m_bs, m_rs;
+    int kv_heads, group, rows, kv_len, q_len, capacity; // rows = q_len * group
+    int causal, mask_f32, splits, split_keys, row_tiles;
+    float scale_log2e;
+};
+
+typedef uint32_t uint4_a8 __attribute__((ext_vector_type(4), aligned(8)));
+typedef uint32_t uint2_a8 __attribute__((ext_vector_type(2), aligned(8)));
+
+// lane group g's register t <- lane group t's register g
+__device__ __forceinline__ void aq_transpose(uint4_t &v) {
+    const auto a = __builtin_amdgcn_permlane16_swap(v[0], v[1], false, false);
+    const auto b = __builtin_amdgcn_permlane16_swap(v[2], v[3], false, false);
+    const auto c = __builtin_amdgcn_permlane32_swap(a[0], b[0], false, false);
+    const auto d = __builtin_amdgcn_permlane32_swap(a[1], b[1], false, false);
+    v = uint4_t{c[0], d[0], c[1], d[1]};
+}
+template <int CTRL> __device__ __forceinline__ float aq_dpp(float v) {
+    return __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, v), CTRL, 0xf, 0xf, true));
+}
+__device__ __forceinline__ float aq_max16(float v) {
+    v = fmaxf(v, aq_dpp<0x128>(v)), v = fmaxf(v, aq_dpp<0x124>(v));
+    v = fmaxf(v, aq_dpp<0x122>(v));
+    return fmaxf(v, aq_dpp<0x121>(v));
+}
+__device__ __forceinline__ float aq_sum16(float v) {
+    v += aq_dpp<0x128>(v), v += aq_dpp<0x124>(v);
+    v += aq_dpp<0x122>(v);
+    return v + aq_dpp<0x121>(v);
+}
+__device__ __forceinline__ uint32_t aq_or16(uint32_t v) {
+    v |= (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x128, 0xf, 0xf, true);
+    v |= (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x124, 0xf, 0xf, true);
+    v |= (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x122, 0xf, 0xf, true);
+    return v | (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x121, 0xf, 0xf, true);
+}
+
+// How a head_dim of 16 NT is read by 16 lanes: a dword of a row each (128), or two bytes (64), a byte (32) and a nibble (16) as they are needed.
+template <int NT> struct AqDims {
+    static constexpr int D = 16 * NT, NF = D / 32, TAIL = NT & 1, NB = NF + TAIL, SR = NB == 3 ? 4 : NB, PB = NF ? NF : 1; // (PB: pieces of 16 bytes of a key, where there are any)
+    static constexpr bool P4 = NT == 8, P2 = NT & 4, P1 = NT & 2, PH = NT & 1;
+    static constexpr int T2 = 0, T1 = P2 ? 4 : 0, TH = T1 + (P1 ? 2 : 0); // first tile of a piece
+    static constexpr int B1 = P2 ? 32 : 0, BH = B1 + (P1 ? 16 : 0);       // its first byte of a row
+    // dimension that lane c's column of tile t stands for
+    __device__ __forceinline__ static int dim(int t, int c) {
+        auto of = [](int nibble) { return 8 * (nibble >> 3) + ((nibble & 3) << 1) + ((nibble >> 2) & 1); }; // of a row's nibble
+        if (P4) return of(8 * c + t);
+        if (P2 && t < 4) return of(4 * c + t);
+        if (P1 && t < T1 + 2) return of(2 * B1 + 2 * c + (t - T1));
+        return of(2 * BH + c);
+    }
+};
+
+// RT: row tiles of 16; VPR: result registers in use with one row tile (1: up to 4 rows, 4: up to 16)
+template <int NT, int RT, int VPR> __global__ __launch_bounds__(RT == 1 ? 512 : 256) void attention_q4_kernel(AttnQ4Args g) {
+    using DM = AqDims<NT>;
+    constexpr int D = DM::D, NF = DM::NF, NB = DM::NB, SR = DM::SR, RB = D / 2;
+    constexpr int ROWS = RT == 1 ? 4 * VPR : 16 * RT; // rows of the tile
+    constexpr int PS = 72;                            // halves between rows of probabilities
+    constexpr int WAVE_LDS = (ROWS * PS + NB * 64) * 2;
+    extern __shared__ __attribute__((aligned(16))) uint8_t smem[];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), waves = blockDim.x >> 6;
+    const int r = lane & 15, fg = lane >> 4;
+    half_t *P = (half_t *)(smem + wave * WAVE_LDS), *S = P + ROWS * PS; // this wavefront's: probabilities [row][position], scales of values [block][position]
+    const int bk = blockIdx.y, b = bk / g.kv_heads, kh = bk - b * g.kv_heads;
+    const int row0 = blockIdx.z * ROWS;
+
+    int len = g.kv_len;
+    if (g.lens) len = min(max(g.lens[b], 0), len);
+    // row m's query row, head and last visible key
+    auto q_row = [&](int m) { return m / g.group; };
+    int m_of[RT][VPR], last[RT][VPR];
+#pragma unroll
+    for (int t = 0; t < RT; t++)
+#pragma unroll
+        for (int v = 0; v < VPR; v++) {
+            m_of[t][v] = row0 + 16 * t + (RT == 1 ? fg * VPR + v : 4 * fg + v);
+            last[t][v] = g.causal ? min(len - 1, q_row(min(m_of[t][v], g.rows - 1)) + len - g.q_len) : len - 1;
+        }
+    // the keys of this workgroup: its share of those that any row of the tile sees
+    int end = len;
+    if (g.causal) end = min(end, q_row(min(row0 + ROWS, g.rows) - 1) + len - g.q_len + 1);
+    const int j_first = blockIdx.x * g.split_keys;
+    const int j_end = min(end, j_first + g.split_keys);
+
+    const int64_t head = (int64_t)bk * g.capacity;
+    const uint8_t *Kc = g.Kc + head * RB, *Vc = g.Vc + head * RB;
+    const half_t *Ks = g.Ks + head * SR, *Vs = g.Vs + head * SR;
+
+    half8_t qf[RT][NB];
+#pragma unroll
+    for (int t = 0; t < RT; t++) {
+        const int m = min(row0 + 16 * t + (RT == 1 ? (r >> 2) * VPR + min(r & 3, VPR - 1) : r), g.rows - 1), qi = q_row(m);
+        const half_t *q = g.Q + b * g.q_bs + (int64_t)(kh * g.group + (m - qi * g.group)) * g.q_hs + qi * g.q_rs + 8 * fg;
+#pragma unroll
+        for (int k = 0; k < NF; k++) qf[t][k] = *(const half8_t *)(q + 32 * k);
+        if constexpr (DM::TAIL) qf[t][NF] = fg < 2 ? *(const half8_t *)(q + 32 * NF) : half8_t{};
+    }
+
+    float mx[RT][VPR], sum[RT][VPR];
+    uint32_t bad[RT][VPR];
+    float4_t o[RT][NT];
+#pragma unroll
+    for (int t = 0; t < RT; t++) {
+#pragma unroll
+        for (int v = 0; v < VPR; v++) mx[t][v] = -INFINITY, sum[t][v] = 0.f, bad[t][v] = 0;
+#pragma unroll
+        for (int n = 0; n < NT; n++) o[t][n] = float4_t{0.f, 0.f, 0.f, 0.f};
+    }
+
+    for (int j0 = j_first + 64 * wave; j0 < j_end; j0 += 64 * waves) {
+        const int clamp = len - 1; // > = 0 here; keys past it repeat it
+        // ---- loads
+        uint4_t kc[NF + DM::TAIL];
+#pragma unroll
+        for (int i = 0; i < NF; i++) {
+            const int pc = 4 * i + fg, ks = pc / DM::PB, kb = pc - ks * DM::PB; // piece: key set and block
+            kc[i] = *(const uint4_a8 *)(Kc + (uint32_t)min(j0 + 16 * ks + r, clamp) * (uint64_t)RB + 16 * kb);
+        }
+        if constexpr (DM::TAIL) {
+            const uint2_t w = *(const uint2_a8 *)(Kc + (uint32_t)min(j0 + 16 * fg + r, clamp) * (uint64_t)RB + 16 * NF);
+            kc[NF] = uint4_t{w[0], w[1], 0, 0};
+        }
+        half_t dk[4][SR];
+#pragma unroll
+        for (int s = 0; s < 4; s++) {
+            const half_t *p = Ks + (uint32_t)min(j0 + 16 * s + r, clamp) * (uint64_t)SR;
+            if constexpr (SR == 1) dk[s][0] = *p;
+            else if constexpr (SR == 2) {
+                const half2_t x = *(const half2_t *)p;
+                dk[s][0] = x[0], dk[s][1] = x[1];
+            } else {
+                const half4_t x = *(const half4_t *)p;
+#pragma unroll
+                for (int k = 0; k < 4; k++) dk[s][k] = x[k];
+            }
+        }
+        half_t dv[SR];
+        {
+            const half_t *p = Vs + (uint32_t)min(j0 + 16 * fg + r, clamp) * (uint64_t)SR;
+            if constexpr (SR == 1) dv[0] = *p;
+            else if constexpr (SR == 2) {
+                const half2_t x = *(const half2_t *)p;
+                dv[0] = x[0], dv[1] = x[1];
+            } else {
+                const half4_t x = *(const half4_t *)p;
+#pragma unroll
+                for (int k = 0; k < 4; k++) dv[k] = x[k];
+            }
+        }
+        uint32_t v2[2][8], v1[2][8], vh[2][8]; // (v2: dwords of a head_dim of 128)
+#pragma unroll
+        for (int u = 0; u < 2; u++)
+#pragma unroll
+            for (int e = 0; e < 8; e++) {
+                const uint8_t *p = Vc + (uint32_t)min(j0 + 16 * (e & 3) + 8 * u + 2 * fg + (e >> 2), clamp) * (uint64_t)RB;
+                if constexpr (DM::P4) v2[u][e] = *(const uint32_t *)(p + 4 * r);
+                if constexpr (DM::P2) v2[u][e] = *(const uint16_t *)(p + 2 * r);
+                if constexpr (DM::P1) v1[u][e] = p[DM::B1 + r];
+                if constexpr (DM::PH) vh[u][e] = p[DM::BH + (r >> 1)];
+            }
+
+        // ---- scores
+        float sc[RT][4][VPR];
+#pragma unroll
+        for (int t = 0; t < RT; t++)
+#pragma unroll
+            for (int s = 0; s < 4; s++)
+#pragma unroll
+                for (int v = 0; v < VPR; v++) sc[t][s][v] = 0.f;
+        auto block = [&](uint32_t w, int s, int k) __attribute__((always_inline)) {
+            const half8_t q = q40_codes(w);
+            const float d = (float)dk[s][k];
+#pragma unroll
+            for (int t = 0; t < RT; t++) {
+                const float4_t p = __builtin_amdgcn_mfma_f32_16x16x32_f16(qf[t][k], q, float4_t{0.f, 0.f, 0.f, 0.f}, 0, 0, 0);
+#pragma unroll
+                for (int v = 0; v < VPR; v++) sc[t][s][v] = fmaf(d, p[v], sc[t][s][v]);
+            }
+        };
+#pragma unroll
+        for (int i = 0; i < NF; i++) {
+            aq_transpose(kc[i]);
+#pragma unroll
+            for (int x = 0; x < 4; x++) block(kc[i][x], (4 * i + x) / DM::PB, (4 * i + x) % DM::PB);
+        }
+        if constexpr (DM::TAIL) {
+            aq_transpose(kc[NF]);
+#pragma unroll
+            for (int s = 0; s < 4; s++) block(kc[NF][s], s, NF);
+        }
+
+        // ---- mask, running maximum and sum, probabilities to LDS
+        const bool inside = j0 + 63 < len && !g.causal; // no key hidden
+#pragma unroll
+        for (int t = 0; t < RT; t++)
+#pragma unroll
+            for (int v = 0; v < VPR; v++) {
+                const int64_t mrow = b * g.m_bs + q_row(min(m_of[t][v], g.rows - 1)) * g.m_rs;
+#pragma unroll
+                for (int s = 0; s < 4; s++) {
+                    const int j = j0 + 16 * s + r;
+                    float x = sc[t][s][v] * g.scale_log2e;
+                    if (g.mask) {
+                        const int64_t at = mrow + min(j, clamp);
+                        const float mk = g.mask_f32 ? ((const float *)g.mask)[at] : (float)((const half_t *)g.mask)[at];
+                        // a hidden key's score may be anything; a type's lowest value hides nothing from a row that has nothing else
+                        const float m2 = mk * kLog2eQ4 == -INFINITY ? -3.40282347e38f : mk * kLog2eQ4;
+                        x = mk == -INFINITY ? -INFINITY : x + m2;
+                    }
+                    if (!inside) x = j <= last[t][v] ? x : -INFINITY;
+                    sc[t][s][v] = x;
+                }
+                const float top = fmaxf(mx[t][v], aq_max16(fmaxf(fmaxf(sc[t][0][v], sc[t][1][v]), fmaxf(sc[t][2][v], sc[t][3][v]))));
+                const float base = top == -INFINITY ? 0.f : top;
+                const float a = __builtin_amdgcn_exp2f(mx[t][v] - base);
+                mx[t][v] = top;
+                float l = 0.f;
+                half4_t p4;
+#pragma unroll
+                for (int s = 0; s < 4; s++) {
+                    const float p = __builtin_amdgcn_exp2f(sc[t][s][v] - base);
+                    l += p;
+                    p4[s] = (half_t)p;
+                }
+                sum[t][v] = fmaf(sum[t][v], a, l);
+#pragma unroll
+                for (int n = 0; n < NT; n++) o[t][n][v] *= a;
+                *(half4_t *)(P + (RT == 1 ? fg * VPR + v : 16 * t + 4 * fg + v) * PS + 4 * r) = p4;
+            }
+        // ---- scales of the values to LDS; one that is not finite shows in the rows that see its key and not through the matrix cores
+        uint32_t odd = 0;
+#pragma unroll
+        for (int k = 0; k < NB; k++) {
+            const bool fin = (__builtin_bit_cast(uint16_t, dv[k]) & 0x7C00u) != 0x7C00u;
+            const bool valid = j0 + 16 * fg + r < len;
+            if (valid && !fin) odd |= 1u << k;
+            S[k * 64 + 4 * r + fg] = valid && fin ? dv[k] : (half_t)0.f;
+        }
+        if (__builtin_amdgcn_ballot_w64(odd != 0)) {
+#pragma unroll
+            for (int s = 0; s < 4; s++) {
+                const uint32_t ks = (uint32_t)__builtin_amdgcn_ds_bpermute(4 * (16 * s + r), (int)odd);
+#pragma unroll
+                for (int t = 0; t < RT; t++)
+#pragma unroll
+                    for (int v = 0; v < VPR; v++)
+                        if (!(sc[t][s][v] == -INFINITY)) bad[t][v] |= ks;
+            }
+        }
+        __builtin_amdgcn_wave_barrier();
+        asm volatile("" ::: "memory");
+
+        // ---- values
+#pragma unroll
+        for (int u = 0; u < 2; u++) {
+            half8_t pf[RT];
+#pragma unroll
+            for (int t = 0; t < RT; t++)
+                pf[t] = *(const half8_t *)(P + (RT == 1 ? (r >> 2) * VPR + min(r & 3, VPR - 1) : 16 * t + r) * PS + 32 * u + 8 * fg);
+            // four registers of key pairs: nibble `n` of the halves -> operand of tile `n0 + n`
+            auto product = [&](const uint32_t *w, int n0, int count, const half8_t d) __attribute__((always_inline)) {
+                half8_t c[4];
+#pragma unroll
+                for (int e = 0; e < 4; e++) c[e] = q40_codes(w[e]);
+#pragma unroll
+                for (int n = 0; n < count; n++) {
+                    const half8_t x = half8_t{c[0][2 * n], c[0][2 * n + 1], c[1][2 * n], c[1][2 * n + 1], c[2][2 * n], c[2][2 * n + 1], c[3][2 * n], c[3][2 * n + 1]} * d;
+#pragma unroll
+                    for (int t = 0; t < RT; t++) o[t][n0 + n] = __builtin_amdgcn_mfma_f32_16x16x32_f16(pf[t], x, o[t][n0 + n], 0, 0, 0);
+                }
+            };
+            auto scales = [&](int dim) { return *(const half8_t *)(S + (dim >> 5) * 64 + 32 * u + 8 * fg); };
+            uint32_t w[4];
+            if constexpr (DM::P4) {
+                const half8_t d = scales(8 * r);
+#pragma unroll
+                for (int hf = 0; hf < 2; hf++) {
+#pragma unroll
+                    for (int e = 0; e < 4; e++) w[e] = __builtin_amdgcn_perm(v2[u][2 * e + 1], v2[u][2 * e], hf ? 0x07060302u : 0x05040100u);
+                    product(w, 4 * hf, 4, d);
+                }
+            }
+            if constexpr (DM::P2) {
+#pragma unroll
+                for (int e = 0; e < 4; e++) w[e] = v2[u][2 * e] | (v2[u][2 * e + 1] << 16);
+                product(w, DM::T2, 4, scales(4 * r));
+            }
+            if constexpr (DM::P1) {
+#pragma unroll
+                for (int e = 0; e < 4; e++) w[e] = v1[u][2 * e] | (v1[u][2 * e + 1] << 16);
+                product(w, DM::T1, 2, scales(2 * DM::B1 + 2 * r));
+            }
+            if constexpr (DM::PH) {
+                const int sh = 4 * (r & 1);
+#pragma unroll
+                for (int e = 0; e < 4; e++) w[e] = (vh[u][2 * e] >> sh) | ((vh[u][2 * e + 1] >> sh) << 16);
+                product(w, DM::TH, 1, scales(2 * DM::BH + r));
+            }
+        }
+        __builtin_amdgcn_wave_barrier();
+        asm volatile("" ::: "memory");
+    }
+
+    // ---- this wavefront's rows: the sum over the 16 lanes, and what a scale that is not finite leaves
+#pragma unroll
+    for (int t = 0; t < RT; t++)
+#pragma unroll
+        for (int v = 0; v < VPR; v++) {
+            sum[t][v] = aq_sum16(sum[t][v]);
+            const uint32_t bd = aq_or16(bad[t][v]);
+#pragma unroll
+            for (int n = 0; n < NT; n++)
+                if ((bd >> (DM::dim(n, r) >> 5)) & 1u) o[t][n][v] = __builtin_nanf("");
+        }
+    // ---- the wavefronts' results through LDS: outputs [wave][RT][NT][VPR][64], maxima and sums [wave][row][2]
+    constexpr int PER = RT * NT * VPR * 64;
+    float *red = (float *)smem, *ml = red + waves * PER;
+    __syncthreads();
+#pragma unroll
+    for (int t = 0; t < RT; t++) {
+#pragma unroll
+        for (int n = 0; n < NT; n++)
+#pragma unroll
+            for (int v = 0; v < VPR; v++) red[wave * PER + ((t * NT + n) * VPR + v) * 64 + lane] = o[t][n][v];
+#pragma unroll
+        for (int v = 0; v < VPR; v++) {
+            const int row = RT == 1 ? fg * VPR + v : 16 * t + 4 * fg + v;
+            if (r == 0) ml[(wave * ROWS + row) * 2] = mx[t][v], ml[(wave * ROWS + row) * 2 + 1] = sum[t][v];
+        }
+    }
+    __syncthreads();
+    for (int e = threadIdx.x; e < PER; e += blockDim.x) {
+        const int l = e & 63, tnv = e >> 6, v = tnv % VPR, tn = tnv / VPR, n = tn % NT, t = tn / NT;
+        const int row = RT == 1 ? (l >> 4) * VPR + v : 16 * t + 4 * (l >> 4) + v, m = row0 + row;
+        if (m >= g.rows) continue;
+        float top = -INFINITY;
+        for (int w = 0; w < waves; w++) top = fmaxf(top, ml[(w * ROWS + row) * 2]);
+        const float base = top == -INFINITY ? 0.f : top;
+        float y = 0.f, s = 0.f;
+        for (int w = 0; w < waves; w++) {
+            const float a = __builtin_amdgcn_exp2f(ml[(w * ROWS + row) * 2] - base);
+            y = fmaf(red[w * PER + e], a, y), s = fmaf(ml[(w * ROWS + row) * 2 + 1], a, s);
+        }
+        const int d = DM::dim(n, l & 15);
+        if (g.splits > 1) {
+            const int64_t at = ((int64_t)bk * g.rows + m) * g.splits + blockIdx.x;
+            g.part_o[at * D + d] = y;
+            if (d == 0) g.part_ml[2 * at] = top, g.part_ml[2 * at + 1] = s;
+        } else {
+            const int qi = q_row(m);
+            g.O[b * g.o_bs + (int64_t)(kh * g.group + (m - qi * g.group)) * g.o_hs + qi * g.o_rs + d] = (half_t)(y / s); // no visible key: 0 / 0
+        }
+    }
+}
+
+// One workgroup per row: thread d joins dimension d of its shares.
+__global__ __launch_bounds__(128) void attention_q4_merge_kernel(AttnQ4Args g, int D) {
+    const int64_t row = blockIdx.x;
+    const int bk = (int)(row / g.rows), m = (int)(row - (int64_t)bk * g.rows), b = bk / g.kv_heads, kh = bk - b * g.kv_heads, d = threadIdx.x;
+    if (d >= D) return;
+    const float *ml = g.part_ml + row * g.splits * 2, *po = g.part_o + row * g.splits * D + d;
+    float top = -INFINITY;
+    for (int s = 0; s < g.splits; s++) top = fmaxf(top, ml[2 * s]);
+    const float base = top == -INFINITY ? 0.f : top;
+    float y = 0.f, l = 0.f;
+    for (int s = 0; s < g.splits; s++) {
+        const float a = __builtin_amdgcn_exp2f(ml[2 * s] - base);
+        y = fmaf(po[(int64_t)s * D], a, y), l = fmaf(ml[2 * s + 1], a, l);
+    }
+    const int qi = m / g.group;
+    g.O[b * g.o_bs + (int64_t)(kh * g.group + (m - qi * g.group)) * g.o_hs + qi * g.o_rs + d] = (half_t)(y / l);
+}
+
+static int aq_row_tiles(int rows) { return rows <= 16 ? 1 : (rows + 31) / 32; }
+// keys of a workgroup where several share a row tile's, and how many do
+static void aq_split(const rt_attention_q4_desc &d, int &splits, int &split_keys) {
+    const int rows = d.q_len * (d.heads / d.kv_heads);
+    const int64_t wgs = (int64_t)d.batch * d.kv_heads * aq_row_tiles(rows);
+    const int step = rows <= 16 ? 512 : 256; // of a workgroup's eight or four wavefronts
+    const int steps = (d.kv_len + step - 1) / step;
+    int s = 1;
+    if (wgs < 512 && steps > 1) s = (int)std::min<int64_t>(steps, (512 + wgs - 1) / wgs);
+    const int per = (steps + s - 1) / s;
+    splits = std::max(1, (steps + per - 1) / std::max(per, 1)), split_keys = std::max(per, 1) * step;
+}
+
+uint64_t attention_q4_workspace_bytes(const rt_attention_q4_desc &d) {
+    if (d.batch == 0 || d.heads == 0 || d.q_len == 0) return 0;
+    int splits, keys;
+    aq_split(d, splits, keys);
+    if (splits <= 1) return 0;
+    return (uint64_t)d.batch * d.heads * d.q_len * splits * (d.head_dim + 2) * sizeof(float);
+}
+
+template <int NT, int RT, int VPR> static hipError_t launch_aq(const AttnQ4Args &g, dim3 grid, int waves, hipStream_t st) {
+    using DM = AqDims<NT>;
+    constexpr int ROWS = RT == 1 ? 4 * VPR : 16 * RT;
+    const size_t wave = (ROWS * 72 + DM::NB * 64) * 2, out = ((size_t)RT * NT * VPR * 64 + 2 * ROWS) * sizeof(float);
+    const size_t lds = waves * std::max(wave, out);
+    if (const hipError_t e = ensure_lds_limit<&attention_q4_kernel<NT, RT, VPR>>(); e != hipSuccess) return e;
+    hipLaunchKernelGGL((attention_q4_kernel<NT, RT, VPR>), grid, dim3(64 * waves), lds, st, g);
+    return hipGetLastError();
+}
+template <int NT> static hipError_t launch_aq_rows(const AttnQ4Args &g, dim3 grid, hipStream_t st) {
+    if (g.rows <= 4) return launch_aq<NT, 1, 1>(g, grid, 8, st);
+    if (g.rows <= 16) return launch_aq<NT, 1, 4>(g, grid, 8, st);
+    return launch_aq<NT, 2, 4>(g, grid, 4, st);
+}
+
+hipError_t launch_attention_q4(const rt_attention_q4_desc &d, const void *q, const void *k_cache, const void *v_cache, const void *mask,
+                               const int32_t *kv_lens, void *out, void *workspace, uint64_t workspace_bytes, hipStream_t stream, const DeviceInfo &dev) {
+    AttnQ4Args g{};
+    const uint64_t soff = cache_q4_scale_offset(d.batch, d.kv_heads, d.capacity, d.head_dim);
+    g.Q = (const half_t *)q, g.O = (half_t *)out, g.mask = mask, g.lens = kv_lens;
+    g.Kc = (const uint8_t *)k_cache, g.Vc = (const uint8_t *)v_cache;
+    g.Ks = (const half_t *)(g.Kc + soff), g.Vs = (const half_t *)(g.Vc + soff);
+    g.q_bs = d.q_strides[0], g.q_hs = d.q_strides[1], g.q_rs = d.q_strides[2];
+    g.o_bs = d.o_strides[0], g.o_hs = d.o_strides[1], g.o_rs = d.o_strides[2];
+    g.m_bs = d.mask_strides[0], g.m_rs = d.mask_strides[1], g.mask_f32 = d.mask_dtype == RT_F32;
+    g.kv_heads = d.kv_heads, g.group = d.heads / d.kv_heads, g.rows = d.q_len * g.group;
+    g.kv_len = d.kv_len, g.q_len = d.q_len, g.capacity = d.capacity, g.causal = d.causal;
+    g.scale_log2e = d.scale * kLog2eQ4;
+    aq_split(d, g.splits, g.split_keys);
+    const uint64_t need = attention_q4_workspace_bytes(d);
+    if (need && workspace && workspace_bytes >= need && !((uintptr_t)workspace & 15u)) {
+        g.part_o = (float *)workspace, g.part_ml = g.part_o + (uint64_t)d.batch * d.heads * d.q_len * g.splits * d.head_dim;
+    } else {
+        g.splits = 1, g.split_keys = std::max(d.kv_len, 1);
+    }
+    const int64_t tiles = aq_row_tiles(g.rows);
+    if (tiles > 65535) return hipErrorNotSupported;
+    const dim3 grid((unsigned)g.splits, (unsigned)(d.batch * d.kv_heads), (unsigned)tiles);
+    hipError_t e;
+    switch (d.head_dim / 16) {
+    case 1: e = launch_aq_rows<1>(g, grid, stream); break;
+    case 2: e = launch_aq_rows<2>(g, grid, stream); break;
+    case 3: e = launch_aq_rows<3>(g, grid, stream); break;
+    case 4: e = launch_aq_rows<4>(g, grid, stream); break;
+    case 5: e = launch_aq_rows<5>(g, grid, stream); break;
+    case 6: e = launch_aq_rows<6>(g, grid, stream); break;
+    case 7: e = launch_aq_rows<7>(g, grid, stream); break;
+    default: e = launch_aq_rows<8>(g, grid, stream); break;
+    }
+    if (e != hipSuccess || g.splits <= 1) return e;
+    hipLaunchKernelGGL(attention_q4_merge_kernel, dim3((unsigned)((int64_t)d.batch * d.heads * d.q_len)), dim3(128), 0, stream, g, d.head_dim);
+    return hipGetLastError();
+}
+
+} // namespace rt

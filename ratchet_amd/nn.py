@@ -4,8 +4,6 @@ operators of this library cover end to end (crates/ratchet-models/src/phi2/mlp.r
 Normalisation, rotary embedding and the residual adds of the layer are other operators and not part of it."""
 from typing import List, Optional
 
-import numpy as np
-
 from .tensor import Device, DType, Tensor
 
 
@@ -31,15 +29,15 @@ class MLP:
 
 
 class KVEntry:
-    """kv_cache.rs:3-19: one layer's key and value caches [batch, heads, capacity, head_dim] and the rows in use."""
+    """kv_cache.rs:3-19: one layer's key and value caches [batch, heads, capacity, head_dim] and the rows in use.
+    With dt = DType.Q4_0 they are held in 4-bit blocks, and may have fewer heads than the queries (heads a multiple of them)."""
 
     def __init__(self, k_cache: Tensor, v_cache: Tensor, entries: int = 0):
         self.k_cache, self.v_cache, self.entries = k_cache, v_cache, entries
 
     @staticmethod
     def allocate(shape, device: Device, dt: DType = DType.F16) -> "KVEntry":
-        z = np.zeros(tuple(shape), dtype=dt.numpy())
-        return KVEntry(Tensor.from_data(z).to(device), Tensor.from_data(z).to(device), 0)
+        return KVEntry(Tensor.empty_cache(shape, device, dt), Tensor.empty_cache(shape, device, dt), 0)
 
 
 class KVCache:

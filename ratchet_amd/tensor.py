@@ -323,6 +323,111 @@ class Cache:
         return [self.cache, self.source]
 
 
+def cache_q4_nbytes(shape: Sequence[int]):
+    """(bytes, offset of the scales) of a cache [batch, heads, capacity, head_dim] held in 4-bit blocks."""
+    n, at = ctypes.c_uint64(), ctypes.c_uint64()
+    if len(shape) != 4:
+        raise InvariantError(_ffi.RT_ERR_INVALID_SHAPE, "cache: rank 4 expected")
+    _check(_ffi.lib().rt_cache_q4_nbytes(*map(int, shape), ctypes.byref(n), ctypes.byref(at)))
+    return n.value, at.value
+
+
+class CacheQ4:
+    """The cache write of Cache into a cache held in 4-bit blocks (Tensor.empty_cache with DType.Q4_0), in place: rows offset .. of `cache` <- `source`,
+    F16 or F32.  `offsets`: an int32 GPU tensor of torch, one more offset per sequence; rows outside the cache are then not written."""
+
+    def __init__(self, cache: "Tensor", source: "Tensor", offset: int, offsets=None):
+        self.cache, self.source, self.offset, self.fresh = cache, source, int(offset), False
+        B, H, cap, D = cache.shape
+        if len(source.shape) == 3 and source.shape[0] == B and source.shape[2] == H * D:
+            self.len, self.src_strides = source.shape[1], [source.shape[1] * H * D, D, H * D]
+        elif len(source.shape) == 4 and (source.shape[0], source.shape[1], source.shape[3]) == (B, H, D):
+            self.len, self.src_strides = source.shape[2], [H * source.shape[2] * D, source.shape[2] * D, D]
+        else:
+            raise OperationError(_ffi.RT_ERR_INVALID_SHAPE, f"cache {cache.shape} <- source {source.shape}")
+        if not 0 <= self.offset <= cap or (offsets is None and self.offset + self.len > cap):
+            raise InvariantError(_ffi.RT_ERR_INVALID_SHAPE, "cache: rows beyond the capacity")
+        self.offsets = _lengths(offsets, B, cache.device, "offsets")
+        self.out_shape = cache.shape
+
+    def check_invariants(self):
+        if not self.cache.is_q4_cache:
+            raise InvariantError(_ffi.RT_ERR_DTYPE_MISMATCH, "cache: a Q4_0 weight is no cache (Tensor.empty_cache makes one)")
+        if self.source.dt not in (DType.F16, DType.F32):
+            raise InvariantError(_ffi.RT_ERR_DTYPE_MISMATCH, "cache: the source is F16 or F32")
+
+    def srcs(self):
+        return [self.cache, self.source]
+
+    def _enqueue(self, device, stream, k, ks, v=None, vs=None):
+        B, H, cap, D = self.cache.shape
+        st = _ffi.lib().rt_cache_write_q4_enqueue(device.ctx, int(self.source.dt), k, ks, v, vs, _strides3(*self.src_strides), None, None,
+                                                  None if self.offsets is None else self.offsets.data_ptr(), B, H, cap, self.offset, self.len, D, stream)
+        _check(st, device)
+
+
+def _lengths(t, batch: int, device: "Device", what: str):
+    """A torch int32 tensor [batch] on the device, or None."""
+    if t is None:
+        return None
+    torch = _torch()
+    if t.dtype != torch.int32 or tuple(t.shape) != (batch,) or not t.is_contiguous() or t.device != device.torch_device():
+        raise OperationError(_ffi.RT_ERR_INVALID_ARG, f"{what}: a contiguous int32 tensor [{batch}] on the caches' device")
+    return t
+
+
+class AttentionQ4:
+    """Attention over caches held in 4-bit blocks (rt_attention_q4_enqueue): `k` and `v` are Q4_0 caches [batch, kv_heads, capacity, head_dim], q
+    [batch, heads, len, head_dim] or [batch, len, heads * head_dim], heads a multiple of kv_heads.  `kv_lens`: an int32 GPU tensor of torch, the
+    keys of each sequence."""
+
+    def __init__(self, q: "Tensor", k: "Tensor", v: "Tensor", mask: Optional["Tensor"], scale: Optional[float],
+                 causal: bool, kv_len: Optional[int], merge_heads: bool, kv_lens=None):
+        self.q, self.k, self.v, self.mask = q, k, v, mask
+        self.use_workspace = True
+        if len(k.shape) != 4 or k.shape != v.shape:
+            raise OperationError(_ffi.RT_ERR_INVALID_SHAPE, f"attention: k {k.shape}, v {v.shape}")
+        B, KV, cap, D = k.shape
+        rows_interleaved = len(q.shape) == 3
+        if rows_interleaved and D and q.shape[0] == B and q.shape[2] % D == 0:
+            Lq, H = q.shape[1], q.shape[2] // D
+        elif len(q.shape) == 4 and q.shape[0] == B and q.shape[3] == D:
+            H, Lq = q.shape[1], q.shape[2]
+        else:
+            raise OperationError(_ffi.RT_ERR_INVALID_SHAPE, f"attention: q {q.shape}, k {k.shape}")
+        self.kv_len = cap if kv_len is None else int(kv_len)
+        if not 0 <= self.kv_len <= cap:
+            raise OperationError(_ffi.RT_ERR_INVALID_SHAPE, f"attention: kv_len {self.kv_len} of a cache of {cap}")
+        d = _ffi.AttentionQ4Desc()
+        if mask is not None:
+            lead = math.prod(mask.shape[:-2])
+            if tuple(mask.shape[-2:]) != (Lq, self.kv_len):
+                raise OperationError(_ffi.RT_ERR_INVALID_SHAPE, f"attention: mask {mask.shape} for [{Lq}, {self.kv_len}] scores")
+            if lead != 1 and not (lead == B and len(mask.shape) >= 3 and mask.shape[0] == B):
+                raise OperationError(_ffi.RT_ERR_UNSUPPORTED, f"attention: a mask per head ({mask.shape}) is not supported")
+            d.mask_strides[:] = [Lq * self.kv_len if lead != 1 else 0, self.kv_len]
+        d.batch, d.heads, d.kv_heads, d.q_len, d.kv_len, d.head_dim, d.capacity = B, H, KV, Lq, self.kv_len, D, cap
+        d.q_strides[:] = [Lq * H * D, D, H * D] if rows_interleaved else [H * Lq * D, Lq * D, D]
+        d.o_strides[:] = [Lq * H * D, D, H * D] if merge_heads else [H * Lq * D, Lq * D, D]
+        d.scale = (1.0 / math.sqrt(D) if D > 0 else 1.0) if scale is None else float(scale)
+        d.causal = int(bool(causal))
+        d.mask_dtype = int(mask.dt) if mask is not None else int(DType.F32)
+        self.desc = d
+        self.kv_lens = _lengths(kv_lens, B, k.device, "kv_lens")
+        self.out_shape = (B, Lq, H * D) if merge_heads else (B, H, Lq, D)
+
+    def check_invariants(self):
+        if self.q.dt != DType.F16 or not self.k.is_q4_cache or not self.v.is_q4_cache:
+            raise InvariantError(_ffi.RT_ERR_DTYPE_MISMATCH, "attention: q is F16, k and v are Q4_0 caches")
+        if self.mask is not None and self.mask.dt not in (DType.F32, DType.F16):
+            raise InvariantError(_ffi.RT_ERR_DTYPE_MISMATCH, "attention: the mask is F32 or F16")
+        st = _ffi.lib().rt_attention_q4_validate(self.desc)
+        _check(st, panic=st == _ffi.RT_ERR_INVALID_SHAPE)
+
+    def srcs(self):
+        return [self.q, self.k, self.v] + ([self.mask] if self.mask is not None else [])
+
+
 # An activation whose input is a Matmul node nobody has resolved yet runs in that product's
 # epilogue (one kernel, one rounding) instead of as a second pass over the output.
 FUSE_ACTIVATIONS = True
@@ -352,7 +457,10 @@ def _write_key_and_value(k: "Tensor", v: "Tensor", stream: int):
     source, the values' write.  The launch runs both sources first and has no order between the two writes, so it is taken only where
     the values' source neither reads what the keys' write changes nor writes a cache, and no write touches what the other reads or writes."""
     a, b = k.op, v.op
-    if k.storage is not None or v.storage is not None or type(a) is not Cache or type(b) is not Cache or a.fresh or b.fresh:
+    q4 = type(a) is CacheQ4 and type(b) is CacheQ4
+    if k.storage is not None or v.storage is not None or not (q4 or (type(a) is Cache and type(b) is Cache)) or a.fresh or b.fresh:
+        return
+    if q4 and (a.source.dt != b.source.dt or a.offsets is not b.offsets):
         return
     if (a.cache.storage is None or b.cache.storage is None or k.dt != v.dt or k.shape != v.shape
             or (a.offset, a.len, a.src_strides) != (b.offset, b.len, b.src_strides) or k.device is not v.device or k.device.kind != "gpu"):
@@ -363,7 +471,7 @@ def _write_key_and_value(k: "Tensor", v: "Tensor", stream: int):
     if ks.device.kind != "gpu" or vs.device.kind != "gpu" or (kc < vc_end and vc < kc_end):
         return
     if vs.storage is None:
-        if type(vs.op) is Cache:
+        if type(vs.op) in (Cache, CacheQ4):
             return
         for s in vs.op.srcs():
             if s.storage is None or s.device.kind != "gpu" or _touches(s.storage, kc, kc_end):
@@ -375,6 +483,10 @@ def _write_key_and_value(k: "Tensor", v: "Tensor", stream: int):
     if vs.storage is None:
         vs._execute(stream)
     if _touches(vs.storage, kc, kc_end):
+        return
+    if q4:
+        a._enqueue(k.device, stream, kc, ks.storage.data_ptr(), vc, vs.storage.data_ptr())
+        k.storage, v.storage = a.cache.storage, b.cache.storage
         return
     B, H, cap, D = a.cache.shape
     st = _ffi.lib().rt_cache_write_kv_enqueue(k.device.ctx, int(k.dt), kc, ks.storage.data_ptr(), vc, vs.storage.data_ptr(),
@@ -390,6 +502,7 @@ class Tensor:
         self.shape = tuple(map(int, shape))
         self.dt, self.device, self.storage, self.op = dt if type(dt) is DType else DType(dt), device, storage, op
         self.consumers = 0   # operator nodes built on this tensor
+        self.is_q4_cache = type(op) is CacheQ4   # Q4_0 rows as a key/value cache has them (Tensor.empty_cache), not a weight's
         if op is not None:
             for src in op.srcs():
                 src.consumers += 1
@@ -420,6 +533,17 @@ class Tensor:
         rng = np.random.default_rng(int(seed) if seed is not None else None)
         return Tensor.from_data(rng.standard_normal(tuple(shape)).astype(dt.numpy()), None, device)
 
+    @staticmethod
+    def empty_cache(shape: Sequence[int], device: Device, dt: DType = DType.F16) -> "Tensor":
+        """A key or value cache [batch, heads, capacity, head_dim], zeros: F16 or F32, or Q4_0, held in 4-bit blocks."""
+        shape = tuple(map(int, shape))
+        if DType(dt) != DType.Q4_0:
+            return Tensor.from_data(np.zeros(shape, dtype=DType(dt).numpy())).to(device)
+        n = max(cache_q4_nbytes(shape)[0], 16)
+        t = Tensor(shape, DType.Q4_0, device, _torch().zeros(n, dtype=_torch().uint8, device=device.torch_device()) if device.is_gpu() else np.zeros(n, np.uint8))
+        t.is_q4_cache = True
+        return t
+
     # -- storage movement ---------------------------------------------------
     def _moved(self, device: Device) -> "Tensor":
         return self if device.kind == "cpu" else self.to(device)
@@ -438,8 +562,14 @@ class Tensor:
             host = self.storage.view(np.uint8).reshape(-1)
             dev_t = torch.empty(max(host.size, 16), dtype=torch.uint8, device=f"cuda:{device.ordinal}")
             dev_t[: host.size].copy_(torch.from_numpy(host))
-            return Tensor(self.shape, self.dt, device, dev_t)
+            t = Tensor(self.shape, self.dt, device, dev_t)
+            t.is_q4_cache = self.is_q4_cache
+            return t
         raw = self.storage.cpu().numpy()
+        if self.is_q4_cache:
+            t = Tensor(self.shape, self.dt, Device.CPU, raw[: cache_q4_nbytes(self.shape)[0]].copy())
+            t.is_q4_cache = True
+            return t
         if self.dt.is_quantized():
             return Tensor(self.shape, self.dt, Device.CPU, raw[: tensor_nbytes(self.dt, self.numel())].copy())
         nbytes = self.numel() * (4 if self.dt == DType.F32 else 2)
@@ -467,6 +597,8 @@ class Tensor:
     def gemm(self, rhs: "Tensor", bias: Optional["Tensor"], trans_lhs: bool, trans_rhs: bool,
              trans_out: bool) -> "Tensor":
         """tensor.rs:388-400: builds the lazy Matmul node."""
+        if self.is_q4_cache or rhs.is_q4_cache:
+            raise InvariantError(_ffi.RT_ERR_DTYPE_MISMATCH, "matmul: a Q4_0 cache is no weight")
         op = Matmul(self, rhs, bias, trans_lhs, trans_rhs, trans_out)
         shape, dt = op.compute_view()   # Err on shape failure
         op.check_invariants()           # panics of Matmul::new and the OpGuards
@@ -479,25 +611,38 @@ class Tensor:
         return Tensor(self.shape, self.dt, self.device, None, op)
 
     def attention(self, k: "Tensor", v: "Tensor", mask: Optional["Tensor"] = None, scale: Optional[float] = None,
-                  causal: bool = False, kv_len: Optional[int] = None, merge_heads: bool = False) -> "Tensor":
-        """softmax(scale * self k^T + mask) v as one lazy node; see Attention."""
-        op = Attention(self, k, v, mask, scale, causal, kv_len, merge_heads)
+                  causal: bool = False, kv_len: Optional[int] = None, merge_heads: bool = False, kv_lens=None) -> "Tensor":
+        """softmax(scale * self k^T + mask) v as one lazy node; see Attention, and AttentionQ4 for caches held in 4-bit blocks (which
+        alone take `kv_lens`)."""
+        if DType.Q4_0 in (k.dt, v.dt):
+            op = AttentionQ4(self, k, v, mask, scale, causal, kv_len, merge_heads, kv_lens)
+        elif kv_lens is not None:
+            raise OperationError(_ffi.RT_ERR_UNSUPPORTED, "attention: kv_lens needs caches held in 4-bit blocks")
+        else:
+            op = Attention(self, k, v, mask, scale, causal, kv_len, merge_heads)
         op.check_invariants()
         return Tensor(op.out_shape, self.dt, self.device, None, op)
 
     def cache(self, source: "Tensor", dim: int, offset: int) -> "Tensor":
         """tensor.rs `cache(source, dim, offset)` (ops/cache.rs): self is the cache; the result is the fresh
         tensor cache[.., :offset, :] ++ source, and the cache holds the new rows too."""
+        if self.dt == DType.Q4_0:
+            raise OperationError(_ffi.RT_ERR_UNSUPPORTED, "cache: caches held in 4-bit blocks are written in place (cache_write)")
         if dim != 2:
             raise OperationError(_ffi.RT_ERR_UNSUPPORTED, "cache: dim 2 (the sequence axis of [b, h, s, d])")
         op = Cache(self, source, offset, fresh=True)
         op.check_invariants()
         return Tensor(op.out_shape, self.dt, self.device, None, op)
 
-    def cache_write(self, source: "Tensor", offset: int) -> "Tensor":
+    def cache_write(self, source: "Tensor", offset: int, offsets=None) -> "Tensor":
         """The same write without the copy: the result is the cache itself (same storage), to be passed to
-        attention(kv_len = offset + len)."""
-        op = Cache(self, source, offset, fresh=False)
+        attention(kv_len = offset + len).  `offsets`: see CacheQ4."""
+        if self.dt == DType.Q4_0:
+            op = CacheQ4(self, source, offset, offsets)
+        elif offsets is not None:
+            raise OperationError(_ffi.RT_ERR_UNSUPPORTED, "cache: offsets needs a cache held in 4-bit blocks")
+        else:
+            op = Cache(self, source, offset, fresh=False)
         op.check_invariants()
         return Tensor(op.out_shape, self.dt, self.device, None, op)
 
@@ -560,7 +705,7 @@ class Tensor:
                 and op.input.consumers <= 1):
             act, op = op.act, op.input.op
             kind = Matmul
-        if kind is Attention:
+        if kind is Attention or kind is AttentionQ4:
             if op.q.storage is None:
                 op.q._execute(stream)   # first, as in srcs(): it may read the caches as they were
             _write_key_and_value(op.k, op.v, stream)
@@ -579,6 +724,10 @@ class Tensor:
             B, H, cap, D = op.cache.shape
             _check(L.rt_cache_write_enqueue(dev.ctx, int(self.dt), op.cache._ptr(), op.source._ptr(), _strides3(*op.src_strides), None, B, H, cap,
                                             op.offset, op.len, D, stream), dev)
+            self.storage = op.cache.storage
+            return
+        if kind is CacheQ4:
+            op._enqueue(dev, stream, op.cache._ptr(), op.source._ptr())
             self.storage = op.cache.storage
             return
         out = self._empty(max(self.numel() * (4 if self.dt == DType.F32 else 2), 16))
@@ -602,6 +751,13 @@ class Tensor:
             ws = self._empty(need.value) if need.value and op.use_workspace else None
             _check(L.rt_attention_enqueue(dev.ctx, op.desc, op.q._ptr(), op.k._ptr(), op.v._ptr(), op.mask._ptr() if op.mask is not None else None, ptr,
                                           ws.data_ptr() if ws is not None else None, need.value if ws is not None else 0, stream), dev)
+        elif kind is AttentionQ4:
+            need = ctypes.c_uint64()
+            _check(L.rt_attention_q4_workspace_bytes(op.desc, need), dev)
+            ws = self._empty(need.value) if need.value and op.use_workspace else None
+            _check(L.rt_attention_q4_enqueue(dev.ctx, op.desc, op.q._ptr(), op.k._ptr(), op.v._ptr(), op.mask._ptr() if op.mask is not None else None,
+                                             None if op.kv_lens is None else op.kv_lens.data_ptr(), ptr, ws.data_ptr() if ws is not None else None,
+                                             need.value if ws is not None else 0, stream), dev)
         elif kind is Cache:
             B, H, cap, D = op.cache.shape
             _check(L.rt_cache_write_enqueue(dev.ctx, int(self.dt), op.cache._ptr(), op.source._ptr(), _strides3(*op.src_strides), ptr, B, H, cap,
@@ -690,7 +846,7 @@ class Quantizer:
 
 def dequantize(quantized: Tensor, device: Optional[Device] = None) -> Tensor:
     """Quantized tensor -> f32 tensor on the tensor's own device kind."""
-    assert quantized.dt.is_quantized()
+    assert quantized.dt.is_quantized() and not quantized.is_q4_cache
     dev = quantized.device if quantized.device.is_gpu() else (device or Device.request_device(DeviceRequest.GPU))
     torch = _torch()
     src = quantized.to(dev)
