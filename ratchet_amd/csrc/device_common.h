@@ -145,9 +145,15 @@ __device__ __forceinline__ void q4k_scale_min(int j, const uint8_t *s, int &sc, 
 
 // Q4_0 codes: a dword holds eight values, nibbles 0..3 the values 0, 2, 4, 6 and nibbles 4..7 the values 1, 3, 5, 7, so that nibble i of
 // both halfwords is the pair (2 i, 2 i + 1).  A nibble in the low bits of an f16 of exponent 2^10 is 1024 + q, in the next four 1024 + 16 q:
-// one subtraction, or one fused multiply-add by 1/16, leaves q - 8.  All of it is exact; nine instructions for eight values.
-__device__ __forceinline__ half8_t q40_codes(uint32_t w) {
-    constexpr uint32_t kLow = 0x000F000Fu, kHigh = 0x00F000F0u, kBias = 0x64006400u;
+// one subtraction, or one fused multiply-add by 1/16, leaves q - 8.  All of it is exact; nine instructions for eight values, where the bias comes in a
+// vector register (q40_bias): and-or takes one constant, and the compiler, which sees two, makes two instructions of it.
+__device__ __forceinline__ uint32_t q40_bias() {
+    uint32_t v = 0x64006400u;
+    asm("" : "+v"(v));
+    return v;
+}
+__device__ __forceinline__ half8_t q40_codes(uint32_t w, uint32_t kBias = 0x64006400u) {
+    constexpr uint32_t kLow = 0x000F000Fu, kHigh = 0x00F000F0u;
     const half2_t off = {(half_t)1032.f, (half_t)1032.f}, mul = {(half_t)0.0625f, (half_t)0.0625f}, add = {(half_t)-72.f, (half_t)-72.f};
     const uint32_t v = w >> 8;
     const half2_t a = __builtin_bit_cast(half2_t, (w & kLow) | kBias) - off;
@@ -182,6 +188,7 @@ hipError_t launch_gemv_q4k_rowdot(const Problem &p, const void *A, const void *B
 hipError_t launch_gemv_q4k_mfma(const Problem &p, const void *A, const void *B, const void *bias, void *out,
                                 hipStream_t stream, const DeviceInfo &dev);
 hipError_t launch_gemv_q40(const Problem &p, const void *A, const void *B, const void *bias, void *out, hipStream_t stream, const DeviceInfo &dev);
+hipError_t launch_gemm_q40(const Problem &p, const void *A, const void *B, const void *bias, void *out, hipStream_t stream, const DeviceInfo &dev);
 hipError_t launch_gemv_chunked(const Problem &p, const void *A, const void *B, const void *bias, void *out, hipStream_t stream,
                                const DeviceInfo &dev);
 hipError_t launch_gemm_q4k(const Problem &p, const void *A, const void *B, const void *bias, void *out, hipStream_t stream,
@@ -199,6 +206,7 @@ hipError_t launch_gemm(const Problem &p, const void *A, const void *B, const voi
 hipError_t launch_gemm_stream(const Problem &p, const void *A, const void *B, const void *bias, void *out, hipStream_t stream,
                               const DeviceInfo &dev);
 uint64_t gemm_nt_workspace_bytes(const Problem &p, const DeviceInfo &dev);
+bool gemm_nt_leaves_q4(const Problem &p, const DeviceInfo &dev);
 bool gemm_nt_static_split(const Problem &p, const DeviceInfo &dev);
 bool gemv_chunks_unless_shared(const Problem &p, const DeviceInfo &dev);
 bool gemv_q8f_chunks(const Problem &p);

@@ -780,8 +780,10 @@ __global__ __launch_bounds__(64 * WI * WJ) void gemm_nt_wide_kernel(GemmNtArgs g
 // iterations ago (everything older has landed with them, the activation rows of tile j + 1 included);
 // widen and store them into stage (j + 1) % 4; barrier.  Requires K % 256 == 0 (scales in groups of 8).
 // ---------------------------------------------------------------------------
-template <int BM, int BN, int LW>
+// Q4: the same for Q4_0 weights; a loading lane's 16 codes are 8 bytes, and q40_codes widens them to q - 8.
+template <int BM, int BN, int LW, bool Q4>
 __global__ __launch_bounds__(NT_THREADS + 64 * LW) void gemm_nt_q8w_kernel(GemmNtArgs g) {
+    using Raw = std::conditional_t<Q4, uint2_t, uint4_t>; // 16 codes
     constexpr int STAGES = 4, AHEAD = 2;
     constexpr int WM = BM / 2, WN = BN / 2, TM = WM / 16, TN = WN / 16;
     constexpr int STAGE_HALFS = (BM + BN) * NT_LDK;
@@ -817,7 +819,7 @@ __global__ __launch_bounds__(NT_THREADS + 64 * LW) void gemm_nt_q8w_kernel(GemmN
             const int ch = lw + c * LW;
             alive[c] = ch < ACH; // wave-uniform
             const int row = min(ch, ACH - 1) * 16 + (lane >> 2);
-            ga[c] = (const uint8_t *)g.A + a_el + min(i0 + row, g.M - 1) * g.a_rs + 16 * piece;
+            ga[c] = (const uint8_t *)g.A + ((a_el + min(i0 + row, g.M - 1) * g.a_rs + 16 * piece) >> (Q4 ? 1 : 0));
             adst[c] = row;
         }
         const half_t *gb[LCHB];
@@ -827,7 +829,8 @@ __global__ __launch_bounds__(NT_THREADS + 64 * LW) void gemm_nt_q8w_kernel(GemmN
             const int kv = (lane & 7) ^ ((row >> 1) & 7);
             gb[c] = g.B + b_el + min(j0 + row, g.N - 1) * g.b_js + 8 * kv;
         }
-        uint4_t ra[STAGES][NA];
+        Raw ra[STAGES][NA];
+        const uint32_t bias4 = q40_bias();
         auto request = [&](int slot, int64_t tile) __attribute__((always_inline)) {
             const int64_t k0 = min(tile, nk - 1) * NT_BK; // past the last tile: re-read it, never used
             half_t *st = ring + slot * STAGE_HALFS + BM * NT_LDK;
@@ -837,7 +840,7 @@ __global__ __launch_bounds__(NT_THREADS + 64 * LW) void gemm_nt_q8w_kernel(GemmN
                                                  (__attribute__((address_space(3))) void *)(st + (lw + c * LW) * 8 * NT_LDK), 16, 0, 0);
             __builtin_amdgcn_sched_barrier(0); // the wait in widen_store counts the loads in this order
 #pragma unroll
-            for (int c = 0; c < NA; c++) ra[slot][c] = *(const uint4_t *)(ga[c] + k0);
+            for (int c = 0; c < NA; c++) ra[slot][c] = *(const Raw *)(ga[c] + (k0 >> (Q4 ? 1 : 0)));
             __builtin_amdgcn_sched_barrier(0);
         };
         auto widen_store = [&](int slot) __attribute__((always_inline)) {
@@ -847,13 +850,18 @@ __global__ __launch_bounds__(NT_THREADS + 64 * LW) void gemm_nt_q8w_kernel(GemmN
 #pragma unroll
             for (int c = 0; c < NA; c++) {
                 if (alive[c]) {
-                    half2_t h[8];
+                    uint4_t lo, hi;
+                    if constexpr (Q4) {
+                        lo = __builtin_bit_cast(uint4_t, q40_codes(ra[slot][c][0], bias4)), hi = __builtin_bit_cast(uint4_t, q40_codes(ra[slot][c][1], bias4));
+                    } else {
+                        half2_t h[8];
 #pragma unroll
-                    for (int d = 0; d < 4; d++) nt_cvt_i8x4(ra[slot][c][d], h[2 * d], h[2 * d + 1]);
-                    const uint4_t lo = {__builtin_bit_cast(uint32_t, h[0]), __builtin_bit_cast(uint32_t, h[1]),
-                                        __builtin_bit_cast(uint32_t, h[2]), __builtin_bit_cast(uint32_t, h[3])};
-                    const uint4_t hi = {__builtin_bit_cast(uint32_t, h[4]), __builtin_bit_cast(uint32_t, h[5]),
-                                        __builtin_bit_cast(uint32_t, h[6]), __builtin_bit_cast(uint32_t, h[7])};
+                        for (int d = 0; d < 4; d++) nt_cvt_i8x4(ra[slot][c][d], h[2 * d], h[2 * d + 1]);
+                        lo = uint4_t{__builtin_bit_cast(uint32_t, h[0]), __builtin_bit_cast(uint32_t, h[1]),
+                                     __builtin_bit_cast(uint32_t, h[2]), __builtin_bit_cast(uint32_t, h[3])};
+                        hi = uint4_t{__builtin_bit_cast(uint32_t, h[4]), __builtin_bit_cast(uint32_t, h[5]),
+                                     __builtin_bit_cast(uint32_t, h[6]), __builtin_bit_cast(uint32_t, h[7])};
+                    }
                     // the four lanes of a row store four of its eight slots, and two neighbouring rows have the same
                     // swizzle: odd rows store their odd slots first, so that eight consecutive lanes cover eight
                     // different 16-byte bank groups
@@ -1271,12 +1279,12 @@ hipError_t launch_splitk_sums(const Problem &p, const void *bias, void *out, flo
     return launch_splitk_reduce(g, p.stacks, st);
 }
 
-template <int BM, int BN, int LW>
+template <int BM, int BN, int LW, bool Q4>
 static hipError_t launch_nt_q8w(const GemmNtArgs &g, int64_t stacks, hipStream_t st) {
     const size_t lds = (size_t)4 * (BM + BN) * NT_LDK * 2;
-    if (const hipError_t e = ensure_lds_limit<&gemm_nt_q8w_kernel<BM, BN, LW>>(); e != hipSuccess) return e;
+    if (const hipError_t e = ensure_lds_limit<&gemm_nt_q8w_kernel<BM, BN, LW, Q4>>(); e != hipSuccess) return e;
     dim3 grid((unsigned)((int64_t)g.tiles_i * g.tiles_j), (unsigned)stacks, (unsigned)g.ksplit);
-    hipLaunchKernelGGL((gemm_nt_q8w_kernel<BM, BN, LW>), grid, dim3(NT_THREADS + 64 * LW), lds, st, g);
+    hipLaunchKernelGGL((gemm_nt_q8w_kernel<BM, BN, LW, Q4>), grid, dim3(NT_THREADS + 64 * LW), lds, st, g);
     if (const hipError_t e = hipGetLastError(); e != hipSuccess) return e;
     return g.ksplit > 1 ? launch_splitk_reduce(g, stacks, st) : hipSuccess;
 }
@@ -1510,8 +1518,10 @@ struct NtChoice {
 };
 // gemm_nt_q8w_kernel's shapes among those with Q8_0H weights
 static bool nt_q8_whole(const Problem &p) { return p.K % 256 == 0 && p.a_bs % 512 == 0; }
+// Q4_0 weights that gemm_nt_q8w_kernel takes from launch_gemm_q40
+static bool nt_q4(const Problem &p) { return p.a_dt == RT_Q4_0 && nt_q8_whole(p) && p.N > kGemvQ40MaxCols; }
 static NtChoice nt_choose(const Problem &p, const DeviceInfo &dev, bool may_split) {
-    const bool q8 = p.a_dt == RT_Q8_0H;
+    const bool q8 = p.a_dt == RT_Q8_0H || p.a_dt == RT_Q4_0;
     const NtTile *tiles = !q8 ? kTilesF16 : nt_q8_whole(p) ? kTilesQ8w : kTilesQ8r;
     const float crowd = q8 ? 0.23f : 0.37f, pass = q8 ? 1.7f : 2.4f;
     const int64_t nk = (p.K + NT_BK - 1) / NT_BK;
@@ -1542,6 +1552,16 @@ static NtChoice nt_choose(const Problem &p, const DeviceInfo &dev, bool may_spli
     return best;
 }
 
+// Q4_0 weights against more activation rows than launch_gemv_q40 takes: left to launch_gemm_q40 where that kernel's tiles of 16 x 32 all run at once, or nearly, and
+// the tiles here would not share a long K (us here and there: 2560 x 2560 at 128 / 160 rows 13.2 / 13.6 and 9.6 / 10.8, 2560 x 10240 at 160 without a workspace 47 and
+// 35; sharing K 30, and 1280 x 5120 at 128 13.2 and 14.2; with more tiles 4096 x 4096 at 160 20.6 and 21.9, 20000 x 2560 at 160 42 and 47).
+bool gemm_nt_leaves_q4(const Problem &p, const DeviceInfo &dev) {
+    if (p.a_dt != RT_Q4_0 || (p.M + 15) / 16 * ((p.N + 31) / 32) * p.stacks > 4 * (int64_t)dev.num_cus) return false;
+    if (p.K <= 2560) return true;
+    const int ks = nt_choose(p, dev, true).ks;
+    return ks == 1 || !p.workspace || ((uintptr_t)p.workspace & 15u) || p.workspace_bytes < (uint64_t)p.stacks * ks * p.M * p.N * sizeof(float);
+}
+
 // exchanges the operands' roles when that makes the output's contiguous axis the kernel's i axis
 static bool nt_orient(Problem &p) {
     if (p.a_dt == RT_F16 && p.act_dt == RT_F16 && p.o_js == 1 && p.o_is != 1) {
@@ -1562,7 +1582,8 @@ uint64_t gemm_nt_workspace_bytes(const Problem &p0, const DeviceInfo &dev) {
     Problem p = p0;
     nt_orient(p);
     if (p.a_ks != 1 || p.b_ks != 1 || p.M < 160 || p.N < 5) return 0;
-    if ((p.a_dt != RT_F16 && p.a_dt != RT_Q8_0H) || p.K % 32 != 0 || p.K <= 256) return 0;
+    if ((p.a_dt != RT_F16 && p.a_dt != RT_Q8_0H && !nt_q4(p)) || p.K % 32 != 0 || p.K <= 256) return 0;
+    if (p.a_dt == RT_Q4_0 && p.K <= 2560 && gemm_nt_leaves_q4(p, dev)) return 0;
     const int ks = nt_choose(p, dev, true).ks;
     return ks > 1 ? (uint64_t)p.stacks * ks * p.M * p.N * sizeof(float) : 0;
 }
@@ -1589,10 +1610,10 @@ hipError_t launch_gemm_nt(const Problem &p0, const void *A, const void *B, const
     // kernel's contiguous output axis, the one its 128-bit epilogue writes along, is this
     // problem's column axis.
     if (nt_orient(p)) std::swap(A, B);
-    if (p.act_dt != RT_F16 || (p.a_dt != RT_F16 && p.a_dt != RT_Q8_0H)) return hipErrorNotSupported;
+    if (p.act_dt != RT_F16 || (p.a_dt != RT_F16 && p.a_dt != RT_Q8_0H && !nt_q4(p))) return hipErrorNotSupported;
     if (p.a_ks != 1 || p.b_ks != 1 || p.K % 8 != 0 || p.K < 8) return hipErrorNotSupported;
     if (p.stacks > 65535 || p.M < 1 || p.N < 1) return hipErrorNotSupported;
-    const bool q8 = p.a_dt == RT_Q8_0H;
+    const bool q8 = p.a_dt != RT_F16; // codes: Q8_0H, or Q4_0 with gemm_nt_q8w_kernel's shapes
     if (((uintptr_t)A & 15u) || ((uintptr_t)B & 15u) || (p.b_js * 2) % 16 || (p.b_bs * 2) % 16) return hipErrorNotSupported;
     if (q8 ? (p.K % 32 != 0) : ((p.a_rs * 2) % 16 != 0 || (p.a_bs * 2) % 16 != 0)) return hipErrorNotSupported;
     // small problems do not fill the tiles; the generic kernel handles them (at 10240 x 2560 f16 weights it takes
@@ -1600,11 +1621,13 @@ hipError_t launch_gemm_nt(const Problem &p0, const void *A, const void *B, const
     if (p.M < 160 || p.N < 5) return hipErrorNotSupported;
     if (!RT_NT_ABLATION && q8 && p.N <= 8 && p.K % 256 == 0 && !gemv_q8h_mfma_well(p, dev) && !gemv_q8h_few_leave(p, dev)) return hipErrorNotSupported; // launch_gemv's
 
+    if (gemm_nt_leaves_q4(p, dev)) return hipErrorNotSupported;
+
     GemmNtArgs g{};
     g.A = A, g.B = (const half_t *)B, g.bias = (const half_t *)bias, g.out = (half_t *)out;
     if (q8) {
         const uint64_t n = (uint64_t)p.a_stack * p.M * p.K;
-        g.scales = (const half_t *)((const uint8_t *)A + rt_q8_0_scale_offset(n));
+        g.scales = (const half_t *)((const uint8_t *)A + (p.a_dt == RT_Q4_0 ? q40_scale_offset(n) : rt_q8_0_scale_offset(n)));
         g.scale_dwords = (int64_t)((n / 32 * 2 + 255) / 256 * 64);
     }
     g.M = p.M, g.N = p.N, g.K = p.K;
@@ -1671,11 +1694,15 @@ hipError_t launch_gemm_nt(const Problem &p0, const void *A, const void *B, const
         return launch_nt_dl<160, 128, 3, 2>(g, p.stacks, stream);
     }
     if (nt_q8_whole(p)) {
-        if (c.bn == 64) return launch_nt_q8w<64, 64, 4>(g, p.stacks, stream);
-        if (c.bm == 64) return launch_nt_q8w<64, 128, 4>(g, p.stacks, stream);
-        if (c.bm == 96) return launch_nt_q8w<96, 128, 4>(g, p.stacks, stream);
-        if (c.bm == 128) return launch_nt_q8w<128, 128, 4>(g, p.stacks, stream);
-        return launch_nt_q8w<160, 128, 4>(g, p.stacks, stream);
+        auto go = [&](auto q4) -> hipError_t {
+            constexpr bool Q4 = decltype(q4)::value;
+            if (c.bn == 64) return launch_nt_q8w<64, 64, 4, Q4>(g, p.stacks, stream);
+            if (c.bm == 64) return launch_nt_q8w<64, 128, 4, Q4>(g, p.stacks, stream);
+            if (c.bm == 96) return launch_nt_q8w<96, 128, 4, Q4>(g, p.stacks, stream);
+            if (c.bm == 128) return launch_nt_q8w<128, 128, 4, Q4>(g, p.stacks, stream);
+            return launch_nt_q8w<160, 128, 4, Q4>(g, p.stacks, stream);
+        };
+        return p.a_dt == RT_Q4_0 ? go(std::true_type{}) : go(std::false_type{});
     }
     if (c.bn == 64) return launch_nt_q8r<64, 64, 2>(g, p.stacks, stream);
     if (c.bm == 64) return launch_nt_q8r<64, 128, 1>(g, p.stacks, stream);
