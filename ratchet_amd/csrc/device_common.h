@@ -143,6 +143,29 @@ __device__ __forceinline__ void q4k_scale_min(int j, const uint8_t *s, int &sc, 
     }
 }
 
+// Maximum / sum over the four lanes l, l ^ 16, l ^ 32, l ^ 48 (the four lane groups that share a query row),
+// left in all of them: v_permlane16_swap and v_permlane32_swap of a register with itself put the partner
+// row's (half's) value beside the lane's own, so each step is two vector instructions and no trip through
+// the LDS crossbar (ds_bpermute, which __shfl_xor is, costs an LDS round trip per step).
+__device__ __forceinline__ float rt_groups_max(float v) {
+    const uint32_t u = __builtin_bit_cast(uint32_t, v);
+    const auto a = __builtin_amdgcn_permlane16_swap(u, u, false, false);
+    // the instruction itself: fmaxf() of values that come out of a bit cast first quiets each of them (two more instructions)
+    float w;
+    asm("v_max_f32 %0, %1, %2" : "=v"(w) : "v"((uint32_t)a[0]), "v"((uint32_t)a[1]));
+    const uint32_t x = __builtin_bit_cast(uint32_t, w);
+    const auto b = __builtin_amdgcn_permlane32_swap(x, x, false, false);
+    return fmaxf(__builtin_bit_cast(float, (uint32_t)b[0]), __builtin_bit_cast(float, (uint32_t)b[1]));
+}
+__device__ __forceinline__ float rt_groups_sum(float v) {
+    const uint32_t u = __builtin_bit_cast(uint32_t, v);
+    const auto a = __builtin_amdgcn_permlane16_swap(u, u, false, false);
+    const float w = __builtin_bit_cast(float, (uint32_t)a[0]) + __builtin_bit_cast(float, (uint32_t)a[1]);
+    const uint32_t x = __builtin_bit_cast(uint32_t, w);
+    const auto b = __builtin_amdgcn_permlane32_swap(x, x, false, false);
+    return __builtin_bit_cast(float, (uint32_t)b[0]) + __builtin_bit_cast(float, (uint32_t)b[1]);
+}
+
 // Q4_0 codes: a dword holds eight values, nibbles 0..3 the values 0, 2, 4, 6 and nibbles 4..7 the values 1, 3, 5, 7, so that nibble i of
 // both halfwords is the pair (2 i, 2 i + 1).  A nibble in the low bits of an f16 of exponent 2^10 is 1024 + q, in the next four 1024 + 16 q:
 // one subtraction, or one fused multiply-add by 1/16, leaves q - 8.  All of it is exact; nine instructions for eight values, where the bias comes in a

@@ -69,29 +69,6 @@ __device__ __forceinline__ int at_chunk_pos(int r, int c, int dvec) {
 // s_waitcnt vmcnt(n) lgkmcnt(0): at most n of this wavefront's loads outstanding, all LDS reads returned
 __device__ __forceinline__ constexpr int at_waitcnt(int n) { return 0x0070 | (n & 0xF) | (((n >> 4) & 0x3) << 14); }
 
-// Maximum / sum over the four lanes l, l ^ 16, l ^ 32, l ^ 48 (the four lane groups that share a query row),
-// left in all of them: v_permlane16_swap and v_permlane32_swap of a register with itself put the partner
-// row's (half's) value beside the lane's own, so each step is two vector instructions and no trip through
-// the LDS crossbar (ds_bpermute, which __shfl_xor is, costs an LDS round trip per step).
-__device__ __forceinline__ float at_groups_max(float v) {
-    const uint32_t u = __builtin_bit_cast(uint32_t, v);
-    const auto a = __builtin_amdgcn_permlane16_swap(u, u, false, false);
-    // the instruction itself: fmaxf() of values that come out of a bit cast first quiets each of them (two more instructions)
-    float w;
-    asm("v_max_f32 %0, %1, %2" : "=v"(w) : "v"((uint32_t)a[0]), "v"((uint32_t)a[1]));
-    const uint32_t x = __builtin_bit_cast(uint32_t, w);
-    const auto b = __builtin_amdgcn_permlane32_swap(x, x, false, false);
-    return fmaxf(__builtin_bit_cast(float, (uint32_t)b[0]), __builtin_bit_cast(float, (uint32_t)b[1]));
-}
-__device__ __forceinline__ float at_groups_sum(float v) {
-    const uint32_t u = __builtin_bit_cast(uint32_t, v);
-    const auto a = __builtin_amdgcn_permlane16_swap(u, u, false, false);
-    const float w = __builtin_bit_cast(float, (uint32_t)a[0]) + __builtin_bit_cast(float, (uint32_t)a[1]);
-    const uint32_t x = __builtin_bit_cast(uint32_t, w);
-    const auto b = __builtin_amdgcn_permlane32_swap(x, x, false, false);
-    return __builtin_bit_cast(float, (uint32_t)b[0]) + __builtin_bit_cast(float, (uint32_t)b[1]);
-}
-
 // stages of the key / value ring: blocks of 32 nkq keys, at most 160 KB
 constexpr int at_stages(int dp, int nkq) { return nkq == 4 ? 3 : (dp <= 96 ? 4 : 3); }
 
@@ -448,7 +425,7 @@ __global__ __launch_bounds__(256 * NKQ) void attention_kernel(AttnArgs g) {
                     bmax = fmaxf(bmax, s);
                 }
         }
-        bmax = at_groups_max(bmax);
+        bmax = rt_groups_max(bmax);
         const float m_new = fmaxf(m_run, bmax);
         // a row that has seen no finite score yet keeps a reference of 0: exp2(-inf - 0) = 0
         const float m_use = m_new == -INFINITY ? 0.f : m_new;
@@ -547,7 +524,7 @@ __global__ __launch_bounds__(256 * NKQ) void attention_kernel(AttnArgs g) {
         m_run = m_new; // what the sums and outputs are now relative to (a split launch hands it on)
     }
     // the row's sum over its four lanes, then O / l; lane (fr, fg) holds columns 16 d + 4 fg + r of row fr
-    l_run = at_groups_sum(l_run);
+    l_run = rt_groups_sum(l_run);
     if (g.splits > 1) {
         // this workgroup saw only its share of the keys: hand (m, l, O) of every row to the merge kernel
         // (rows past q_len are never merged: a decode step has one live row of 64)
@@ -766,7 +743,7 @@ __global__ __launch_bounds__(256, 2) void attention_long_kernel(AttnArgs g) {
                     bmax = fmaxf(bmax, s);
                 }
             }
-            bmax = at_groups_max(bmax);
+            bmax = rt_groups_max(bmax);
             // The reference is the block's own maximum, whose probability is then exact, or 2^8 below the row's where that is more: what
             // rounding the probabilities to f16 costs is mostly the error of the largest ones.  One running maximum
             // for the whole row left only one of them exact (2048 x 2048, N(0, 1) scores: 1.03 times the error of the kernel
@@ -839,7 +816,7 @@ __global__ __launch_bounds__(256, 2) void attention_long_kernel(AttnArgs g) {
 #pragma unroll
     for (int u = 0; u < 2; u++) {
         const int row = qw + 16 * u + fr;
-        const float inv = 1.f / at_groups_sum(l_run[u]); // no visible key: 0 / 0 = NaN, what the unfused sequence yields
+        const float inv = 1.f / rt_groups_sum(l_run[u]); // no visible key: 0 / 0 = NaN, what the unfused sequence yields
         if (row >= g.q_len) continue;
         half_t *op = O + (int64_t)row * g.o_rs;
 #pragma unroll

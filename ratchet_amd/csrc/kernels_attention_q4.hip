@@ -27,6 +27,7 @@
 namespace rt {
 
 constexpr float kLog2eQ4 = 1.4426950408889634f;
+constexpr int AQ_MAX_SPLITS = 64; // a lane of the merge for each
 
 struct AttnQ4Args {
     const half_t *Q;
@@ -38,7 +39,7 @@ struct AttnQ4Args {
     float *part_o, *part_ml; // [row][split][D], [row][split][2]
     int64_t q_bs, q_hs, q_rs, o_bs, o_hs, o_rs, m_bs, m_rs;
     int kv_heads, group, rows, kv_len, q_len, capacity; // rows = q_len * group
-    int causal, mask_f32, splits, split_keys, row_tiles;
+    int causal, mask_f32, splits, split_keys, row_tiles, resident;
     float scale_log2e;
 };
 
@@ -392,33 +393,335 @@ template <int NT, int RT, int VPR> __global__ __launch_bounds__(RT == 1 ? 512 : 
     }
 }
 
-// One workgroup per row: thread d joins dimension d of its shares.
-__global__ __launch_bounds__(128) void attention_q4_merge_kernel(AttnQ4Args g, int D) {
-    const int64_t row = blockIdx.x;
-    const int bk = (int)(row / g.rows), m = (int)(row - (int64_t)bk * g.rows), b = bk / g.kv_heads, kh = bk - b * g.kv_heads, d = threadIdx.x;
-    if (d >= D) return;
-    const float *ml = g.part_ml + row * g.splits * 2, *po = g.part_o + row * g.splits * D + d;
-    float top = -INFINITY;
-    for (int s = 0; s < g.splits; s++) top = fmaxf(top, ml[2 * s]);
-    const float base = top == -INFINITY ? 0.f : top;
-    float y = 0.f, l = 0.f;
-    for (int s = 0; s < g.splits; s++) {
-        const float a = __builtin_amdgcn_exp2f(ml[2 * s] - base);
-        y = fmaf(po[(int64_t)s * D], a, y), l = fmaf(ml[2 * s + 1], a, l);
+// ---------------------------------------------------------------------------------------------
+// More rows (prompts, and steps of a few tokens with heads that share keys): a workgroup of four wavefronts has 128 rows of one head of keys, a wavefront 32 of
+// them, against blocks of 64 keys that all four widen to f16 in LDS: d (q - 8), which is exact for scales of eight significant bits, as the cache's write makes
+// them (others round here).  Widening costs 15 instructions for eight values, once for 128 rows; the kernel above does it for every 16.  A thread's share of
+// the next block (a dword of codes per 16 dimensions) is requested before this block's products and widened behind them, into the other of two stages.
+// LDS rows are 16 bytes longer than the values: the fragments' reads then meet no bank twice.
+//   S = K Q^T: keys first, so that a lane holds one row's scores of 16 keys, and the maximum needs two steps across lanes.
+//   O += V^T P: the lane's probabilities are an operand as they lie; the values' comes transposed out of LDS (ds_read_b64_tr_b16).
+// The exponentials refer to the block's own maximum, or 2^8 below the row's where that is more: what rounding the probabilities to f16 costs is mostly the
+// error of the largest, and these are then exact.  The sum is that of the rounded probabilities.
+// ---------------------------------------------------------------------------------------------
+constexpr int AP_ROWS = 128, AP_KEYS = 64;
+typedef half_t half4_u __attribute__((ext_vector_type(4), aligned(2))); // outputs start anywhere
+typedef __fp16 aq_fp16x4 __attribute__((ext_vector_type(4)));
+
+// MK: no mask tensor, an f32 one, an f16 one
+template <int NT, int MK> __global__ __launch_bounds__(256, 2) void attention_q4_tile_kernel(AttnQ4Args g) {
+    constexpr int D = 16 * NT, KK = (NT + 1) / 2, LD = D + 8, BLK = AP_KEYS * LD, RB = D / 2, SR = KK == 3 ? 4 : KK, DW = 2 * NT; // (DW: dwords of a row)
+    extern __shared__ __attribute__((aligned(16))) uint8_t smem[];
+    half_t *const ring = (half_t *)smem;                         // [2][keys | values][64][LD]
+    uint32_t *const odd_flags = (uint32_t *)(ring + 4 * BLK);    // [2][wavefront]: whether the block has a scale of values that is not finite
+    const int t = threadIdx.x, lane = t & 63, wave = __builtin_amdgcn_readfirstlane(t >> 6);
+    const int fr = lane & 15, fg = lane >> 4;
+
+    // (head of keys, tile of rows, share of keys): XCD x takes the x-th eighth, so that a head's tiles share an L2; with the causal flag the long (late) tiles
+    // come first, and where every workgroup is resident at once (two per compute unit) the second half in the opposite order
+    uint32_t lin = blockIdx.x, bk, tile, sp = 0;
+    const uint32_t total = gridDim.x, nt = (uint32_t)g.row_tiles;
+    const uint32_t chunk = total >> 3, rr = lin >> 3, x8 = lin & 7u;
+    if ((total & 7u) == 0 && g.causal && g.splits == 1 && chunk % nt == 0) {
+        const uint32_t hx = chunk / nt, q = rr / hx;
+        bk = x8 * hx + (rr - q * hx);
+        tile = total <= (uint32_t)g.resident && nt % 2 == 0 && 2 * q >= nt ? q - nt / 2 : nt - 1 - q;
+    } else {
+        if ((total & 7u) == 0) lin = x8 * chunk + rr;
+        const uint32_t u = lin / (uint32_t)g.splits;
+        sp = lin - u * (uint32_t)g.splits;
+        bk = u / nt, tile = u - bk * nt;
     }
-    const int qi = m / g.group;
-    g.O[b * g.o_bs + (int64_t)(kh * g.group + (m - qi * g.group)) * g.o_hs + qi * g.o_rs + d] = (half_t)(y / l);
+    const int b = (int)bk / g.kv_heads, kh = (int)bk - b * g.kv_heads;
+    const int row0 = (int)tile * AP_ROWS, rw = row0 + 32 * wave; // first row of the workgroup, of the wavefront
+    int len = g.kv_len;
+    if (g.lens) len = min(max(__builtin_amdgcn_readfirstlane(g.lens[b]), 0), len);
+    const int off = len - g.q_len; // causal: query row i sees keys <= i + off
+    auto sees = [&](int m) { return g.causal ? max(0, min(len, min(m, g.rows - 1) / g.group + off + 1)) : len; }; // keys that row m sees
+    const int j_first = (int)sp * g.split_keys;
+    const int j_end = min(sees(row0 + AP_ROWS - 1), j_first + g.split_keys), w_end = rw < g.rows ? min(j_end, sees(rw + 31)) : 0;
+    const int w_lean = MK || g.scale_log2e > 0.f ? min(w_end, sees(rw)) : 0; // blocks up to here: every key is seen by all of the wavefront's rows
+
+    const int64_t head = (int64_t)bk * g.capacity;
+    const uint8_t *const Kc = g.Kc + head * RB, *const Vc = g.Vc + head * RB;
+    const half_t *const Ks = g.Ks + head * SR, *const Vs = g.Vs + head * SR;
+
+    // rows rw + 16 u + fr: fragments of dimensions 32 kk + 8 fg .. + 7 (zero past head_dim)
+    half8_t fq[2][KK];
+    int last[2]; // the last key that the row sees
+    const half_t *mrow[2];
+#pragma unroll
+    for (int u = 0; u < 2; u++) {
+        const int m = min(rw + 16 * u + fr, g.rows - 1), qi = m / g.group;
+        last[u] = (g.causal ? min(len, qi + off + 1) : len) - 1;
+        const half_t *qp = g.Q + b * g.q_bs + (int64_t)(kh * g.group + (m - qi * g.group)) * g.q_hs + qi * g.q_rs;
+#pragma unroll
+        for (int kk = 0; kk < KK; kk++) fq[u][kk] = 32 * kk + 8 * fg < D ? *(const half8_t *)(qp + 32 * kk + 8 * fg) : half8_t{};
+        mrow[u] = (const half_t *)g.mask + (b * g.m_bs + qi * g.m_rs) * (MK == 1 ? 2 : 1);
+    }
+
+    // ---- this thread's dwords of a block: number i is dword i * 256 + t of [keys | values][64][DW]
+    uint32_t raw[NT];
+    half_t ds[NT];
+    auto load = [&](int j0) __attribute__((always_inline)) {
+#pragma unroll
+        for (int i = 0; i < NT; i++) {
+            const bool val = __builtin_amdgcn_readfirstlane(i * 256 + t) >= 128 * NT;
+            const int f = i * 256 + t - (val ? 128 * NT : 0), key = f / DW, w = f - key * DW;
+            const uint32_t j = (uint32_t)min(key, len - 1 - j0); // keys past the last repeat it: their scores are masked
+            raw[i] = *(const uint32_t *)((val ? Vc : Kc) + (int64_t)j0 * RB + (j * RB + 4 * w));
+            ds[i] = *((val ? Vs : Ks) + (int64_t)j0 * SR + (j * SR + (w >> 2)));
+        }
+    };
+    const uint32_t bias = q40_bias();
+    auto widen = [&](int stage) __attribute__((always_inline)) {
+        bool odd = false;
+#pragma unroll
+        for (int i = 0; i < NT; i++) {
+            const bool val = __builtin_amdgcn_readfirstlane(i * 256 + t) >= 128 * NT;
+            const int f = i * 256 + t - (val ? 128 * NT : 0), key = f / DW, w = f - key * DW;
+            half_t d = ds[i];
+            if (val) { // a value that is not finite shows in the rows that see its key, and not through the matrix cores
+                const bool fin = (__builtin_bit_cast(uint16_t, d) & 0x7C00u) != 0x7C00u;
+                odd |= !fin;
+                d = fin ? d : (half_t)0.f;
+            }
+            *(half8_t *)(ring + stage * 2 * BLK + (val ? BLK : 0) + key * LD + 8 * w) = q40_codes(raw[i], bias) * half8_t{d, d, d, d, d, d, d, d};
+        }
+        const bool any = __builtin_amdgcn_ballot_w64(odd) != 0;
+        if (lane == 0) odd_flags[4 * stage + wave] = any;
+    };
+    using MT = std::conditional_t<MK == 1, float, half_t>;
+    typedef MT mask4_t __attribute__((ext_vector_type(4)));
+    typedef MT mask4_u __attribute__((ext_vector_type(4), aligned(sizeof(MT)))); // rows start anywhere
+    constexpr int MU = MK ? 2 : 1, MB = MK ? 4 : 1;
+    mask4_t mk[MU][MB]; // the block's, requested before the first product
+    auto load_mask = [&](int j0) __attribute__((always_inline)) {
+        if constexpr (MK != 0) {
+#pragma unroll
+            for (int u = 0; u < 2; u++) {
+                const MT *p = (const MT *)mrow[u];
+                if (j0 + AP_KEYS <= len) { // uniform
+#pragma unroll
+                    for (int bt = 0; bt < 4; bt++) mk[u][bt] = *(const mask4_u *)(p + j0 + 16 * bt + 4 * fg);
+                } else {
+#pragma unroll
+                    for (int e = 0; e < 16; e++) mk[u][e >> 2][e & 3] = p[min(j0 + 16 * (e >> 2) + 4 * fg + (e & 3), len - 1)];
+                }
+            }
+        }
+    };
+
+    float4_t acc[2][NT];
+    float m_run[2], m_top[2], l_run[2]; // base 2: the exponentials' reference and the maximum so far; this lane's share of the sum
+    uint32_t bad[2];
+#pragma unroll
+    for (int u = 0; u < 2; u++) {
+        m_run[u] = m_top[u] = -INFINITY, l_run[u] = 0.f, bad[u] = 0;
+#pragma unroll
+        for (int d = 0; d < NT; d++) acc[u][d] = float4_t{0.f, 0.f, 0.f, 0.f};
+    }
+    int koff[KK];
+#pragma unroll
+    for (int kk = 0; kk < KK; kk++) koff[kk] = fr * LD + 8 * min(4 * kk + fg, DW - 1);
+    const int voff = BLK + (4 * fg + (fr >> 2)) * LD + 4 * (fr & 3);
+
+    auto step = [&](int stage, int j0, auto lean_c) __attribute__((always_inline)) {
+        constexpr bool LEAN = decltype(lean_c)::value;
+        const half_t *const st = ring + stage * 2 * BLK;
+        const uint4_t fl = *(const uint4_t *)(odd_flags + 4 * stage);
+        load_mask(j0);
+        float4_t S[2][4];
+#pragma unroll
+        for (int bt = 0; bt < 4; bt++) {
+            half8_t fk[KK];
+#pragma unroll
+            for (int kk = 0; kk < KK; kk++) fk[kk] = *(const half8_t *)(st + koff[kk] + 16 * bt * LD);
+#pragma unroll
+            for (int u = 0; u < 2; u++) S[u][bt] = float4_t{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int kk = 0; kk < KK; kk++)
+#pragma unroll
+                for (int u = 0; u < 2; u++) S[u][bt] = __builtin_amdgcn_mfma_f32_16x16x32_f16(fk[kk], fq[u][kk], S[u][bt], 0, 0, 0);
+        }
+        const bool odd = __builtin_amdgcn_readfirstlane((int)(fl[0] | fl[1] | fl[2] | fl[3])) != 0;
+        half8_t fp[2][2];
+#pragma unroll
+        for (int u = 0; u < 2; u++) {
+            float bmax = -INFINITY;
+            if constexpr (LEAN && MK == 0) { // scale > 0: the maximum of the raw scores, the scale folded into the exponent's argument
+#pragma unroll
+                for (int e = 0; e < 16; e++) bmax = fmaxf(bmax, S[u][e >> 2][e & 3]);
+                bmax *= g.scale_log2e;
+            } else {
+#pragma unroll
+                for (int e = 0; e < 16; e++) {
+                    float s = S[u][e >> 2][e & 3] * g.scale_log2e;
+                    if constexpr (MK != 0) {
+                        const float mv = (float)mk[u][e >> 2][e & 3], m2 = mv * kLog2eQ4;
+                        // a hidden key's score may be anything; a type's lowest value hides nothing from a row that has nothing else
+                        s = mv == -INFINITY ? -INFINITY : s + (MK == 1 && m2 == -INFINITY ? -3.40282347e38f : m2);
+                    }
+                    if (!LEAN && j0 + 16 * (e >> 2) + 4 * fg + (e & 3) > last[u]) s = -INFINITY;
+                    S[u][e >> 2][e & 3] = s;
+                    bmax = fmaxf(bmax, s);
+                }
+            }
+            if (odd) {
+                uint32_t seen = 0;
+#pragma unroll
+                for (int e = 0; e < 16; e++) seen |= S[u][e >> 2][e & 3] == -INFINITY ? 0u : 1u << e;
+#pragma unroll 1
+                for (int e = 0; e < 16 * KK; e++) {
+                    const int k = e >> 4;
+                    const uint32_t j = (uint32_t)min(j0 + 4 * (e & 12) + 4 * fg + (e & 3), len - 1);
+                    const bool fin = (__builtin_bit_cast(uint16_t, Vs[j * SR + k]) & 0x7C00u) != 0x7C00u;
+                    if (!fin && ((seen >> (e & 15)) & 1u)) bad[u] |= 1u << k;
+                }
+            }
+            bmax = rt_groups_max(bmax);
+            m_top[u] = fmaxf(m_top[u], bmax);
+            const float m_new = fmaxf(m_top[u] - 8.f, bmax);
+            const float m_use = m_new == -INFINITY ? 0.f : m_new; // a row without a key yet: exp2(-inf - 0) = 0
+            const float alpha = __builtin_amdgcn_exp2f(m_run[u] - m_use);
+            m_run[u] = m_new;
+            const float sc = LEAN && MK == 0 ? g.scale_log2e : 1.f;
+            float psum = 0.f;
+#pragma unroll
+            for (int e = 0; e < 16; e += 2) {
+                const float p0 = __builtin_amdgcn_exp2f(fmaf(S[u][e >> 2][e & 3], sc, -m_use)), p1 = __builtin_amdgcn_exp2f(fmaf(S[u][e >> 2][(e & 3) + 1], sc, -m_use));
+                const half2_t p = {(half_t)p0, (half_t)p1};
+                psum = __builtin_amdgcn_fdot2(p, half2_t{(half_t)1, (half_t)1}, psum, false);
+                fp[u][e >> 3][e & 7] = p[0], fp[u][e >> 3][(e & 7) + 1] = p[1];
+            }
+            l_run[u] = l_run[u] * alpha + psum;
+#pragma unroll
+            for (int d = 0; d < NT; d++) acc[u][d] *= alpha;
+        }
+#pragma unroll
+        for (int hh = 0; hh < 2; hh++)
+#pragma unroll
+            for (int d = 0; d < NT; d++) {
+                typedef uint64_t u64x2_t __attribute__((ext_vector_type(2)));
+                typedef __attribute__((address_space(3))) aq_fp16x4 *lds4;
+                const half_t *vp = st + voff + 16 * d + 32 * hh * LD;
+                const uint64_t v0 = __builtin_bit_cast(uint64_t, __builtin_amdgcn_ds_read_tr16_b64_v4f16((lds4)vp));
+                const uint64_t v1 = __builtin_bit_cast(uint64_t, __builtin_amdgcn_ds_read_tr16_b64_v4f16((lds4)(vp + 16 * LD)));
+                const half8_t fv = __builtin_bit_cast(half8_t, u64x2_t{v0, v1});
+#pragma unroll
+                for (int u = 0; u < 2; u++) acc[u][d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(fv, fp[u][hh], acc[u][d], 0, 0, 0);
+            }
+    };
+
+    if (j_first < j_end) {
+        load(j_first);
+        widen(0);
+        __syncthreads();
+        int stage = 0, j0 = j_first;
+        auto turn = [&](auto body) __attribute__((always_inline)) {
+            const bool more = j0 + AP_KEYS < j_end;
+            if (more) load(j0 + AP_KEYS);
+            __builtin_amdgcn_sched_barrier(0);
+            body();
+            __builtin_amdgcn_sched_barrier(0);
+            if (more) widen(stage ^ 1);
+            __syncthreads();
+            stage ^= 1, j0 += AP_KEYS;
+        };
+        while (j0 + AP_KEYS <= w_lean) turn([&]() { step(stage, j0, std::true_type{}); });
+        while (j0 < w_end) turn([&]() { step(stage, j0, std::false_type{}); });
+        while (j0 < j_end) turn([]() {}); // blocks that only other wavefronts need
+    }
+#pragma unroll
+    for (int u = 0; u < 2; u++) {
+        const int m = rw + 16 * u + fr;
+        const float l = rt_groups_sum(l_run[u]);
+        uint32_t bd = bad[u];
+        bd |= (uint32_t)__shfl_xor((int)bd, 16);
+        bd |= (uint32_t)__shfl_xor((int)bd, 32);
+        if (bd) {
+#pragma unroll
+            for (int d = 0; d < NT; d++)
+                if ((bd >> (d >> 1)) & 1u) acc[u][d] = float4_t{1.f, 1.f, 1.f, 1.f} * __builtin_nanf("");
+        }
+        if (m >= g.rows) continue;
+        if (g.splits > 1) {
+            const int64_t at = ((int64_t)bk * g.rows + m) * g.splits + sp;
+            if (fg == 0) *(float2_t *)(g.part_ml + 2 * at) = float2_t{m_run[u], l};
+            if (j_first < j_end) { // (a share with a sum of 0 is not read)
+#pragma unroll
+                for (int d = 0; d < NT; d++) *(float4_t *)(g.part_o + at * D + 16 * d + 4 * fg) = acc[u][d];
+            }
+        } else {
+            const int qi = m / g.group;
+            const float inv = 1.f / l; // no visible key: 0 * inf, NaN
+            half_t *const op = g.O + b * g.o_bs + (int64_t)(kh * g.group + (m - qi * g.group)) * g.o_hs + qi * g.o_rs;
+#pragma unroll
+            for (int d = 0; d < NT; d++) {
+                const half4_t o4 = {(half_t)(acc[u][d][0] * inv), (half_t)(acc[u][d][1] * inv), (half_t)(acc[u][d][2] * inv), (half_t)(acc[u][d][3] * inv)};
+                *(half4_u *)(op + 16 * d + 4 * fg) = o4;
+            }
+        }
+    }
 }
 
-static int aq_row_tiles(int rows) { return rows <= 16 ? 1 : (rows + 31) / 32; }
+// Joins the shares of a row, four columns a thread.  A row's threads are CG = D / 4 to the next power of two columns by SG groups of shares, all of whose loads are
+// requested at once; the groups meet in LDS, in a fixed order.  (One thread a column that walked the shares took 20.9 us for 32 rows of 64 shares of 128.)
+template <int CG> __global__ __launch_bounds__(256) void attention_q4_merge_kernel(AttnQ4Args g, int D) {
+    constexpr int SG = 256 / CG, PER = (AQ_MAX_SPLITS + SG - 1) / SG;
+    __shared__ __attribute__((aligned(16))) float part[SG][4 * CG];
+    const int64_t row = blockIdx.x;
+    const int t = threadIdx.x, lane = t & 63, c = t % CG, sg = t / CG;
+    const bool live = 4 * c < D;
+    const float *const po = g.part_o + row * g.splits * D + (live ? 4 * c : 0);
+    float4_t v[PER];
+#pragma unroll
+    for (int i = 0; i < PER; i++)
+        if (i * SG < g.splits) v[i] = *(const float4_t *)(po + (int64_t)min(i * SG + sg, g.splits - 1) * D);
+    // lane s has share s's weight
+    const float2_t ml = *(const float2_t *)(g.part_ml + (row * g.splits + min(lane, g.splits - 1)) * 2);
+    float top = ml[0];
+#pragma unroll
+    for (int x = 1; x < 64; x *= 2) top = fmaxf(top, __shfl_xor(top, x));
+    const float base = top == -INFINITY ? 0.f : top;
+    const float a = lane < g.splits && ml[1] != 0.f ? __builtin_amdgcn_exp2f(ml[0] - base) : 0.f; // (a share without a key: nothing to read)
+    float l = lane < g.splits && ml[1] != 0.f ? a * ml[1] : 0.f;
+#pragma unroll
+    for (int x = 1; x < 64; x *= 2) l += __shfl_xor(l, x);
+    const uint64_t some = __builtin_amdgcn_ballot_w64(lane < g.splits && ml[1] != 0.f);
+    float4_t y = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int i = 0; i < PER; i++) {
+        const int s = i * SG + sg;
+        const float w = __shfl(a, s & 63);
+        if (i * SG < g.splits && ((some >> (s & 63)) & 1u)) {
+#pragma unroll
+            for (int k = 0; k < 4; k++) y[k] = fmaf(v[i][k], w, y[k]);
+        }
+    }
+    *(float4_t *)&part[sg][4 * c] = y;
+    __syncthreads();
+    if (t >= D) return;
+    float sum = 0.f;
+#pragma unroll
+    for (int s = 0; s < SG; s++) sum += part[s][t];
+    const int bk = (int)(row / g.rows), m = (int)(row - (int64_t)bk * g.rows), b = bk / g.kv_heads, kh = bk - b * g.kv_heads, qi = m / g.group;
+    g.O[b * g.o_bs + (int64_t)(kh * g.group + (m - qi * g.group)) * g.o_hs + qi * g.o_rs + t] = (half_t)(sum / l); // no visible key: 0 / 0
+}
+
+// the two kernels: rows of a tile, and the keys that shares are counted in
+static bool aq_streams(int rows) { return rows <= 16; }
+static int64_t aq_row_tiles(int rows) { return aq_streams(rows) ? 1 : (rows + AP_ROWS - 1) / AP_ROWS; }
+RT_TUNABLE(g_aq_target, 512);
+RT_TUNABLE(g_aq_least, 128);
 // keys of a workgroup where several share a row tile's, and how many do
 static void aq_split(const rt_attention_q4_desc &d, int &splits, int &split_keys) {
     const int rows = d.q_len * (d.heads / d.kv_heads);
     const int64_t wgs = (int64_t)d.batch * d.kv_heads * aq_row_tiles(rows);
-    const int step = rows <= 16 ? 512 : 256; // of a workgroup's eight or four wavefronts
+    const int step = aq_streams(rows) ? 512 : g_aq_least; // of a workgroup's eight wavefronts; two blocks
     const int steps = (d.kv_len + step - 1) / step;
     int s = 1;
-    if (wgs < 512 && steps > 1) s = (int)std::min<int64_t>(steps, (512 + wgs - 1) / wgs);
+    if (wgs < g_aq_target && steps > 1) s = (int)std::min<int64_t>(std::min(steps, AQ_MAX_SPLITS), aq_streams(rows) ? (g_aq_target + wgs - 1) / wgs : g_aq_target / wgs);
     const int per = (steps + s - 1) / s;
     splits = std::max(1, (steps + per - 1) / std::max(per, 1)), split_keys = std::max(per, 1) * step;
 }
@@ -442,8 +745,13 @@ template <int NT, int RT, int VPR> static hipError_t launch_aq(const AttnQ4Args 
 }
 template <int NT> static hipError_t launch_aq_rows(const AttnQ4Args &g, dim3 grid, hipStream_t st) {
     if (g.rows <= 4) return launch_aq<NT, 1, 1>(g, grid, 8, st);
-    if (g.rows <= 16) return launch_aq<NT, 1, 4>(g, grid, 8, st);
-    return launch_aq<NT, 2, 4>(g, grid, 4, st);
+    return launch_aq<NT, 1, 4>(g, grid, 8, st);
+}
+template <int NT, int MK> static hipError_t launch_aq_tile(const AttnQ4Args &g, unsigned wgs, hipStream_t st) {
+    constexpr size_t lds = (size_t)4 * AP_KEYS * (16 * NT + 8) * sizeof(half_t) + 8 * sizeof(uint32_t);
+    if (const hipError_t e = ensure_lds_limit<&attention_q4_tile_kernel<NT, MK>>(); e != hipSuccess) return e;
+    hipLaunchKernelGGL((attention_q4_tile_kernel<NT, MK>), dim3(wgs), dim3(256), lds, st, g);
+    return hipGetLastError();
 }
 
 hipError_t launch_attention_q4(const rt_attention_q4_desc &d, const void *q, const void *k_cache, const void *v_cache, const void *mask,
@@ -466,22 +774,31 @@ hipError_t launch_attention_q4(const rt_attention_q4_desc &d, const void *q, con
     } else {
         g.splits = 1, g.split_keys = std::max(d.kv_len, 1);
     }
-    const int64_t tiles = aq_row_tiles(g.rows);
-    if (tiles > 65535) return hipErrorNotSupported;
-    const dim3 grid((unsigned)g.splits, (unsigned)(d.batch * d.kv_heads), (unsigned)tiles);
+    const int64_t tiles = aq_row_tiles(g.rows), stacks = (int64_t)d.batch * d.kv_heads;
+    g.row_tiles = (int)tiles, g.resident = 2 * dev.num_cus;
+    if (tiles * stacks * g.splits > 0xffffff || (g.splits > 1 && stacks * g.rows > 0xffffff)) return hipErrorNotSupported; // (a grid's threads along an axis are fewer than 2^32)
+    const dim3 grid((unsigned)g.splits, (unsigned)stacks);
+    auto go = [&](auto nt) -> hipError_t {
+        constexpr int NT = decltype(nt)::value;
+        if (aq_streams(g.rows)) return launch_aq_rows<NT>(g, grid, stream);
+        const unsigned wgs = (unsigned)(tiles * stacks * g.splits);
+        return !mask ? launch_aq_tile<NT, 0>(g, wgs, stream) : g.mask_f32 ? launch_aq_tile<NT, 1>(g, wgs, stream) : launch_aq_tile<NT, 2>(g, wgs, stream);
+    };
     hipError_t e;
     switch (d.head_dim / 16) {
-    case 1: e = launch_aq_rows<1>(g, grid, stream); break;
-    case 2: e = launch_aq_rows<2>(g, grid, stream); break;
-    case 3: e = launch_aq_rows<3>(g, grid, stream); break;
-    case 4: e = launch_aq_rows<4>(g, grid, stream); break;
-    case 5: e = launch_aq_rows<5>(g, grid, stream); break;
-    case 6: e = launch_aq_rows<6>(g, grid, stream); break;
-    case 7: e = launch_aq_rows<7>(g, grid, stream); break;
-    default: e = launch_aq_rows<8>(g, grid, stream); break;
+    case 1: e = go(std::integral_constant<int, 1>{}); break;
+    case 2: e = go(std::integral_constant<int, 2>{}); break;
+    case 3: e = go(std::integral_constant<int, 3>{}); break;
+    case 4: e = go(std::integral_constant<int, 4>{}); break;
+    case 5: e = go(std::integral_constant<int, 5>{}); break;
+    case 6: e = go(std::integral_constant<int, 6>{}); break;
+    case 7: e = go(std::integral_constant<int, 7>{}); break;
+    default: e = go(std::integral_constant<int, 8>{}); break;
     }
     if (e != hipSuccess || g.splits <= 1) return e;
-    hipLaunchKernelGGL(attention_q4_merge_kernel, dim3((unsigned)((int64_t)d.batch * d.heads * d.q_len)), dim3(128), 0, stream, g, d.head_dim);
+    const dim3 rows((unsigned)(stacks * g.rows));
+    if (d.head_dim <= 64) hipLaunchKernelGGL(attention_q4_merge_kernel<16>, rows, dim3(256), 0, stream, g, d.head_dim);
+    else hipLaunchKernelGGL(attention_q4_merge_kernel<32>, rows, dim3(256), 0, stream, g, d.head_dim);
     return hipGetLastError();
 }
 
