@@ -188,6 +188,27 @@ __device__ __forceinline__ half8_t q40_codes(uint32_t w, uint32_t kBias = 0x6400
 // byte offset of the scales of a Q4_0 tensor: its codes, half a byte each, fill whole 256 bytes
 inline uint64_t q40_scale_offset(uint64_t numel) { return (numel / 2 + 255u) & ~(uint64_t)255u; }
 
+// lane group g's register t <- lane group t's register g
+__device__ __forceinline__ void q40_transpose(uint4_t &v) {
+    const auto a = __builtin_amdgcn_permlane16_swap(v[0], v[1], false, false);
+    const auto b = __builtin_amdgcn_permlane16_swap(v[2], v[3], false, false);
+    const auto c = __builtin_amdgcn_permlane32_swap(a[0], b[0], false, false);
+    const auto d = __builtin_amdgcn_permlane32_swap(a[1], b[1], false, false);
+    v = uint4_t{c[0], d[0], c[1], d[1]};
+}
+
+// a dword of lane group u -> all lane groups, for u below UC (2: lane groups 2 and 3 have what 0 and 1 have)
+template <int UC> __device__ __forceinline__ void q40_spread(uint32_t x, uint32_t *to) {
+    if constexpr (UC == 2) {
+        const auto a = __builtin_amdgcn_permlane16_swap(x, x, false, false); // lane groups 0 0 2 2, and 1 1 3 3
+        to[0] = a[0], to[1] = a[1];
+    } else {
+        const auto h = __builtin_amdgcn_permlane32_swap(x, x, false, false); // 0 1 0 1, and 2 3 2 3
+        const auto a = __builtin_amdgcn_permlane16_swap(h[0], h[0], false, false), b = __builtin_amdgcn_permlane16_swap(h[1], h[1], false, false);
+        to[0] = a[0], to[1] = a[1], to[2] = b[0], to[3] = b[1];
+    }
+}
+
 // A 4-bit key/value cache [batch, heads, capacity, head_dim] in one buffer: codes, head_dim / 2 bytes a row, to whole 256 bytes, then a row's
 // scales, one f16 per 32 values (the last block may have 16), as many as the next of 1, 2 and 4.
 inline int cache_q4_scales(int head_dim) { return head_dim <= 32 ? 1 : head_dim <= 64 ? 2 : 4; }

@@ -39,21 +39,10 @@ struct AttnQ4Args {
     float *part_o, *part_ml; // [row][split][D], [row][split][2]
     int64_t q_bs, q_hs, q_rs, o_bs, o_hs, o_rs, m_bs, m_rs;
     int kv_heads, group, rows, kv_len, q_len, capacity; // rows = q_len * group
-    int causal, mask_f32, splits, split_keys, row_tiles, resident;
+    int causal, mask_f32, splits, split_keys, row_tiles;
     float scale_log2e;
 };
 
-typedef uint32_t uint4_a8 __attribute__((ext_vector_type(4), aligned(8)));
-typedef uint32_t uint2_a8 __attribute__((ext_vector_type(2), aligned(8)));
-
-// lane group g's register t <- lane group t's register g
-__device__ __forceinline__ void aq_transpose(uint4_t &v) {
-    const auto a = __builtin_amdgcn_permlane16_swap(v[0], v[1], false, false);
-    const auto b = __builtin_amdgcn_permlane16_swap(v[2], v[3], false, false);
-    const auto c = __builtin_amdgcn_permlane32_swap(a[0], b[0], false, false);
-    const auto d = __builtin_amdgcn_permlane32_swap(a[1], b[1], false, false);
-    v = uint4_t{c[0], d[0], c[1], d[1]};
-}
 template <int CTRL> __device__ __forceinline__ float aq_dpp(float v) {
     return __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, v), CTRL, 0xf, 0xf, true));
 }
@@ -74,217 +63,202 @@ __device__ __forceinline__ uint32_t aq_or16(uint32_t v) {
     return v | (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x121, 0xf, 0xf, true);
 }
 
-// How a head_dim of 16 NT is read by 16 lanes: a dword of a row each (128), or two bytes (64), a byte (32) and a nibble (16) as they are needed.
+// How a row of values, 8 NT bytes, is read by 16 lanes: W bytes each, by CL of them
 template <int NT> struct AqDims {
-    static constexpr int D = 16 * NT, NF = D / 32, TAIL = NT & 1, NB = NF + TAIL, SR = NB == 3 ? 4 : NB, PB = NF ? NF : 1; // (PB: pieces of 16 bytes of a key, where there are any)
-    static constexpr bool P4 = NT == 8, P2 = NT & 4, P1 = NT & 2, PH = NT & 1;
-    static constexpr int T2 = 0, T1 = P2 ? 4 : 0, TH = T1 + (P1 ? 2 : 0); // first tile of a piece
-    static constexpr int B1 = P2 ? 32 : 0, BH = B1 + (P1 ? 16 : 0);       // its first byte of a row
+    static constexpr int D = 16 * NT, RB = 8 * NT, NF = D / 32, TAIL = NT & 1, NB = NF + TAIL, SR = NB == 3 ? 4 : NB, PB = NF ? NF : 1; // (PB: pieces of 16 bytes of a key, where there are any)
+    static constexpr int W = NT > 4 ? 4 : NT > 2 ? 2 : 1, CL = RB / W, T = 2 * W;
     // dimension that lane c's column of tile t stands for
     __device__ __forceinline__ static int dim(int t, int c) {
-        auto of = [](int nibble) { return 8 * (nibble >> 3) + ((nibble & 3) << 1) + ((nibble >> 2) & 1); }; // of a row's nibble
-        if (P4) return of(8 * c + t);
-        if (P2 && t < 4) return of(4 * c + t);
-        if (P1 && t < T1 + 2) return of(2 * B1 + 2 * c + (t - T1));
-        return of(2 * BH + c);
+        const int nibble = T * c + t; // of the row
+        return 8 * (nibble >> 3) + ((nibble & 3) << 1) + ((nibble >> 2) & 1);
     }
 };
 
-// RT: row tiles of 16; VPR: result registers in use with one row tile (1: up to 4 rows, 4: up to 16)
-template <int NT, int RT, int VPR> __global__ __launch_bounds__(RT == 1 ? 512 : 256) void attention_q4_kernel(AttnQ4Args g) {
+// Loads with a bound: past `bytes` the hardware returns zeros, and so codes of keys past the last have scales of zero.
+__device__ __forceinline__ __amdgpu_buffer_rsrc_t aq_bounded(const void *p, int bytes) {
+    return __builtin_amdgcn_make_buffer_rsrc(const_cast<void *>(p), 0, bytes, 0x00027000); // raw, 32-bit data
+}
+
+// VPR: result registers in use (1: up to 4 rows, 4: up to 16).  MK: a mask tensor
+template <int NT, int VPR, int MK> __global__ __launch_bounds__(512) void attention_q4_kernel(AttnQ4Args g) {
     using DM = AqDims<NT>;
-    constexpr int D = DM::D, NF = DM::NF, NB = DM::NB, SR = DM::SR, RB = D / 2;
-    constexpr int ROWS = RT == 1 ? 4 * VPR : 16 * RT; // rows of the tile
-    constexpr int PS = 72;                            // halves between rows of probabilities
+    constexpr int D = DM::D, NF = DM::NF, TAIL = DM::TAIL, NB = DM::NB, SR = DM::SR, SW = (SR + 1) / 2, RB = DM::RB, W = DM::W, T = DM::T;
+    constexpr int ROWS = 4 * VPR, PS = 72; // halves between rows of probabilities
     constexpr int WAVE_LDS = (ROWS * PS + NB * 64) * 2;
     extern __shared__ __attribute__((aligned(16))) uint8_t smem[];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), waves = blockDim.x >> 6;
-    const int r = lane & 15, fg = lane >> 4;
+    const int r = lane & 15, fg = lane >> 4, cc = min(r, DM::CL - 1);
     half_t *P = (half_t *)(smem + wave * WAVE_LDS), *S = P + ROWS * PS; // this wavefront's: probabilities [row][position], scales of values [block][position]
     const int bk = blockIdx.y, b = bk / g.kv_heads, kh = bk - b * g.kv_heads;
-    const int row0 = blockIdx.z * ROWS;
 
     int len = g.kv_len;
     if (g.lens) len = min(max(g.lens[b], 0), len);
-    // row m's query row, head and last visible key
-    auto q_row = [&](int m) { return m / g.group; };
-    int m_of[RT][VPR], last[RT][VPR];
+    // row fg VPR + v: its query row, head and last visible key
+    auto q_row = [&](int m) { return min(m, g.rows - 1) / g.group; };
+    int last[VPR];
 #pragma unroll
-    for (int t = 0; t < RT; t++)
-#pragma unroll
-        for (int v = 0; v < VPR; v++) {
-            m_of[t][v] = row0 + 16 * t + (RT == 1 ? fg * VPR + v : 4 * fg + v);
-            last[t][v] = g.causal ? min(len - 1, q_row(min(m_of[t][v], g.rows - 1)) + len - g.q_len) : len - 1;
-        }
-    // the keys of this workgroup: its share of those that any row of the tile sees
-    int end = len;
-    if (g.causal) end = min(end, q_row(min(row0 + ROWS, g.rows) - 1) + len - g.q_len + 1);
+    for (int v = 0; v < VPR; v++) last[v] = g.causal ? min(len - 1, q_row(fg * VPR + v) + len - g.q_len) : len - 1;
+    // the keys of this workgroup: its share of those that any row sees; up to `whole` all rows see them all
+    const int end = g.causal ? min(len, q_row(g.rows - 1) + len - g.q_len + 1) : len, whole = g.causal ? min(len, len - g.q_len + 1) : len;
     const int j_first = blockIdx.x * g.split_keys;
     const int j_end = min(end, j_first + g.split_keys);
 
     const int64_t head = (int64_t)bk * g.capacity;
-    const uint8_t *Kc = g.Kc + head * RB, *Vc = g.Vc + head * RB;
-    const half_t *Ks = g.Ks + head * SR, *Vs = g.Vs + head * SR;
+    const uint8_t *const Kc = g.Kc + head * RB, *const Vc = g.Vc + head * RB;
+    const half_t *const Ks = g.Ks + head * SR, *const Vs = g.Vs + head * SR;
 
-    half8_t qf[RT][NB];
-#pragma unroll
-    for (int t = 0; t < RT; t++) {
-        const int m = min(row0 + 16 * t + (RT == 1 ? (r >> 2) * VPR + min(r & 3, VPR - 1) : r), g.rows - 1), qi = q_row(m);
+    half8_t qf[NB];
+    {
+        const int m = min((r >> 2) * VPR + min(r & 3, VPR - 1), g.rows - 1), qi = m / g.group;
         const half_t *q = g.Q + b * g.q_bs + (int64_t)(kh * g.group + (m - qi * g.group)) * g.q_hs + qi * g.q_rs + 8 * fg;
 #pragma unroll
-        for (int k = 0; k < NF; k++) qf[t][k] = *(const half8_t *)(q + 32 * k);
-        if constexpr (DM::TAIL) qf[t][NF] = fg < 2 ? *(const half8_t *)(q + 32 * NF) : half8_t{};
+        for (int k = 0; k < NF; k++) qf[k] = *(const half8_t *)(q + 32 * k);
+        if constexpr (TAIL) qf[NF] = fg < 2 ? *(const half8_t *)(q + 32 * NF) : half8_t{};
     }
 
-    float mx[RT][VPR], sum[RT][VPR];
-    uint32_t bad[RT][VPR];
-    float4_t o[RT][NT];
+    // ---- 64 keys' loads
+    struct Unit {
+        uint4_t kc[NF + TAIL];
+        uint32_t dk[SW], dv[SW]; // lane group fg has the scales of keys 16 fg + r
+        uint32_t v[2][8];
+    };
+    uint32_t ko[NF ? NF : 1];
 #pragma unroll
-    for (int t = 0; t < RT; t++) {
-#pragma unroll
-        for (int v = 0; v < VPR; v++) mx[t][v] = -INFINITY, sum[t][v] = 0.f, bad[t][v] = 0;
-#pragma unroll
-        for (int n = 0; n < NT; n++) o[t][n] = float4_t{0.f, 0.f, 0.f, 0.f};
+    for (int i = 0; i < NF; i++) {
+        const int pc = 4 * i + fg, ks = pc / DM::PB, kb = pc - ks * DM::PB; // piece: key set and block
+        ko[i] = (16 * ks + r) * RB + 16 * kb;
     }
-
-    for (int j0 = j_first + 64 * wave; j0 < j_end; j0 += 64 * waves) {
-        const int clamp = len - 1; // > = 0 here; keys past it repeat it
-        // ---- loads
-        uint4_t kc[NF + DM::TAIL];
+    const uint32_t kt = lane * RB + 16 * NF, so = lane * SR * 2, vo = 2 * fg * RB + W * cc;
+    auto load = [&](int j0, Unit &k) __attribute__((always_inline)) {
+        const int n = max(0, min(64, j_end - j0));
+        const int64_t at = min(j0, max(j_end - 1, 0)); // (of nothing where n is 0)
+        const auto kr = aq_bounded(Kc + at * RB, n * RB), vr = aq_bounded(Vc + at * RB, n * RB), ksr = aq_bounded(Ks + at * SR, n * SR * 2), vsr = aq_bounded(Vs + at * SR, n * SR * 2);
 #pragma unroll
-        for (int i = 0; i < NF; i++) {
-            const int pc = 4 * i + fg, ks = pc / DM::PB, kb = pc - ks * DM::PB; // piece: key set and block
-            kc[i] = *(const uint4_a8 *)(Kc + (uint32_t)min(j0 + 16 * ks + r, clamp) * (uint64_t)RB + 16 * kb);
+        for (int i = 0; i < NF; i++) k.kc[i] = __builtin_bit_cast(uint4_t, __builtin_amdgcn_raw_buffer_load_b128(kr, ko[i], 0, 0));
+        if constexpr (TAIL) {
+            const uint2_t w = __builtin_bit_cast(uint2_t, __builtin_amdgcn_raw_buffer_load_b64(kr, kt, 0, 0));
+            k.kc[NF] = uint4_t{w[0], w[1], 0, 0};
         }
-        if constexpr (DM::TAIL) {
-            const uint2_t w = *(const uint2_a8 *)(Kc + (uint32_t)min(j0 + 16 * fg + r, clamp) * (uint64_t)RB + 16 * NF);
-            kc[NF] = uint4_t{w[0], w[1], 0, 0};
-        }
-        half_t dk[4][SR];
-#pragma unroll
-        for (int s = 0; s < 4; s++) {
-            const half_t *p = Ks + (uint32_t)min(j0 + 16 * s + r, clamp) * (uint64_t)SR;
-            if constexpr (SR == 1) dk[s][0] = *p;
-            else if constexpr (SR == 2) {
-                const half2_t x = *(const half2_t *)p;
-                dk[s][0] = x[0], dk[s][1] = x[1];
-            } else {
-                const half4_t x = *(const half4_t *)p;
-#pragma unroll
-                for (int k = 0; k < 4; k++) dk[s][k] = x[k];
+        auto scales = [&](__amdgpu_buffer_rsrc_t p, uint32_t *d) __attribute__((always_inline)) {
+            if constexpr (SR == 1) d[0] = __builtin_amdgcn_raw_buffer_load_b16(p, so, 0, 0);
+            else if constexpr (SR == 2) d[0] = __builtin_amdgcn_raw_buffer_load_b32(p, so, 0, 0);
+            else {
+                const uint2_t x = __builtin_bit_cast(uint2_t, __builtin_amdgcn_raw_buffer_load_b64(p, so, 0, 0));
+                d[0] = x[0], d[SW - 1] = x[1];
             }
-        }
-        half_t dv[SR];
-        {
-            const half_t *p = Vs + (uint32_t)min(j0 + 16 * fg + r, clamp) * (uint64_t)SR;
-            if constexpr (SR == 1) dv[0] = *p;
-            else if constexpr (SR == 2) {
-                const half2_t x = *(const half2_t *)p;
-                dv[0] = x[0], dv[1] = x[1];
-            } else {
-                const half4_t x = *(const half4_t *)p;
-#pragma unroll
-                for (int k = 0; k < 4; k++) dv[k] = x[k];
-            }
-        }
-        uint32_t v2[2][8], v1[2][8], vh[2][8]; // (v2: dwords of a head_dim of 128)
+        };
+        scales(ksr, k.dk), scales(vsr, k.dv);
 #pragma unroll
         for (int u = 0; u < 2; u++)
 #pragma unroll
             for (int e = 0; e < 8; e++) {
-                const uint8_t *p = Vc + (uint32_t)min(j0 + 16 * (e & 3) + 8 * u + 2 * fg + (e >> 2), clamp) * (uint64_t)RB;
-                if constexpr (DM::P4) v2[u][e] = *(const uint32_t *)(p + 4 * r);
-                if constexpr (DM::P2) v2[u][e] = *(const uint16_t *)(p + 2 * r);
-                if constexpr (DM::P1) v1[u][e] = p[DM::B1 + r];
-                if constexpr (DM::PH) vh[u][e] = p[DM::BH + (r >> 1)];
+                const uint32_t o = vo + (16 * (e & 3) + 8 * u + (e >> 2)) * RB;
+                if constexpr (W == 4) k.v[u][e] = __builtin_amdgcn_raw_buffer_load_b32(vr, o, 0, 0);
+                else if constexpr (W == 2) k.v[u][e] = __builtin_amdgcn_raw_buffer_load_b16(vr, o, 0, 0);
+                else k.v[u][e] = __builtin_amdgcn_raw_buffer_load_b8(vr, o, 0, 0);
             }
+    };
+    uint32_t mk[MK ? VPR : 1][4]; // the block's mask values, as they are; requested before the next block's loads, so that nothing waits for those
+    auto load_mask = [&](int j0) __attribute__((always_inline)) {
+        if constexpr (MK != 0) {
+#pragma unroll
+            for (int v = 0; v < VPR; v++) {
+                const int64_t row = b * g.m_bs + q_row(fg * VPR + v) * g.m_rs;
+#pragma unroll
+                for (int s = 0; s < 4; s++) {
+                    const int64_t i = row + min(j0 + 16 * s + r, len - 1);
+                    mk[v][s] = g.mask_f32 ? ((const uint32_t *)g.mask)[i] : ((const uint16_t *)g.mask)[i];
+                }
+            }
+        }
+    };
 
+    float mx[VPR], sum[VPR];
+    uint32_t bad[VPR];
+    float4_t o[T];
+#pragma unroll
+    for (int v = 0; v < VPR; v++) mx[v] = -INFINITY, sum[v] = 0.f, bad[v] = 0;
+#pragma unroll
+    for (int n = 0; n < T; n++) o[n] = float4_t{0.f, 0.f, 0.f, 0.f};
+    const uint32_t bias = q40_bias();
+
+    auto multiply = [&](int j0, Unit &k) __attribute__((always_inline)) {
         // ---- scores
-        float sc[RT][4][VPR];
+        uint32_t dk[SW][4]; // of key 16 s + r
 #pragma unroll
-        for (int t = 0; t < RT; t++)
+        for (int w = 0; w < SW; w++) q40_spread<4>(k.dk[w], dk[w]);
+        float sc[4][VPR];
 #pragma unroll
-            for (int s = 0; s < 4; s++)
+        for (int s = 0; s < 4; s++)
 #pragma unroll
-                for (int v = 0; v < VPR; v++) sc[t][s][v] = 0.f;
-        auto block = [&](uint32_t w, int s, int k) __attribute__((always_inline)) {
-            const half8_t q = q40_codes(w);
-            const float d = (float)dk[s][k];
+            for (int v = 0; v < VPR; v++) sc[s][v] = 0.f;
+        auto block = [&](uint32_t w, int s, int n) __attribute__((always_inline)) {
+            const float d = (float)__builtin_bit_cast(half2_t, dk[n >> 1][s])[n & 1];
+            const float4_t p = __builtin_amdgcn_mfma_f32_16x16x32_f16(qf[n], q40_codes(w, bias), float4_t{0.f, 0.f, 0.f, 0.f}, 0, 0, 0);
 #pragma unroll
-            for (int t = 0; t < RT; t++) {
-                const float4_t p = __builtin_amdgcn_mfma_f32_16x16x32_f16(qf[t][k], q, float4_t{0.f, 0.f, 0.f, 0.f}, 0, 0, 0);
-#pragma unroll
-                for (int v = 0; v < VPR; v++) sc[t][s][v] = fmaf(d, p[v], sc[t][s][v]);
-            }
+            for (int v = 0; v < VPR; v++) sc[s][v] = fmaf(d, p[v], sc[s][v]);
         };
 #pragma unroll
         for (int i = 0; i < NF; i++) {
-            aq_transpose(kc[i]);
+            q40_transpose(k.kc[i]);
 #pragma unroll
-            for (int x = 0; x < 4; x++) block(kc[i][x], (4 * i + x) / DM::PB, (4 * i + x) % DM::PB);
+            for (int x = 0; x < 4; x++) block(k.kc[i][x], (4 * i + x) / DM::PB, (4 * i + x) % DM::PB);
         }
-        if constexpr (DM::TAIL) {
-            aq_transpose(kc[NF]);
+        if constexpr (TAIL) {
+            q40_transpose(k.kc[NF]);
 #pragma unroll
-            for (int s = 0; s < 4; s++) block(kc[NF][s], s, NF);
+            for (int s = 0; s < 4; s++) block(k.kc[NF][s], s, NF);
         }
 
         // ---- mask, running maximum and sum, probabilities to LDS
-        const bool inside = j0 + 63 < len && !g.causal; // no key hidden
+        const bool inside = j0 + 64 <= whole; // no key hidden
 #pragma unroll
-        for (int t = 0; t < RT; t++)
+        for (int v = 0; v < VPR; v++) {
 #pragma unroll
-            for (int v = 0; v < VPR; v++) {
-                const int64_t mrow = b * g.m_bs + q_row(min(m_of[t][v], g.rows - 1)) * g.m_rs;
-#pragma unroll
-                for (int s = 0; s < 4; s++) {
-                    const int j = j0 + 16 * s + r;
-                    float x = sc[t][s][v] * g.scale_log2e;
-                    if (g.mask) {
-                        const int64_t at = mrow + min(j, clamp);
-                        const float mk = g.mask_f32 ? ((const float *)g.mask)[at] : (float)((const half_t *)g.mask)[at];
-                        // a hidden key's score may be anything; a type's lowest value hides nothing from a row that has nothing else
-                        const float m2 = mk * kLog2eQ4 == -INFINITY ? -3.40282347e38f : mk * kLog2eQ4;
-                        x = mk == -INFINITY ? -INFINITY : x + m2;
-                    }
-                    if (!inside) x = j <= last[t][v] ? x : -INFINITY;
-                    sc[t][s][v] = x;
+            for (int s = 0; s < 4; s++) {
+                float x = sc[s][v] * g.scale_log2e;
+                if constexpr (MK != 0) {
+                    const float mv = g.mask_f32 ? __builtin_bit_cast(float, mk[v][s]) : (float)__builtin_bit_cast(half_t, (uint16_t)mk[v][s]);
+                    // a hidden key's score may be anything; a type's lowest value hides nothing from a row that has nothing else
+                    const float m2 = mv * kLog2eQ4 == -INFINITY ? -3.40282347e38f : mv * kLog2eQ4;
+                    x = mv == -INFINITY ? -INFINITY : x + m2;
                 }
-                const float top = fmaxf(mx[t][v], aq_max16(fmaxf(fmaxf(sc[t][0][v], sc[t][1][v]), fmaxf(sc[t][2][v], sc[t][3][v]))));
-                const float base = top == -INFINITY ? 0.f : top;
-                const float a = __builtin_amdgcn_exp2f(mx[t][v] - base);
-                mx[t][v] = top;
-                float l = 0.f;
-                half4_t p4;
-#pragma unroll
-                for (int s = 0; s < 4; s++) {
-                    const float p = __builtin_amdgcn_exp2f(sc[t][s][v] - base);
-                    l += p;
-                    p4[s] = (half_t)p;
-                }
-                sum[t][v] = fmaf(sum[t][v], a, l);
-#pragma unroll
-                for (int n = 0; n < NT; n++) o[t][n][v] *= a;
-                *(half4_t *)(P + (RT == 1 ? fg * VPR + v : 16 * t + 4 * fg + v) * PS + 4 * r) = p4;
+                if (!inside) x = j0 + 16 * s + r <= last[v] ? x : -INFINITY;
+                sc[s][v] = x;
             }
+            const float top = fmaxf(mx[v], aq_max16(fmaxf(fmaxf(sc[0][v], sc[1][v]), fmaxf(sc[2][v], sc[3][v]))));
+            const float base = top == -INFINITY ? 0.f : top;
+            const float a = __builtin_amdgcn_exp2f(mx[v] - base);
+            mx[v] = top;
+            float l = 0.f;
+            half4_t p4;
+#pragma unroll
+            for (int s = 0; s < 4; s++) {
+                const float p = __builtin_amdgcn_exp2f(sc[s][v] - base);
+                l += p;
+                p4[s] = (half_t)p;
+            }
+            sum[v] = fmaf(sum[v], a, l);
+#pragma unroll
+            for (int n = 0; n < T; n++) o[n][v] *= a;
+            *(half4_t *)(P + (fg * VPR + v) * PS + 4 * r) = p4;
+        }
         // ---- scales of the values to LDS; one that is not finite shows in the rows that see its key and not through the matrix cores
         uint32_t odd = 0;
 #pragma unroll
-        for (int k = 0; k < NB; k++) {
-            const bool fin = (__builtin_bit_cast(uint16_t, dv[k]) & 0x7C00u) != 0x7C00u;
-            const bool valid = j0 + 16 * fg + r < len;
-            if (valid && !fin) odd |= 1u << k;
-            S[k * 64 + 4 * r + fg] = valid && fin ? dv[k] : (half_t)0.f;
+        for (int n = 0; n < NB; n++) {
+            const half_t d = __builtin_bit_cast(half2_t, k.dv[n >> 1])[n & 1];
+            const bool fin = (__builtin_bit_cast(uint16_t, d) & 0x7C00u) != 0x7C00u;
+            if (!fin) odd |= 1u << n;
+            S[n * 64 + 4 * r + fg] = fin ? d : (half_t)0.f;
         }
         if (__builtin_amdgcn_ballot_w64(odd != 0)) {
 #pragma unroll
             for (int s = 0; s < 4; s++) {
                 const uint32_t ks = (uint32_t)__builtin_amdgcn_ds_bpermute(4 * (16 * s + r), (int)odd);
 #pragma unroll
-                for (int t = 0; t < RT; t++)
-#pragma unroll
-                    for (int v = 0; v < VPR; v++)
-                        if (!(sc[t][s][v] == -INFINITY)) bad[t][v] |= ks;
+                for (int v = 0; v < VPR; v++)
+                    if (!(sc[s][v] == -INFINITY)) bad[v] |= ks;
             }
         }
         __builtin_amdgcn_wave_barrier();
@@ -293,93 +267,92 @@ template <int NT, int RT, int VPR> __global__ __launch_bounds__(RT == 1 ? 512 : 
         // ---- values
 #pragma unroll
         for (int u = 0; u < 2; u++) {
-            half8_t pf[RT];
-#pragma unroll
-            for (int t = 0; t < RT; t++)
-                pf[t] = *(const half8_t *)(P + (RT == 1 ? (r >> 2) * VPR + min(r & 3, VPR - 1) : 16 * t + r) * PS + 32 * u + 8 * fg);
+            const half8_t pf = *(const half8_t *)(P + ((r >> 2) * VPR + min(r & 3, VPR - 1)) * PS + 32 * u + 8 * fg);
+            const half8_t d = *(const half8_t *)(S + ((T * cc) >> 5) * 64 + 32 * u + 8 * fg);
             // four registers of key pairs: nibble `n` of the halves -> operand of tile `n0 + n`
-            auto product = [&](const uint32_t *w, int n0, int count, const half8_t d) __attribute__((always_inline)) {
+            auto product = [&](const uint32_t *w, int n0, int count) __attribute__((always_inline)) {
                 half8_t c[4];
 #pragma unroll
-                for (int e = 0; e < 4; e++) c[e] = q40_codes(w[e]);
+                for (int e = 0; e < 4; e++) c[e] = q40_codes(w[e], bias);
 #pragma unroll
                 for (int n = 0; n < count; n++) {
                     const half8_t x = half8_t{c[0][2 * n], c[0][2 * n + 1], c[1][2 * n], c[1][2 * n + 1], c[2][2 * n], c[2][2 * n + 1], c[3][2 * n], c[3][2 * n + 1]} * d;
-#pragma unroll
-                    for (int t = 0; t < RT; t++) o[t][n0 + n] = __builtin_amdgcn_mfma_f32_16x16x32_f16(pf[t], x, o[t][n0 + n], 0, 0, 0);
+                    o[n0 + n] = __builtin_amdgcn_mfma_f32_16x16x32_f16(pf, x, o[n0 + n], 0, 0, 0);
                 }
             };
-            auto scales = [&](int dim) { return *(const half8_t *)(S + (dim >> 5) * 64 + 32 * u + 8 * fg); };
             uint32_t w[4];
-            if constexpr (DM::P4) {
-                const half8_t d = scales(8 * r);
+            if constexpr (W == 4) {
 #pragma unroll
                 for (int hf = 0; hf < 2; hf++) {
 #pragma unroll
-                    for (int e = 0; e < 4; e++) w[e] = __builtin_amdgcn_perm(v2[u][2 * e + 1], v2[u][2 * e], hf ? 0x07060302u : 0x05040100u);
-                    product(w, 4 * hf, 4, d);
+                    for (int e = 0; e < 4; e++) w[e] = __builtin_amdgcn_perm(k.v[u][2 * e + 1], k.v[u][2 * e], hf ? 0x07060302u : 0x05040100u);
+                    product(w, 4 * hf, 4);
                 }
-            }
-            if constexpr (DM::P2) {
+            } else {
 #pragma unroll
-                for (int e = 0; e < 4; e++) w[e] = v2[u][2 * e] | (v2[u][2 * e + 1] << 16);
-                product(w, DM::T2, 4, scales(4 * r));
-            }
-            if constexpr (DM::P1) {
-#pragma unroll
-                for (int e = 0; e < 4; e++) w[e] = v1[u][2 * e] | (v1[u][2 * e + 1] << 16);
-                product(w, DM::T1, 2, scales(2 * DM::B1 + 2 * r));
-            }
-            if constexpr (DM::PH) {
-                const int sh = 4 * (r & 1);
-#pragma unroll
-                for (int e = 0; e < 4; e++) w[e] = (vh[u][2 * e] >> sh) | ((vh[u][2 * e + 1] >> sh) << 16);
-                product(w, DM::TH, 1, scales(2 * DM::BH + r));
+                for (int e = 0; e < 4; e++) w[e] = k.v[u][2 * e] | (k.v[u][2 * e + 1] << 16);
+                product(w, 0, T);
             }
         }
         __builtin_amdgcn_wave_barrier();
         asm volatile("" ::: "memory");
+    };
+
+    // 64 keys are multiplied while the wavefront's next 64 are on their way
+    const int step = 64 * waves;
+    int j0 = j_first + 64 * wave;
+    Unit ring[2];
+    if (j0 < j_end) {
+        load(j0, ring[0]);
+        __builtin_amdgcn_sched_barrier(0);
+#pragma unroll 1
+        for (; j0 + step < j_end; j0 += 2 * step) {
+            auto turn = [&](int j, Unit &now, Unit &next) __attribute__((always_inline)) {
+                load_mask(j);
+                load(j + step, next);
+                __builtin_amdgcn_sched_barrier(0);
+                multiply(j, now);
+                __builtin_amdgcn_sched_barrier(0);
+            };
+            turn(j0, ring[0], ring[1]);
+            turn(j0 + step, ring[1], ring[0]);
+        }
+        if (j0 < j_end) load_mask(j0), multiply(j0, ring[0]);
     }
 
     // ---- this wavefront's rows: the sum over the 16 lanes, and what a scale that is not finite leaves
 #pragma unroll
-    for (int t = 0; t < RT; t++)
+    for (int v = 0; v < VPR; v++) {
+        sum[v] = aq_sum16(sum[v]);
+        const uint32_t bd = aq_or16(bad[v]);
 #pragma unroll
-        for (int v = 0; v < VPR; v++) {
-            sum[t][v] = aq_sum16(sum[t][v]);
-            const uint32_t bd = aq_or16(bad[t][v]);
-#pragma unroll
-            for (int n = 0; n < NT; n++)
-                if ((bd >> (DM::dim(n, r) >> 5)) & 1u) o[t][n][v] = __builtin_nanf("");
-        }
-    // ---- the wavefronts' results through LDS: outputs [wave][RT][NT][VPR][64], maxima and sums [wave][row][2]
-    constexpr int PER = RT * NT * VPR * 64;
+        for (int n = 0; n < T; n++)
+            if ((bd >> (DM::dim(n, cc) >> 5)) & 1u) o[n][v] = __builtin_nanf("");
+    }
+    // ---- the wavefronts' results through LDS: outputs [wave][T][VPR][64], maxima and sums [wave][row][2]
+    constexpr int PER = T * VPR * 64;
     float *red = (float *)smem, *ml = red + waves * PER;
     __syncthreads();
 #pragma unroll
-    for (int t = 0; t < RT; t++) {
+    for (int n = 0; n < T; n++)
 #pragma unroll
-        for (int n = 0; n < NT; n++)
+        for (int v = 0; v < VPR; v++) red[wave * PER + (n * VPR + v) * 64 + lane] = o[n][v];
 #pragma unroll
-            for (int v = 0; v < VPR; v++) red[wave * PER + ((t * NT + n) * VPR + v) * 64 + lane] = o[t][n][v];
-#pragma unroll
-        for (int v = 0; v < VPR; v++) {
-            const int row = RT == 1 ? fg * VPR + v : 16 * t + 4 * fg + v;
-            if (r == 0) ml[(wave * ROWS + row) * 2] = mx[t][v], ml[(wave * ROWS + row) * 2 + 1] = sum[t][v];
-        }
+    for (int v = 0; v < VPR; v++) {
+        const int row = fg * VPR + v;
+        if (r == 0) ml[(wave * ROWS + row) * 2] = mx[v], ml[(wave * ROWS + row) * 2 + 1] = sum[v];
     }
     __syncthreads();
     for (int e = threadIdx.x; e < PER; e += blockDim.x) {
-        const int l = e & 63, tnv = e >> 6, v = tnv % VPR, tn = tnv / VPR, n = tn % NT, t = tn / NT;
-        const int row = RT == 1 ? (l >> 4) * VPR + v : 16 * t + 4 * (l >> 4) + v, m = row0 + row;
-        if (m >= g.rows) continue;
+        const int l = e & 63, v = (e >> 6) % VPR, n = (e >> 6) / VPR, m = (l >> 4) * VPR + v;
+        if (m >= g.rows || (l & 15) >= DM::CL) continue;
         float top = -INFINITY;
-        for (int w = 0; w < waves; w++) top = fmaxf(top, ml[(w * ROWS + row) * 2]);
+        for (int w = 0; w < waves; w++) top = fmaxf(top, ml[(w * ROWS + m) * 2]);
         const float base = top == -INFINITY ? 0.f : top;
         float y = 0.f, s = 0.f;
         for (int w = 0; w < waves; w++) {
-            const float a = __builtin_amdgcn_exp2f(ml[(w * ROWS + row) * 2] - base);
-            y = fmaf(red[w * PER + e], a, y), s = fmaf(ml[(w * ROWS + row) * 2 + 1], a, s);
+            const float a = __builtin_amdgcn_exp2f(ml[(w * ROWS + m) * 2] - base);
+            y = fmaf(red[w * PER + e], a, y), s = fmaf(ml[(w * ROWS + m) * 2 + 1], a, s);
         }
         const int d = DM::dim(n, l & 15);
         if (g.splits > 1) {
@@ -387,7 +360,7 @@ template <int NT, int RT, int VPR> __global__ __launch_bounds__(RT == 1 ? 512 : 
             g.part_o[at * D + d] = y;
             if (d == 0) g.part_ml[2 * at] = top, g.part_ml[2 * at + 1] = s;
         } else {
-            const int qi = q_row(m);
+            const int qi = m / g.group;
             g.O[b * g.o_bs + (int64_t)(kh * g.group + (m - qi * g.group)) * g.o_hs + qi * g.o_rs + d] = (half_t)(y / s); // no visible key: 0 / 0
         }
     }
@@ -404,28 +377,33 @@ template <int NT, int RT, int VPR> __global__ __launch_bounds__(RT == 1 ? 512 : 
 // The exponentials refer to the block's own maximum, or 2^8 below the row's where that is more: what rounding the probabilities to f16 costs is mostly the
 // error of the largest, and these are then exact.  The sum is that of the rounded probabilities.
 // ---------------------------------------------------------------------------------------------
-constexpr int AP_ROWS = 128, AP_KEYS = 64;
+constexpr int AP_ROWS = 128, AP_KEYS = 128; // of a workgroup's step
 typedef half_t half4_u __attribute__((ext_vector_type(4), aligned(2))); // outputs start anywhere
 typedef __fp16 aq_fp16x4 __attribute__((ext_vector_type(4)));
 
+// halves of a row of values in LDS, of a stage
+constexpr int aq_value_row(int nt) { return 16 * nt + (nt % 2 ? 0 : 16); }
+constexpr int aq_stage(int nt) { return AP_KEYS * (16 * nt + 8 + aq_value_row(nt)); }
+
 // MK: no mask tensor, an f32 one, an f16 one
-template <int NT, int MK> __global__ __launch_bounds__(256, 2) void attention_q4_tile_kernel(AttnQ4Args g) {
-    constexpr int D = 16 * NT, KK = (NT + 1) / 2, LD = D + 8, BLK = AP_KEYS * LD, RB = D / 2, SR = KK == 3 ? 4 : KK, DW = 2 * NT; // (DW: dwords of a row)
+template <int NT, int MK> __global__ __launch_bounds__(512, 2) void attention_q4_tile_kernel(AttnQ4Args g) {
+    constexpr int D = 16 * NT, KK = (NT + 1) / 2, RB = D / 2, SR = KK == 3 ? 4 : KK, DW = 2 * NT;            // (DW: dwords of a row)
+    constexpr int LD = D + 8, VD = aq_value_row(NT), KBLK = AP_KEYS * LD, STAGE = aq_stage(NT); // halves: a row of keys, of values; a block of keys, both
     extern __shared__ __attribute__((aligned(16))) uint8_t smem[];
-    half_t *const ring = (half_t *)smem;                         // [2][keys | values][64][LD]
-    uint32_t *const odd_flags = (uint32_t *)(ring + 4 * BLK);    // [2][wavefront]: whether the block has a scale of values that is not finite
+    half_t *const ring = (half_t *)smem;                          // [2][keys | values][128][LD | VD]
+    uint32_t *const odd_flags = (uint32_t *)(ring + 2 * STAGE);   // [2][wavefront]: whether the block has a scale of values that is not finite
     const int t = threadIdx.x, lane = t & 63, wave = __builtin_amdgcn_readfirstlane(t >> 6);
-    const int fr = lane & 15, fg = lane >> 4;
+    const int fr = lane & 15, fg = lane >> 4, rg = wave & 3, kg = wave >> 2; // group of rows, half of the keys
 
     // (head of keys, tile of rows, share of keys): XCD x takes the x-th eighth, so that a head's tiles share an L2; with the causal flag the long (late) tiles
-    // come first, and where every workgroup is resident at once (two per compute unit) the second half in the opposite order
+    // come first
     uint32_t lin = blockIdx.x, bk, tile, sp = 0;
     const uint32_t total = gridDim.x, nt = (uint32_t)g.row_tiles;
     const uint32_t chunk = total >> 3, rr = lin >> 3, x8 = lin & 7u;
     if ((total & 7u) == 0 && g.causal && g.splits == 1 && chunk % nt == 0) {
         const uint32_t hx = chunk / nt, q = rr / hx;
         bk = x8 * hx + (rr - q * hx);
-        tile = total <= (uint32_t)g.resident && nt % 2 == 0 && 2 * q >= nt ? q - nt / 2 : nt - 1 - q;
+        tile = nt - 1 - q;
     } else {
         if ((total & 7u) == 0) lin = x8 * chunk + rr;
         const uint32_t u = lin / (uint32_t)g.splits;
@@ -433,7 +411,7 @@ template <int NT, int MK> __global__ __launch_bounds__(256, 2) void attention_q4
         bk = u / nt, tile = u - bk * nt;
     }
     const int b = (int)bk / g.kv_heads, kh = (int)bk - b * g.kv_heads;
-    const int row0 = (int)tile * AP_ROWS, rw = row0 + 32 * wave; // first row of the workgroup, of the wavefront
+    const int row0 = (int)tile * AP_ROWS, rw = row0 + 32 * rg; // first row of the workgroup, of the wavefront
     int len = g.kv_len;
     if (g.lens) len = min(max(__builtin_amdgcn_readfirstlane(g.lens[b]), 0), len);
     const int off = len - g.q_len; // causal: query row i sees keys <= i + off
@@ -460,36 +438,46 @@ template <int NT, int MK> __global__ __launch_bounds__(256, 2) void attention_q4
         mrow[u] = (const half_t *)g.mask + (b * g.m_bs + qi * g.m_rs) * (MK == 1 ? 2 : 1);
     }
 
-    // ---- this thread's dwords of a block: number i is dword i * 256 + t of [keys | values][64][DW]
-    uint32_t raw[NT];
-    half_t ds[NT];
+    // ---- this thread's dwords of a block: number i is dword i * 512 + t of [keys | values][128][DW], at four times that from the block's first
+    uint32_t raw[NT], ds[NT], so[NT]; // (so: of its scale; the key is so / (2 SR))
+    auto is_key = [&](int i) { return 2 * i + 2 <= NT || (2 * i < NT && wave < 4); }; // (uniform)
+#pragma unroll
+    for (int i = 0; i < NT; i++) {
+        const int f = (i * 512 + t) % (256 * NT), key = f / DW;
+        so[i] = 2 * (key * SR + ((f - key * DW) >> 2));
+    }
     auto load = [&](int j0) __attribute__((always_inline)) {
+        const int n = min(AP_KEYS, len - j0); // past the last key the loads return zeros
+        const auto kr = aq_bounded(Kc + (int64_t)j0 * RB, n * RB), vr = aq_bounded(Vc + (int64_t)j0 * RB, n * RB);
+        const auto ksr = aq_bounded(Ks + (int64_t)j0 * SR, n * SR * 2), vsr = aq_bounded(Vs + (int64_t)j0 * SR, n * SR * 2);
 #pragma unroll
         for (int i = 0; i < NT; i++) {
-            const bool val = __builtin_amdgcn_readfirstlane(i * 256 + t) >= 128 * NT;
-            const int f = i * 256 + t - (val ? 128 * NT : 0), key = f / DW, w = f - key * DW;
-            const uint32_t j = (uint32_t)min(key, len - 1 - j0); // keys past the last repeat it: their scores are masked
-            raw[i] = *(const uint32_t *)((val ? Vc : Kc) + (int64_t)j0 * RB + (j * RB + 4 * w));
-            ds[i] = *((val ? Vs : Ks) + (int64_t)j0 * SR + (j * SR + (w >> 2)));
+            const int e = i * 512 + t;
+            if (is_key(i)) {
+                raw[i] = __builtin_amdgcn_raw_buffer_load_b32(kr, 4 * e, 0, 0), ds[i] = __builtin_amdgcn_raw_buffer_load_b16(ksr, so[i], 0, 0);
+            } else {
+                raw[i] = __builtin_amdgcn_raw_buffer_load_b32(vr, 4 * e - 1024 * NT, 0, 0), ds[i] = __builtin_amdgcn_raw_buffer_load_b16(vsr, so[i], 0, 0);
+            }
         }
     };
     const uint32_t bias = q40_bias();
     auto widen = [&](int stage) __attribute__((always_inline)) {
+        uint8_t *const st = (uint8_t *)(ring + stage * STAGE);
         bool odd = false;
 #pragma unroll
         for (int i = 0; i < NT; i++) {
-            const bool val = __builtin_amdgcn_readfirstlane(i * 256 + t) >= 128 * NT;
-            const int f = i * 256 + t - (val ? 128 * NT : 0), key = f / DW, w = f - key * DW;
-            half_t d = ds[i];
+            const bool val = !is_key(i);
+            const uint32_t f = (uint32_t)(i * 512 + t - (val ? 256 * NT : 0)), key = so[i] / (2 * SR);
+            half_t d = __builtin_bit_cast(half_t, (uint16_t)ds[i]);
             if (val) { // a value that is not finite shows in the rows that see its key, and not through the matrix cores
-                const bool fin = (__builtin_bit_cast(uint16_t, d) & 0x7C00u) != 0x7C00u;
+                const bool fin = (ds[i] & 0x7C00u) != 0x7C00u;
                 odd |= !fin;
                 d = fin ? d : (half_t)0.f;
             }
-            *(half8_t *)(ring + stage * 2 * BLK + (val ? BLK : 0) + key * LD + 8 * w) = q40_codes(raw[i], bias) * half8_t{d, d, d, d, d, d, d, d};
+            *(half8_t *)(st + 16 * f + (val ? 2 * KBLK + (VD - D) * 2 * key : (LD - D) * 2 * key)) = q40_codes(raw[i], bias) * half8_t{d, d, d, d, d, d, d, d};
         }
         const bool any = __builtin_amdgcn_ballot_w64(odd) != 0;
-        if (lane == 0) odd_flags[4 * stage + wave] = any;
+        if (lane == 0) odd_flags[8 * stage + wave] = any;
     };
     using MT = std::conditional_t<MK == 1, float, half_t>;
     typedef MT mask4_t __attribute__((ext_vector_type(4)));
@@ -501,7 +489,7 @@ template <int NT, int MK> __global__ __launch_bounds__(256, 2) void attention_q4
 #pragma unroll
             for (int u = 0; u < 2; u++) {
                 const MT *p = (const MT *)mrow[u];
-                if (j0 + AP_KEYS <= len) { // uniform
+                if (j0 + 64 <= len) { // uniform
 #pragma unroll
                     for (int bt = 0; bt < 4; bt++) mk[u][bt] = *(const mask4_u *)(p + j0 + 16 * bt + 4 * fg);
                 } else {
@@ -513,23 +501,23 @@ template <int NT, int MK> __global__ __launch_bounds__(256, 2) void attention_q4
     };
 
     float4_t acc[2][NT];
-    float m_run[2], m_top[2], l_run[2]; // base 2: the exponentials' reference and the maximum so far; this lane's share of the sum
+    float m_run[2], l_run[2]; // base 2: the exponentials' reference; this lane's share of the sum
     uint32_t bad[2];
 #pragma unroll
     for (int u = 0; u < 2; u++) {
-        m_run[u] = m_top[u] = -INFINITY, l_run[u] = 0.f, bad[u] = 0;
+        m_run[u] = -INFINITY, l_run[u] = 0.f, bad[u] = 0;
 #pragma unroll
         for (int d = 0; d < NT; d++) acc[u][d] = float4_t{0.f, 0.f, 0.f, 0.f};
     }
     int koff[KK];
 #pragma unroll
-    for (int kk = 0; kk < KK; kk++) koff[kk] = fr * LD + 8 * min(4 * kk + fg, DW - 1);
-    const int voff = BLK + (4 * fg + (fr >> 2)) * LD + 4 * (fr & 3);
+    for (int kk = 0; kk < KK; kk++) koff[kk] = (64 * kg + fr) * LD + 8 * min(4 * kk + fg, DW - 1);
+    const int voff = KBLK + (64 * kg + 4 * fg + (fr >> 2)) * VD + 4 * (fr & 3);
 
     auto step = [&](int stage, int j0, auto lean_c) __attribute__((always_inline)) {
         constexpr bool LEAN = decltype(lean_c)::value;
-        const half_t *const st = ring + stage * 2 * BLK;
-        const uint4_t fl = *(const uint4_t *)(odd_flags + 4 * stage);
+        const half_t *const st = ring + stage * STAGE;
+        const uint4_t fl = *(const uint4_t *)(odd_flags + 8 * stage), fh = *(const uint4_t *)(odd_flags + 8 * stage + 4);
         load_mask(j0);
         float4_t S[2][4];
 #pragma unroll
@@ -544,7 +532,7 @@ template <int NT, int MK> __global__ __launch_bounds__(256, 2) void attention_q4
 #pragma unroll
                 for (int u = 0; u < 2; u++) S[u][bt] = __builtin_amdgcn_mfma_f32_16x16x32_f16(fk[kk], fq[u][kk], S[u][bt], 0, 0, 0);
         }
-        const bool odd = __builtin_amdgcn_readfirstlane((int)(fl[0] | fl[1] | fl[2] | fl[3])) != 0;
+        const bool odd = __builtin_amdgcn_readfirstlane((int)(fl[0] | fl[1] | fl[2] | fl[3] | fh[0] | fh[1] | fh[2] | fh[3])) != 0;
         half8_t fp[2][2];
 #pragma unroll
         for (int u = 0; u < 2; u++) {
@@ -580,11 +568,15 @@ template <int NT, int MK> __global__ __launch_bounds__(256, 2) void attention_q4
                 }
             }
             bmax = rt_groups_max(bmax);
-            m_top[u] = fmaxf(m_top[u], bmax);
-            const float m_new = fmaxf(m_top[u] - 8.f, bmax);
-            const float m_use = m_new == -INFINITY ? 0.f : m_new; // a row without a key yet: exp2(-inf - 0) = 0
-            const float alpha = __builtin_amdgcn_exp2f(m_run[u] - m_use);
-            m_run[u] = m_new;
+            // the reference follows the maximum only where that is 2^8 past it (or it has none): the outputs and the sum are seldom rescaled
+            if (__builtin_amdgcn_ballot_w64(bmax > m_run[u] + 8.f)) {
+                const float m_new = fmaxf(m_run[u], bmax), alpha = m_new == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(m_run[u] - m_new);
+                m_run[u] = m_new;
+                l_run[u] *= alpha;
+#pragma unroll
+                for (int d = 0; d < NT; d++) acc[u][d] *= alpha;
+            }
+            const float m_use = m_run[u] == -INFINITY ? 0.f : m_run[u]; // a row without a key yet: exp2(-inf - 0) = 0
             const float sc = LEAN && MK == 0 ? g.scale_log2e : 1.f;
             float psum = 0.f;
 #pragma unroll
@@ -594,9 +586,7 @@ template <int NT, int MK> __global__ __launch_bounds__(256, 2) void attention_q4
                 psum = __builtin_amdgcn_fdot2(p, half2_t{(half_t)1, (half_t)1}, psum, false);
                 fp[u][e >> 3][e & 7] = p[0], fp[u][e >> 3][(e & 7) + 1] = p[1];
             }
-            l_run[u] = l_run[u] * alpha + psum;
-#pragma unroll
-            for (int d = 0; d < NT; d++) acc[u][d] *= alpha;
+            l_run[u] += psum;
         }
 #pragma unroll
         for (int hh = 0; hh < 2; hh++)
@@ -604,9 +594,9 @@ template <int NT, int MK> __global__ __launch_bounds__(256, 2) void attention_q4
             for (int d = 0; d < NT; d++) {
                 typedef uint64_t u64x2_t __attribute__((ext_vector_type(2)));
                 typedef __attribute__((address_space(3))) aq_fp16x4 *lds4;
-                const half_t *vp = st + voff + 16 * d + 32 * hh * LD;
+                const half_t *vp = st + voff + 16 * d + 32 * hh * VD;
                 const uint64_t v0 = __builtin_bit_cast(uint64_t, __builtin_amdgcn_ds_read_tr16_b64_v4f16((lds4)vp));
-                const uint64_t v1 = __builtin_bit_cast(uint64_t, __builtin_amdgcn_ds_read_tr16_b64_v4f16((lds4)(vp + 16 * LD)));
+                const uint64_t v1 = __builtin_bit_cast(uint64_t, __builtin_amdgcn_ds_read_tr16_b64_v4f16((lds4)(vp + 16 * VD)));
                 const half8_t fv = __builtin_bit_cast(half8_t, u64x2_t{v0, v1});
 #pragma unroll
                 for (int u = 0; u < 2; u++) acc[u][d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(fv, fp[u][hh], acc[u][d], 0, 0, 0);
@@ -618,6 +608,7 @@ template <int NT, int MK> __global__ __launch_bounds__(256, 2) void attention_q4
         widen(0);
         __syncthreads();
         int stage = 0, j0 = j_first;
+        const int kj = 64 * kg; // this wavefront's keys
         auto turn = [&](auto body) __attribute__((always_inline)) {
             const bool more = j0 + AP_KEYS < j_end;
             if (more) load(j0 + AP_KEYS);
@@ -628,26 +619,48 @@ template <int NT, int MK> __global__ __launch_bounds__(256, 2) void attention_q4
             __syncthreads();
             stage ^= 1, j0 += AP_KEYS;
         };
-        while (j0 + AP_KEYS <= w_lean) turn([&]() { step(stage, j0, std::true_type{}); });
-        while (j0 < w_end) turn([&]() { step(stage, j0, std::false_type{}); });
+        while (j0 + kj + 64 <= w_lean) turn([&]() { step(stage, j0 + kj, std::true_type{}); });
+        while (j0 + kj < w_end) turn([&]() { step(stage, j0 + kj, std::false_type{}); });
         while (j0 < j_end) turn([]() {}); // blocks that only other wavefronts need
     }
+    // ---- the two halves of the keys through LDS: [group of rows][tile of 16][dimensions' tile][lane] four, and references, sums, flags
 #pragma unroll
     for (int u = 0; u < 2; u++) {
-        const int m = rw + 16 * u + fr;
-        const float l = rt_groups_sum(l_run[u]);
-        uint32_t bd = bad[u];
-        bd |= (uint32_t)__shfl_xor((int)bd, 16);
-        bd |= (uint32_t)__shfl_xor((int)bd, 32);
-        if (bd) {
+        l_run[u] = rt_groups_sum(l_run[u]);
+        bad[u] |= (uint32_t)__shfl_xor((int)bad[u], 16);
+        bad[u] |= (uint32_t)__shfl_xor((int)bad[u], 32);
+    }
+    float4_t *const rest = (float4_t *)smem;
+    float *const sums = (float *)(rest + 8 * NT * 64);
+    if (kg == 1) {
 #pragma unroll
-            for (int d = 0; d < NT; d++)
-                if ((bd >> (d >> 1)) & 1u) acc[u][d] = float4_t{1.f, 1.f, 1.f, 1.f} * __builtin_nanf("");
+        for (int u = 0; u < 2; u++) {
+#pragma unroll
+            for (int d = 0; d < NT; d++) rest[((2 * rg + u) * NT + d) * 64 + lane] = acc[u][d];
+            float *const p = sums + (2 * rg + u) * 192 + lane;
+            p[0] = m_run[u], p[64] = l_run[u], p[128] = __builtin_bit_cast(float, bad[u]);
         }
+    }
+    __syncthreads();
+    if (kg == 1) return;
+#pragma unroll
+    for (int u = 0; u < 2; u++) {
+        const float *const p = sums + (2 * rg + u) * 192 + lane;
+        const float m1 = p[0], top = fmaxf(m_run[u], m1), base = top == -INFINITY ? 0.f : top;
+        const float a0 = __builtin_amdgcn_exp2f(m_run[u] - base), a1 = __builtin_amdgcn_exp2f(m1 - base), l = l_run[u] * a0 + p[64] * a1;
+        const uint32_t bd = bad[u] | __builtin_bit_cast(uint32_t, p[128]);
+#pragma unroll
+        for (int d = 0; d < NT; d++) {
+            const float4_t r = rest[((2 * rg + u) * NT + d) * 64 + lane];
+#pragma unroll
+            for (int k = 0; k < 4; k++) acc[u][d][k] = fmaf(acc[u][d][k], a0, r[k] * a1);
+            if ((bd >> (d >> 1)) & 1u) acc[u][d] = float4_t{1.f, 1.f, 1.f, 1.f} * __builtin_nanf("");
+        }
+        const int m = rw + 16 * u + fr;
         if (m >= g.rows) continue;
         if (g.splits > 1) {
             const int64_t at = ((int64_t)bk * g.rows + m) * g.splits + sp;
-            if (fg == 0) *(float2_t *)(g.part_ml + 2 * at) = float2_t{m_run[u], l};
+            if (fg == 0) *(float2_t *)(g.part_ml + 2 * at) = float2_t{top, l};
             if (j_first < j_end) { // (a share with a sum of 0 is not read)
 #pragma unroll
                 for (int d = 0; d < NT; d++) *(float4_t *)(g.part_o + at * D + 16 * d + 4 * fg) = acc[u][d];
@@ -710,20 +723,21 @@ template <int CG> __global__ __launch_bounds__(256) void attention_q4_merge_kern
 }
 
 // the two kernels: rows of a tile, and the keys that shares are counted in
-static bool aq_streams(int rows) { return rows <= 16; }
+RT_TUNABLE(g_aq_stream_rows, 16);
+RT_TUNABLE(g_aq_waves, 8);
+RT_TUNABLE(g_aq_target, 256);
+RT_TUNABLE(g_aq_least, 1);
+static bool aq_streams(int rows) { return rows <= g_aq_stream_rows; }
 static int64_t aq_row_tiles(int rows) { return aq_streams(rows) ? 1 : (rows + AP_ROWS - 1) / AP_ROWS; }
-RT_TUNABLE(g_aq_target, 512);
-RT_TUNABLE(g_aq_least, 128);
 // keys of a workgroup where several share a row tile's, and how many do
 static void aq_split(const rt_attention_q4_desc &d, int &splits, int &split_keys) {
     const int rows = d.q_len * (d.heads / d.kv_heads);
     const int64_t wgs = (int64_t)d.batch * d.kv_heads * aq_row_tiles(rows);
-    const int step = aq_streams(rows) ? 512 : g_aq_least; // of a workgroup's eight wavefronts; two blocks
-    const int steps = (d.kv_len + step - 1) / step;
-    int s = 1;
-    if (wgs < g_aq_target && steps > 1) s = (int)std::min<int64_t>(std::min(steps, AQ_MAX_SPLITS), aq_streams(rows) ? (g_aq_target + wgs - 1) / wgs : g_aq_target / wgs);
-    const int per = (steps + s - 1) / s;
-    splits = std::max(1, (steps + per - 1) / std::max(per, 1)), split_keys = std::max(per, 1) * step;
+    const int unit = aq_streams(rows) ? 64 * g_aq_waves : AP_KEYS;
+    const int steps = (d.kv_len + unit - 1) / unit;
+    int64_t s = std::min<int64_t>(AQ_MAX_SPLITS, std::min<int64_t>(steps / g_aq_least, g_aq_target / wgs));
+    const int per = s > 1 ? (int)((steps + s - 1) / s) : std::max(steps, 1);
+    splits = std::max(1, (steps + per - 1) / per), split_keys = per * unit;
 }
 
 uint64_t attention_q4_workspace_bytes(const rt_attention_q4_desc &d) {
@@ -734,23 +748,23 @@ uint64_t attention_q4_workspace_bytes(const rt_attention_q4_desc &d) {
     return (uint64_t)d.batch * d.heads * d.q_len * splits * (d.head_dim + 2) * sizeof(float);
 }
 
-template <int NT, int RT, int VPR> static hipError_t launch_aq(const AttnQ4Args &g, dim3 grid, int waves, hipStream_t st) {
+template <int NT, int VPR, int MK> static hipError_t launch_aq(const AttnQ4Args &g, dim3 grid, hipStream_t st) {
     using DM = AqDims<NT>;
-    constexpr int ROWS = RT == 1 ? 4 * VPR : 16 * RT;
-    const size_t wave = (ROWS * 72 + DM::NB * 64) * 2, out = ((size_t)RT * NT * VPR * 64 + 2 * ROWS) * sizeof(float);
-    const size_t lds = waves * std::max(wave, out);
-    if (const hipError_t e = ensure_lds_limit<&attention_q4_kernel<NT, RT, VPR>>(); e != hipSuccess) return e;
-    hipLaunchKernelGGL((attention_q4_kernel<NT, RT, VPR>), grid, dim3(64 * waves), lds, st, g);
+    constexpr int ROWS = 4 * VPR;
+    const size_t wave = (ROWS * 72 + DM::NB * 64) * 2, out = ((size_t)DM::T * VPR * 64 + 2 * ROWS) * sizeof(float);
+    const size_t lds = g_aq_waves * std::max(wave, out);
+    if (const hipError_t e = ensure_lds_limit<&attention_q4_kernel<NT, VPR, MK>>(); e != hipSuccess) return e;
+    hipLaunchKernelGGL((attention_q4_kernel<NT, VPR, MK>), grid, dim3(64 * g_aq_waves), lds, st, g);
     return hipGetLastError();
 }
 template <int NT> static hipError_t launch_aq_rows(const AttnQ4Args &g, dim3 grid, hipStream_t st) {
-    if (g.rows <= 4) return launch_aq<NT, 1, 1>(g, grid, 8, st);
-    return launch_aq<NT, 1, 4>(g, grid, 8, st);
+    if (g.rows <= 4) return g.mask ? launch_aq<NT, 1, 1>(g, grid, st) : launch_aq<NT, 1, 0>(g, grid, st);
+    return g.mask ? launch_aq<NT, 4, 1>(g, grid, st) : launch_aq<NT, 4, 0>(g, grid, st);
 }
 template <int NT, int MK> static hipError_t launch_aq_tile(const AttnQ4Args &g, unsigned wgs, hipStream_t st) {
-    constexpr size_t lds = (size_t)4 * AP_KEYS * (16 * NT + 8) * sizeof(half_t) + 8 * sizeof(uint32_t);
+    constexpr size_t ring = (size_t)2 * aq_stage(NT) * sizeof(half_t) + 16 * sizeof(uint32_t), halves = (size_t)8 * (NT * 64 * 16 + 192 * 4), lds = ring > halves ? ring : halves;
     if (const hipError_t e = ensure_lds_limit<&attention_q4_tile_kernel<NT, MK>>(); e != hipSuccess) return e;
-    hipLaunchKernelGGL((attention_q4_tile_kernel<NT, MK>), dim3(wgs), dim3(256), lds, st, g);
+    hipLaunchKernelGGL((attention_q4_tile_kernel<NT, MK>), dim3(wgs), dim3(512), lds, st, g);
     return hipGetLastError();
 }
 
@@ -775,7 +789,7 @@ hipError_t launch_attention_q4(const rt_attention_q4_desc &d, const void *q, con
         g.splits = 1, g.split_keys = std::max(d.kv_len, 1);
     }
     const int64_t tiles = aq_row_tiles(g.rows), stacks = (int64_t)d.batch * d.kv_heads;
-    g.row_tiles = (int)tiles, g.resident = 2 * dev.num_cus;
+    g.row_tiles = (int)tiles;
     if (tiles * stacks * g.splits > 0xffffff || (g.splits > 1 && stacks * g.rows > 0xffffff)) return hipErrorNotSupported; // (a grid's threads along an axis are fewer than 2^32)
     const dim3 grid((unsigned)g.splits, (unsigned)stacks);
     auto go = [&](auto nt) -> hipError_t {

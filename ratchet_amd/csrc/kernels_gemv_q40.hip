@@ -48,29 +48,8 @@ struct GemvQ40Args {
 
 typedef uint64_t uint64_a2 __attribute__((aligned(2)));
 
-// lane group g's register t <- lane group t's register g
-__device__ __forceinline__ void q40_transpose(uint4_t &v) {
-    const auto a = __builtin_amdgcn_permlane16_swap(v[0], v[1], false, false);
-    const auto b = __builtin_amdgcn_permlane16_swap(v[2], v[3], false, false);
-    const auto c = __builtin_amdgcn_permlane32_swap(a[0], b[0], false, false);
-    const auto d = __builtin_amdgcn_permlane32_swap(a[1], b[1], false, false);
-    v = uint4_t{c[0], d[0], c[1], d[1]};
-}
-
 // floats between activation rows of sums in LDS: a multiple of 4 that keeps a wavefront's four rows of 16 apart
 __host__ __device__ constexpr int q40_ld(int rows) { return rows + 4; }
-
-// a dword of lane group u -> all lane groups, for u below UC (2: lane groups 2 and 3 have what 0 and 1 have)
-template <int UC> __device__ __forceinline__ void q40_spread(uint32_t x, uint32_t *to) {
-    if constexpr (UC == 2) {
-        const auto a = __builtin_amdgcn_permlane16_swap(x, x, false, false); // lane groups 0 0 2 2, and 1 1 3 3
-        to[0] = a[0], to[1] = a[1];
-    } else {
-        const auto h = __builtin_amdgcn_permlane32_swap(x, x, false, false); // 0 1 0 1, and 2 3 2 3
-        const auto a = __builtin_amdgcn_permlane16_swap(h[0], h[0], false, false), b = __builtin_amdgcn_permlane16_swap(h[1], h[1], false, false);
-        to[0] = a[0], to[1] = a[1], to[2] = b[0], to[3] = b[1];
-    }
-}
 
 // MT: groups of 16 activation rows; VPR: result registers in use (1, 2 or 4; 4 with MT > 1); XI: pieces of a panel's activations per
 // thread, at least NV UC / (4 wr); UC: chunks of 128 in a unit of K (4, or 2 where registers are short); DEPTH: panels of weights in flight
