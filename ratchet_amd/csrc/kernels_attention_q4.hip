@@ -11,14 +11,18 @@
 // Softmax: running maximum and sum in f32, base 2; a row's keys are spread over 16 lanes, which four DPP rotations join for the maximum, and only at
 // the end for the sum.
 // Values: the operand of the second product holds, for one dimension, eight keys in a lane.  Codes of one key are neighbours along the dimensions, so
-// lane c (of 16) reads a dword (half, byte, nibble for what is left of head_dim) of each key's row, and a byte permutation of two keys' puts the same
-// nibble of both into the two halves of a register: the unpacking of q40_codes with pairs of keys in place of pairs of dimensions.  The
+// lane c (of 16) reads four bytes of each key's row (two up to a head_dim of 64, one up to 32; a row of 80 takes ten lanes, which costs less than the second load
+// that would occupy all), and a byte permutation of two keys' puts the same nibble of both into the two halves of a register: the unpacking of q40_codes with pairs of keys in place of pairs of dimensions.  The
 // order of keys in that product is free: 4 r + s is key 16 s + r, so that a lane's four probabilities are neighbours.  dv (q - 8) is exact in f16 for
 // scales of eight significant bits, which is what the cache's write makes (others round here); dv = 0 past the last key.  The probabilities enter as
 // f16, as in kernels_attention.hip.
 //
 // Wavefronts of a workgroup take 64 keys in turn and are merged through LDS; where there are few heads several workgroups share the keys and a second
 // kernel merges them, in a fixed order.
+//
+// 32 sequences of 8192 keys, 8 heads of 128, one row of 32 heads: 62 us, 4.8 TB/s, which is what a copy reaches; of lengths between, whose longest bounds it, 50.
+// Small ones wait: 32768 keys of one sequence 16 us (7.4 at a copy's rate) in a launch, a trip to memory and two steps of 1.7 us in which two wavefronts of a SIMD unpack
+// (500 instructions for 64 keys), and 3 of the second launch.
 #include "device_common.h"
 
 #include <algorithm>
@@ -27,7 +31,8 @@
 namespace rt {
 
 constexpr float kLog2eQ4 = 1.4426950408889634f;
-constexpr int AQ_MAX_SPLITS = 64; // a lane of the merge for each
+constexpr int AQ_MAX_SPLITS = 64; // shares of a row
+constexpr int AQ_WAVES = 8;       // of a streaming workgroup
 
 struct AttnQ4Args {
     const half_t *Q;
@@ -79,14 +84,15 @@ __device__ __forceinline__ __amdgpu_buffer_rsrc_t aq_bounded(const void *p, int 
     return __builtin_amdgcn_make_buffer_rsrc(const_cast<void *>(p), 0, bytes, 0x00027000); // raw, 32-bit data
 }
 
-// VPR: result registers in use (1: up to 4 rows, 4: up to 16).  MK: a mask tensor
+// VPR: result registers in use (1: up to 4 rows, 2: up to 8, 4: up to 16).  MK: a mask tensor
 template <int NT, int VPR, int MK> __global__ __launch_bounds__(512) void attention_q4_kernel(AttnQ4Args g) {
     using DM = AqDims<NT>;
     constexpr int D = DM::D, NF = DM::NF, TAIL = DM::TAIL, NB = DM::NB, SR = DM::SR, SW = (SR + 1) / 2, RB = DM::RB, W = DM::W, T = DM::T;
     constexpr int ROWS = 4 * VPR, PS = 72; // halves between rows of probabilities
     constexpr int WAVE_LDS = (ROWS * PS + NB * 64) * 2;
     extern __shared__ __attribute__((aligned(16))) uint8_t smem[];
-    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), waves = blockDim.x >> 6;
+    constexpr int waves = AQ_WAVES;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int r = lane & 15, fg = lane >> 4, cc = min(r, DM::CL - 1);
     half_t *P = (half_t *)(smem + wave * WAVE_LDS), *S = P + ROWS * PS; // this wavefront's: probabilities [row][position], scales of values [block][position]
     const int bk = blockIdx.y, b = bk / g.kv_heads, kh = bk - b * g.kv_heads;
@@ -116,25 +122,31 @@ template <int NT, int VPR, int MK> __global__ __launch_bounds__(512) void attent
         if constexpr (TAIL) qf[NF] = fg < 2 ? *(const half8_t *)(q + 32 * NF) : half8_t{};
     }
 
-    // ---- 64 keys' loads
+    // ---- 64 keys' loads, the wavefront's next
+    const int step = 64 * waves;
     struct Unit {
         uint4_t kc[NF + TAIL];
         uint32_t dk[SW], dv[SW]; // lane group fg has the scales of keys 16 fg + r
         uint32_t v[2][8];
     };
-    uint32_t ko[NF ? NF : 1];
+    // offsets of this lane's loads in 32 bits from the first key of a window of 2^24: pieces of 16 bytes of keys (a constant apart but where a key has three), a
+    // block of 16, scales, values
+    uint32_t ko[DM::PB == 3 ? 3 : 1], kt, so, vo;
+    __amdgpu_buffer_rsrc_t kr, vr, ksr, vsr;
+    auto window = [&](int j0, int j1) __attribute__((always_inline)) { // the keys j0 .. j1 - 1; this wavefront's start 64 wave behind
 #pragma unroll
-    for (int i = 0; i < NF; i++) {
-        const int pc = 4 * i + fg, ks = pc / DM::PB, kb = pc - ks * DM::PB; // piece: key set and block
-        ko[i] = (16 * ks + r) * RB + 16 * kb;
-    }
-    const uint32_t kt = lane * RB + 16 * NF, so = lane * SR * 2, vo = 2 * fg * RB + W * cc;
-    auto load = [&](int j0, Unit &k) __attribute__((always_inline)) {
-        const int n = max(0, min(64, j_end - j0));
-        const int64_t at = min(j0, max(j_end - 1, 0)); // (of nothing where n is 0)
-        const auto kr = aq_bounded(Kc + at * RB, n * RB), vr = aq_bounded(Vc + at * RB, n * RB), ksr = aq_bounded(Ks + at * SR, n * SR * 2), vsr = aq_bounded(Vs + at * SR, n * SR * 2);
+        for (int i = 0; i < (DM::PB == 3 ? 3 : 1); i++) {
+            const int pc = 4 * i + fg, ks = pc / DM::PB, kb = pc - ks * DM::PB; // piece: key set and block
+            ko[i] = (64 * wave + 16 * ks + r) * RB + 16 * kb;
+        }
+        kt = (64 * wave + lane) * RB + 16 * NF, so = (64 * wave + lane) * SR * 2, vo = (64 * wave + 2 * fg) * RB + W * cc;
+        kr = aq_bounded(Kc + (int64_t)j0 * RB, (j1 - j0) * RB), vr = aq_bounded(Vc + (int64_t)j0 * RB, (j1 - j0) * RB);
+        ksr = aq_bounded(Ks + (int64_t)j0 * SR, (j1 - j0) * SR * 2), vsr = aq_bounded(Vs + (int64_t)j0 * SR, (j1 - j0) * SR * 2);
+    };
+    auto load = [&](Unit &k) __attribute__((always_inline)) {
 #pragma unroll
-        for (int i = 0; i < NF; i++) k.kc[i] = __builtin_bit_cast(uint4_t, __builtin_amdgcn_raw_buffer_load_b128(kr, ko[i], 0, 0));
+        for (int i = 0; i < NF; i++)
+            k.kc[i] = __builtin_bit_cast(uint4_t, DM::PB == 3 ? __builtin_amdgcn_raw_buffer_load_b128(kr, ko[i], 0, 0) : __builtin_amdgcn_raw_buffer_load_b128(kr, ko[0] + i * (64 / DM::PB) * RB, 0, 0));
         if constexpr (TAIL) {
             const uint2_t w = __builtin_bit_cast(uint2_t, __builtin_amdgcn_raw_buffer_load_b64(kr, kt, 0, 0));
             k.kc[NF] = uint4_t{w[0], w[1], 0, 0};
@@ -157,6 +169,9 @@ template <int NT, int VPR, int MK> __global__ __launch_bounds__(512) void attent
                 else if constexpr (W == 2) k.v[u][e] = __builtin_amdgcn_raw_buffer_load_b16(vr, o, 0, 0);
                 else k.v[u][e] = __builtin_amdgcn_raw_buffer_load_b8(vr, o, 0, 0);
             }
+#pragma unroll
+        for (int i = 0; i < (DM::PB == 3 ? 3 : 1); i++) ko[i] += step * RB;
+        kt += step * RB, so += step * SR * 2, vo += step * RB;
     };
     uint32_t mk[MK ? VPR : 1][4]; // the block's mask values, as they are; requested before the next block's loads, so that nothing waits for those
     auto load_mask = [&](int j0) __attribute__((always_inline)) {
@@ -192,11 +207,20 @@ template <int NT, int VPR, int MK> __global__ __launch_bounds__(512) void attent
         for (int s = 0; s < 4; s++)
 #pragma unroll
             for (int v = 0; v < VPR; v++) sc[s][v] = 0.f;
-        auto block = [&](uint32_t w, int s, int n) __attribute__((always_inline)) {
-            const float d = (float)__builtin_bit_cast(half2_t, dk[n >> 1][s])[n & 1];
-            const float4_t p = __builtin_amdgcn_mfma_f32_16x16x32_f16(qf[n], q40_codes(w, bias), float4_t{0.f, 0.f, 0.f, 0.f}, 0, 0, 0);
+        // a block's sums are folded behind the next block's instructions: left alone the compiler waits for the matrix cores after each
+        float4_t part = {0.f, 0.f, 0.f, 0.f};
+        float scale = 0.f;
+        int set = 0;
+        auto fold = [&]() __attribute__((always_inline)) {
+            asm volatile("" : "+v"(part));
 #pragma unroll
-            for (int v = 0; v < VPR; v++) sc[s][v] = fmaf(d, p[v], sc[s][v]);
+            for (int v = 0; v < VPR; v++) sc[set][v] = fmaf(scale, part[v], sc[set][v]);
+        };
+        auto block = [&](uint32_t w, int s, int n) __attribute__((always_inline)) {
+            const float4_t now = __builtin_amdgcn_mfma_f32_16x16x32_f16(qf[n], q40_codes(w, bias), float4_t{0.f, 0.f, 0.f, 0.f}, 0, 0, 0);
+            fold();
+            part = now, scale = (float)__builtin_bit_cast(half2_t, dk[n >> 1][s])[n & 1], set = s;
+            __builtin_amdgcn_sched_barrier(0);
         };
 #pragma unroll
         for (int i = 0; i < NF; i++) {
@@ -209,6 +233,7 @@ template <int NT, int VPR, int MK> __global__ __launch_bounds__(512) void attent
 #pragma unroll
             for (int s = 0; s < 4; s++) block(k.kc[NF][s], s, NF);
         }
+        fold();
 
         // ---- mask, running maximum and sum, probabilities to LDS
         const bool inside = j0 + 64 <= whole; // no key hidden
@@ -299,25 +324,28 @@ template <int NT, int VPR, int MK> __global__ __launch_bounds__(512) void attent
     };
 
     // 64 keys are multiplied while the wavefront's next 64 are on their way
-    const int step = 64 * waves;
-    int j0 = j_first + 64 * wave;
+    constexpr int WINDOW = 1 << 24;
     Unit ring[2];
-    if (j0 < j_end) {
-        load(j0, ring[0]);
-        __builtin_amdgcn_sched_barrier(0);
 #pragma unroll 1
-        for (; j0 + step < j_end; j0 += 2 * step) {
-            auto turn = [&](int j, Unit &now, Unit &next) __attribute__((always_inline)) {
-                load_mask(j);
-                load(j + step, next);
-                __builtin_amdgcn_sched_barrier(0);
-                multiply(j, now);
-                __builtin_amdgcn_sched_barrier(0);
-            };
+    for (int w0 = j_first; w0 < j_end; w0 += WINDOW) {
+        const int w1 = min(j_end - w0, WINDOW) + w0;
+        window(w0, w1);
+        int j0 = w0 + 64 * wave;
+        load(ring[0]);
+        __builtin_amdgcn_sched_barrier(0);
+        auto turn = [&](int j, Unit &now, Unit &next) __attribute__((always_inline)) {
+            load_mask(j);
+            load(next); // (past the end: zeros)
+            __builtin_amdgcn_sched_barrier(0);
+            multiply(j, now);
+            __builtin_amdgcn_sched_barrier(0);
+        };
+#pragma unroll 1
+        for (; j0 + step < w1; j0 += 2 * step) {
             turn(j0, ring[0], ring[1]);
             turn(j0 + step, ring[1], ring[0]);
         }
-        if (j0 < j_end) load_mask(j0), multiply(j0, ring[0]);
+        if (j0 < w1) load_mask(j0), multiply(j0, ring[0]);
     }
 
     // ---- this wavefront's rows: the sum over the 16 lanes, and what a scale that is not finite leaves
@@ -678,66 +706,85 @@ template <int NT, int MK> __global__ __launch_bounds__(512, 2) void attention_q4
     }
 }
 
-// Joins the shares of a row, four columns a thread.  A row's threads are CG = D / 4 to the next power of two columns by SG groups of shares, all of whose loads are
-// requested at once; the groups meet in LDS, in a fixed order.  (One thread a column that walked the shares took 20.9 us for 32 rows of 64 shares of 128.)
-template <int CG> __global__ __launch_bounds__(256) void attention_q4_merge_kernel(AttnQ4Args g, int D) {
-    constexpr int SG = 256 / CG, PER = (AQ_MAX_SPLITS + SG - 1) / SG;
-    __shared__ __attribute__((aligned(16))) float part[SG][4 * CG];
-    const int64_t row = blockIdx.x;
-    const int t = threadIdx.x, lane = t & 63, c = t % CG, sg = t / CG;
+// Joins the shares of a row, four columns a thread: CG threads have the columns of a row, SG groups of them its shares, and the workgroup 256 / (CG SG) rows.  All
+// loads are requested at once, and the groups meet in LDS, in a fixed order.  (One thread a column that walked the shares took 20.9 us for 32 rows of 64 shares
+// of 128, this 2.9; 4800 rows of 6 shares of 64 with 16 groups, ten of them idle, and a row a workgroup 7.0.)
+template <int CG, int SG> __global__ __launch_bounds__(256) void attention_q4_merge_kernel(AttnQ4Args g, int D, int64_t rows) {
+    constexpr int R = 256 / (CG * SG), PER = SG < 8 ? 1 : AQ_MAX_SPLITS / SG; // (four groups: up to four shares)
+    __shared__ __attribute__((aligned(16))) float part[R][SG][4 * CG];
+    const int t = threadIdx.x, c = t % CG, sg = t / CG % SG, rl = t / (CG * SG);
+    const int64_t row = min((int64_t)blockIdx.x * R + rl, rows - 1);
     const bool live = 4 * c < D;
-    const float *const po = g.part_o + row * g.splits * D + (live ? 4 * c : 0);
+    const float *const po = g.part_o + row * g.splits * D + (live ? 4 * c : 0), *const pm = g.part_ml + row * g.splits * 2;
     float4_t v[PER];
+    float2_t ml[PER];
 #pragma unroll
     for (int i = 0; i < PER; i++)
-        if (i * SG < g.splits) v[i] = *(const float4_t *)(po + (int64_t)min(i * SG + sg, g.splits - 1) * D);
-    // lane s has share s's weight
-    const float2_t ml = *(const float2_t *)(g.part_ml + (row * g.splits + min(lane, g.splits - 1)) * 2);
-    float top = ml[0];
+        if (i * SG < g.splits) { // (uniform)
+            const int s = min(i * SG + sg, g.splits - 1);
+            ml[i] = *(const float2_t *)(pm + 2 * s), v[i] = *(const float4_t *)(po + (int64_t)s * D);
+        }
+    // this group's shares; one whose sum is 0 has no key, and no outputs were written
+    float top = -INFINITY;
 #pragma unroll
-    for (int x = 1; x < 64; x *= 2) top = fmaxf(top, __shfl_xor(top, x));
+    for (int i = 0; i < PER; i++)
+        if (i * SG < g.splits) top = fmaxf(top, ml[i][0]);
     const float base = top == -INFINITY ? 0.f : top;
-    const float a = lane < g.splits && ml[1] != 0.f ? __builtin_amdgcn_exp2f(ml[0] - base) : 0.f; // (a share without a key: nothing to read)
-    float l = lane < g.splits && ml[1] != 0.f ? a * ml[1] : 0.f;
-#pragma unroll
-    for (int x = 1; x < 64; x *= 2) l += __shfl_xor(l, x);
-    const uint64_t some = __builtin_amdgcn_ballot_w64(lane < g.splits && ml[1] != 0.f);
+    float l = 0.f;
     float4_t y = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-    for (int i = 0; i < PER; i++) {
-        const int s = i * SG + sg;
-        const float w = __shfl(a, s & 63);
-        if (i * SG < g.splits && ((some >> (s & 63)) & 1u)) {
+    for (int i = 0; i < PER; i++)
+        if (i * SG < g.splits && i * SG + sg < g.splits && ml[i][1] != 0.f) {
+            const float a = __builtin_amdgcn_exp2f(ml[i][0] - base);
+            l = fmaf(a, ml[i][1], l);
 #pragma unroll
-            for (int k = 0; k < 4; k++) y[k] = fmaf(v[i][k], w, y[k]);
+            for (int k = 0; k < 4; k++) y[k] = fmaf(a, v[i][k], y[k]);
         }
-    }
-    *(float4_t *)&part[sg][4 * c] = y;
+    __shared__ float mls[R][SG][2];
+    *(float4_t *)&part[rl][sg][4 * c] = y;
+    if (c == 0) mls[rl][sg][0] = top, mls[rl][sg][1] = l;
     __syncthreads();
-    if (t >= D) return;
-    float sum = 0.f;
+    for (int e = t; e < R * D; e += 256) {
+        const int rr = e / D, d = e - rr * D;
+        const int64_t out = (int64_t)blockIdx.x * R + rr;
+        if (out >= rows) break;
+        float all = -INFINITY, sum = 0.f, total = 0.f;
 #pragma unroll
-    for (int s = 0; s < SG; s++) sum += part[s][t];
-    const int bk = (int)(row / g.rows), m = (int)(row - (int64_t)bk * g.rows), b = bk / g.kv_heads, kh = bk - b * g.kv_heads, qi = m / g.group;
-    g.O[b * g.o_bs + (int64_t)(kh * g.group + (m - qi * g.group)) * g.o_hs + qi * g.o_rs + t] = (half_t)(sum / l); // no visible key: 0 / 0
+        for (int s = 0; s < SG; s++) all = fmaxf(all, mls[rr][s][0]);
+        const float ref = all == -INFINITY ? 0.f : all;
+#pragma unroll
+        for (int s = 0; s < SG; s++) {
+            const float a = __builtin_amdgcn_exp2f(mls[rr][s][0] - ref);
+            sum = fmaf(part[rr][s][d], a, sum), total = fmaf(mls[rr][s][1], a, total);
+        }
+        const int bk = (int)(out / g.rows), m = (int)(out - (int64_t)bk * g.rows), b = bk / g.kv_heads, kh = bk - b * g.kv_heads, qi = m / g.group;
+        g.O[b * g.o_bs + (int64_t)(kh * g.group + (m - qi * g.group)) * g.o_hs + qi * g.o_rs + d] = (half_t)(sum / total); // no visible key: 0 / 0
+    }
+}
+template <int CG, int SG> static hipError_t launch_aq_merge(const AttnQ4Args &g, int D, int64_t rows, hipStream_t st) {
+    constexpr int R = 256 / (CG * SG);
+    hipLaunchKernelGGL((attention_q4_merge_kernel<CG, SG>), dim3((unsigned)((rows + R - 1) / R)), dim3(256), 0, st, g, D, rows);
+    return hipGetLastError();
 }
 
-// the two kernels: rows of a tile, and the keys that shares are counted in
-RT_TUNABLE(g_aq_stream_rows, 16);
-RT_TUNABLE(g_aq_waves, 8);
-RT_TUNABLE(g_aq_target, 256);
-RT_TUNABLE(g_aq_least, 1);
-static bool aq_streams(int rows) { return rows <= g_aq_stream_rows; }
+// Up to 16 rows per head of keys stream (us, that kernel and the other: 4 x 32 heads on 2001 keys of 96 at 7 rows 15.5 and 24.3, on 2048 of 128 at 8 / 16 rows 22.2 /
+// 23.6 and 26.8 / 28.3).
+constexpr int AQ_STREAM_ROWS = 16;
+static bool aq_streams(int rows) { return rows <= AQ_STREAM_ROWS; }
 static int64_t aq_row_tiles(int rows) { return aq_streams(rows) ? 1 : (rows + AP_ROWS - 1) / AP_ROWS; }
-// keys of a workgroup where several share a row tile's, and how many do
+// Keys of a workgroup where several share a row tile's, and how many do: as many as fill the 256 compute units once (a workgroup's eight wavefronts leave no room
+// for a second; two rounds of half the keys, 32 x 8 heads on 8192 keys of 128: 62 -> 69 us), down to one step each.
+// The streaming kernel does two steps (1024 keys) in one launch (32 heads of 80: 8.0 us, in two shares 8.7; four steps 12.3, in four shares 9.1).  The other takes
+// shares of two steps from 2048 rows on, where joining them costs more than the second step (32 x 128 rows on 1024 keys of 80: one step each 20.0 us, two 16.2; 32 x 32
+// rows on 544 keys 10.7 and 13.6).
 static void aq_split(const rt_attention_q4_desc &d, int &splits, int &split_keys) {
     const int rows = d.q_len * (d.heads / d.kv_heads);
-    const int64_t wgs = (int64_t)d.batch * d.kv_heads * aq_row_tiles(rows);
-    const int unit = aq_streams(rows) ? 64 * g_aq_waves : AP_KEYS;
-    const int steps = (d.kv_len + unit - 1) / unit;
-    int64_t s = std::min<int64_t>(AQ_MAX_SPLITS, std::min<int64_t>(steps / g_aq_least, g_aq_target / wgs));
-    const int per = s > 1 ? (int)((steps + s - 1) / s) : std::max(steps, 1);
-    splits = std::max(1, (steps + per - 1) / per), split_keys = per * unit;
+    const int64_t stacks = (int64_t)d.batch * d.kv_heads, wgs = stacks * aq_row_tiles(rows);
+    const int unit = aq_streams(rows) ? 64 * AQ_WAVES : AP_KEYS, steps = std::max(1, (d.kv_len + unit - 1) / unit);
+    const int least = aq_streams(rows) ? (steps <= 2 ? 2 : 1) : stacks * rows >= 2048 ? 2 : 1;
+    const int64_t s = std::min<int64_t>({AQ_MAX_SPLITS, steps / least, 256 / wgs});
+    const int per = s > 1 ? (int)((steps + s - 1) / s) : steps;
+    splits = (steps + per - 1) / per, split_keys = (int)std::min<int64_t>((int64_t)per * unit, 1 << 30);
 }
 
 uint64_t attention_q4_workspace_bytes(const rt_attention_q4_desc &d) {
@@ -752,13 +799,14 @@ template <int NT, int VPR, int MK> static hipError_t launch_aq(const AttnQ4Args 
     using DM = AqDims<NT>;
     constexpr int ROWS = 4 * VPR;
     const size_t wave = (ROWS * 72 + DM::NB * 64) * 2, out = ((size_t)DM::T * VPR * 64 + 2 * ROWS) * sizeof(float);
-    const size_t lds = g_aq_waves * std::max(wave, out);
+    const size_t lds = AQ_WAVES * std::max(wave, out);
     if (const hipError_t e = ensure_lds_limit<&attention_q4_kernel<NT, VPR, MK>>(); e != hipSuccess) return e;
-    hipLaunchKernelGGL((attention_q4_kernel<NT, VPR, MK>), grid, dim3(64 * g_aq_waves), lds, st, g);
+    hipLaunchKernelGGL((attention_q4_kernel<NT, VPR, MK>), grid, dim3(64 * AQ_WAVES), lds, st, g);
     return hipGetLastError();
 }
 template <int NT> static hipError_t launch_aq_rows(const AttnQ4Args &g, dim3 grid, hipStream_t st) {
     if (g.rows <= 4) return g.mask ? launch_aq<NT, 1, 1>(g, grid, st) : launch_aq<NT, 1, 0>(g, grid, st);
+    if (g.rows <= 8) return g.mask ? launch_aq<NT, 2, 1>(g, grid, st) : launch_aq<NT, 2, 0>(g, grid, st);
     return g.mask ? launch_aq<NT, 4, 1>(g, grid, st) : launch_aq<NT, 4, 0>(g, grid, st);
 }
 template <int NT, int MK> static hipError_t launch_aq_tile(const AttnQ4Args &g, unsigned wgs, hipStream_t st) {
@@ -810,10 +858,9 @@ hipError_t launch_attention_q4(const rt_attention_q4_desc &d, const void *q, con
     default: e = go(std::integral_constant<int, 8>{}); break;
     }
     if (e != hipSuccess || g.splits <= 1) return e;
-    const dim3 rows((unsigned)(stacks * g.rows));
-    if (d.head_dim <= 64) hipLaunchKernelGGL(attention_q4_merge_kernel<16>, rows, dim3(256), 0, stream, g, d.head_dim);
-    else hipLaunchKernelGGL(attention_q4_merge_kernel<32>, rows, dim3(256), 0, stream, g, d.head_dim);
-    return hipGetLastError();
+    const int64_t rows = stacks * g.rows;
+    if (d.head_dim <= 64) return g.splits <= 4 ? launch_aq_merge<16, 4>(g, d.head_dim, rows, stream) : g.splits <= 8 ? launch_aq_merge<16, 8>(g, d.head_dim, rows, stream) : launch_aq_merge<16, 16>(g, d.head_dim, rows, stream);
+    return g.splits <= 4 ? launch_aq_merge<32, 4>(g, d.head_dim, rows, stream) : launch_aq_merge<32, 8>(g, d.head_dim, rows, stream);
 }
 
 } // namespace rt
