@@ -45,7 +45,7 @@ struct AttnQ4Args {
     int64_t q_bs, q_hs, q_rs, o_bs, o_hs, o_rs, m_bs, m_rs;
     int kv_heads, group, rows, kv_len, q_len, capacity; // rows = q_len * group
     int causal, mask_f32, splits, split_keys, row_tiles;
-    float scale_log2e;
+    float scale, scale_log2e;
 };
 
 template <int CTRL> __device__ __forceinline__ float aq_dpp(float v) {
@@ -419,7 +419,7 @@ template <int NT, int MK> __global__ __launch_bounds__(512, 2) void attention_q4
     constexpr int LD = D + 8, VD = aq_value_row(NT), KBLK = AP_KEYS * LD, STAGE = aq_stage(NT); // halves: a row of keys, of values; a block of keys, both
     extern __shared__ __attribute__((aligned(16))) uint8_t smem[];
     half_t *const ring = (half_t *)smem;                          // [2][keys | values][128][LD | VD]
-    uint32_t *const odd_flags = (uint32_t *)(ring + 2 * STAGE);   // [2][wavefront]: whether the block has a scale of values that is not finite
+    uint32_t *const odd_flags = (uint32_t *)(ring + 2 * STAGE);   // [2][wavefront]: whether the block has a scale of values, of keys that is not finite
     const int t = threadIdx.x, lane = t & 63, wave = __builtin_amdgcn_readfirstlane(t >> 6);
     const int fr = lane & 15, fg = lane >> 4, rg = wave & 3, kg = wave >> 2; // group of rows, half of the keys
 
@@ -455,6 +455,7 @@ template <int NT, int MK> __global__ __launch_bounds__(512, 2) void attention_q4
     // rows rw + 16 u + fr: fragments of dimensions 32 kk + 8 fg .. + 7 (zero past head_dim)
     half8_t fq[2][KK];
     int last[2]; // the last key that the row sees
+    bool wild = false; // whether a query that is not finite is among them
     const half_t *mrow[2];
 #pragma unroll
     for (int u = 0; u < 2; u++) {
@@ -463,9 +464,15 @@ template <int NT, int MK> __global__ __launch_bounds__(512, 2) void attention_q4
         const half_t *qp = g.Q + b * g.q_bs + (int64_t)(kh * g.group + (m - qi * g.group)) * g.q_hs + qi * g.q_rs;
 #pragma unroll
         for (int kk = 0; kk < KK; kk++) fq[u][kk] = 32 * kk + 8 * fg < D ? *(const half8_t *)(qp + 32 * kk + 8 * fg) : half8_t{};
+        if (MK)
+#pragma unroll
+            for (int kk = 0; kk < KK; kk++)
+#pragma unroll
+                for (int e = 0; e < 8; e++) wild |= !(__builtin_fabsf((float)fq[u][kk][e]) <= 65504.f);
         mrow[u] = (const half_t *)g.mask + (b * g.m_bs + qi * g.m_rs) * (MK == 1 ? 2 : 1);
     }
 
+    wild = __builtin_amdgcn_ballot_w64(wild) != 0;
     // ---- this thread's dwords of a block: number i is dword i * 512 + t of [keys | values][128][DW], at four times that from the block's first
     uint32_t raw[NT], ds[NT], so[NT]; // (so: of its scale; the key is so / (2 SR))
     auto is_key = [&](int i) { return 2 * i + 2 <= NT || (2 * i < NT && wave < 4); }; // (uniform)
@@ -491,27 +498,29 @@ template <int NT, int MK> __global__ __launch_bounds__(512, 2) void attention_q4
     const uint32_t bias = q40_bias();
     auto widen = [&](int stage) __attribute__((always_inline)) {
         uint8_t *const st = (uint8_t *)(ring + stage * STAGE);
-        bool odd = false;
+        bool odd = false, odd_key = false;
 #pragma unroll
         for (int i = 0; i < NT; i++) {
             const bool val = !is_key(i);
             const uint32_t f = (uint32_t)(i * 512 + t - (val ? 256 * NT : 0)), key = so[i] / (2 * SR);
             half_t d = __builtin_bit_cast(half_t, (uint16_t)ds[i]);
+            const bool fin = (ds[i] & 0x7C00u) != 0x7C00u;
             if (val) { // a value that is not finite shows in the rows that see its key, and not through the matrix cores
-                const bool fin = (ds[i] & 0x7C00u) != 0x7C00u;
                 odd |= !fin;
                 d = fin ? d : (half_t)0.f;
+            } else if (MK) {
+                odd_key |= !fin;
             }
             *(half8_t *)(st + 16 * f + (val ? 2 * KBLK + (VD - D) * 2 * key : (LD - D) * 2 * key)) = q40_codes(raw[i], bias) * half8_t{d, d, d, d, d, d, d, d};
         }
-        const bool any = __builtin_amdgcn_ballot_w64(odd) != 0;
+        const uint32_t any = (__builtin_amdgcn_ballot_w64(odd) != 0 ? 1u : 0u) | (__builtin_amdgcn_ballot_w64(odd_key) != 0 ? 2u : 0u);
         if (lane == 0) odd_flags[8 * stage + wave] = any;
     };
     using MT = std::conditional_t<MK == 1, float, half_t>;
     typedef MT mask4_t __attribute__((ext_vector_type(4)));
     typedef MT mask4_u __attribute__((ext_vector_type(4), aligned(sizeof(MT)))); // rows start anywhere
     constexpr int MU = MK ? 2 : 1, MB = MK ? 4 : 1;
-    mask4_t mk[MU][MB]; // the block's, requested before the first product
+    mask4_t mk[MU][MB]; // the wavefront's next block's, requested before the second product of the one before it
     auto load_mask = [&](int j0) __attribute__((always_inline)) {
         if constexpr (MK != 0) {
 #pragma unroll
@@ -529,7 +538,10 @@ template <int NT, int MK> __global__ __launch_bounds__(512, 2) void attention_q4
     };
 
     float4_t acc[2][NT];
-    float m_run[2], l_run[2]; // base 2: the exponentials' reference; this lane's share of the sum
+    // the exponentials' reference and this lane's share of the sum.  Scores are in units of log2(e), and with a mask tensor as they are: its type's lowest value, which hides
+    // nothing from a row that has nothing else, would be infinite in the others.
+    constexpr float unit = MK ? kLog2eQ4 : 1.f;
+    float m_run[2], l_run[2];
     uint32_t bad[2];
 #pragma unroll
     for (int u = 0; u < 2; u++) {
@@ -546,7 +558,6 @@ template <int NT, int MK> __global__ __launch_bounds__(512, 2) void attention_q4
         constexpr bool LEAN = decltype(lean_c)::value;
         const half_t *const st = ring + stage * STAGE;
         const uint4_t fl = *(const uint4_t *)(odd_flags + 8 * stage), fh = *(const uint4_t *)(odd_flags + 8 * stage + 4);
-        load_mask(j0);
         float4_t S[2][4];
 #pragma unroll
         for (int bt = 0; bt < 4; bt++) {
@@ -560,7 +571,8 @@ template <int NT, int MK> __global__ __launch_bounds__(512, 2) void attention_q4
 #pragma unroll
                 for (int u = 0; u < 2; u++) S[u][bt] = __builtin_amdgcn_mfma_f32_16x16x32_f16(fk[kk], fq[u][kk], S[u][bt], 0, 0, 0);
         }
-        const bool odd = __builtin_amdgcn_readfirstlane((int)(fl[0] | fl[1] | fl[2] | fl[3] | fh[0] | fh[1] | fh[2] | fh[3])) != 0;
+        const uint32_t flags = (uint32_t)__builtin_amdgcn_readfirstlane((int)(fl[0] | fl[1] | fl[2] | fl[3] | fh[0] | fh[1] | fh[2] | fh[3]));
+        const bool odd = flags & 1u;
         half8_t fp[2][2];
 #pragma unroll
         for (int u = 0; u < 2; u++) {
@@ -572,15 +584,18 @@ template <int NT, int MK> __global__ __launch_bounds__(512, 2) void attention_q4
             } else {
 #pragma unroll
                 for (int e = 0; e < 16; e++) {
-                    float s = S[u][e >> 2][e & 3] * g.scale_log2e;
-                    if constexpr (MK != 0) {
-                        const float mv = (float)mk[u][e >> 2][e & 3], m2 = mv * kLog2eQ4;
-                        // a hidden key's score may be anything; a type's lowest value hides nothing from a row that has nothing else
-                        s = mv == -INFINITY ? -INFINITY : s + (MK == 1 && m2 == -INFINITY ? -3.40282347e38f : m2);
-                    }
-                    if (!LEAN && j0 + 16 * (e >> 2) + 4 * fg + (e & 3) > last[u]) s = -INFINITY;
-                    S[u][e >> 2][e & 3] = s;
-                    bmax = fmaxf(bmax, s);
+                    const float s = S[u][e >> 2][e & 3];
+                    S[u][e >> 2][e & 3] = MK ? fmaf(s, g.scale, (float)mk[MK ? u : 0][MK ? e >> 2 : 0][e & 3]) : s * g.scale_log2e;
+                }
+                if (MK && ((flags & 2u) || wild)) { // a hidden key's score may be anything
+#pragma unroll
+                    for (int e = 0; e < 16; e++)
+                        if ((float)mk[MK ? u : 0][MK ? e >> 2 : 0][e & 3] == -INFINITY) S[u][e >> 2][e & 3] = -INFINITY;
+                }
+#pragma unroll
+                for (int e = 0; e < 16; e++) {
+                    if (!LEAN && j0 + 16 * (e >> 2) + 4 * fg + (e & 3) > last[u]) S[u][e >> 2][e & 3] = -INFINITY;
+                    bmax = fmaxf(bmax, S[u][e >> 2][e & 3]);
                 }
             }
             if (odd) {
@@ -596,9 +611,9 @@ template <int NT, int MK> __global__ __launch_bounds__(512, 2) void attention_q4
                 }
             }
             bmax = rt_groups_max(bmax);
-            // the reference follows the maximum only where that is 2^8 past it (or it has none): the outputs and the sum are seldom rescaled
-            if (__builtin_amdgcn_ballot_w64(bmax > m_run[u] + 8.f)) {
-                const float m_new = fmaxf(m_run[u], bmax), alpha = m_new == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(m_run[u] - m_new);
+            // the reference follows the maximum only where that is some 2^8 past it (or it has none): the outputs and the sum are seldom rescaled
+            if (__builtin_amdgcn_ballot_w64(bmax > m_run[u] + (MK ? 5.5f : 8.f))) {
+                const float m_new = fmaxf(m_run[u], bmax), alpha = m_new == -INFINITY ? 1.f : __builtin_amdgcn_exp2f((m_run[u] - m_new) * unit);
                 m_run[u] = m_new;
                 l_run[u] *= alpha;
 #pragma unroll
@@ -609,13 +624,15 @@ template <int NT, int MK> __global__ __launch_bounds__(512, 2) void attention_q4
             float psum = 0.f;
 #pragma unroll
             for (int e = 0; e < 16; e += 2) {
-                const float p0 = __builtin_amdgcn_exp2f(fmaf(S[u][e >> 2][e & 3], sc, -m_use)), p1 = __builtin_amdgcn_exp2f(fmaf(S[u][e >> 2][(e & 3) + 1], sc, -m_use));
+                const float s0 = S[u][e >> 2][e & 3], s1 = S[u][e >> 2][(e & 3) + 1];
+                const float p0 = __builtin_amdgcn_exp2f(MK ? (s0 - m_use) * unit : fmaf(s0, sc, -m_use)), p1 = __builtin_amdgcn_exp2f(MK ? (s1 - m_use) * unit : fmaf(s1, sc, -m_use));
                 const half2_t p = {(half_t)p0, (half_t)p1};
                 psum = __builtin_amdgcn_fdot2(p, half2_t{(half_t)1, (half_t)1}, psum, false);
                 fp[u][e >> 3][e & 7] = p[0], fp[u][e >> 3][(e & 7) + 1] = p[1];
             }
             l_run[u] += psum;
         }
+        load_mask(j0 + AP_KEYS); // in registers that are free from here on
 #pragma unroll
         for (int hh = 0; hh < 2; hh++)
 #pragma unroll
@@ -632,7 +649,7 @@ template <int NT, int MK> __global__ __launch_bounds__(512, 2) void attention_q4
     };
 
     if (j_first < j_end) {
-        load(j_first);
+        load(j_first), load_mask(j_first + 64 * kg);
         widen(0);
         __syncthreads();
         int stage = 0, j0 = j_first;
@@ -654,6 +671,7 @@ template <int NT, int MK> __global__ __launch_bounds__(512, 2) void attention_q4
     // ---- the two halves of the keys through LDS: [group of rows][tile of 16][dimensions' tile][lane] four, and references, sums, flags
 #pragma unroll
     for (int u = 0; u < 2; u++) {
+        if (MK && m_run[u] != -INFINITY) m_run[u] = fmaxf(m_run[u] * unit, -3.40282347e38f);
         l_run[u] = rt_groups_sum(l_run[u]);
         bad[u] |= (uint32_t)__shfl_xor((int)bad[u], 16);
         bad[u] |= (uint32_t)__shfl_xor((int)bad[u], 32);
@@ -772,18 +790,29 @@ template <int CG, int SG> static hipError_t launch_aq_merge(const AttnQ4Args &g,
 constexpr int AQ_STREAM_ROWS = 16;
 static bool aq_streams(int rows) { return rows <= AQ_STREAM_ROWS; }
 static int64_t aq_row_tiles(int rows) { return aq_streams(rows) ? 1 : (rows + AP_ROWS - 1) / AP_ROWS; }
-// Keys of a workgroup where several share a row tile's, and how many do: as many as fill the 256 compute units once (a workgroup's eight wavefronts leave no room
-// for a second; two rounds of half the keys, 32 x 8 heads on 8192 keys of 128: 62 -> 69 us), down to one step each.
-// The streaming kernel does two steps (1024 keys) in one launch (32 heads of 80: 8.0 us, in two shares 8.7; four steps 12.3, in four shares 9.1).  The other takes
-// shares of two steps from 2048 rows on, where joining them costs more than the second step (32 x 128 rows on 1024 keys of 80: one step each 20.0 us, two 16.2; 32 x 32
-// rows on 544 keys 10.7 and 13.6).
+// Keys of a workgroup where several share a row tile's, and how many do.
+// The streaming kernel: as many as fill the 256 compute units once (a workgroup's eight wavefronts leave no room for a second; two rounds of half the keys, 32 x 8
+// heads on 8192 keys of 128: 62 -> 69 us), down to one step each, but two steps (1024 keys) in one launch (32 heads of 80: 8.0 us, in two shares 8.7; four steps 12.3,
+// in four shares 9.1).
+// The other: the least of what its rounds of workgroups, the partial results and the second launch take.  A step is some 1.4 + 0.017 head_dim us (2.5, 3.1 and 3.6
+// measured at 64, 96 and 128), partial results are written and read at 2.5 TB/s (us for shares: 32 x 128 rows on 1024 keys of 80: 1: 21.3, 4: 16.2, 8: 20.0; 32 x 32 on 544: 1:
+// 13.9, 2: 13.6, 5: 10.7; 2 x 4 x 600 on 1373 keys of 64: 3: 21.6, 6: 19.6, 11: 26.4).
 static void aq_split(const rt_attention_q4_desc &d, int &splits, int &split_keys) {
     const int rows = d.q_len * (d.heads / d.kv_heads);
     const int64_t stacks = (int64_t)d.batch * d.kv_heads, wgs = stacks * aq_row_tiles(rows);
     const int unit = aq_streams(rows) ? 64 * AQ_WAVES : AP_KEYS, steps = std::max(1, (d.kv_len + unit - 1) / unit);
-    const int least = aq_streams(rows) ? (steps <= 2 ? 2 : 1) : stacks * rows >= 2048 ? 2 : 1;
-    const int64_t s = std::min<int64_t>({AQ_MAX_SPLITS, steps / least, 256 / wgs});
-    const int per = s > 1 ? (int)((steps + s - 1) / s) : steps;
+    int64_t s = 1;
+    if (aq_streams(rows)) {
+        s = steps <= 2 ? 1 : std::max<int64_t>(1, std::min<int64_t>({AQ_MAX_SPLITS, steps, 256 / wgs}));
+    } else if (wgs < 2048) { // (more rounds than eight lose little at their end)
+        const double step = 1.4 + 0.017 * d.head_dim, part = (double)stacks * rows * (d.head_dim + 2) * 8 / 2.5e6;
+        double best = 0;
+        for (int n = 1; n <= std::min(steps, AQ_MAX_SPLITS); n++) {
+            const double t = (double)((wgs * n + 255) / 256) * ((steps + n - 1) / n) * step + (n > 1 ? 4 + n * part : 0);
+            if (n == 1 || t < best) best = t, s = n;
+        }
+    }
+    const int per = (int)((steps + s - 1) / s);
     splits = (steps + per - 1) / per, split_keys = (int)std::min<int64_t>((int64_t)per * unit, 1 << 30);
 }
 
@@ -828,7 +857,7 @@ hipError_t launch_attention_q4(const rt_attention_q4_desc &d, const void *q, con
     g.m_bs = d.mask_strides[0], g.m_rs = d.mask_strides[1], g.mask_f32 = d.mask_dtype == RT_F32;
     g.kv_heads = d.kv_heads, g.group = d.heads / d.kv_heads, g.rows = d.q_len * g.group;
     g.kv_len = d.kv_len, g.q_len = d.q_len, g.capacity = d.capacity, g.causal = d.causal;
-    g.scale_log2e = d.scale * kLog2eQ4;
+    g.scale = d.scale, g.scale_log2e = d.scale * kLog2eQ4;
     aq_split(d, g.splits, g.split_keys);
     const uint64_t need = attention_q4_workspace_bytes(d);
     if (need && workspace && workspace_bytes >= need && !((uintptr_t)workspace & 15u)) {
