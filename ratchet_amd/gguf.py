@@ -127,16 +127,17 @@ class Header:
             raise OperationError(_ffi.RT_ERR_INVALID_ARG, f"missing key {key}")
         return self.metadata[key]
 
-    def tensor(self, name: str, device: Device, q8_dtype: DType = DType.Q8_0H) -> Tensor:
+    def tensor(self, name: str, device: Device, q8_dtype: DType = DType.Q8_0H, q4_0: bool = False) -> Tensor:
         """Header::tensor (gguf.rs:483-496).  The reference picks Q8_0H when the device has f16
-        shaders (gguf.rs:130-136); every gfx950 does, so that is the default here."""
+        shaders (gguf.rs:130-136); every gfx950 does, so that is the default here.  Q4_0 tensors, on which the
+        reference bails (gguf.rs:140), load with `q4_0` only."""
         if name not in self.tensor_infos:
             raise OperationError(_ffi.RT_ERR_INVALID_ARG, f"cannot find tensor info for {name}")
         if not device.is_gpu():
             raise OperationError(_ffi.RT_ERR_NO_DEVICE, "tensors are loaded to a GPU device")
         ti = self.tensor_infos[name]
         dst_dt = {GgmlDType.F32: DType.F32, GgmlDType.F16: DType.F16, GgmlDType.Q8_0: q8_dtype,
-                  GgmlDType.Q4K: DType.Q4_K, GgmlDType.Q4_0: DType.Q4_0}.get(ti.ggml_dtype)
+                  GgmlDType.Q4K: DType.Q4_K, GgmlDType.Q4_0: DType.Q4_0 if q4_0 else None}.get(ti.ggml_dtype)
         if dst_dt is None:
             raise OperationError(_ffi.RT_ERR_UNSUPPORTED, f"unsupported ggml dtype {ti.ggml_dtype.name}")
         numel = int(np.prod(ti.shape, dtype=np.int64)) if ti.shape else 1

@@ -107,7 +107,9 @@ def image(name, shape, blocks):
 def test_gguf_tensor_through_a_linear(device):
     codes, d = draw(48 * 160, 5)
     head = gguf.Header.read(image(b"blk.0.ffn_up.weight", (48, 160), gguf_blocks(codes, d)))
-    w = head.tensor("blk.0.ffn_up.weight", device)
+    with pytest.raises(OperationError):  # as the reference does
+        head.tensor("blk.0.ffn_up.weight", device)
+    w = head.tensor("blk.0.ffn_up.weight", device, q4_0=True)
     assert w.dt == DType.Q4_0 and w.shape == (48, 160) and np.array_equal(w.to(Device.CPU).storage, segments(codes, d))
     st = _ffi.lib().rt_gguf_load_tensor(device.ctx, head._h, head._buf, len(head._image), 0, _ffi.RT_Q4_0, None, w.data_ptr(), None)
     assert st == _ffi.RT_ERR_INVALID_ARG  # no staging buffer
