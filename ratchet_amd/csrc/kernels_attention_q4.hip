@@ -473,6 +473,11 @@ template <int NT, int MK> __global__ __launch_bounds__(512, 2) void attention_q4
     }
 
     wild = __builtin_amdgcn_ballot_w64(wild) != 0;
+    // awaited here: a first use in the loop, where the compiler does not know them from the block's loads, waited for those in every step
+#pragma unroll
+    for (int u = 0; u < 2; u++)
+#pragma unroll
+        for (int kk = 0; kk < KK; kk++) asm volatile("" : "+v"(fq[u][kk]));
     // ---- this thread's dwords of a block: number i is dword i * 512 + t of [keys | values][128][DW], at four times that from the block's first
     uint32_t raw[NT], ds[NT], so[NT]; // (so: of its scale; the key is so / (2 SR))
     auto is_key = [&](int i) { return 2 * i + 2 <= NT || (2 * i < NT && wave < 4); }; // (uniform)
@@ -481,8 +486,8 @@ template <int NT, int MK> __global__ __launch_bounds__(512, 2) void attention_q4
         const int f = (i * 512 + t) % (256 * NT), key = f / DW;
         so[i] = 2 * (key * SR + ((f - key * DW) >> 2));
     }
-    auto load = [&](int j0) __attribute__((always_inline)) {
-        const int n = min(AP_KEYS, len - j0); // past the last key the loads return zeros
+    auto load = [&](int j) __attribute__((always_inline)) {
+        const int j0 = __builtin_amdgcn_readfirstlane(j), n = min(AP_KEYS, len - j0); // past the last key the loads return zeros
         const auto kr = aq_bounded(Kc + (int64_t)j0 * RB, n * RB), vr = aq_bounded(Vc + (int64_t)j0 * RB, n * RB);
         const auto ksr = aq_bounded(Ks + (int64_t)j0 * SR, n * SR * 2), vsr = aq_bounded(Vs + (int64_t)j0 * SR, n * SR * 2);
 #pragma unroll
