@@ -290,3 +290,50 @@ def test_one_workgroup_past_its_window(device, lq):
     # beside what holds elsewhere: the sum, in f32 over 2^15 steps of a lane, off by at most half a step of a partial sum that grows evenly: 2^-10 of the zeros' part
     tol = (2.0**-11 + 2.0**-20 + 2 * e) * mag + 2.0**-25 * np.abs(vv).sum(0) / l + 2.0**-11 * np.abs(want) + 2.0**-25 + 2.0**-10 * zeros / l * np.abs(want)
     assert (np.abs(got - want) <= tol).all(), float((np.abs(got - want) / tol).max())
+
+
+@gpu
+@pytest.mark.parametrize("lq", [1, 20])
+def test_no_keys_and_no_caches(device, lq):
+    """kv_len = 0: every row is NaN, and the caches may be NULL."""
+    desc = attention_desc(2, 4, 2, lq, 0, 64, 8)
+    q = torch.zeros((2, lq, 4, 64), dtype=torch.float16, device="cuda:0")
+    out = torch.zeros_like(q)
+    for causal in (0, 1):
+        desc.causal = causal
+        out.zero_()
+        assert _ffi.lib().rt_attention_q4_enqueue(device.ctx, ctypes.byref(desc), q.data_ptr(), None, None, None, None, out.data_ptr(), None, 0,
+                                                  torch.cuda.current_stream().cuda_stream) == 0
+        assert torch.isnan(out).all()
+
+
+@gpu
+@pytest.mark.parametrize("lq", [1, 5, 17])
+def test_as_many_sequences_as_a_call_takes(device, lq):
+    """65535 heads of keys in one call; one more is refused."""
+    rng = np.random.default_rng(lq)
+    b, kv, n, d = 13107, 5, 3, 16
+    kbuf, kval = drawn_cache(rng, b, kv, n, d)
+    vbuf, vval = drawn_cache(rng, b, kv, n, d)
+    q = rng.standard_normal((b, kv, lq, d)).astype(np.float16)
+    got = run(device, q, kbuf, vbuf, kv, n, n, 0.2)
+    for i in (0, 1, 6000, b - 1):
+        want, tol = reference(q[i : i + 1], kval[i : i + 1], vval[i : i + 1], 0.2)
+        check(got[i : i + 1], want, tol)
+    desc = attention_desc(65536, 1, 1, lq, n, d, n)
+    assert _ffi.lib().rt_attention_q4_validate(ctypes.byref(desc)) == _ffi.RT_ERR_UNSUPPORTED
+
+
+@gpu
+@pytest.mark.parametrize("h,kv,lq", [(64, 1, 1), (16, 1, 1), (17, 1, 1), (40, 8, 3), (64, 2, 9)])
+def test_many_heads_on_one(device, h, kv, lq):
+    """Groups that make a tile of one query row, that fill the streaming kernel's rows and that pass them by one; a mask's row belongs to all heads of its query."""
+    rng = np.random.default_rng(h)
+    b, n, d = 2, 640, 80
+    kbuf, kval = drawn_cache(rng, b, kv, n, d)
+    vbuf, vval = drawn_cache(rng, b, kv, n, d)
+    q = rng.standard_normal((b, h, lq, d)).astype(np.float16)
+    mask = np.where(rng.random((b, lq, n)) < 0.3, -np.inf, rng.uniform(-2, 2, (b, lq, n))).astype(np.float16)
+    for causal, m, lens in ((False, None, None), (True, None, [600, 11]), (True, mask, None)):
+        want, tol = reference(q, kval, vval, 0.2, mask=m, causal=causal, lens=lens)
+        check(run(device, q, kbuf, vbuf, kv, n, n, 0.2, mask=m, causal=causal, lens=lens), want, tol)

@@ -108,3 +108,25 @@ def test_products_captured_into_a_graph(device, n):
         torch.cuda.synchronize()
         assert torch.isfinite(z[0]).all() and torch.equal(z[0].view(torch.int16), z[1].view(torch.int16)), i
 
+
+@gpu
+@pytest.mark.parametrize("m,k,n", [(40, 288, 4097), (163, 128, 1500), (33, 96, 700)])
+def test_many_activation_rows_against_few_weights(device, m, k, n):
+    weight, x, bias, exact, mag = operands(device, (), m, k, n)
+    got, _ = call(device, weight, torch.from_numpy(x).to("cuda:0"), m, k, n)
+    check(got, exact[0], mag[0], k)
+
+
+@gpu
+@pytest.mark.parametrize("m,k,n", [(2560, 10240, 96), (512, 2048, 4), (640, 2048, 512)])
+def test_the_form_without_a_workspace_argument(device, m, k, n):
+    """rt_matmul_enqueue_static: Q4_0 weights run there as they do without a workspace."""
+    weight, x, _, exact, mag = operands(device, (), m, k, n)
+    xt = torch.from_numpy(x).to("cuda:0")
+    plain, _ = call(device, weight, xt, m, k, n, workspace=False)
+    desc = _ffi.make_desc(_ffi.RT_Q4_0, (m, k), _ffi.RT_F16, (n, k), False, True, True)
+    out = torch.full((n, m), float("nan"), dtype=torch.float16, device="cuda:0")
+    assert _ffi.lib().rt_matmul_enqueue_static(device.ctx, ctypes.byref(desc), weight.data_ptr(), xt.data_ptr(), None, out.data_ptr(), _ffi.RT_ACT_NONE,
+                                               torch.cuda.current_stream().cuda_stream) == 0
+    assert torch.equal(out.view(torch.int16), plain.view(torch.int16))
+    check(out, exact[0], mag[0], k)
