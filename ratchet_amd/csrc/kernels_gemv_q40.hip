@@ -1,4 +1,5 @@
-// Q4_0 weights x f16 activations on the matrix cores, one pass over the weight for up to 64 activation rows (decode steps of one or many sequences)
+// Q4_0 weights x f16 activations on the matrix cores, one pass over the weight for 3 to 64 activation rows (decode steps of some sequences; one or two rows are
+// kernels_gemv_q40_rowdot.hip's up to a K of 10240)
 // and tiles of 32 for more (prompts that launch_gemm_nt leaves).
 //
 //   y[j, i] = act(sum_b d[i, b] * sum_{k in b} (q[i, k] - 8) x[j, k] + bias)        b: blocks of 32 of K
@@ -21,8 +22,8 @@
 // A K-vector (16 bytes) v of activation row j of a panel is at slot v * NV + j of LDS, j exchanged within its 16 by 4 (v % 4): reads
 // (16 rows of one vector by a lane group) and writes (four vectors of a row by neighbouring lanes) then meet no bank twice.
 //
-// Measured (weights from HBM, us): 10240 x 2560 at 1 / 16 / 64 rows 8.3 / 9.9 / 16.5, 2560 x 10240 9.5 / 14.6 / 25.9, 51865 x 2560 at 1 / 16 rows 20.5 / 23.8
-// (3.2 TB/s).  The large ones are bound by the issue of the unpacking: the same kernel without its loads takes 14 us, with nothing but its loads 19,
+// Measured (weights from HBM, us): 10240 x 2560 at 4 / 16 / 64 rows 8.3 / 9.9 / 16.5, 2560 x 10240 9.5 / 14.6 / 25.9, 51865 x 2560 at 16 rows 23.8
+// (3.2 TB/s).  The large ones are bound by the issue of the unpacking: with one row 20.5 us, without its loads 14, with nothing but its loads 19,
 // and a kernel that only reads the codes 12 (5.5 TB/s).  The small ones by latency: a launch, one trip to HBM and the sum over K are 5.4 us at 2560 x 2560.
 #include "device_common.h"
 
@@ -321,7 +322,9 @@ static hipError_t q40_run(const Problem &p, const void *A, const void *B, const 
 }
 
 hipError_t launch_gemv_q40(const Problem &p, const void *A, const void *B, const void *bias, void *out, hipStream_t stream, const DeviceInfo &dev) {
-    return p.N <= kGemvQ40MaxCols ? q40_run(p, A, B, bias, out, stream, dev) : hipErrorNotSupported;
+    if (p.N > kGemvQ40MaxCols) return hipErrorNotSupported;
+    const hipError_t e = launch_gemv_q40_rowdot(p, A, B, bias, out, stream, dev); // one or two vectors
+    return e == hipErrorNotSupported ? q40_run(p, A, B, bias, out, stream, dev) : e;
 }
 // More rows: whole units of 256 of K against 160 weight rows and more are launch_gemm_nt's, but for what it leaves.  (Asked here too: a plan offers its product to
 // the family that took it last time first, and whether that one takes it may go by the workspace.)

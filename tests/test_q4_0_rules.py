@@ -6,8 +6,8 @@ import numpy as np
 import pytest
 import torch
 
-from ratchet_amd import _ffi
-from test_q4_0 import check, operands
+from ratchet_amd import DType, Tensor, _ffi
+from test_q4_0 import check, draw, operands, segments, values
 
 gpu = pytest.mark.gpu
 
@@ -130,3 +130,37 @@ def test_the_form_without_a_workspace_argument(device, m, k, n):
                                                torch.cuda.current_stream().cuda_stream) == 0
     assert torch.equal(out.view(torch.int16), plain.view(torch.int16))
     check(out, exact[0], mag[0], k)
+
+
+@gpu
+@pytest.mark.parametrize("n", [1, 2, 3, 9, 40, 200])
+def test_subnormal_activations(device, n):
+    """Activations below f16's normal range count like any others; weights of the largest scales keep the products in it."""
+    rng = np.random.default_rng(n)
+    m, k = 170, 2048
+    codes, d = draw(m * k, n)
+    d = np.full_like(d, 8000)
+    x = (rng.integers(-1023, 1024, (n, k)) * 2.0**-24).astype(np.float16)
+    w = values(codes, d).reshape(m, k)
+    weight = Tensor.from_quantized(segments(codes, d), DType.Q4_0, (m, k), device)
+    got, _ = call(device, weight, torch.from_numpy(x).to("cuda:0"), m, k, n)
+    xd = x.astype(np.float64)
+    check(got, xd @ w.T, np.abs(xd) @ np.abs(w).T, k)
+
+
+# K that lanes of a row share evenly, that leaves lanes without a block, one block; K that two, three, four wavefronts share; rows that end in a group of four and many passes
+@gpu
+@pytest.mark.parametrize("k", [32, 64, 512, 544, 2528, 2560, 2592, 5120, 5152, 7680, 10240, 10272])
+@pytest.mark.parametrize("m", [1, 7, 2050, 9001])
+def test_one_and_two_vectors(device, m, k):
+    for n in (1, 2):
+        weight, x, bias, exact, mag = operands(device, (), m, k, n)
+        xt, bt = torch.from_numpy(x).to("cuda:0"), torch.from_numpy(bias[0]).to("cuda:0")
+        off = bias[0].astype(np.float64)
+        got, _ = call(device, weight, xt, m, k, n, bt)
+        check(got, exact[0] + off, mag[0] + np.abs(off), k)
+        if m == 7:
+            x[n - 1, k - 1] = np.inf  # the last value of the last vector: others are untouched, and no lane without a block sees it
+            clean = got
+            got, _ = call(device, weight, torch.from_numpy(x).to("cuda:0"), m, k, n, bt)
+            assert torch.equal(got[: n - 1], clean[: n - 1]) and not torch.isfinite(got[n - 1]).any()
