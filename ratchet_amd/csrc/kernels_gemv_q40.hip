@@ -22,8 +22,8 @@
 // A K-vector (16 bytes) v of activation row j of a panel is at slot v * NV + j of LDS, j exchanged within its 16 by 4 (v % 4): reads
 // (16 rows of one vector by a lane group) and writes (four vectors of a row by neighbouring lanes) then meet no bank twice.
 //
-// Measured (weights from HBM, us): 10240 x 2560 at 4 / 16 / 64 rows 8.3 / 9.9 / 16.5, 2560 x 10240 9.5 / 14.6 / 25.9, 51865 x 2560 at 16 rows 23.8
-// (3.2 TB/s).  The large ones are bound by the issue of the unpacking: with one row 20.5 us, without its loads 14, with nothing but its loads 19,
+// Measured (weights from HBM, us): 10240 x 2560 at 4 / 16 / 64 rows 7.9 / 9.4 / 16.1, 2560 x 10240 9.0 / 13.8 / 25.0, 51865 x 2560 at 16 rows 25
+// (3.0 TB/s).  The large ones are bound by the issue of the unpacking: with one row and no bias 20.5 us, without its loads 14, with nothing but its loads 19,
 // and a kernel that only reads the codes 12 (5.5 TB/s).  The small ones by latency: a launch, one trip to HBM and the sum over K are 5.4 us at 2560 x 2560.
 #include "device_common.h"
 
@@ -45,6 +45,7 @@ struct GemvQ40Args {
     int wr, wk;         // wavefronts along the weight rows, and that share K
     int vec_out;        // outputs along the weight rows are contiguous and start on 16 bytes
     int tiles_j, remap; // tiles of activation rows; whether workgroups are dealt to the XCDs in ranges
+    int bias_at;        // bytes of LDS before the tile's biases
 };
 
 typedef uint64_t uint64_a2 __attribute__((aligned(2)));
@@ -167,6 +168,10 @@ template <int MT, int VPR, int XI, int UC, int DEPTH> __global__ __launch_bounds
         }
     };
 
+    // the tile's biases, asked for with the first activations: behind the last sum they would be another trip to memory (2560 x 2560 at 4 rows 5.9 us, so 5.5; 10240 x 2560 8.4 and 7.9)
+    half_t *const biases = (half_t *)(smem + g.bias_at);
+    const half_t *const from = g.has_bias ? g.bias : g.X;
+    const half_t bias_t = from[!g.has_bias ? 0 : g.bias_on_rows ? min((int64_t)ti * 16 * WR + t, g.M - 1) : min(j0 + t, g.N - 1)];
     // panel p: multiplied from ring[p % (DEPTH + 1)], while panel p + DEPTH's weights and panel p + 1's activations are requested
     Unit ring[DEPTH + 1];
     load_x(0);
@@ -175,6 +180,7 @@ template <int MT, int VPR, int XI, int UC, int DEPTH> __global__ __launch_bounds
     for (int u = 0; u < DEPTH; u++) load(u, ring[u]);
     __builtin_amdgcn_sched_barrier(0);
     store_x(0);
+    if (t < max(16 * WR, NV)) biases[t] = bias_t;
     __syncthreads();
     auto panel = [&](int p, Unit &now, Unit &next) __attribute__((always_inline)) {
         load_x(p + 1);
@@ -230,7 +236,7 @@ template <int MT, int VPR, int XI, int UC, int DEPTH> __global__ __launch_bounds
             const int64_t left = g.M - first - i;
 #pragma unroll
             for (int x = 0; x < 8; x++) {
-                if (g.has_bias) y[x] += (float)g.bias[g.bias_on_rows ? first + min<int64_t>(i + x, g.M - 1 - first) : j0 + j];
+                if (g.has_bias) y[x] += (float)biases[g.bias_on_rows ? i + x : j];
                 h[x] = (half_t)rt_act_k<decltype(has_act)::value>(y[x]);
             }
             half_t *const o = out + (first + i) * g.o_is + (j0 + j) * g.o_js;
@@ -253,7 +259,8 @@ template <int MT, int VPR, int XI, int UC, int DEPTH> static hipError_t launch_q
     if (ti * tj > 0x3fffff) return hipErrorNotSupported; // (a grid's threads along an axis are fewer than 2^32)
     g.tiles_j = (int)tj, g.remap = tj > 1 && ti * tj % 8 == 0;
     const size_t panel = (size_t)NV * wk * UC * 256, x = g.K > 128 * UC * wk ? 2 * panel : panel, red = (size_t)wk * NV * q40_ld(16 * wr) * sizeof(float);
-    const size_t lds = std::max(x, red);
+    g.bias_at = (int)std::max(x, red); // (whole 16 bytes)
+    const size_t lds = (size_t)g.bias_at + std::max(16 * wr, NV) * sizeof(half_t);
     if (lds > 160 * 1024) return hipErrorNotSupported;
     if (lds > 48 * 1024)
         if (const hipError_t e = ensure_lds_limit<&gemv_q40_kernel<MT, VPR, XI, UC, DEPTH>>(); e != hipSuccess) return e;

@@ -10,7 +10,7 @@
 // q40_codes, exact, and four dot products; a block's sum is scaled in f32.  The sixteen lanes are joined by DPP, the wavefronts that share K through LDS, in a
 // fixed order.
 //
-// 10240 x 2560 from HBM 6.6 us, 51865 x 2560 16.6 (4.5 TB/s, near a copy's 5.1), 2560 x 2560 4.0: the small ones are a launch, one trip to memory and 1 us of
+// With a bias 10240 x 2560 from HBM 6.3 us, 51865 x 2560 17.0 (4.4 TB/s, near a copy's 5.1), 2560 x 2560 4.1: the small ones are a launch, one trip to memory and 1 us of
 // instructions.
 #include "device_common.h"
 
@@ -45,8 +45,9 @@ template <int NB, int NV> __global__ __launch_bounds__(512, NV == 1 ? 4 : 3) voi
     const half_t *const scales = g.scales + (g.a_stack == 1 ? 0 : s) * g.M * nb;
     struct Rows {
         uint4_t w[NB];
-        half_t d[NB];
+        half_t d[NB], bias;
     };
+    const half_t *const from = g.has_bias ? g.bias : g.X; // (read in any case, so that the loads in flight are the same number)
     auto load = [&](int64_t group, Rows &k) __attribute__((always_inline)) { // (rows and blocks past the end repeat the last)
         const int64_t row = min(4 * group + (lane >> 4), g.M - 1);
         const uint8_t *const w = codes + row * (g.K >> 1);
@@ -55,6 +56,7 @@ template <int NB, int NV> __global__ __launch_bounds__(512, NV == 1 ? 4 : 3) voi
         for (int i = 0; i < NB; i++) k.w[i] = *(const uint4_t *)(w + 16 * (uint32_t)min(b0 + 16 * i, nb - 1));
 #pragma unroll
         for (int i = 0; i < NB; i++) k.d[i] = d[min(b0 + 16 * i, nb - 1)];
+        k.bias = from[!g.has_bias ? 0 : g.bias_on_rows ? row : min(seg, NV - 1)];
     };
     const int64_t first = (int64_t)blockIdx.x * (threads / (64 * wk));
     Rows ring[2];
@@ -134,7 +136,7 @@ template <int NB, int NV> __global__ __launch_bounds__(512, NV == 1 ? 4 : 3) voi
         }
         const int64_t row = 4 * at + (lane >> 4);
         if (kc == 0 && seg < NV && row < g.M) {
-            if (g.has_bias) y += (float)g.bias[g.bias_on_rows ? row : seg];
+            if (g.has_bias) y += (float)k.bias;
             rt_with_act(g.act, [&](auto has_act) { y = rt_act_k<decltype(has_act)::value>(y); });
             g.out[s * g.o_bs + row * g.o_is + seg * g.o_js] = (half_t)y;
         }
@@ -169,7 +171,7 @@ template <int NB> static hipError_t launch_rowdot(const RowdotQ40Args &g, int wr
     return hipGetLastError();
 }
 
-// One or two vectors and K up to 10240, four wavefronts a workgroup (all sharing K where that is long), two workgroups per compute unit (us for 10240 x 2560 / 51865 x 2560, one vector:
+// One or two vectors and K up to 10240, four wavefronts a workgroup (all sharing K where that is long), two workgroups per compute unit (us without a bias for 10240 x 2560 / 51865 x 2560, one vector:
 // two 6.6 / 16.6, three 7.0 / 17.4; eight wavefronts 7.1 / 17.9).  The matrix-core kernel at one and two vectors and this: 10240 x 2560 8.4 / 8.3 and 6.6 / 7.5, 2560 x 10240 9.4 / 9.4 and 7.5 /
 // 10.0, 2560 x 2560 5.9 / 5.9 and 4.0 / 4.9, 51865 x 2560 21.5 / 21.8 and 16.6 / 20.4, 8192 x 8192 13.0 / 14.4 and 11.2 / 12.9, 640 x 1024 4.1 and 2.5; 4096 x 14336 13.0 / 13.0, here with six
 // wavefronts that share K 12.2 / 20.
