@@ -31,7 +31,7 @@
 namespace rt {
 
 constexpr float kLog2eQ4 = 1.4426950408889634f;
-constexpr int AQ_MAX_SPLITS = 64; // shares of a row
+constexpr int AQ_MAX_SPLITS = 64; // shares of a row of the prompt kernel
 constexpr int AQ_WAVES = 8;       // of a streaming workgroup
 
 struct AttnQ4Args {
@@ -737,36 +737,42 @@ template <int NT, int MK> __global__ __launch_bounds__(512, 2) void attention_q4
 // loads are requested at once, and the groups meet in LDS, in a fixed order.  (One thread a column that walked the shares took 20.9 us for 32 rows of 64 shares
 // of 128, this 2.9; 4800 rows of 6 shares of 64 with 16 groups, ten of them idle, and a row a workgroup 7.0.)
 template <int CG, int SG> __global__ __launch_bounds__(256) void attention_q4_merge_kernel(AttnQ4Args g, int D, int64_t rows) {
-    constexpr int R = 256 / (CG * SG), PER = SG < 8 ? 1 : AQ_MAX_SPLITS / SG; // (four groups: up to four shares)
+    constexpr int R = 256 / (CG * SG), PER = SG < 8 ? 1 : 64 / SG; // (four groups: up to four shares; others 64 at a time)
     __shared__ __attribute__((aligned(16))) float part[R][SG][4 * CG];
     const int t = threadIdx.x, c = t % CG, sg = t / CG % SG, rl = t / (CG * SG);
     const int64_t row = min((int64_t)blockIdx.x * R + rl, rows - 1);
     const bool live = 4 * c < D;
     const float *const po = g.part_o + row * g.splits * D + (live ? 4 * c : 0), *const pm = g.part_ml + row * g.splits * 2;
-    float4_t v[PER];
-    float2_t ml[PER];
-#pragma unroll
-    for (int i = 0; i < PER; i++)
-        if (i * SG < g.splits) { // (uniform)
-            const int s = min(i * SG + sg, g.splits - 1);
-            ml[i] = *(const float2_t *)(pm + 2 * s), v[i] = *(const float4_t *)(po + (int64_t)s * D);
-        }
     // this group's shares; one whose sum is 0 has no key, and no outputs were written
-    float top = -INFINITY;
-#pragma unroll
-    for (int i = 0; i < PER; i++)
-        if (i * SG < g.splits) top = fmaxf(top, ml[i][0]);
-    const float base = top == -INFINITY ? 0.f : top;
-    float l = 0.f;
+    float top = -INFINITY, l = 0.f;
     float4_t y = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll 1
+    for (int s0 = 0; s0 < g.splits; s0 += SG * PER) {
+        float4_t v[PER];
+        float2_t ml[PER];
 #pragma unroll
-    for (int i = 0; i < PER; i++)
-        if (i * SG < g.splits && i * SG + sg < g.splits && ml[i][1] != 0.f) {
-            const float a = __builtin_amdgcn_exp2f(ml[i][0] - base);
-            l = fmaf(a, ml[i][1], l);
+        for (int i = 0; i < PER; i++)
+            if (s0 + i * SG < g.splits) { // (uniform)
+                const int s = min(s0 + i * SG + sg, g.splits - 1);
+                ml[i] = *(const float2_t *)(pm + 2 * s), v[i] = *(const float4_t *)(po + (int64_t)s * D);
+            }
+        float now = top;
 #pragma unroll
-            for (int k = 0; k < 4; k++) y[k] = fmaf(a, v[i][k], y[k]);
-        }
+        for (int i = 0; i < PER; i++)
+            if (s0 + i * SG < g.splits) now = fmaxf(now, ml[i][0]);
+        const float base = now == -INFINITY ? 0.f : now, old = __builtin_amdgcn_exp2f(top - base);
+        top = now, l *= old;
+#pragma unroll
+        for (int k = 0; k < 4; k++) y[k] *= old;
+#pragma unroll
+        for (int i = 0; i < PER; i++)
+            if (s0 + i * SG < g.splits && s0 + i * SG + sg < g.splits && ml[i][1] != 0.f) {
+                const float a = __builtin_amdgcn_exp2f(ml[i][0] - base);
+                l = fmaf(a, ml[i][1], l);
+#pragma unroll
+                for (int k = 0; k < 4; k++) y[k] = fmaf(a, v[i][k], y[k]);
+            }
+    }
     __shared__ float mls[R][SG][2];
     *(float4_t *)&part[rl][sg][4 * c] = y;
     if (c == 0) mls[rl][sg][0] = top, mls[rl][sg][1] = l;
@@ -802,7 +808,7 @@ static int64_t aq_row_tiles(int rows) { return aq_streams(rows) ? 1 : (rows + AP
 // Keys of a workgroup where several share a row tile's, and how many do.
 // The streaming kernel: as many as fill the 256 compute units once (a workgroup's eight wavefronts leave no room for a second; two rounds of half the keys, 32 x 8
 // heads on 8192 keys of 128: 62 -> 69 us), down to one step each, but two steps (1024 keys) in one launch (32 heads of 80: 8.0 us, in two shares 8.7; four steps 12.3,
-// in four shares 9.1).
+// in four shares 9.1; 8 heads on one of 128, 131072 keys: 256 shares 16.4, 64 of four steps 20.1).
 // The other: the least of what its rounds of workgroups, the partial results and the second launch take.  A step is some 1.4 + 0.017 head_dim us (2.5, 3.1 and 3.6
 // measured at 64, 96 and 128), partial results are written and read at 2.5 TB/s (us for shares: 32 x 128 rows on 1024 keys of 80: 1: 21.3, 4: 16.2, 8: 20.0; 32 x 32 on 544: 1:
 // 13.9, 2: 13.6, 5: 10.7; 2 x 4 x 600 on 1373 keys of 64: 3: 21.6, 6: 19.6, 11: 26.4).
@@ -812,7 +818,7 @@ static void aq_split(const rt_attention_q4_desc &d, int &splits, int &split_keys
     const int unit = aq_streams(rows) ? 64 * AQ_WAVES : AP_KEYS, steps = std::max(1, (d.kv_len + unit - 1) / unit);
     int64_t s = 1;
     if (aq_streams(rows)) {
-        s = steps <= 2 ? 1 : std::max<int64_t>(1, std::min<int64_t>({AQ_MAX_SPLITS, steps, 256 / wgs}));
+        s = steps <= 2 ? 1 : std::max<int64_t>(1, std::min<int64_t>(steps, 256 / wgs));
     } else if (wgs < 2048) { // (more rounds than eight lose little at their end)
         const double step = 1.4 + 0.017 * d.head_dim, part = (double)stacks * rows * (d.head_dim + 2) * 8 / 2.5e6;
         double best = 0;
