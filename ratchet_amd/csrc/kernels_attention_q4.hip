@@ -552,6 +552,7 @@ template <int NT, int MK> __global__ __launch_bounds__(512, 2) void attention_q4
     constexpr float unit = MK ? kLog2eQ4 : 1.f;
     float m_run[2], l_run[2];
     uint32_t bad[2];
+    bool coarse = false; // whether a reference was too large for scores that are not rounded (uniform)
 #pragma unroll
     for (int u = 0; u < 2; u++) {
         m_run[u] = -INFINITY, l_run[u] = 0.f, bad[u] = 0;
@@ -620,16 +621,25 @@ template <int NT, int MK> __global__ __launch_bounds__(512, 2) void attention_q4
                 }
             }
             bmax = rt_groups_max(bmax);
-            // the reference follows the maximum only where that is some 2^8 past it (or it has none): the outputs and the sum are seldom rescaled
-            if (__builtin_amdgcn_ballot_w64(bmax > m_run[u] + (MK ? 5.5f : 8.f))) {
+            // the reference follows the maximum only where that is some 2^8 past it (or it has none): the outputs and the sum are seldom rescaled.  (Their difference, which
+            // is exact where it is small: between 2^27 and 2^28 the reference plus 8 may round to the next f32, 16 away, and a probability of 2^16 is no f16.)
+            float sc = LEAN && MK == 0 ? g.scale_log2e : 1.f;
+            if (__builtin_amdgcn_ballot_w64(bmax - m_run[u] > (MK ? 5.5f : 8.f))) {
                 const float m_new = fmaxf(m_run[u], bmax), alpha = m_new == -INFINITY ? 1.f : __builtin_amdgcn_exp2f((m_run[u] - m_new) * unit);
                 m_run[u] = m_new;
                 l_run[u] *= alpha;
 #pragma unroll
                 for (int d = 0; d < NT; d++) acc[u][d] *= alpha;
+                // The reference is a rounded product and a score meets it in the fused multiply-add without a rounding of its own: past 4096 that shows, 2^-12 and more between
+                // blocks here and those that round their scores, and past 2^28 a probability would leave f16.  From there on scores are rounded first.
+                if (LEAN && MK == 0 && __builtin_amdgcn_ballot_w64(!(__builtin_fabsf(m_new) < 4096.f))) {
+                    coarse = true;
+#pragma unroll
+                    for (int e = 0; e < 16; e++) S[u][e >> 2][e & 3] *= g.scale_log2e;
+                    sc = 1.f;
+                }
             }
             const float m_use = m_run[u] == -INFINITY ? 0.f : m_run[u]; // a row without a key yet: exp2(-inf - 0) = 0
-            const float sc = LEAN && MK == 0 ? g.scale_log2e : 1.f;
             float psum = 0.f;
 #pragma unroll
             for (int e = 0; e < 16; e += 2) {
@@ -673,7 +683,7 @@ template <int NT, int MK> __global__ __launch_bounds__(512, 2) void attention_q4
             __syncthreads();
             stage ^= 1, j0 += AP_KEYS;
         };
-        while (j0 + kj + 64 <= w_lean) turn([&]() { step(stage, j0 + kj, std::true_type{}); });
+        while (j0 + kj + 64 <= w_lean && !coarse) turn([&]() { step(stage, j0 + kj, std::true_type{}); });
         while (j0 + kj < w_end) turn([&]() { step(stage, j0 + kj, std::false_type{}); });
         while (j0 < j_end) turn([]() {}); // blocks that only other wavefronts need
     }
