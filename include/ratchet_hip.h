@@ -527,7 +527,10 @@ RT_API rt_status rt_cache_write_q4_enqueue(rt_ctx *ctx, int32_t src_dtype, void 
  *             F32 or F16; a key whose mask is -inf is not seen, whatever its score or value
  * A row that sees no key is NaN, as in rt_attention_enqueue.  Rows of the caches past a sequence's length are not used.
  * Sums, maxima and scores are f32; the probabilities enter the second product as f16; a scale of the cache with more
- * than eight significant bits makes values that round to f16.
+ * than eight significant bits makes values that round to f16.  A scale that is not finite, or above 8188 in magnitude
+ * (eight times that is the last f16; rt_cache_write_q4_enqueue makes none past 8160): of values, its dimensions are NaN in the
+ * rows that see the key; of keys, the rows that see the key are NaN where the scale is, and not defined else; rows that do
+ * not see it are untouched by either.
  * Limits (RT_ERR_UNSUPPORTED beyond): 65535 sequences times kv_heads, 2^30 keys, 2^21 query rows of the heads that share a head of
  * keys, and 2^24 tiles of 128 of them in a call. */
 typedef struct rt_attention_q4_desc {

@@ -79,6 +79,10 @@ template <int NT> struct AqDims {
     }
 };
 
+// Whether the f16 values of a scale are finite: eight times 8188 is 65504, the largest.  One past it (the cache's write makes none) counts as one that is not finite: as
+// an infinite operand of the matrix cores, a key that a row does not see would reach it as 0 * inf.
+__device__ __forceinline__ bool aq_finite(uint32_t bits) { return (bits & 0x7FFFu) <= 0x6FFFu; }
+
 // Loads with a bound: past `bytes` the hardware returns zeros, and so codes of keys past the last have scales of zero.
 __device__ __forceinline__ __amdgpu_buffer_rsrc_t aq_bounded(const void *p, int bytes) {
     return __builtin_amdgcn_make_buffer_rsrc(const_cast<void *>(p), 0, bytes, 0x00027000); // raw, 32-bit data
@@ -273,7 +277,7 @@ template <int NT, int VPR, int MK> __global__ __launch_bounds__(512) void attent
 #pragma unroll
         for (int n = 0; n < NB; n++) {
             const half_t d = __builtin_bit_cast(half2_t, k.dv[n >> 1])[n & 1];
-            const bool fin = (__builtin_bit_cast(uint16_t, d) & 0x7C00u) != 0x7C00u;
+            const bool fin = aq_finite(__builtin_bit_cast(uint16_t, d));
             if (!fin) odd |= 1u << n;
             S[n * 64 + 4 * r + fg] = fin ? d : (half_t)0.f;
         }
@@ -513,7 +517,7 @@ template <int NT, int MK> __global__ __launch_bounds__(512, 2) void attention_q4
             const bool val = !is_key(i);
             const uint32_t f = (uint32_t)(i * 512 + t - (val ? 256 * NT : 0)), key = so[i] / (2 * SR);
             half_t d = __builtin_bit_cast(half_t, (uint16_t)ds[i]);
-            const bool fin = (ds[i] & 0x7C00u) != 0x7C00u;
+            const bool fin = aq_finite(ds[i]);
             if (val) { // a value that is not finite shows in the rows that see its key, and not through the matrix cores
                 odd |= !fin;
                 d = fin ? d : (half_t)0.f;
@@ -616,7 +620,7 @@ template <int NT, int MK> __global__ __launch_bounds__(512, 2) void attention_q4
                 for (int e = 0; e < 16 * KK; e++) {
                     const int k = e >> 4;
                     const uint32_t j = (uint32_t)min(j0 + 4 * (e & 12) + 4 * fg + (e & 3), len - 1);
-                    const bool fin = (__builtin_bit_cast(uint16_t, Vs[j * SR + k]) & 0x7C00u) != 0x7C00u;
+                    const bool fin = aq_finite(__builtin_bit_cast(uint16_t, Vs[j * SR + k]));
                     if (!fin && ((seen >> (e & 15)) & 1u)) bad[u] |= 1u << k;
                 }
             }

@@ -2,7 +2,7 @@
 import numpy as np
 import pytest
 
-from test_cache_q4 import blocks, buffer, run
+from test_cache_q4 import blocks, buffer, check, reference, run, values
 
 gpu = pytest.mark.gpu
 
@@ -56,3 +56,52 @@ def test_large_scores_a_step_apart(device, step):
             for ws in (True, False):
                 got = run(device, q, kbuf, vbuf, 1, n, length, 1.0, workspace=ws).astype(np.float64)
                 assert ((got >= 1 - 2.0**-10) & (got <= 2 + 2.0**-9)).all(), (base, got[0, 0, :, 0])
+
+
+@gpu
+@pytest.mark.parametrize("lq", [1, 6, 13, 17, 40, 150])
+@pytest.mark.parametrize("d", [48, 96, 128])
+def test_scales_above_what_a_value_can_follow(device, lq, d):
+    """8188 is the last scale whose values, up to eight times it, are f16 numbers; from 8192 on a block counts as one that is not finite.  Hidden, by a mask or by the causal flag, it
+    changes nothing; seen it leaves other rows alone, and is NaN in its dimensions (values; a row that sees such keys is not defined)."""
+    rng = np.random.default_rng(d + lq)
+    n = 333
+    codes = rng.integers(0, 16, (1, 1, n, d), dtype=np.uint8)
+    vcodes = rng.integers(0, 16, (1, 1, n, d), dtype=np.uint8)
+    ds = np.full((1, 1, n, blocks(d)), 0.125, np.float16)
+    q = rng.standard_normal((1, 1, lq, d)).astype(np.float16)
+    q[..., 32:] *= np.float16(0.01)
+    mask = rng.uniform(-2, 2, (lq, n)).astype(np.float32)
+    hidden = [7, 64, 200, 332]
+    mask[:, hidden] = -np.inf
+    for big in (16384.0, -8192.0, 65504.0, np.inf):
+        kds, vds = ds.copy(), ds.copy()
+        kds[0, 0, hidden, 1], vds[0, 0, hidden, 1] = big, big
+        codes[0, 0, hidden, 32:], vcodes[0, 0, hidden, 32:] = 0, 0
+        plain = lambda c: values(c, ds)
+        want, tol = reference(q, plain(codes), plain(vcodes), 0.1, mask=mask)
+        for ws in (True, False):
+            check(run(device, q, buffer(codes, kds), buffer(vcodes, vds), 1, n, n, 0.1, mask=mask, workspace=ws), want, tol)
+        # seen, by the last row alone
+        open_ = mask.copy()
+        open_[lq - 1, 200] = 0
+        got = run(device, q, buffer(codes, kds), buffer(vcodes, ds), 1, n, n, 0.1, mask=open_)
+        check(got[:, :, : lq - 1], *(x[:, :, : lq - 1] for x in reference(q, plain(codes), plain(vcodes), 0.1, mask=open_)))
+        got = run(device, q, buffer(codes, ds), buffer(vcodes, vds), 1, n, n, 0.1, mask=open_)
+        assert np.isnan(got[0, 0, lq - 1, 32:64]).all() and np.isfinite(got[0, 0, lq - 1, :32]).all() and np.isfinite(got[0, 0, lq - 1, 64:]).all(), big
+        # the last key is seen by the last row alone
+        kds, vds = ds.copy(), ds.copy()
+        kds[0, 0, n - 1, 1], vds[0, 0, n - 1, 1] = big, big
+        want, tol = (x[:, :, : lq - 1] for x in reference(q, plain(codes), plain(vcodes), 0.1, causal=True))
+        check(run(device, q, buffer(codes, kds), buffer(vcodes, vds), 1, n, n, 0.1, causal=True)[:, :, : lq - 1], want, tol)
+        got = run(device, q, buffer(codes, ds), buffer(vcodes, vds), 1, n, n, 0.1, causal=True)
+        assert np.isnan(got[0, 0, lq - 1, 32:64]).all()
+        check(got[:, :, : lq - 1], want, tol)
+    # 8188: values up to 65504, all of them f16 numbers
+    kds, vds = ds.copy(), ds.copy()
+    kds[0, 0, 200, 1] = vds[0, 0, 200, 1] = 8188
+    codes[0, 0, 200, 32:64] = 8
+    codes[0, 0, 200, 32], vcodes[0, 0, 200, 32:64] = 0, rng.integers(0, 2, min(d, 64) - 32) * 15
+    q[..., 32] = np.float16(2.0**-14)  # a score of -4
+    want, tol = reference(q, values(codes, kds), values(vcodes, vds), 0.1)
+    check(run(device, q, buffer(codes, kds), buffer(vcodes, vds), 1, n, n, 0.1), want, tol)
