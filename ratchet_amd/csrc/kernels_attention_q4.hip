@@ -8,7 +8,7 @@
 // block's sum scaled by dk in f32.  A load is 16 bytes a lane of consecutive pieces of consecutive keys, and a 4 x 4 transposition among lane
 // groups puts dword g of a block into lane group g, as the operand wants it (kernels_gemv_q40.hip has the same step).  Rows up to 4 (8) are put at
 // MFMA rows 4 m (4 m, 4 m + 1), where one result register (two) holds them all.
-// Softmax: running maximum and sum in f32, base 2; a row's keys are spread over 16 lanes, which four DPP rotations join for the maximum, and only at
+// Softmax: running reference and sum in f32, base 2; a row's keys are spread over 16 lanes, which four DPP rotations join for the maximum, and only at
 // the end for the sum.
 // Values: the operand of the second product holds, for one dimension, eight keys in a lane.  Codes of one key are neighbours along the dimensions, so
 // lane c (of 16) reads four bytes of each key's row (two up to a head_dim of 64, one up to 32; a row of 80 takes ten lanes, which costs less than the second load
@@ -33,6 +33,10 @@ namespace rt {
 constexpr float kLog2eQ4 = 1.4426950408889634f;
 constexpr int AQ_MAX_SPLITS = 64; // shares of a row of the prompt kernel
 constexpr int AQ_WAVES = 8;       // of a streaming workgroup
+// The exponentials' reference (mx, m_run below, in base 2) is this much below a block's maximum.  As f16 a probability goes down to 2^-25, so that against the largest none of
+// more than 2^-32 is lost (with the maximum itself as reference 2^16 keys of 2^-25.5 each beside one of 1 were, an eighth or half of them, those of its wavefront).  Below 8, since
+// what is left of a difference of 8 and more may round to 16 where an f32's step is that, between 2^27 and 2^28, and 2^16 is no f16.
+constexpr float AQ_BELOW = 7.f;
 
 struct AttnQ4Args {
     const half_t *Q;
@@ -255,7 +259,7 @@ template <int NT, int VPR, int MK> __global__ __launch_bounds__(512) void attent
                 if (!inside) x = j0 + 16 * s + r <= last[v] ? x : -INFINITY;
                 sc[s][v] = x;
             }
-            const float top = fmaxf(mx[v], aq_max16(fmaxf(fmaxf(sc[0][v], sc[1][v]), fmaxf(sc[2][v], sc[3][v]))));
+            const float top = fmaxf(mx[v], aq_max16(fmaxf(fmaxf(sc[0][v], sc[1][v]), fmaxf(sc[2][v], sc[3][v]))) - AQ_BELOW);
             const float base = top == -INFINITY ? 0.f : top;
             const float a = __builtin_amdgcn_exp2f(mx[v] - base);
             mx[v] = top;
@@ -407,7 +411,7 @@ template <int NT, int VPR, int MK> __global__ __launch_bounds__(512) void attent
 //   S = K Q^T: keys first, so that a lane holds one row's scores of 16 keys, and the maximum needs two steps across lanes.
 //   O += V^T P: the lane's probabilities are an operand as they lie; the values' comes transposed out of LDS (ds_read_b64_tr_b16).
 // The exponentials' reference follows the row's maximum only where that has risen by some 2^8, so that outputs and sums are seldom rescaled; f16 rounds a probability
-// of 2^8 as it does one of 1, relatively.  The sum is that of the rounded probabilities.
+// of 2^15 as it does one of 1, relatively.  The sum is that of the rounded probabilities.
 // Two groups of four wavefronts have halves of the 128 keys of a step and are joined at the end: one workgroup per compute unit then has two wavefronts per SIMD at any
 // length (four wavefronts and two workgroups took as long as the longer of the two: 2048 x 2048 x 32 heads x 96 causal 70 us, this 50).
 // us: 2048 x 2048 x 32 heads, causal, of 96 / 128 dimensions 50 / 59; 2 x 512 rows of 32 heads on 8 x 4096 keys of 128 87 (790 TFLOP/s), of 64 59.  Bound by instruction
@@ -625,11 +629,11 @@ template <int NT, int MK> __global__ __launch_bounds__(512, 2) void attention_q4
                 }
             }
             bmax = rt_groups_max(bmax);
-            // the reference follows the maximum only where that is some 2^8 past it (or it has none): the outputs and the sum are seldom rescaled.  (Their difference, which
-            // is exact where it is small: between 2^27 and 2^28 the reference plus 8 may round to the next f32, 16 away, and a probability of 2^16 is no f16.)
+            // the reference follows the maximum only where that is some 2^15 past it (or it has none), and then 2^8 past where it was: the outputs and the sum are seldom rescaled.
+            // (Their difference, which is exact where it is small: a sum may round.  2^15 is below f16's last, 2^16 is not.)
             float sc = LEAN && MK == 0 ? g.scale_log2e : 1.f;
-            if (__builtin_amdgcn_ballot_w64(bmax - m_run[u] > (MK ? 5.5f : 8.f))) {
-                const float m_new = fmaxf(m_run[u], bmax), alpha = m_new == -INFINITY ? 1.f : __builtin_amdgcn_exp2f((m_run[u] - m_new) * unit);
+            if (__builtin_amdgcn_ballot_w64(bmax - m_run[u] > 15.f / unit)) {
+                const float m_new = fmaxf(m_run[u], bmax - AQ_BELOW / unit), alpha = m_new == -INFINITY ? 1.f : __builtin_amdgcn_exp2f((m_run[u] - m_new) * unit);
                 m_run[u] = m_new;
                 l_run[u] *= alpha;
 #pragma unroll

@@ -105,3 +105,30 @@ def test_scales_above_what_a_value_can_follow(device, lq, d):
     q[..., 32] = np.float16(2.0**-14)  # a score of -4
     want, tol = reference(q, values(codes, kds), values(vcodes, vds), 0.1)
     check(run(device, q, buffer(codes, kds), buffer(vcodes, vds), 1, n, n, 0.1), want, tol)
+
+
+@gpu
+@pytest.mark.parametrize("lq", [1, 6, 13, 17, 150])
+@pytest.mark.parametrize("masked", [False, True])
+def test_a_long_tail_beside_one_large_probability(device, lq, masked):
+    """One key 25.5 powers of two above 2^16 others, that weigh 2^-9.5 together and, since its value is 0, are all that a row consists of.  As f16 numbers
+    relative to the largest they would be lost: what a probability is rounded to, 2^-25 of the largest at least, is more than they are.  With one workgroup, and so on the keys of one wavefront in eight
+    (one half of them), or with shares.  Tolerance: as in test_cache_q4, but for its 2^-25 sum_j |v| / l, which is 2^-32 here: a probability of the largest is held at 2^7 or more of f16."""
+    n, d = 1 << 16, 32
+    rng = np.random.default_rng(lq)
+    kc, kd = np.full((1, 1, n, d), 8, np.uint8), np.full((1, 1, n, 1), 0.5, np.float16)
+    at = 1000
+    kc[0, 0, at, 0] = 12  # 2 in dimension 0
+    vc, vd = rng.integers(9, 16, (1, 1, n, d), dtype=np.uint8), np.full((1, 1, n, 1), 8.0, np.float16)
+    vc[0, 0, at] = 8
+    q = np.zeros((1, 1, lq, d), np.float16)
+    q[..., 0] = np.linspace(0.99, 1, lq)
+    scale = np.float32(25.5 * np.log(2) / 2)
+    mask = np.zeros((lq, n), np.float16) if masked else None
+    kval, vval = values(kc, kd), values(vc, vd)
+    want, tol = reference(q, kval, vval, float(scale), mask=mask)
+    s = q[0, 0, :, 0].astype(np.float64) * 2 * float(scale)
+    tol -= ((2.0**-25 - 2.0**-32) * vval[0, 0].sum(0)[None] / (1 + n * np.exp(-s))[:, None])[None, None]
+    assert (want > 0.01).all() and (tol < 0.02 * want).all()
+    for ws in (True, False):
+        check(run(device, q, buffer(kc, kd), buffer(vc, vd), 1, n, n, scale, mask=mask, workspace=ws), want, tol)
