@@ -532,7 +532,7 @@ RT_API rt_status rt_cache_write_q4_enqueue(rt_ctx *ctx, int32_t src_dtype, void 
  * rows that see the key; of keys, the rows that see the key are NaN where the scale is, and not defined else; rows that do
  * not see it are untouched by either.
  * Limits (RT_ERR_UNSUPPORTED beyond): 65535 sequences times kv_heads, 2^30 keys, 2^21 query rows of the heads that share a head of
- * keys, and 2^24 tiles of 128 of them in a call. */
+ * keys, and, where these are more than 16, 2^23 - 1 tiles of 128 of them in a call. */
 typedef struct rt_attention_q4_desc {
     int32_t batch, heads, kv_heads;
     int32_t q_len, kv_len;

@@ -725,6 +725,7 @@ rt_status rt_attention_q4_validate(const rt_attention_q4_desc *d) {
     if (!(d->scale == d->scale)) return RT_ERR_INVALID_ARG;
     if ((int64_t)d->batch * d->kv_heads > 65535 || d->kv_len > (1 << 30)) return RT_ERR_UNSUPPORTED;
     if (d->heads > 0 && (int64_t)d->q_len * (d->heads / d->kv_heads) > 32 * 65535) return RT_ERR_UNSUPPORTED;
+    if (!rt::attention_q4_fits(*d)) return RT_ERR_UNSUPPORTED;
     return RT_OK;
 }
 
@@ -754,7 +755,6 @@ rt_status rt_attention_q4_enqueue(rt_ctx *ctx, const rt_attention_q4_desc *desc,
     DeviceGuard dg(ctx->dev.ordinal);
     if (!dg.ok) return fail(ctx, RT_ERR_NO_DEVICE, "hipSetDevice failed");
     hipError_t e = rt::launch_attention_q4(*desc, q, k_cache, v_cache, mask, kv_lens, out, workspace, workspace_bytes, (hipStream_t)stream, ctx->dev);
-    if (e == hipErrorNotSupported) return fail(ctx, RT_ERR_UNSUPPORTED, "attention: too many rows");
     if (e != hipSuccess) return hip_fail(ctx, "attention launch", e);
     return RT_OK;
     RT_GUARD_END(ctx)

@@ -276,6 +276,7 @@ hipError_t launch_cache_write(void *cache, const void *src, void *cache2, const 
 hipError_t launch_cache_write_q4(int src_dtype, void *k_cache, const void *k_src, void *v_cache, const void *v_src, const int64_t *strides, void *k_values,
                                  void *v_values, const int32_t *offsets, int batch, int heads, int capacity, int offset, int len, int head_dim,
                                  hipStream_t stream);
+bool attention_q4_fits(const rt_attention_q4_desc &d); // (of a descriptor that is valid else)
 uint64_t attention_q4_workspace_bytes(const rt_attention_q4_desc &d);
 hipError_t launch_attention_q4(const rt_attention_q4_desc &d, const void *q, const void *k_cache, const void *v_cache, const void *mask,
                                const int32_t *kv_lens, void *out, void *workspace, uint64_t workspace_bytes, hipStream_t stream, const DeviceInfo &dev);

@@ -849,6 +849,13 @@ static void aq_split(const rt_attention_q4_desc &d, int &splits, int &split_keys
     splits = (steps + per - 1) / per, split_keys = (int)std::min<int64_t>((int64_t)per * unit, 1 << 30);
 }
 
+// A grid's threads along an axis are fewer than 2^32, and the prompt kernel's workgroups, of 512, lie along one.  Shares take no call past that: there are none from 2048
+// workgroups on, and at most 64 of a tile (the streaming kernel's lie along the other axis); the join then has at most 2^18 rows.
+bool attention_q4_fits(const rt_attention_q4_desc &d) {
+    if (d.batch == 0 || d.heads == 0 || d.q_len == 0) return true;
+    return aq_row_tiles(d.q_len * (d.heads / d.kv_heads)) * d.batch * d.kv_heads <= 0x7fffff;
+}
+
 uint64_t attention_q4_workspace_bytes(const rt_attention_q4_desc &d) {
     if (d.batch == 0 || d.heads == 0 || d.q_len == 0) return 0;
     int splits, keys;
@@ -900,7 +907,6 @@ hipError_t launch_attention_q4(const rt_attention_q4_desc &d, const void *q, con
     }
     const int64_t tiles = aq_row_tiles(g.rows), stacks = (int64_t)d.batch * d.kv_heads;
     g.row_tiles = (int)tiles;
-    if (tiles * stacks * g.splits > 0xffffff || (g.splits > 1 && stacks * g.rows > 0xffffff)) return hipErrorNotSupported; // (a grid's threads along an axis are fewer than 2^32)
     const dim3 grid((unsigned)g.splits, (unsigned)stacks);
     auto go = [&](auto nt) -> hipError_t {
         constexpr int NT = decltype(nt)::value;

@@ -1,10 +1,33 @@
 """Attention over 4-bit caches at the ends of its numbers' range.  Caches and the call are those of test_cache_q4."""
+import ctypes
+
 import numpy as np
 import pytest
 
-from test_cache_q4 import blocks, buffer, check, reference, run, values
+from ratchet_amd import _ffi
+from test_cache_q4 import attention_desc, blocks, buffer, check, reference, run, values
 
 gpu = pytest.mark.gpu
+
+
+def test_tiles_of_a_call():
+    """A launch has fewer than 2^32 threads along an axis, 2^23 - 1 workgroups of 512, a tile of 128 rows each; up to 16 rows per head of keys take no tiles."""
+    L, need = _ffi.lib(), ctypes.c_uint64()
+    for batch, kv, heads, lq, want in ((65535, 1, 1, 128 * 128, 0), (65535, 1, 1, 128 * 128 + 1, _ffi.RT_ERR_UNSUPPORTED), (8191, 8, 64, 2048, 0), (8191, 8, 64, 2049, _ffi.RT_ERR_UNSUPPORTED),
+                                       (511, 1, 1, 32 * 65535, 0), (512, 1, 1, 32 * 65535, _ffi.RT_ERR_UNSUPPORTED), (65535, 1, 16, 1, 0), (1, 1, 1, 32 * 65535, 0)):
+        for n in (1, 1000, 1 << 30):
+            d = attention_desc(batch, heads, kv, lq, n, 16, n)
+            assert L.rt_attention_q4_validate(ctypes.byref(d)) == want, (batch, kv, lq, n)
+            assert L.rt_attention_q4_workspace_bytes(ctypes.byref(d), ctypes.byref(need)) == want
+            if want == 0:  # and the shares that a workspace makes are no more, nor the rows that a second launch joins
+                tiles, shares = batch * kv * -(-lq * heads // kv // 128), need.value // (batch * heads * lq * 18 * 4)
+                assert lq * heads // kv <= 16 or tiles * max(shares, 1) < 1 << 23
+                assert not shares or batch * heads * lq <= 1 << 18
+    for k in (dict(batch=0), dict(heads=0, kv_heads=0), dict(q_len=0)):
+        d = attention_desc(2, 8, 4, 3, 50, 64, 60)
+        for name, v in k.items():
+            setattr(d, name, v)
+        assert L.rt_attention_q4_validate(ctypes.byref(d)) == 0
 
 
 def one_dimension(n, d, k0, v0, extra=None):
