@@ -337,6 +337,8 @@ class CacheQ4:
     F16 or F32.  `offsets`: an int32 GPU tensor of torch, one more offset per sequence; rows outside the cache are then not written."""
 
     def __init__(self, cache: "Tensor", source: "Tensor", offset: int, offsets=None):
+        if not cache.is_q4_cache:
+            raise InvariantError(_ffi.RT_ERR_DTYPE_MISMATCH, "cache: a Q4_0 weight is no cache (Tensor.empty_cache makes one)")
         self.cache, self.source, self.offset, self.fresh = cache, source, int(offset), False
         B, H, cap, D = cache.shape
         if len(source.shape) == 3 and source.shape[0] == B and source.shape[2] == H * D:
@@ -351,8 +353,6 @@ class CacheQ4:
         self.out_shape = cache.shape
 
     def check_invariants(self):
-        if not self.cache.is_q4_cache:
-            raise InvariantError(_ffi.RT_ERR_DTYPE_MISMATCH, "cache: a Q4_0 weight is no cache (Tensor.empty_cache makes one)")
         if self.source.dt not in (DType.F16, DType.F32):
             raise InvariantError(_ffi.RT_ERR_DTYPE_MISMATCH, "cache: the source is F16 or F32")
 
