@@ -328,6 +328,8 @@ def cache_q4_nbytes(shape: Sequence[int]):
     n, at = ctypes.c_uint64(), ctypes.c_uint64()
     if len(shape) != 4:
         raise InvariantError(_ffi.RT_ERR_INVALID_SHAPE, "cache: rank 4 expected")
+    if any(s > 0x7fffffff for s in shape):   # (ctypes would pass such a size modulo 2^32)
+        raise OperationError(_ffi.RT_ERR_INVALID_SHAPE, f"cache: {tuple(shape)}")
     _check(_ffi.lib().rt_cache_q4_nbytes(*map(int, shape), ctypes.byref(n), ctypes.byref(at)))
     return n.value, at.value
 

@@ -3,6 +3,7 @@ import numpy as np
 import pytest
 
 from ratchet_amd import DType, Device, InvariantError, OperationError, Tensor, _ffi
+from ratchet_amd.tensor import cache_q4_nbytes
 
 CPU = Device.CPU
 
@@ -17,3 +18,12 @@ def test_a_weight_of_any_rank_is_no_cache(shape):
     with pytest.raises(InvariantError) as e:
         w.cache_write(halves(2, 3, 1, 64), 0)
     assert e.value.status == _ffi.RT_ERR_DTYPE_MISMATCH
+
+
+def test_sizes_past_31_bits():
+    """What does not fit the interface's int32 is refused, not taken modulo 2^32: a cache of 2^32 + 5 rows had the bytes of one of 5, and a write at row 2^32 + 1 went to row 1."""
+    for shape in ((1, 1, 2**32 + 5, 64), (2**32 + 1, 1, 8, 64), (1, 2**32 + 1, 8, 64), (1, 1, 8, 2**32 + 64), (1, 1, 2**31, 64), (1, 1, -1, 64)):
+        with pytest.raises(OperationError) as e:
+            Tensor.empty_cache(shape, CPU, DType.Q4_0)
+        assert e.value.status == _ffi.RT_ERR_INVALID_SHAPE, shape
+    assert cache_q4_nbytes((1, 1, 2**31 - 1, 64)) == (2**31 * 36, 2**31 * 32)
