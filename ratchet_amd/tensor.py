@@ -540,6 +540,8 @@ class Tensor:
         """A key or value cache [batch, heads, capacity, head_dim], zeros: F16 or F32, or Q4_0, held in 4-bit blocks."""
         shape = tuple(map(int, shape))
         if DType(dt) != DType.Q4_0:
+            if DType(dt).is_quantized():
+                raise OperationError(_ffi.RT_ERR_UNSUPPORTED, f"cache: {DType(dt).name}")
             return Tensor.from_data(np.zeros(shape, dtype=DType(dt).numpy())).to(device)
         n = max(cache_q4_nbytes(shape)[0], 16)
         t = Tensor(shape, DType.Q4_0, device, _torch().zeros(n, dtype=_torch().uint8, device=device.torch_device()) if device.is_gpu() else np.zeros(n, np.uint8))

@@ -2,7 +2,7 @@
 import numpy as np
 import pytest
 
-from ratchet_amd import DType, Device, InvariantError, OperationError, Tensor, _ffi
+from ratchet_amd import DType, Device, InvariantError, OperationError, Tensor, _ffi, nn
 from ratchet_amd.tensor import cache_q4_nbytes
 
 CPU = Device.CPU
@@ -27,3 +27,15 @@ def test_sizes_past_31_bits():
             Tensor.empty_cache(shape, CPU, DType.Q4_0)
         assert e.value.status == _ffi.RT_ERR_INVALID_SHAPE, shape
     assert cache_q4_nbytes((1, 1, 2**31 - 1, 64)) == (2**31 * 36, 2**31 * 32)
+
+
+def test_types_of_a_cache():
+    """F16, F32 and Q4_0; others are refused with the library's error, also through the modules."""
+    for dt in (DType.F16, DType.F32):
+        c = Tensor.empty_cache((1, 2, 8, 64), CPU, dt)
+        assert c.dt == dt and not c.is_q4_cache and not c.storage.any()
+    for make in (lambda dt: Tensor.empty_cache((1, 2, 8, 64), CPU, dt), lambda dt: nn.KVCache(1, (1, 2, 8, 64), CPU, dt)):
+        for dt in (DType.Q8_0H, DType.Q8_0F, DType.Q4_K):
+            with pytest.raises(OperationError) as e:
+                make(dt)
+            assert e.value.status == _ffi.RT_ERR_UNSUPPORTED
