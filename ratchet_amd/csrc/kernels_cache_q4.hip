@@ -4,12 +4,12 @@
 //   d = -sign(m) * min(r(t), 8160),  r: rounded to eight significant bits, and to multiples of 2^-24,
 //   q = clamp(floor(x / d + 8.5), 0, 15)   (d = 0: 8),   the value held: d * (q - 8).
 // Eight significant bits of d and three of q - 8 (or a power of two) fit an f16, so the values held are f16 numbers and a reader may scale codes in f16
-// without a rounding; m itself is met to 2^-9.  A block with a NaN or an infinity gets d = NaN.
+// without a rounding; m itself is met to 2^-8 from 2^-14 up (the limit included: 65504 is held as 65280) and to 2^-22 below.  A block with a NaN or an infinity gets d = NaN.
 //
 // The quotient is x * rcp(d) here.  Where x / d is not half way between two codes it is at least 2^-12 away from that: x has 11 significant bits
-// and d eight, |x| >= |d| / 2 there, so 2 x - (2 n + 1) d is a multiple of 2^-3 units of d's last place, and 2 |d| is at most 510 of them.  The product is
-// within 2^-18 of the quotient (|x / d| < 8.1, the reciprocal within an ulp or so), and 2^-15 added before the floor sends every half way up, as the
-// formula does, and nothing else.
+// and d eight, |x| >= |d| / 2 there, so 2 x - (2 n + 1) d is a multiple of 2^-3 units of d's last place, and 2 |d| is at most 510 of them.  (Where d is k < 256 times 2^-24, x is a
+// multiple of 2^-24 too, and the distance at least 1 / (2 k).)  |x / d| is below 12: about 8, and up to 11 where d is 2^-24.  The product is within 2^-18 of it, the reciprocal
+// being right to an ulp or so and the sum with 8.5 rounded to 2^-20, and 2^-15 added before the floor sends every half way up, as the formula does, and nothing else.
 #include "device_common.h"
 
 #include <algorithm>
