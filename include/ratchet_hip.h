@@ -523,7 +523,7 @@ RT_API rt_status rt_cache_write_q4_enqueue(rt_ctx *ctx, int32_t src_dtype, void 
  *   kv_len    rows of the caches that are in use; with `kv_lens` (batch int32 in device memory, or NULL) sequence b has
  *             kv_lens[b] of them, taken between 0 and kv_len
  *   causal    key j is visible to query i iff j <= i + (the sequence's length - q_len)
- *   mask      NULL, or additive, [q_len, kv_len] per sequence (mask_strides: sequence, 0 for one that all share, and row),
+ *   mask      NULL, or additive, [q_len, kv_len] per sequence (mask_strides: sequence, 0 for one that all share, and row, at least kv_len),
  *             F32 or F16; a key whose mask is -inf is not seen, whatever its score or value
  * A row that sees no key is NaN, as in rt_attention_enqueue.  Rows of the caches past a sequence's length are not used.
  * Sums, maxima and scores are f32; the probabilities enter the second product as f16; a scale of the cache with more

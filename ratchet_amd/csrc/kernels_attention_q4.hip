@@ -20,9 +20,9 @@
 // Wavefronts of a workgroup take 64 keys in turn and are merged through LDS; where there are few heads several workgroups share the keys and a second
 // kernel merges them, in a fixed order.
 //
-// 32 sequences of 8192 keys, 8 heads of 128, one row of 32 heads: 62 us, 4.8 TB/s, which is what a copy reaches; of lengths between, whose longest bounds it, 50.
-// Small ones wait: 32768 keys of one sequence 16 us (7.4 at a copy's rate) in a launch, a trip to memory and two steps of 1.7 us in which two wavefronts of a SIMD unpack
-// (500 instructions for 64 keys), and 3 of the second launch.
+// 32 sequences of 8192 keys, 8 heads of 128, one row of 32 heads: 61 us from HBM, 4.9 TB/s, near a copy's 5.1 (53 over and over on one state, of which the last-level cache
+// keeps some); of lengths between, whose longest bounds it, 51 (46).  Small ones wait: 32768 keys of one sequence 16.0 us from HBM, 14.3 on one state (7.4 at a copy's rate), in a
+// launch, a trip to memory and two steps of 1.7 us in which two wavefronts of a SIMD unpack (500 instructions for 64 keys), and 3 of the second launch.
 #include "device_common.h"
 
 #include <algorithm>
@@ -826,7 +826,8 @@ static int64_t aq_row_tiles(int rows) { return aq_streams(rows) ? 1 : (rows + AP
 // Keys of a workgroup where several share a row tile's, and how many do.
 // The streaming kernel: as many as fill the 256 compute units once (a workgroup's eight wavefronts leave no room for a second; two rounds of half the keys, 32 x 8
 // heads on 8192 keys of 128: 62 -> 69 us), down to one step each, but two steps (1024 keys) in one launch (32 heads of 80: 8.0 us, in two shares 8.7; four steps 12.3,
-// in four shares 9.1; 8 heads on one of 128, 131072 keys: 256 shares 16.4, 64 of four steps 20.1).
+// in four shares 9.1; 8 heads on one of 128, 131072 keys: 256 shares 16.4, 64 of four steps 20.1).  More than 128 heads of keys have a share each, so that the last round may leave
+// compute units idle (8192 keys of 128: 128 heads 33 us, 136 43, 256 53, 264 89, 512 116): rounds and shares are not weighed against each other here.
 // The other: the least of what its rounds of workgroups, the partial results and the second launch take.  A step is some 1.4 + 0.017 head_dim us (2.5, 3.1 and 3.6
 // measured at 64, 96 and 128), partial results are written and read at 2.5 TB/s (us for shares: 32 x 128 rows on 1024 keys of 80: 1: 21.3, 4: 16.2, 8: 20.0; 32 x 32 on 544: 1:
 // 13.9, 2: 13.6, 5: 10.7; 2 x 4 x 600 on 1373 keys of 64: 3: 21.6, 6: 19.6, 11: 26.4).

@@ -22,8 +22,8 @@
 // A K-vector (16 bytes) v of activation row j of a panel is at slot v * NV + j of LDS, j exchanged within its 16 by 4 (v % 4): reads
 // (16 rows of one vector by a lane group) and writes (four vectors of a row by neighbouring lanes) then meet no bank twice.
 //
-// Measured (weights from HBM, us): 10240 x 2560 at 4 / 16 / 64 rows 7.9 / 9.4 / 16.1, 2560 x 10240 9.0 / 13.8 / 25.0, 51865 x 2560 at 16 rows 25
-// (3.0 TB/s).  The large ones are bound by the issue of the unpacking: with one row and no bias 20.5 us, without its loads 14, with nothing but its loads 19,
+// Measured (weights from HBM, a captured graph, us): 10240 x 2560 at 4 / 16 / 32 / 64 rows 8.4 / 9.7 / 12.1 / 16.4, 2560 x 10240 9.4 / 15.0 / 26.8 / 27.1, 51865 x 2560
+// 22 / 26 / 34 / 56 (16 rows: 3.0 TB/s).  The large ones are bound by the issue of the unpacking: with one row and no bias 20.5 us, without its loads 14, with nothing but its loads 19,
 // and a kernel that only reads the codes 12 (5.5 TB/s).  The small ones by latency: a launch, one trip to HBM and the sum over K are 5.4 us at 2560 x 2560.
 #include "device_common.h"
 
@@ -269,9 +269,11 @@ template <int MT, int VPR, int XI, int UC, int DEPTH> static hipError_t launch_q
 }
 
 // Wavefronts along the rows and along K, by the number of tiles of 16 weight rows (and 32 activation rows) and the units of 512 of K.  All (wr, wk) of up to
-// 16 wavefronts were timed over M 320 .. 51865, K 512 .. 10240 and N 1, 3, 8, 16, 32, 64, 160; the rules stay within 1 .. 12 % of the best there.
-// Few tiles: one row of tiles a workgroup, K shared (2560 x 10240, 1 row: (1, 8) 9.3 us, (4, 1) 21.9).  More rows than compute units take at once: whole rows, K shared only
-// where it is long (51865 x 2560, 1 row: (2, 1) 20.4 us, (1, 4) 30.5).
+// 16 wavefronts were timed over M 320 .. 51865, K 512 .. 10240 and N 3, 8, 16, 32, 64, 160; the rules stay within 1 .. 12 % of the best there.  (Of (wr, wk): 33 to 64 rows take
+// two tiles of 32, and every weight is unpacked for each; a tile of 64 was not built.)
+// Few tiles: one row of tiles a workgroup, K shared (2560 x 10240: 4 rows (1, 4) 9.5 us, (4, 1) 22.3; 8 rows 11.8 and 23.8).  Some: (4, 1) (10240 x 2560: 4 rows 8.3, (1, 4)
+// 10.4; 8 rows 8.7 and 14.1).  More rows than compute units take at once: whole rows, K shared only where it is long (51865 x 2560: 4 rows (2, 1) 22.1, (1, 4) 32; 8 rows 25.1 and
+// 50; 20000 x 10240, 4 rows: (2, 4) 33.4, (2, 1) 35).
 struct Q40Shape {
     int wr, wk;
 };

@@ -10,8 +10,8 @@
 // q40_codes, exact, and four dot products; a block's sum is scaled in f32.  The sixteen lanes are joined by DPP, the wavefronts that share K through LDS, in a
 // fixed order.
 //
-// With a bias 10240 x 2560 from HBM 6.3 us, 51865 x 2560 17.0 (4.4 TB/s, near a copy's 5.1), 2560 x 2560 4.1: the small ones are a launch, one trip to memory and 1 us of
-// instructions.
+// With a bias, from HBM in a captured graph, 10240 x 2560 6.7 us, 51865 x 2560 17.1 (4.4 TB/s, near a copy's 5.1), 2560 x 10240 7.9, 2560 x 2560 3.9: the small ones are a launch,
+// one trip to memory and 1 us of instructions.  Two vectors, with four more dot products for eight weights: 7.8, 21.6, 9.4 and 4.4.
 #include "device_common.h"
 
 #include <algorithm>
@@ -171,10 +171,10 @@ template <int NB> static hipError_t launch_rowdot(const RowdotQ40Args &g, int wr
     return hipGetLastError();
 }
 
-// One or two vectors and K up to 10240, four wavefronts a workgroup (all sharing K where that is long), two workgroups per compute unit (us without a bias for 10240 x 2560 / 51865 x 2560, one vector:
+// One or two vectors and K up to 10240, which four wavefronts of five blocks a lane hold, four wavefronts a workgroup (all sharing K where that is long), two workgroups per compute unit (us without a bias for 10240 x 2560 / 51865 x 2560, one vector:
 // two 6.6 / 16.6, three 7.0 / 17.4; eight wavefronts 7.1 / 17.9).  The matrix-core kernel at one and two vectors and this: 10240 x 2560 8.4 / 8.3 and 6.6 / 7.5, 2560 x 10240 9.4 / 9.4 and 7.5 /
-// 10.0, 2560 x 2560 5.9 / 5.9 and 4.0 / 4.9, 51865 x 2560 21.5 / 21.8 and 16.6 / 20.4, 8192 x 8192 13.0 / 14.4 and 11.2 / 12.9, 640 x 1024 4.1 and 2.5; 4096 x 14336 13.0 / 13.0, here with six
-// wavefronts that share K 12.2 / 20.
+// 10.0, 2560 x 2560 5.9 / 5.9 and 4.0 / 4.9, 51865 x 2560 21.5 / 21.8 and 16.6 / 20.4, 8192 x 8192 13.0 / 14.4 and 11.2 / 12.9, 640 x 1024 4.1 and 2.5; 4096 x 14336 12.4 / 12.4, here with six
+// wavefronts that share K 12.2 / 20: nothing to be had past 10240.
 hipError_t launch_gemv_q40_rowdot(const Problem &p, const void *A, const void *B, const void *bias, void *out, hipStream_t stream, const DeviceInfo &dev) {
     if (p.a_dt != RT_Q4_0 || p.act_dt != RT_F16 || p.N < 1 || p.N > 2 || p.b_ks != 1 || p.K < 32 || p.K % 32 != 0 || p.K > 10240) return hipErrorNotSupported;
     const int units = (int)((p.K / 32 + 15) / 16), wk = (units + 4) / 5, nb = (units + wk - 1) / wk;
