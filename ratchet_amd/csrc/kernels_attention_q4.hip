@@ -8,7 +8,7 @@
 // block's sum scaled by dk in f32.  A load is 16 bytes a lane of consecutive pieces of consecutive keys, and a 4 x 4 transposition among lane
 // groups puts dword g of a block into lane group g, as the operand wants it (kernels_gemv_q40.hip has the same step).  Rows up to 4 (8) are put at
 // MFMA rows 4 m (4 m, 4 m + 1), where one result register (two) holds them all.
-// Softmax: running reference and sum in f32, base 2; a row's keys are spread over 16 lanes, which four DPP rotations join for the maximum, and only at
+// Softmax: running reference and sum in f32; a row's keys are spread over 16 lanes, which four DPP rotations join for the maximum, and only at
 // the end for the sum.
 // Values: the operand of the second product holds, for one dimension, eight keys in a lane.  Codes of one key are neighbours along the dimensions, so
 // lane c (of 16) reads four bytes of each key's row (two up to a head_dim of 64, one up to 32; a row of 80 takes ten lanes, which costs less than the second load
@@ -33,7 +33,7 @@ namespace rt {
 constexpr float kLog2eQ4 = 1.4426950408889634f;
 constexpr int AQ_MAX_SPLITS = 64; // shares of a row of the prompt kernel
 constexpr int AQ_WAVES = 8;       // of a streaming workgroup
-// The exponentials' reference (mx, m_run below, in base 2) is this much below a block's maximum.  As f16 a probability goes down to 2^-25, so that against the largest none of
+// The exponentials' reference (mx, m_run below) is this much, in base 2, below a block's maximum.  As f16 a probability goes down to 2^-25, so that against the largest none of
 // more than 2^-32 is lost (with the maximum itself as reference 2^16 keys of 2^-25.5 each beside one of 1 were, an eighth or half of them, those of its wavefront).  Below 8, since
 // what is left of a difference of 8 and more may round to 16 where an f32's step is that, between 2^27 and 2^28, and 2^16 is no f16.
 constexpr float AQ_BELOW = 7.f;
@@ -51,6 +51,10 @@ struct AttnQ4Args {
     int causal, mask_f32, splits, split_keys, row_tiles;
     float scale, scale_log2e;
 };
+
+// Scores and references are in units of log2(e), and with a mask tensor as they are, in the kernels and in the partial results: f32's lowest number, which hides nothing from a row
+// that has nothing else, and its neighbours would be infinite in the others.
+__host__ __device__ constexpr float aq_unit(bool masked) { return masked ? kLog2eQ4 : 1.f; }
 
 template <int CTRL> __device__ __forceinline__ float aq_dpp(float v) {
     return __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, v), CTRL, 0xf, 0xf, true));
@@ -196,6 +200,7 @@ template <int NT, int VPR, int MK> __global__ __launch_bounds__(512) void attent
         }
     };
 
+    constexpr float unit = aq_unit(MK);
     float mx[VPR], sum[VPR];
     uint32_t bad[VPR];
     float4_t o[T];
@@ -249,27 +254,33 @@ template <int NT, int VPR, int MK> __global__ __launch_bounds__(512) void attent
         for (int v = 0; v < VPR; v++) {
 #pragma unroll
             for (int s = 0; s < 4; s++) {
-                float x = sc[s][v] * g.scale_log2e;
+                float x;
                 if constexpr (MK != 0) {
                     const float mv = g.mask_f32 ? __builtin_bit_cast(float, mk[v][s]) : (float)__builtin_bit_cast(half_t, (uint16_t)mk[v][s]);
-                    // a hidden key's score may be anything; a type's lowest value hides nothing from a row that has nothing else
-                    const float m2 = mv * kLog2eQ4 == -INFINITY ? -3.40282347e38f : mv * kLog2eQ4;
-                    x = mv == -INFINITY ? -INFINITY : x + m2;
+                    x = mv == -INFINITY ? -INFINITY : fmaf(sc[s][v], g.scale, mv); // (a hidden key's score may be anything)
+                } else {
+                    x = sc[s][v] * g.scale_log2e;
                 }
                 if (!inside) x = j0 + 16 * s + r <= last[v] ? x : -INFINITY;
                 sc[s][v] = x;
             }
-            const float top = fmaxf(mx[v], aq_max16(fmaxf(fmaxf(sc[0][v], sc[1][v]), fmaxf(sc[2][v], sc[3][v]))) - AQ_BELOW);
+            const float top = fmaxf(mx[v], aq_max16(fmaxf(fmaxf(sc[0][v], sc[1][v]), fmaxf(sc[2][v], sc[3][v]))) - AQ_BELOW / unit);
             const float base = top == -INFINITY ? 0.f : top;
-            const float a = __builtin_amdgcn_exp2f(mx[v] - base);
+            const float a = __builtin_amdgcn_exp2f((mx[v] - base) * unit);
             mx[v] = top;
             float l = 0.f;
             half4_t p4;
 #pragma unroll
             for (int s = 0; s < 4; s++) {
-                const float p = __builtin_amdgcn_exp2f(sc[s][v] - base);
-                l += p;
+                const float p = __builtin_amdgcn_exp2f((sc[s][v] - base) * unit);
                 p4[s] = (half_t)p;
+                if (MK == 0) l += p;
+            }
+            // In base 2 the largest probability is a power of two, as f16 too.  In other units it is one only where a score's step is small beside 1: the sum is that of the rounded
+            // probabilities there, so that what the largest, or equal ones, lose is in both.
+            if constexpr (MK != 0) {
+                const half2_t one = {(half_t)1, (half_t)1};
+                l = __builtin_amdgcn_fdot2(half2_t{p4[2], p4[3]}, one, __builtin_amdgcn_fdot2(half2_t{p4[0], p4[1]}, one, 0.f, false), false);
             }
             sum[v] = fmaf(sum[v], a, l);
 #pragma unroll
@@ -387,7 +398,7 @@ template <int NT, int VPR, int MK> __global__ __launch_bounds__(512) void attent
         const float base = top == -INFINITY ? 0.f : top;
         float y = 0.f, s = 0.f;
         for (int w = 0; w < waves; w++) {
-            const float a = __builtin_amdgcn_exp2f(ml[(w * ROWS + m) * 2] - base);
+            const float a = __builtin_amdgcn_exp2f((ml[(w * ROWS + m) * 2] - base) * unit);
             y = fmaf(red[w * PER + e], a, y), s = fmaf(ml[(w * ROWS + m) * 2 + 1], a, s);
         }
         const int d = DM::dim(n, l & 15);
@@ -555,9 +566,8 @@ template <int NT, int MK> __global__ __launch_bounds__(512, 2) void attention_q4
     };
 
     float4_t acc[2][NT];
-    // the exponentials' reference and this lane's share of the sum.  Scores are in units of log2(e), and with a mask tensor as they are: its type's lowest value, which hides
-    // nothing from a row that has nothing else, would be infinite in the others.
-    constexpr float unit = MK ? kLog2eQ4 : 1.f;
+    // the exponentials' reference and this lane's share of the sum
+    constexpr float unit = aq_unit(MK);
     float m_run[2], l_run[2];
     uint32_t bad[2];
     bool coarse = false; // whether a reference was too large for scores that are not rounded (uniform)
@@ -698,7 +708,6 @@ template <int NT, int MK> __global__ __launch_bounds__(512, 2) void attention_q4
     // ---- the two halves of the keys through LDS: [group of rows][tile of 16][dimensions' tile][lane] four, and references, sums, flags
 #pragma unroll
     for (int u = 0; u < 2; u++) {
-        if (MK && m_run[u] != -INFINITY) m_run[u] = fmaxf(m_run[u] * unit, -3.40282347e38f);
         l_run[u] = rt_groups_sum(l_run[u]);
         bad[u] |= (uint32_t)__shfl_xor((int)bad[u], 16);
         bad[u] |= (uint32_t)__shfl_xor((int)bad[u], 32);
@@ -720,7 +729,7 @@ template <int NT, int MK> __global__ __launch_bounds__(512, 2) void attention_q4
     for (int u = 0; u < 2; u++) {
         const float *const p = sums + (2 * rg + u) * 192 + lane;
         const float m1 = p[0], top = fmaxf(m_run[u], m1), base = top == -INFINITY ? 0.f : top;
-        const float a0 = __builtin_amdgcn_exp2f(m_run[u] - base), a1 = __builtin_amdgcn_exp2f(m1 - base), l = l_run[u] * a0 + p[64] * a1;
+        const float a0 = __builtin_amdgcn_exp2f((m_run[u] - base) * unit), a1 = __builtin_amdgcn_exp2f((m1 - base) * unit), l = l_run[u] * a0 + p[64] * a1;
         const uint32_t bd = bad[u] | __builtin_bit_cast(uint32_t, p[128]);
 #pragma unroll
         for (int d = 0; d < NT; d++) {
@@ -754,12 +763,13 @@ template <int NT, int MK> __global__ __launch_bounds__(512, 2) void attention_q4
 // Joins the shares of a row, four columns a thread: CG threads have the columns of a row, SG groups of them its shares, and the workgroup 256 / (CG SG) rows.  All
 // loads are requested at once, and the groups meet in LDS, in a fixed order.  (One thread a column that walked the shares took 20.9 us for 32 rows of 64 shares
 // of 128, this 2.9; 4800 rows of 6 shares of 64 with 16 groups, ten of them idle, and a row a workgroup 7.0.)
-template <int CG, int SG> __global__ __launch_bounds__(256) void attention_q4_merge_kernel(AttnQ4Args g, int D, int64_t rows) {
+template <int CG, int SG, bool MASK> __global__ __launch_bounds__(256) void attention_q4_merge_kernel(AttnQ4Args g, int D, int64_t rows) {
     constexpr int R = 256 / (CG * SG), PER = SG < 8 ? 1 : 64 / SG; // (four groups: up to four shares; others 64 at a time)
     __shared__ __attribute__((aligned(16))) float part[R][SG][4 * CG];
     const int t = threadIdx.x, c = t % CG, sg = t / CG % SG, rl = t / (CG * SG);
     const int64_t row = min((int64_t)blockIdx.x * R + rl, rows - 1);
     const bool live = 4 * c < D;
+    constexpr float unit = aq_unit(MASK);
     const float *const po = g.part_o + row * g.splits * D + (live ? 4 * c : 0), *const pm = g.part_ml + row * g.splits * 2;
     // this group's shares; one whose sum is 0 has no key, and no outputs were written
     float top = -INFINITY, l = 0.f;
@@ -778,14 +788,14 @@ template <int CG, int SG> __global__ __launch_bounds__(256) void attention_q4_me
 #pragma unroll
         for (int i = 0; i < PER; i++)
             if (s0 + i * SG < g.splits) now = fmaxf(now, ml[i][0]);
-        const float base = now == -INFINITY ? 0.f : now, old = __builtin_amdgcn_exp2f(top - base);
+        const float base = now == -INFINITY ? 0.f : now, old = __builtin_amdgcn_exp2f((top - base) * unit);
         top = now, l *= old;
 #pragma unroll
         for (int k = 0; k < 4; k++) y[k] *= old;
 #pragma unroll
         for (int i = 0; i < PER; i++)
             if (s0 + i * SG < g.splits && s0 + i * SG + sg < g.splits && ml[i][1] != 0.f) {
-                const float a = __builtin_amdgcn_exp2f(ml[i][0] - base);
+                const float a = __builtin_amdgcn_exp2f((ml[i][0] - base) * unit);
                 l = fmaf(a, ml[i][1], l);
 #pragma unroll
                 for (int k = 0; k < 4; k++) y[k] = fmaf(a, v[i][k], y[k]);
@@ -805,7 +815,7 @@ template <int CG, int SG> __global__ __launch_bounds__(256) void attention_q4_me
         const float ref = all == -INFINITY ? 0.f : all;
 #pragma unroll
         for (int s = 0; s < SG; s++) {
-            const float a = __builtin_amdgcn_exp2f(mls[rr][s][0] - ref);
+            const float a = __builtin_amdgcn_exp2f((mls[rr][s][0] - ref) * unit);
             sum = fmaf(part[rr][s][d], a, sum), total = fmaf(mls[rr][s][1], a, total);
         }
         const int bk = (int)(out / g.rows), m = (int)(out - (int64_t)bk * g.rows), b = bk / g.kv_heads, kh = bk - b * g.kv_heads, qi = m / g.group;
@@ -814,7 +824,9 @@ template <int CG, int SG> __global__ __launch_bounds__(256) void attention_q4_me
 }
 template <int CG, int SG> static hipError_t launch_aq_merge(const AttnQ4Args &g, int D, int64_t rows, hipStream_t st) {
     constexpr int R = 256 / (CG * SG);
-    hipLaunchKernelGGL((attention_q4_merge_kernel<CG, SG>), dim3((unsigned)((rows + R - 1) / R)), dim3(256), 0, st, g, D, rows);
+    const dim3 grid((unsigned)((rows + R - 1) / R));
+    if (g.mask) hipLaunchKernelGGL((attention_q4_merge_kernel<CG, SG, true>), grid, dim3(256), 0, st, g, D, rows);
+    else hipLaunchKernelGGL((attention_q4_merge_kernel<CG, SG, false>), grid, dim3(256), 0, st, g, D, rows);
     return hipGetLastError();
 }
 

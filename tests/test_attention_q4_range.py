@@ -155,3 +155,28 @@ def test_a_long_tail_beside_one_large_probability(device, lq, masked):
     assert (want > 0.01).all() and (tol < 0.02 * want).all()
     for ws in (True, False):
         check(run(device, q, buffer(kc, kd), buffer(vc, vd), 1, n, n, scale, mask=mask, workspace=ws), want, tol)
+
+
+@gpu
+@pytest.mark.parametrize("lq", [1, 6, 13, 20, 150])
+@pytest.mark.parametrize("near", [0.999, 0.9, 0.72, 0.5])
+def test_masks_near_the_lowest_number(device, lq, near):
+    """A mask of f32's lowest number and a few keys above it by a part of that: differences of 10^35 and more, so that a row is the mean of the values of those few (next to such a mask
+    their scores vanish in f32).  They lie in one block of 64 keys, in two of them, or at both ends."""
+    n, d = 1500, 64
+    rng = np.random.default_rng(lq)
+    v0 = rng.integers(-64, 65, n) / 16
+    kbuf, vbuf = one_dimension(n, d, rng.uniform(-0.1, 0.1, n), v0)
+    q = rng.standard_normal((1, 1, lq, d)).astype(np.float16)
+    low = np.finfo(np.float32).min
+    for best in ([70, 71], [3, 700], [0, 1499], [1490]):
+        mask = np.full((lq, n), low, np.float32)
+        mask[:, best] = np.float32(near * float(low))
+        want = v0[best].mean()
+        for ws in (True, False):
+            got = run(device, q, kbuf, vbuf, 1, n, n, 0.125, mask=mask, workspace=ws).astype(np.float64)
+            assert (np.abs(got - want) <= 2.0**-11 * abs(want) + 2.0**-20).all(), (best, ws, got[0, 0, :, 0], want)
+    mask[:] = low  # all alike: the mean of all, each probability and the sum of them rounded
+    for ws in (True, False):
+        got = run(device, q, kbuf, vbuf, 1, n, n, 0.125, mask=mask, workspace=ws).astype(np.float64)
+        assert (np.abs(got - v0.mean()) <= 2.0**-11 * abs(v0.mean()) + 2.0**-11 * np.abs(v0).mean()).all()
