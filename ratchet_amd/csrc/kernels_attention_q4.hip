@@ -20,7 +20,7 @@
 // Wavefronts of a workgroup take 64 keys in turn and are merged through LDS; where there are few heads several workgroups share the keys and a second
 // kernel merges them, in a fixed order.
 //
-// 32 sequences of 8192 keys, 8 heads of 128, one row of 32 heads: 61 us from HBM, 4.9 TB/s, near a copy's 5.1 (53 over and over on one state, of which the last-level cache
+// 32 sequences of 8192 keys, 8 heads of 128, one row of 32 heads: 60 us from HBM, 5.0 TB/s, near a copy's 5.1 (53 over and over on one state, of which the last-level cache
 // keeps some); of lengths between, whose longest bounds it, 51 (46).  Small ones wait: 32768 keys of one sequence 16.0 us from HBM, 14.3 on one state (7.4 at a copy's rate), in a
 // launch, a trip to memory and two steps of 1.7 us in which two wavefronts of a SIMD unpack (500 instructions for 64 keys), and 3 of the second launch.
 #include "device_common.h"
