@@ -116,6 +116,51 @@ pub struct rt_attention_q4_desc {
 }
 
 #[repr(C)]
+#[derive(Clone, Copy, Default)]
+pub struct rt_paged_cache_desc {
+    pub batch: i32,
+    pub kv_heads: i32,
+    pub head_dim: i32,
+    pub pages: i32,
+    pub page_size: i32,
+    pub table_width: i32,
+    pub table_stride: i64, // entries
+}
+
+#[repr(C)]
+#[derive(Clone, Copy, Default)]
+pub struct rt_attention_paged_desc {
+    pub cache: rt_paged_cache_desc,
+    pub heads: i32,
+    pub rows: i32,
+    pub max_rows: i32,
+    pub max_keys: i32,
+    pub causal: i32,
+    pub scale: f32,
+    pub q_strides: [i64; 2], // row, head; in elements
+    pub o_strides: [i64; 2],
+}
+
+#[repr(C)]
+#[derive(Clone, Copy, Default)]
+pub struct rt_attention_packed_desc {
+    pub batch: i32,
+    pub heads: i32,
+    pub kv_heads: i32,
+    pub head_dim: i32,
+    pub rows: i32,
+    pub kv_rows: i32,
+    pub max_rows: i32,
+    pub max_keys: i32,
+    pub causal: i32,
+    pub scale: f32,
+    pub q_strides: [i64; 2], // row, head; in elements
+    pub k_strides: [i64; 2],
+    pub v_strides: [i64; 2],
+    pub o_strides: [i64; 2],
+}
+
+#[repr(C)]
 #[derive(Clone, Copy)]
 pub struct rt_gguf_tensor_info {
     pub name: *const c_char, // NUL-terminated, owned by the rt_gguf
@@ -225,6 +270,20 @@ extern "C" {
     pub fn rt_attention_q4_enqueue(ctx: *mut rt_ctx, desc: *const rt_attention_q4_desc, q: *const c_void, k_cache: *const c_void,
                                    v_cache: *const c_void, mask: *const c_void, kv_lens: *const i32, out: *mut c_void,
                                    workspace: *mut c_void, workspace_bytes: u64, stream: *mut c_void) -> rt_status;
+    // sequences of different lengths: a key/value cache held in pages, attention over it, attention of packed prompts
+    pub fn rt_cache_write_paged_enqueue(ctx: *mut rt_ctx, desc: *const rt_paged_cache_desc, src_dtype: i32, k_pool: *mut c_void,
+                                        k_src: *const c_void, v_pool: *mut c_void, v_src: *const c_void, src_strides: *const i64,
+                                        table: *const i32, lens: *const i32, starts: *const i32, rows: i32, stream: *mut c_void) -> rt_status;
+    pub fn rt_attention_paged_validate(desc: *const rt_attention_paged_desc) -> rt_status;
+    pub fn rt_attention_paged_workspace_bytes(desc: *const rt_attention_paged_desc, bytes: *mut u64) -> rt_status;
+    pub fn rt_attention_paged_enqueue(ctx: *mut rt_ctx, desc: *const rt_attention_paged_desc, q: *const c_void, k_pool: *const c_void,
+                                      v_pool: *const c_void, table: *const i32, lens: *const i32, starts: *const i32, out: *mut c_void,
+                                      workspace: *mut c_void, workspace_bytes: u64, stream: *mut c_void) -> rt_status;
+    pub fn rt_attention_packed_validate(desc: *const rt_attention_packed_desc) -> rt_status;
+    pub fn rt_attention_packed_workspace_bytes(desc: *const rt_attention_packed_desc, bytes: *mut u64) -> rt_status;
+    pub fn rt_attention_packed_enqueue(ctx: *mut rt_ctx, desc: *const rt_attention_packed_desc, q: *const c_void, k: *const c_void,
+                                       v: *const c_void, starts: *const i32, kv_starts: *const i32, out: *mut c_void,
+                                       workspace: *mut c_void, workspace_bytes: u64, stream: *mut c_void) -> rt_status;
     // GGUF container (host-side parse; load = upload + layout conversion on `stream`)
     pub fn rt_gguf_parse(image: *const c_void, size: u64, out: *mut *mut rt_gguf) -> rt_status;
     pub fn rt_gguf_free(g: *mut rt_gguf);

@@ -554,6 +554,93 @@ RT_API rt_status rt_attention_q4_enqueue(rt_ctx *ctx, const rt_attention_q4_desc
                                          const void *v_cache, const void *mask, const int32_t *kv_lens, void *out, void *workspace,
                                          uint64_t workspace_bytes, void *stream);
 
+/* ------------------------------------------------------------------------
+ * Sequences of different lengths in one call: a key/value cache held in pages, attention over it, and attention of
+ * prompts that lie packed (no counterpart in the reference, whose batch has one length and whose Cache is one tensor,
+ * ops/cache.rs:20-140).
+ *
+ * Packed rows: sequence b has the rows starts[b] .. starts[b + 1] - 1 of a tensor [rows, heads, head_dim], whose rows and
+ * heads are strided and whose head_dim is contiguous.  `starts` is batch + 1 ascending int32 in device memory, so that a
+ * captured graph may be replayed with other lengths, or NULL: every sequence has the same number of rows, one behind
+ * another.  Sequences may be empty.  Rows before the first and behind the last sequence are not read, and what would be
+ * written there is left as it was.
+ *
+ * Pages: a pool is [pages, kv_heads, page_size, head_dim], F16, contiguous: that of the keys and that of the values.  Entry j of
+ * a sequence's row of `table` (int32 in device memory, rows table_stride entries apart) is the page that holds its positions
+ * j * page_size .. (j + 1) * page_size - 1.  lens[b] (int32 in device memory) positions of sequence b are in use, the call's rows
+ * of the sequence among them: those are the last.  An entry outside 0 .. pages - 1 is no page: nothing is written there, and
+ * its positions are seen by no row.
+ * ------------------------------------------------------------------------ */
+typedef struct rt_paged_cache_desc {
+    int32_t batch;              /* sequences */
+    int32_t kv_heads;
+    int32_t head_dim;           /* a multiple of 8, 8 .. 128 */
+    int32_t pages;              /* of a pool */
+    int32_t page_size;          /* positions of a page: a power of two, 16 .. 65536 */
+    int32_t table_width;        /* entries of a sequence's row of the table */
+    int64_t table_stride;       /* entries between them, at least table_width */
+} rt_paged_cache_desc;
+
+/* Writes the new rows of every sequence into the pools, one launch:
+ *   src     packed [rows, kv_heads, head_dim], F16, or F32 (rounded to f16); src_strides: row, head, in elements, both tensors'
+ *   starts  as above; NULL: rows / batch each
+ * Row i of the n rows of sequence b goes to position lens[b] - n + i; one below 0, past the table or without a page is not
+ * written.  Everything else in the pools keeps its bytes.  v_pool and v_src may both be NULL: one tensor.  Two rows of a call that
+ * name the same place of a page (sequences that share one): one of the two is there afterwards. */
+RT_API rt_status rt_cache_write_paged_enqueue(rt_ctx *ctx, const rt_paged_cache_desc *desc, int32_t src_dtype, void *k_pool, const void *k_src,
+                                              void *v_pool, const void *v_src, const int64_t *src_strides, const int32_t *table,
+                                              const int32_t *lens, const int32_t *starts, int32_t rows, void *stream);
+
+/* Attention over the pages: out = softmax(scale * q k^T) v for the packed query rows, F16, of every sequence.  Head h reads the pools'
+ * head h / (heads / kv_heads).
+ *   lens      keys of each sequence, taken between 0 and max_keys
+ *   causal    row i of the n rows of a sequence sees the keys up to position lens[b] - n + i; without it all of the sequence's
+ *   max_rows  no sequence has more rows than this: rows past it are left as they were.  starts == NULL: each has so many
+ *   max_keys  likewise for the keys; at most table_width * page_size
+ * A row that sees no key is NaN, as in rt_attention_enqueue.  Keys that a row does not see, and what lies in pages behind a sequence's keys, have no effect on
+ * it, whatever they hold; a row that sees a value that is not finite is not finite in that dimension.
+ * Sums, references and scores are f32; the probabilities enter the second product as f16.
+ * Limits (RT_ERR_UNSUPPORTED beyond): 2^25 rows, 2^30 keys of a sequence, rows times heads below 2^31, 65535 sequences. */
+typedef struct rt_attention_paged_desc {
+    rt_paged_cache_desc cache;
+    int32_t heads;              /* a multiple of cache.kv_heads */
+    int32_t rows;               /* of q and out, of all sequences */
+    int32_t max_rows, max_keys;
+    int32_t causal;             /* 0 / 1 */
+    float scale;
+    int64_t q_strides[2];       /* row, head; multiples of 8 */
+    int64_t o_strides[2];
+} rt_attention_paged_desc;
+
+RT_API rt_status rt_attention_paged_validate(const rt_attention_paged_desc *desc);
+/* Bytes of workspace with which the keys of a row are shared among workgroups; as rt_attention_workspace_bytes. */
+RT_API rt_status rt_attention_paged_workspace_bytes(const rt_attention_paged_desc *desc, uint64_t *bytes);
+RT_API rt_status rt_attention_paged_enqueue(rt_ctx *ctx, const rt_attention_paged_desc *desc, const void *q, const void *k_pool, const void *v_pool,
+                                            const int32_t *table, const int32_t *lens, const int32_t *starts, void *out, void *workspace,
+                                            uint64_t workspace_bytes, void *stream);
+
+/* Attention of packed prompts: keys and values are packed rows too, [kv_rows, kv_heads, head_dim], those of sequence b at kv_starts[b] ..
+ * kv_starts[b + 1] - 1; kv_starts == NULL: where its query rows are (kv_rows == rows), each prompt seeing itself.  q, k and v may be parts of one fused
+ * projection's output.  All else as rt_attention_paged_enqueue; with the causal flag row i of n sees the first (keys - n + i + 1) keys. */
+typedef struct rt_attention_packed_desc {
+    int32_t batch, heads, kv_heads;
+    int32_t head_dim;           /* a multiple of 8, 8 .. 128 */
+    int32_t rows, kv_rows;
+    int32_t max_rows, max_keys;
+    int32_t causal;             /* 0 / 1 */
+    float scale;
+    int64_t q_strides[2];       /* row, head; multiples of 8 */
+    int64_t k_strides[2];
+    int64_t v_strides[2];
+    int64_t o_strides[2];
+} rt_attention_packed_desc;
+
+RT_API rt_status rt_attention_packed_validate(const rt_attention_packed_desc *desc);
+RT_API rt_status rt_attention_packed_workspace_bytes(const rt_attention_packed_desc *desc, uint64_t *bytes);
+RT_API rt_status rt_attention_packed_enqueue(rt_ctx *ctx, const rt_attention_packed_desc *desc, const void *q, const void *k, const void *v,
+                                             const int32_t *starts, const int32_t *kv_starts, void *out, void *workspace, uint64_t workspace_bytes,
+                                             void *stream);
+
 #ifdef __cplusplus
 }
 #endif

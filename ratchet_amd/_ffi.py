@@ -91,6 +91,35 @@ class AttentionQ4Desc(ctypes.Structure):
     ]
 
 
+class PagedCacheDesc(ctypes.Structure):
+    """rt_paged_cache_desc."""
+    _fields_ = [
+        ("batch", ctypes.c_int32), ("kv_heads", ctypes.c_int32), ("head_dim", ctypes.c_int32),
+        ("pages", ctypes.c_int32), ("page_size", ctypes.c_int32), ("table_width", ctypes.c_int32),
+        ("table_stride", ctypes.c_int64),
+    ]
+
+
+class AttentionPagedDesc(ctypes.Structure):
+    """rt_attention_paged_desc."""
+    _fields_ = [
+        ("cache", PagedCacheDesc),
+        ("heads", ctypes.c_int32), ("rows", ctypes.c_int32), ("max_rows", ctypes.c_int32), ("max_keys", ctypes.c_int32),
+        ("causal", ctypes.c_int32), ("scale", ctypes.c_float),
+        ("q_strides", ctypes.c_int64 * 2), ("o_strides", ctypes.c_int64 * 2),
+    ]
+
+
+class AttentionPackedDesc(ctypes.Structure):
+    """rt_attention_packed_desc."""
+    _fields_ = [
+        ("batch", ctypes.c_int32), ("heads", ctypes.c_int32), ("kv_heads", ctypes.c_int32), ("head_dim", ctypes.c_int32),
+        ("rows", ctypes.c_int32), ("kv_rows", ctypes.c_int32), ("max_rows", ctypes.c_int32), ("max_keys", ctypes.c_int32),
+        ("causal", ctypes.c_int32), ("scale", ctypes.c_float),
+        ("q_strides", ctypes.c_int64 * 2), ("k_strides", ctypes.c_int64 * 2), ("v_strides", ctypes.c_int64 * 2), ("o_strides", ctypes.c_int64 * 2),
+    ]
+
+
 # name -> (restype, argtypes); the single source the symbol test walks too
 _vp, _u64, _i32 = ctypes.c_void_p, ctypes.c_uint64, ctypes.c_int32
 _P = ctypes.POINTER
@@ -138,6 +167,13 @@ SIGNATURES = {
     "rt_attention_q4_validate": (_i32, [_P(AttentionQ4Desc)]),
     "rt_attention_q4_workspace_bytes": (_i32, [_P(AttentionQ4Desc), _P(_u64)]),
     "rt_attention_q4_enqueue": (_i32, [_vp, _P(AttentionQ4Desc), _vp, _vp, _vp, _vp, _vp, _vp, _vp, _u64, _vp]),
+    "rt_cache_write_paged_enqueue": (_i32, [_vp, _P(PagedCacheDesc), _i32, _vp, _vp, _vp, _vp, _P(ctypes.c_int64), _vp, _vp, _vp, _i32, _vp]),
+    "rt_attention_paged_validate": (_i32, [_P(AttentionPagedDesc)]),
+    "rt_attention_paged_workspace_bytes": (_i32, [_P(AttentionPagedDesc), _P(_u64)]),
+    "rt_attention_paged_enqueue": (_i32, [_vp, _P(AttentionPagedDesc), _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _u64, _vp]),
+    "rt_attention_packed_validate": (_i32, [_P(AttentionPackedDesc)]),
+    "rt_attention_packed_workspace_bytes": (_i32, [_P(AttentionPackedDesc), _P(_u64)]),
+    "rt_attention_packed_enqueue": (_i32, [_vp, _P(AttentionPackedDesc), _vp, _vp, _vp, _vp, _vp, _vp, _vp, _u64, _vp]),
     "rt_gguf_parse": (_i32, [_vp, _u64, _P(_vp)]),
     "rt_gguf_free": (None, [_vp]),
     "rt_gguf_error": (ctypes.c_char_p, [_vp]),

@@ -4,6 +4,7 @@
 #include <hip/hip_runtime.h>
 
 #include <atomic>
+#include <cmath>
 #include <cstdlib>
 #include <cstring>
 #include <memory>
@@ -755,6 +756,143 @@ rt_status rt_attention_q4_enqueue(rt_ctx *ctx, const rt_attention_q4_desc *desc,
     DeviceGuard dg(ctx->dev.ordinal);
     if (!dg.ok) return fail(ctx, RT_ERR_NO_DEVICE, "hipSetDevice failed");
     hipError_t e = rt::launch_attention_q4(*desc, q, k_cache, v_cache, mask, kv_lens, out, workspace, workspace_bytes, (hipStream_t)stream, ctx->dev);
+    if (e != hipSuccess) return hip_fail(ctx, "attention launch", e);
+    return RT_OK;
+    RT_GUARD_END(ctx)
+}
+
+// What the paged cache's operators ask of its description.
+static rt_status paged_validate(const rt_paged_cache_desc &c) {
+    if (c.batch < 0 || c.kv_heads < 0 || c.pages < 0 || c.table_width < 0) return RT_ERR_INVALID_SHAPE;
+    if (c.head_dim < 8 || c.head_dim > 128 || c.head_dim % 8) return RT_ERR_INVALID_SHAPE;
+    if (c.page_size < 16 || c.page_size > 65536 || (c.page_size & (c.page_size - 1))) return RT_ERR_INVALID_SHAPE;
+    if (c.table_stride < c.table_width) return RT_ERR_INVALID_SHAPE;
+    if (c.batch > 65535 || c.kv_heads > 65535 || c.table_stride > (int64_t(1) << 31)) return RT_ERR_UNSUPPORTED;
+    return RT_OK;
+}
+
+// Of packed rows: sizes, and strides in elements.
+static rt_status ragged_validate(int32_t batch, int32_t heads, int32_t kv_heads, int32_t rows, int32_t max_rows, int32_t max_keys, int32_t causal, float scale,
+                                 const int64_t *q_strides, const int64_t *o_strides) {
+    if (batch < 0 || heads < 0 || kv_heads < 0 || rows < 0 || max_rows < 0 || max_keys < 0) return RT_ERR_INVALID_SHAPE;
+    if (heads > 0 && (kv_heads == 0 || heads % kv_heads)) return RT_ERR_INVALID_SHAPE;
+    for (int j = 0; j < 2; j++) {
+        if (q_strides[j] < 0 || o_strides[j] < 0) return RT_ERR_INVALID_SHAPE;
+        if (q_strides[j] % 8) return RT_ERR_UNSUPPORTED; // rows are read as 16-byte vectors
+        if (q_strides[j] > (int64_t(1) << 31) || o_strides[j] > (int64_t(1) << 31)) return RT_ERR_UNSUPPORTED;
+    }
+    if (causal != 0 && causal != 1) return RT_ERR_INVALID_ARG;
+    if (!(std::fabs(scale) <= 3.4e38f)) return RT_ERR_INVALID_ARG;
+    if (batch > 65535 || rows > (1 << 25) || max_keys > (1 << 30) || (int64_t)rows * heads >= (int64_t(1) << 31)) return RT_ERR_UNSUPPORTED;
+    return RT_OK;
+}
+
+rt_status rt_cache_write_paged_enqueue(rt_ctx *ctx, const rt_paged_cache_desc *desc, int32_t src_dtype, void *k_pool, const void *k_src, void *v_pool,
+                                       const void *v_src, const int64_t *src_strides, const int32_t *table, const int32_t *lens, const int32_t *starts,
+                                       int32_t rows, void *stream) {
+    if (!ctx || !desc || !src_strides) return RT_ERR_INVALID_ARG;
+    RT_GUARD_BEGIN
+    if (src_dtype != RT_F32 && src_dtype != RT_F16) return fail(ctx, RT_ERR_DTYPE_MISMATCH, "cache: the source is F32 or F16");
+    const rt_status st = paged_validate(*desc);
+    if (st != RT_OK) return fail(ctx, st, "cache: invalid descriptor");
+    if (rows < 0 || (!starts && (desc->batch == 0 ? rows != 0 : rows % desc->batch != 0)))
+        return fail(ctx, RT_ERR_INVALID_SHAPE, "cache: without starts the rows are shared evenly");
+    const int64_t esz = src_dtype == RT_F32 ? 4 : 2;
+    for (int i = 0; i < 2; i++)
+        if (src_strides[i] < 0 || src_strides[i] > (int64_t(1) << 31) || (src_strides[i] * esz) % 16)
+            return fail(ctx, RT_ERR_UNSUPPORTED, "cache: source strides must keep rows 16-byte aligned");
+    if (rows > (1 << 25)) return fail(ctx, RT_ERR_UNSUPPORTED, "cache: more than 2^25 rows at once");
+    if (rows == 0 || desc->batch == 0 || desc->kv_heads == 0 || desc->pages == 0 || desc->table_width == 0) return RT_OK; // nothing to write
+    if (!k_pool || !k_src || (!v_pool != !v_src) || !table || !lens) return fail(ctx, RT_ERR_INVALID_ARG, "null device pointer");
+    if (((uintptr_t)k_pool | (uintptr_t)k_src | (uintptr_t)v_pool | (uintptr_t)v_src) & 15u)
+        return fail(ctx, RT_ERR_INVALID_ARG, "cache: pools and sources must be 16-byte aligned");
+    if (((uintptr_t)table | (uintptr_t)lens | (uintptr_t)starts) & 3u) return fail(ctx, RT_ERR_INVALID_ARG, "cache: table, lens and starts must be 4-byte aligned");
+    DeviceGuard dg(ctx->dev.ordinal);
+    if (!dg.ok) return fail(ctx, RT_ERR_NO_DEVICE, "hipSetDevice failed");
+    hipError_t e = rt::launch_cache_write_paged(*desc, src_dtype, k_pool, k_src, v_pool, v_src, src_strides, table, lens, starts, rows, (hipStream_t)stream);
+    if (e != hipSuccess) return hip_fail(ctx, "cache write launch", e);
+    return RT_OK;
+    RT_GUARD_END(ctx)
+}
+
+rt_status rt_attention_paged_validate(const rt_attention_paged_desc *d) {
+    if (!d) return RT_ERR_INVALID_ARG;
+    rt_status st = paged_validate(d->cache);
+    if (st != RT_OK) return st;
+    st = ragged_validate(d->cache.batch, d->heads, d->cache.kv_heads, d->rows, d->max_rows, d->max_keys, d->causal, d->scale, d->q_strides, d->o_strides);
+    if (st != RT_OK) return st;
+    if (d->max_keys > (int64_t)d->cache.table_width * d->cache.page_size) return RT_ERR_INVALID_SHAPE;
+    return rt::attention_paged_fits(*d) ? RT_OK : RT_ERR_UNSUPPORTED;
+}
+
+rt_status rt_attention_paged_workspace_bytes(const rt_attention_paged_desc *desc, uint64_t *bytes) {
+    if (!desc || !bytes) return RT_ERR_INVALID_ARG;
+    const rt_status st = rt_attention_paged_validate(desc);
+    if (st != RT_OK) return st;
+    *bytes = rt::attention_paged_workspace_bytes(*desc);
+    return RT_OK;
+}
+
+rt_status rt_attention_paged_enqueue(rt_ctx *ctx, const rt_attention_paged_desc *desc, const void *q, const void *k_pool, const void *v_pool, const int32_t *table,
+                                     const int32_t *lens, const int32_t *starts, void *out, void *workspace, uint64_t workspace_bytes, void *stream) {
+    if (!ctx || !desc) return RT_ERR_INVALID_ARG;
+    RT_GUARD_BEGIN
+    const rt_status st = rt_attention_paged_validate(desc);
+    if (st != RT_OK) return fail(ctx, st, "attention: invalid descriptor");
+    if (!starts && desc->rows != (int64_t)desc->cache.batch * desc->max_rows)
+        return fail(ctx, RT_ERR_INVALID_SHAPE, "attention: without starts every sequence has max_rows rows");
+    if (desc->cache.batch == 0 || desc->heads == 0 || desc->rows == 0 || desc->max_rows == 0) return RT_OK; // empty output
+    if (!q || !out || !lens || (desc->max_keys > 0 && desc->cache.pages > 0 && (!k_pool || !v_pool || !table))) return fail(ctx, RT_ERR_INVALID_ARG, "null device pointer");
+    if (((uintptr_t)q | (uintptr_t)k_pool | (uintptr_t)v_pool) & 15u) return fail(ctx, RT_ERR_INVALID_ARG, "attention: q and the pools must be 16-byte aligned");
+    if (((uintptr_t)out & 1u) || (((uintptr_t)table | (uintptr_t)lens | (uintptr_t)starts) & 3u))
+        return fail(ctx, RT_ERR_INVALID_ARG, "attention: out, table, lens and starts must be aligned to their types");
+    DeviceGuard dg(ctx->dev.ordinal);
+    if (!dg.ok) return fail(ctx, RT_ERR_NO_DEVICE, "hipSetDevice failed");
+    hipError_t e = rt::launch_attention_paged(*desc, q, k_pool, v_pool, table, lens, starts, out, workspace, workspace_bytes, (hipStream_t)stream, ctx->dev);
+    if (e != hipSuccess) return hip_fail(ctx, "attention launch", e);
+    return RT_OK;
+    RT_GUARD_END(ctx)
+}
+
+rt_status rt_attention_packed_validate(const rt_attention_packed_desc *d) {
+    if (!d) return RT_ERR_INVALID_ARG;
+    const rt_status st = ragged_validate(d->batch, d->heads, d->kv_heads, d->rows, d->max_rows, d->max_keys, d->causal, d->scale, d->q_strides, d->o_strides);
+    if (st != RT_OK) return st;
+    if (d->head_dim < 8 || d->head_dim > 128 || d->head_dim % 8 || d->kv_rows < 0) return RT_ERR_INVALID_SHAPE;
+    const int64_t *strides[2] = {d->k_strides, d->v_strides};
+    for (int i = 0; i < 2; i++)
+        for (int j = 0; j < 2; j++) {
+            if (strides[i][j] < 0) return RT_ERR_INVALID_SHAPE;
+            if (strides[i][j] % 8 || strides[i][j] > (int64_t(1) << 27)) return RT_ERR_UNSUPPORTED; // a few rows' offsets are 32 bits
+        }
+    return rt::attention_packed_fits(*d) ? RT_OK : RT_ERR_UNSUPPORTED;
+}
+
+rt_status rt_attention_packed_workspace_bytes(const rt_attention_packed_desc *desc, uint64_t *bytes) {
+    if (!desc || !bytes) return RT_ERR_INVALID_ARG;
+    const rt_status st = rt_attention_packed_validate(desc);
+    if (st != RT_OK) return st;
+    *bytes = rt::attention_packed_workspace_bytes(*desc);
+    return RT_OK;
+}
+
+rt_status rt_attention_packed_enqueue(rt_ctx *ctx, const rt_attention_packed_desc *desc, const void *q, const void *k, const void *v, const int32_t *starts,
+                                      const int32_t *kv_starts, void *out, void *workspace, uint64_t workspace_bytes, void *stream) {
+    if (!ctx || !desc) return RT_ERR_INVALID_ARG;
+    RT_GUARD_BEGIN
+    const rt_status st = rt_attention_packed_validate(desc);
+    if (st != RT_OK) return fail(ctx, st, "attention: invalid descriptor");
+    if (!starts && desc->rows != (int64_t)desc->batch * desc->max_rows)
+        return fail(ctx, RT_ERR_INVALID_SHAPE, "attention: without starts every sequence has max_rows rows");
+    if (!kv_starts && desc->kv_rows != desc->rows) return fail(ctx, RT_ERR_INVALID_SHAPE, "attention: without kv_starts the keys are where the queries are");
+    if (desc->batch == 0 || desc->heads == 0 || desc->rows == 0 || desc->max_rows == 0) return RT_OK; // empty output
+    if (!q || !out || (desc->max_keys > 0 && desc->kv_rows > 0 && (!k || !v))) return fail(ctx, RT_ERR_INVALID_ARG, "null device pointer");
+    if (((uintptr_t)q | (uintptr_t)k | (uintptr_t)v) & 15u) return fail(ctx, RT_ERR_INVALID_ARG, "attention: q, k and v must be 16-byte aligned");
+    if (((uintptr_t)out & 1u) || (((uintptr_t)starts | (uintptr_t)kv_starts) & 3u))
+        return fail(ctx, RT_ERR_INVALID_ARG, "attention: out, starts and kv_starts must be aligned to their types");
+    DeviceGuard dg(ctx->dev.ordinal);
+    if (!dg.ok) return fail(ctx, RT_ERR_NO_DEVICE, "hipSetDevice failed");
+    hipError_t e = rt::launch_attention_packed(*desc, q, k, v, starts, kv_starts, out, workspace, workspace_bytes, (hipStream_t)stream, ctx->dev);
     if (e != hipSuccess) return hip_fail(ctx, "attention launch", e);
     return RT_OK;
     RT_GUARD_END(ctx)

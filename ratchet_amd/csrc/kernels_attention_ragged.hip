@@ -1,0 +1,471 @@
+// Attention of sequences of different lengths, many query rows: prompts that lie packed one behind another, and rows against a cache held in pages (ragged.h).
+//
+//   out[r, h] = sum_j p_j v_j,  p = softmax_j(scale * q[r, h] . k_j) over the keys j that row r sees
+//
+// The rows of the heads that share a head of keys are one matrix, row m = query row * group + head of the group, so that a block of keys and values is read
+// once for all of them.  A workgroup of four wavefronts has 128 such rows of a sequence, a wavefront 32, against blocks of 64 keys that go from memory straight into LDS
+// (no registers; two stages of the ring at head_dim above 64, four below), rows of 64 or 128 halves, 16-byte chunks XOR-swizzled by the row.
+//   S^T = K Q^T, v_mfma_f32_32x32x16_f16 with the keys as first operand: a lane has 16 of a tile's 32 keys of one row, and its neighbour 32 lanes on the others.
+//   softmax: scores stay as the product has them; p = exp2(s * sc - c) with the row's running reference c (RG_BELOW).  Sums and references are f32; probabilities enter the
+//     second product as f16 and the sum is that of the rounded ones.
+//   O^T += V^T P^T: eight probabilities of a lane are an operand as they lie, in an order of keys of their own; the values' operand comes in that order, transposed, out of
+//     LDS (ds_read_b64_tr_b16).
+// Which tile of which sequence a workgroup has it finds out by itself (rg_locate): the host knows no lengths.
+#include "ragged.h"
+
+#include <algorithm>
+#include <cmath>
+
+namespace rt {
+
+constexpr int RR_ROWS = 128, RR_KEYS = 64;
+constexpr int RR_MAX_SPLITS = 64;
+constexpr int rr_pitch(int ks) { return ks <= 4 ? 64 : 128; } // halves of a row in LDS
+constexpr int rr_stages(int ks) { return ks <= 4 ? 4 : 2; }
+typedef __fp16 rr_fp16x4 __attribute__((ext_vector_type(4)));
+typedef half_t half4_ru __attribute__((ext_vector_type(4), aligned(2)));
+
+__device__ __forceinline__ constexpr int rr_waitcnt(int n) { return 0x0070 | (n & 0xF) | (((n >> 4) & 0x3) << 14); } // vmcnt(n) lgkmcnt(0)
+
+// What chunk numbers of row r are XORed with.  The reads of keys take one chunk of 32 rows, those of values 64 bytes of four neighbouring rows (and of four others): rows four apart differ
+// in the low bits and neighbours in the high ones, so that each covers the banks evenly.
+template <int PITCH> __device__ __forceinline__ int rr_swizzle(int r) {
+    return PITCH == 128 ? ((r & 3) << 2) | ((r >> 2) & 3) : (((r >> 1) & 1) << 2) | ((r >> 2) & 3);
+}
+
+// maximum / sum of lanes l and l ^ 32
+__device__ __forceinline__ float rr_pair_max(float v) {
+    const uint32_t u = __builtin_bit_cast(uint32_t, v);
+    const auto a = __builtin_amdgcn_permlane32_swap(u, u, false, false);
+    return fmaxf(__builtin_bit_cast(float, (uint32_t)a[0]), __builtin_bit_cast(float, (uint32_t)a[1]));
+}
+__device__ __forceinline__ float rr_pair_sum(float v) {
+    const uint32_t u = __builtin_bit_cast(uint32_t, v);
+    const auto a = __builtin_amdgcn_permlane32_swap(u, u, false, false);
+    return __builtin_bit_cast(float, (uint32_t)a[0]) + __builtin_bit_cast(float, (uint32_t)a[1]);
+}
+
+// KS: steps of 16 over head_dim (the last one may be half)
+template <int KS, bool PAGED> __global__ __launch_bounds__(256, 2) void attention_ragged_kernel(RaggedArgs g) {
+    constexpr int P = rr_pitch(KS), CPR = P / 8, DT = (KS + 1) / 2, STAGES = rr_stages(KS);
+    constexpr int BLK = RR_KEYS * P;              // halves of a block of keys (or of values)
+    constexpr int RPI = 64 / CPR;                 // rows of a load instruction
+    constexpr int NI = RR_KEYS / RPI / 4;         // of them a wavefront issues per block and tensor
+    extern __shared__ __attribute__((aligned(16))) uint8_t smem[];
+    const half_t *const ring = (const half_t *)smem; // [STAGES][keys | values][64][P]
+    const int t = threadIdx.x, lane = t & 63, wave = __builtin_amdgcn_readfirstlane(t >> 6);
+    const int r = lane & 31, hi = lane >> 5;
+
+    int b, tile, first, key0;
+    const int line = blockIdx.x / g.kv_heads, kh = blockIdx.x - line * g.kv_heads, place = line / g.splits, share = line - place * g.splits;
+    if (!rg_locate<RR_ROWS>(g, place, b, tile)) return;
+    b = __builtin_amdgcn_readfirstlane(b), tile = __builtin_amdgcn_readfirstlane(tile);
+    const int n = __builtin_amdgcn_readfirstlane(rg_rows(g, b, first)), len = __builtin_amdgcn_readfirstlane(rg_keys<PAGED>(g, b, key0));
+    first = __builtin_amdgcn_readfirstlane(first), key0 = __builtin_amdgcn_readfirstlane(key0);
+    const int rows = n * g.group, off = len - n; // causal: query row i sees keys up to i + off
+    const int row0 = tile * RR_ROWS, rw = row0 + 32 * wave;
+    auto sees = [&](int m) { return g.causal ? max(0, min(len, min(m, rows - 1) / g.group + off + 1)) : len; }; // keys that row m sees: the first so many
+    // this share's blocks of those that a row of the tile sees
+    const int nkb = (sees(row0 + RR_ROWS - 1) + RR_KEYS - 1) / RR_KEYS;
+    const int kb0 = __builtin_amdgcn_readfirstlane((int)((int64_t)nkb * share / g.splits)), kb1 = __builtin_amdgcn_readfirstlane((int)((int64_t)nkb * (share + 1) / g.splits));
+    const int seen_all = __builtin_amdgcn_readfirstlane(rw < rows ? sees(rw) : 0), seen_any = __builtin_amdgcn_readfirstlane(rw < rows ? sees(rw + 31) : 0); // by each, by any of the wavefront's rows
+
+    // queries: row rw + r, dimensions 16 k + 8 hi .. + 7
+    const int m = min(rw + r, rows - 1), qi = m / g.group, qh = kh * g.group + (m - qi * g.group);
+    const int last = min(len - 1, g.causal ? qi + off : len - 1);
+    half8_t fq[KS];
+    {
+        const half_t *q = g.Q + (int64_t)(first + qi) * g.q_rs + (int64_t)qh * g.q_hs;
+        const half_t sign = (half_t)g.sign;
+#pragma unroll
+        for (int k = 0; k < KS; k++) {
+            const int d = 16 * k + 8 * hi;
+            fq[k] = d < g.D ? *(const half8_t *)(q + d) * half8_t{sign, sign, sign, sign, sign, sign, sign, sign} : half8_t{};
+        }
+    }
+    // awaited here: a first use in the loop would wait there, for these and with them for every load into LDS
+#pragma unroll
+    for (int k = 0; k < KS; k++) asm volatile("" : "+v"(fq[k]));
+
+    // columns behind head_dim are zeros: no load writes them
+    if (g.D < P)
+        for (int i = t; i < STAGES * 2 * BLK / 8; i += 256) ((uint4_t *)smem)[i] = uint4_t{0, 0, 0, 0};
+    __syncthreads();
+
+    // ---- loads: instruction i of this wavefront brings the rows RPI (wave + 4 i) .. of the block; lane l the chunk l % CPR of row l / CPR
+    const int lr = lane / CPR;
+    const half_t *const K = g.K + (int64_t)kh * g.k_hs, *const V = g.V + (int64_t)kh * g.v_hs;
+    typedef __attribute__((address_space(4))) const int32_t *scalar_t; // read through the scalar cache: no vector load is awaited for them
+    const scalar_t table = PAGED ? (scalar_t)(uintptr_t)(g.table + b * g.table_stride) : (scalar_t)0;
+    const int last_entry = PAGED ? max(0, len - 1) >> g.page_shift : 0;
+    int pages[4]; // of the 16 keys each of a block
+    auto look = [&](int kb) __attribute__((always_inline)) {
+        if constexpr (PAGED) {
+#pragma unroll
+            for (int i = 0; i < 4; i++) pages[i] = table[min((kb * RR_KEYS + 16 * i) >> g.page_shift, last_entry)];
+        }
+    };
+    int chunk[NI];      // this lane's chunk of its row
+    uint64_t lanes[NI]; // those whose chunk is a part of the row
+#pragma unroll
+    for (int i = 0; i < NI; i++) {
+        chunk[i] = (lane % CPR) ^ rr_swizzle<P>(RPI * (wave + 4 * i) + lr);
+        lanes[i] = __builtin_amdgcn_ballot_w64(8 * chunk[i] < g.D);
+    }
+    const uint32_t lds0 = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) uint8_t *)smem;
+    // block kb into a stage, from the pages that `pages` has; -> whether its four sixteenths are there, as bits
+    auto issue = [&](int stage, int kb) __attribute__((always_inline)) {
+        uint32_t there = 15u;
+#pragma unroll
+        for (int i = 0; i < NI; i++) {
+            const int row = RPI * (wave + 4 * i), c = chunk[i]; // row of the block; this lane's chunk
+            const half_t *kp, *vp;
+            uint32_t ko, vo;
+            if constexpr (PAGED) {
+                const int x = RPI == 4 ? pages[i] : wave < 2 ? pages[(2 * i) & 3] : pages[(2 * i + 1) & 3], page = (uint32_t)x < (uint32_t)g.pages ? x : 0; // (of row / 16)
+                const int64_t at = (int64_t)page * g.k_rs + (int64_t)((kb * RR_KEYS + row) & ((1 << g.page_shift) - 1)) * g.D;
+                kp = K + at, vp = V + at;
+                ko = vo = 2u * (uint32_t)(lr * g.D + 8 * c);
+            } else {
+                const int j = min(kb * RR_KEYS + row, len - 1), more = min(lr, len - 1 - j); // rows behind the last: the last again
+                kp = K + (key0 + j) * g.k_rs, vp = V + (key0 + j) * g.v_rs;
+                ko = 2u * (uint32_t)(more * (int)g.k_rs + 8 * c), vo = 2u * (uint32_t)(more * (int)g.v_rs + 8 * c);
+            }
+            const uint32_t dst = __builtin_amdgcn_readfirstlane(lds0 + (uint32_t)(2 * (stage * 2 * BLK + row * P)));
+            // (every lane is active here, and is again)
+            asm volatile("s_mov_b64 exec, %6\n\ts_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %2, %3\n\t"
+                         "s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %4, %5\n\ts_mov_b64 exec, -1" ::"s"(dst),
+                         "s"(dst + 2 * BLK), "v"(ko), "s"(kp), "v"(vo), "s"(vp), "s"(lanes[i])
+                         : "m0", "memory");
+        }
+        if constexpr (PAGED) {
+#pragma unroll
+            for (int i = 0; i < 4; i++)
+                if ((uint32_t)pages[i] >= (uint32_t)g.pages) there &= ~(1u << i);
+        }
+        return there;
+    };
+    // all but the newest `keep` blocks' loads of this wavefront have landed, and its LDS reads have returned; then everybody's have
+    auto publish = [&](auto keep) __attribute__((always_inline)) {
+        __builtin_amdgcn_sched_barrier(0);
+        asm volatile("" ::: "memory");
+        __builtin_amdgcn_s_waitcnt(rr_waitcnt(decltype(keep)::value * 2 * NI));
+        __builtin_amdgcn_s_barrier();
+        asm volatile("" ::: "memory");
+        __builtin_amdgcn_sched_barrier(0);
+    };
+
+    float16_t acc[DT];
+    float c_run = -INFINITY, l_run = 0.f; // the reference, this lane's share of the sum
+    bool coarse = false; // whether scores are rounded before the reference is taken away (uniform)
+#pragma unroll
+    for (int d = 0; d < DT; d++) acc[d] = float16_t{};
+
+    // fragment offsets in a stage, halves
+    int koff[KS], voff[DT][2];
+#pragma unroll
+    for (int k = 0; k < KS; k++) koff[k] = r * P + 8 * ((2 * k + hi) ^ rr_swizzle<P>(r));
+    auto value_at = [&](int d, int w) { // dimensions 32 d .., of 16 keys the row 4 hi + (lane % 16) / 4, and 8 more
+        const int s = lane & 15, half = (lane >> 4) & 1, row = 4 * hi + (s >> 2) + 8 * w;
+        return BLK + row * P + 8 * ((4 * d + 2 * half + ((s & 3) >> 1)) ^ rr_swizzle<P>(row)) + 4 * (s & 1);
+    };
+#pragma unroll
+    for (int d = 0; d < DT; d++) voff[d][0] = value_at(d, 0), voff[d][1] = value_at(d, 1);
+    auto transposed = [&](const half_t *p0, const half_t *p1) __attribute__((always_inline)) {
+        typedef uint64_t u64x2_t __attribute__((ext_vector_type(2)));
+        typedef __attribute__((address_space(3))) rr_fp16x4 *lds4;
+        const uint64_t v0 = __builtin_bit_cast(uint64_t, __builtin_amdgcn_ds_read_tr16_b64_v4f16((lds4)p0));
+        const uint64_t v1 = __builtin_bit_cast(uint64_t, __builtin_amdgcn_ds_read_tr16_b64_v4f16((lds4)p1));
+        return __builtin_bit_cast(half8_t, u64x2_t{v0, v1});
+    };
+    auto values = [&](const half_t *st, int d, int s) __attribute__((always_inline)) { // dimensions 32 d .., keys 16 s ..
+        return transposed(st + voff[d][0] + 16 * s * P, st + voff[d][1] + 16 * s * P);
+    };
+
+    auto step = [&](int stage, int kb, uint32_t there, auto lean_c) __attribute__((always_inline)) {
+        constexpr bool LEAN = decltype(lean_c)::value;
+        const half_t *const st = ring + stage * 2 * BLK;
+        float16_t S[2];
+#pragma unroll
+        for (int u = 0; u < 2; u++) {
+            S[u] = float16_t{};
+#pragma unroll
+            for (int k = 0; k < KS; k++) {
+                const half8_t fk = *(const half8_t *)(st + koff[k] + 32 * u * P);
+                S[u] = __builtin_amdgcn_mfma_f32_32x32x16_f16(fk, fq[k], S[u], 0, 0, 0);
+            }
+        }
+        // register i of S[u]: key 32 u + 8 (i / 4) + 4 hi + i % 4 of the block
+        int left = last - kb * RR_KEYS - 4 * hi;
+        auto sees_key = [&](int u, int i) { return 32 * u + 8 * (i >> 2) + (i & 3) <= left && ((there >> (2 * u + (i >> 3))) & 1u); };
+        float top = -INFINITY;
+#pragma unroll
+        for (int u = 0; u < 2; u++)
+#pragma unroll
+            for (int i = 0; i < 16; i++) {
+                if constexpr (!LEAN) S[u][i] = sees_key(u, i) ? S[u][i] : -INFINITY;
+                top = fmaxf(top, S[u][i]);
+            }
+        top = rr_pair_max(top) * g.sc;
+        float sc = g.sc;
+        if (__builtin_amdgcn_ballot_w64(top - c_run > RG_ABOVE)) {
+            const float c = fmaxf(c_run, top - RG_BELOW), alpha = c == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(c_run - c);
+            c_run = c;
+            l_run *= alpha;
+#pragma unroll
+            for (int d = 0; d < DT; d++) acc[d] *= alpha;
+            // The reference is a rounded product, which a score meets in the fused multiply-add without a rounding of its own: past 4096 the difference shows, and past 2^24 a
+            // probability could leave f16.  From there on scores are rounded first.
+            coarse = __builtin_amdgcn_ballot_w64(c != -INFINITY && !(__builtin_fabsf(c) < 4096.f)) != 0;
+        }
+        if (coarse) {
+#pragma unroll
+            for (int u = 0; u < 2; u++)
+#pragma unroll
+                for (int i = 0; i < 16; i++) S[u][i] *= sc;
+            sc = 1.f;
+        }
+        const float c = c_run == -INFINITY ? 0.f : c_run; // a row that has seen no key: exp2(-inf)
+        half8_t fp[4];
+        float sum = 0.f;
+#pragma unroll
+        for (int u = 0; u < 2; u++)
+#pragma unroll
+            for (int i = 0; i < 16; i += 2) {
+                const half2_t p = {(half_t)__builtin_amdgcn_exp2f(fmaf(S[u][i], sc, -c)), (half_t)__builtin_amdgcn_exp2f(fmaf(S[u][i + 1], sc, -c))};
+                sum = __builtin_amdgcn_fdot2(p, half2_t{(half_t)1, (half_t)1}, sum, false);
+                fp[2 * u + (i >> 3)][i & 7] = p[0], fp[2 * u + (i >> 3)][(i & 7) + 1] = p[1];
+            }
+        l_run += sum;
+        bool odd = false;
+        if constexpr (!LEAN) { // a value that is not finite must not reach, as 0 * inf, the rows that do not see its key
+            float x = 0.f;
+#pragma unroll
+            for (int s = 0; s < 4; s++)
+#pragma unroll
+                for (int d = 0; d < DT; d++) {
+                    x = rg_odd(values(st, d, s), x);
+                    __builtin_amdgcn_sched_barrier(0);
+                }
+            odd = __builtin_amdgcn_ballot_w64(x != 0.f) != 0; // (NaN is)
+        }
+        if (!LEAN && odd) {
+            // Such values enter as 0, and a second product counts, for each row and dimension, how many it sees that are +inf (1 each), -inf (256) or NaN (both)
+#pragma unroll
+            for (int d = 0; d < DT; d++) {
+                float16_t mark = {};
+                asm volatile("" : "+v"(left), "+s"(there)::"memory"); // (read and compared again: nothing of this is worth registers outside)
+#pragma unroll
+                for (int s = 0; s < 4; s++) {
+                    half8_t v = values(st, d, s), vis;
+                    const half8_t code = rg_take_odd(v);
+#pragma unroll
+                    for (int e = 0; e < 8; e++) vis[e] = __builtin_bit_cast(half_t, (uint16_t)(sees_key(s >> 1, 8 * (s & 1) + e) ? 0x3C00 : 0));
+                    acc[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v, fp[s], acc[d], 0, 0, 0);
+                    mark = __builtin_amdgcn_mfma_f32_32x32x16_f16(code, vis, mark, 0, 0, 0);
+                    __builtin_amdgcn_sched_barrier(0);
+                }
+#pragma unroll
+                for (int i = 0; i < 16; i++) {
+                    acc[d][i] += (int)mark[i] & 255 ? INFINITY : 0.f;
+                    acc[d][i] += mark[i] >= 256.f ? -INFINITY : 0.f;
+                }
+                __builtin_amdgcn_sched_barrier(0);
+            }
+        } else {
+#pragma unroll
+            for (int s = 0; s < 4; s++)
+#pragma unroll
+                for (int d = 0; d < DT; d++) acc[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(values(st, d, s), fp[s], acc[d], 0, 0, 0);
+        }
+    };
+
+    if (kb0 < kb1) {
+        uint32_t there[STAGES];
+        look(kb0);
+#pragma unroll
+        for (int s = 0; s < STAGES - 1; s++) {
+            there[s] = issue(s, min(kb0 + s, kb1 - 1)); // past the end: the last block again, into a stage that nobody reads
+            look(min(kb0 + s + 1, kb1 - 1));
+        }
+        publish(std::integral_constant<int, STAGES - 2>{});
+        int cur = 0, fill = STAGES - 1, kb = kb0;
+        auto turn = [&](auto body) __attribute__((always_inline)) {
+            const uint32_t now = there[0];
+#pragma unroll
+            for (int s = 0; s + 2 < STAGES; s++) there[s] = there[s + 1];
+            there[STAGES - 2] = issue(fill, min(kb + STAGES - 1, kb1 - 1));
+            look(min(kb + STAGES, kb1 - 1));
+            body(now);
+            publish(std::integral_constant<int, STAGES - 2>{});
+            cur = cur + 1 == STAGES ? 0 : cur + 1, fill = fill + 1 == STAGES ? 0 : fill + 1;
+            kb++;
+        };
+        const int lean = min(kb1, seen_all / RR_KEYS), any = min(kb1, (seen_any + RR_KEYS - 1) / RR_KEYS);
+        while (kb < lean && there[0] == 15u) turn([&](uint32_t) { step(cur, kb, 15u, std::true_type{}); });
+        while (kb < any) turn([&](uint32_t now) { step(cur, kb, now, std::false_type{}); });
+        while (kb < kb1) turn([](uint32_t) {}); // blocks that only other wavefronts need
+    }
+    __builtin_amdgcn_s_waitcnt(rr_waitcnt(0)); // nothing lands after the workgroup has ended
+    const float l = rr_pair_sum(l_run);
+    if (rw + r >= rows) return;
+    const int64_t row = first + qi;
+    if (g.splits > 1) {
+        const int64_t at = ((row * g.kv_heads + kh) * g.group + (m - qi * g.group)) * g.splits + share;
+        if (hi == 0) *(float2_t *)(g.part_ml + 2 * at) = float2_t{c_run, l};
+        if (kb0 < kb1) { // (a share with a sum of 0 is not read)
+            float *const po = g.part_o + at * g.D;
+#pragma unroll
+            for (int d = 0; d < DT; d++)
+#pragma unroll
+                for (int i = 0; i < 16; i += 4) {
+                    const int x = 32 * d + 2 * i + 4 * hi;
+                    if (x < g.D) *(float4_t *)(po + x) = float4_t{acc[d][i], acc[d][i + 1], acc[d][i + 2], acc[d][i + 3]};
+                }
+        }
+    } else {
+        const float inv = 1.f / l; // no visible key: 0 * inf, NaN
+        half_t *const o = g.O + row * g.o_rs + (int64_t)qh * g.o_hs;
+#pragma unroll
+        for (int d = 0; d < DT; d++)
+#pragma unroll
+            for (int i = 0; i < 16; i += 4) {
+                const int x = 32 * d + 2 * i + 4 * hi;
+                if (x < g.D) *(half4_ru *)(o + x) = half4_ru{(half_t)(acc[d][i] * inv), (half_t)(acc[d][i + 1] * inv), (half_t)(acc[d][i + 2] * inv), (half_t)(acc[d][i + 3] * inv)};
+            }
+    }
+}
+
+// Joins the shares of a row in a fixed order.  A workgroup has 16 of a tile's 128 rows (blockIdx.y), 16 threads each, four columns a thread at a time.
+__global__ __launch_bounds__(256) void attention_ragged_join_kernel(RaggedArgs g) {
+    int b, tile, first;
+    const int place = blockIdx.x / g.kv_heads, kh = blockIdx.x - place * g.kv_heads;
+    if (!rg_locate<RR_ROWS>(g, place, b, tile)) return;
+    const int n = rg_rows(g, b, first), m = tile * RR_ROWS + blockIdx.y * 16 + (threadIdx.x >> 4);
+    if (m >= n * g.group) return;
+    const int qi = m / g.group, h = kh * g.group + (m - qi * g.group);
+    const int64_t row = first + qi, at = (row * g.kv_heads * g.group + h) * g.splits;
+    float top = -INFINITY;
+    for (int s = 0; s < g.splits; s++) top = fmaxf(top, g.part_ml[2 * (at + s)]);
+    const float base = top == -INFINITY ? 0.f : top;
+    float l = 0.f;
+    for (int s = 0; s < g.splits; s++) l = fmaf(__builtin_amdgcn_exp2f(g.part_ml[2 * (at + s)] - base), g.part_ml[2 * (at + s) + 1], l);
+    for (int d = 4 * (threadIdx.x & 15); d < g.D; d += 64) {
+        float4_t y = {0.f, 0.f, 0.f, 0.f};
+        for (int s = 0; s < g.splits; s++) {
+            const float2_t ml = *(const float2_t *)(g.part_ml + 2 * (at + s));
+            if (ml[1] == 0.f) continue; // no key, and no outputs were written
+            const float a = __builtin_amdgcn_exp2f(ml[0] - base);
+            const float4_t v = *(const float4_t *)(g.part_o + (at + s) * g.D + d);
+#pragma unroll
+            for (int k = 0; k < 4; k++) y[k] = fmaf(a, v[k], y[k]);
+        }
+        *(half4_ru *)(g.O + row * g.o_rs + (int64_t)h * g.o_hs + d) = half4_ru{(half_t)(y[0] / l), (half_t)(y[1] / l), (half_t)(y[2] / l), (half_t)(y[3] / l)};
+    }
+}
+
+// Tiles of a call, at most: sequences have `rows` rows in all, and each may leave one tile begun.
+static int64_t rr_tiles(int batch, int group, int rows, int max_rows) {
+    return std::min<int64_t>((int64_t)batch * (((int64_t)max_rows * group + RR_ROWS - 1) / RR_ROWS), (int64_t)rows * group / RR_ROWS + batch);
+}
+static int rr_splits(int64_t wgs, int max_keys) {
+    const int64_t steps = (max_keys + RR_KEYS - 1) / RR_KEYS;
+    return (int)std::max<int64_t>(1, std::min<int64_t>({(int64_t)RR_MAX_SPLITS, steps / 4, 512 / std::max<int64_t>(wgs, 1)}));
+}
+static uint64_t rr_workspace(int heads, int rows, int head_dim, int splits) {
+    return splits <= 1 ? 0 : (uint64_t)rows * heads * splits * (head_dim + 2) * sizeof(float);
+}
+
+static bool rr_fits(int batch, int kv_heads, int group, int rows, int max_rows) {
+    return rr_tiles(batch, group, rows, max_rows) * kv_heads <= 0xffffff; // a grid's threads are fewer than 2^32; shares take no call past that
+}
+static uint64_t rr_workspace_bytes(int batch, int heads, int kv_heads, int rows, int max_rows, int max_keys, int head_dim) {
+    return rr_workspace(heads, rows, head_dim, rr_splits(rr_tiles(batch, heads / kv_heads, rows, max_rows) * kv_heads, max_keys));
+}
+
+template <int KS, bool PAGED> static hipError_t launch_rr(const RaggedArgs &g, hipStream_t st) {
+    constexpr size_t lds = (size_t)rr_stages(KS) * 2 * RR_KEYS * rr_pitch(KS) * sizeof(half_t);
+    if (const hipError_t e = ensure_lds_limit<&attention_ragged_kernel<KS, PAGED>>(); e != hipSuccess) return e;
+    hipLaunchKernelGGL((attention_ragged_kernel<KS, PAGED>), dim3((unsigned)((int64_t)g.tiles * g.kv_heads * g.splits)), dim3(256), lds, st, g);
+    return hipGetLastError();
+}
+
+// exp(scale * s) as exp2(sc * s) with sc above 0, whatever the scale's sign; a scale of 0 leaves scores of 0
+static void rr_scale(RaggedArgs &g, float scale) {
+    g.sign = scale > 0.f ? 1.f : scale < 0.f ? -1.f : 0.f;
+    g.sc = scale == 0.f ? 1.f : std::fabs(scale) * kLog2eR;
+}
+
+// `g` has the operands; the shares, and where partial results go, are chosen here.
+static hipError_t launch_ragged(RaggedArgs &g, bool paged, void *workspace, uint64_t workspace_bytes, hipStream_t stream) {
+    g.tiles = (int)rr_tiles(g.batch, g.group, g.rows, g.max_rows);
+    g.splits = rr_splits((int64_t)g.tiles * g.kv_heads, g.max_keys);
+    const uint64_t need = rr_workspace(g.kv_heads * g.group, g.rows, g.D, g.splits);
+    if (need && workspace && workspace_bytes >= need && !((uintptr_t)workspace & 15u))
+        g.part_o = (float *)workspace, g.part_ml = g.part_o + (uint64_t)g.rows * g.kv_heads * g.group * g.splits * g.D;
+    else
+        g.splits = 1;
+    auto go = [&](auto ks) -> hipError_t {
+        constexpr int KS = decltype(ks)::value;
+        return paged ? launch_rr<KS, true>(g, stream) : launch_rr<KS, false>(g, stream);
+    };
+    hipError_t e;
+    switch ((g.D + 15) / 16) {
+    case 1: e = go(std::integral_constant<int, 1>{}); break;
+    case 2: e = go(std::integral_constant<int, 2>{}); break;
+    case 3: e = go(std::integral_constant<int, 3>{}); break;
+    case 4: e = go(std::integral_constant<int, 4>{}); break;
+    case 5: e = go(std::integral_constant<int, 5>{}); break;
+    case 6: e = go(std::integral_constant<int, 6>{}); break;
+    case 7: e = go(std::integral_constant<int, 7>{}); break;
+    default: e = go(std::integral_constant<int, 8>{}); break;
+    }
+    if (e != hipSuccess || g.splits <= 1) return e;
+    hipLaunchKernelGGL(attention_ragged_join_kernel, dim3((unsigned)((int64_t)g.tiles * g.kv_heads), RR_ROWS / 16), dim3(256), 0, stream, g);
+    return hipGetLastError();
+}
+
+bool attention_packed_fits(const rt_attention_packed_desc &d) {
+    if (d.batch == 0 || d.heads == 0 || d.rows == 0) return true;
+    return rr_fits(d.batch, d.kv_heads, d.heads / d.kv_heads, d.rows, d.max_rows);
+}
+uint64_t attention_packed_workspace_bytes(const rt_attention_packed_desc &d) {
+    if (d.batch == 0 || d.heads == 0 || d.rows == 0) return 0;
+    return rr_workspace_bytes(d.batch, d.heads, d.kv_heads, d.rows, d.max_rows, d.max_keys, d.head_dim);
+}
+hipError_t launch_attention_packed(const rt_attention_packed_desc &d, const void *q, const void *k, const void *v, const int32_t *starts, const int32_t *kv_starts,
+                                   void *out, void *workspace, uint64_t workspace_bytes, hipStream_t stream, const DeviceInfo &dev) {
+    RaggedArgs g{};
+    g.Q = (const half_t *)q, g.K = (const half_t *)k, g.V = (const half_t *)v, g.O = (half_t *)out, g.starts = starts, g.kv_starts = kv_starts;
+    g.q_rs = d.q_strides[0], g.q_hs = d.q_strides[1], g.o_rs = d.o_strides[0], g.o_hs = d.o_strides[1];
+    g.k_rs = d.k_strides[0], g.k_hs = d.k_strides[1], g.v_rs = d.v_strides[0], g.v_hs = d.v_strides[1];
+    g.batch = d.batch, g.kv_heads = d.kv_heads, g.group = d.heads / d.kv_heads, g.D = d.head_dim;
+    g.rows = d.rows, g.kv_rows = d.kv_rows, g.max_rows = d.max_rows, g.max_keys = d.max_keys, g.causal = d.causal;
+    rr_scale(g, d.scale);
+    return launch_ragged(g, false, workspace, workspace_bytes, stream);
+}
+
+bool attention_paged_fits(const rt_attention_paged_desc &d) {
+    if (d.cache.batch == 0 || d.heads == 0 || d.rows == 0) return true;
+    return rr_fits(d.cache.batch, d.cache.kv_heads, d.heads / d.cache.kv_heads, d.rows, d.max_rows);
+}
+uint64_t attention_paged_workspace_bytes(const rt_attention_paged_desc &d) {
+    if (d.cache.batch == 0 || d.heads == 0 || d.rows == 0) return 0;
+    return rr_workspace_bytes(d.cache.batch, d.heads, d.cache.kv_heads, d.rows, d.max_rows, d.max_keys, d.cache.head_dim);
+}
+hipError_t launch_attention_paged(const rt_attention_paged_desc &d, const void *q, const void *k_pool, const void *v_pool, const int32_t *table, const int32_t *lens,
+                                  const int32_t *starts, void *out, void *workspace, uint64_t workspace_bytes, hipStream_t stream, const DeviceInfo &dev) {
+    RaggedArgs g{};
+    const rt_paged_cache_desc &c = d.cache;
+    g.Q = (const half_t *)q, g.K = (const half_t *)k_pool, g.V = (const half_t *)v_pool, g.O = (half_t *)out, g.starts = starts, g.table = table, g.lens = lens;
+    g.q_rs = d.q_strides[0], g.q_hs = d.q_strides[1], g.o_rs = d.o_strides[0], g.o_hs = d.o_strides[1];
+    g.k_hs = g.v_hs = (int64_t)c.page_size * c.head_dim, g.k_rs = g.v_rs = g.k_hs * c.kv_heads; // a head's part of a page, a page
+    g.table_stride = c.table_stride, g.pages = c.pages, g.page_shift = __builtin_ctz(c.page_size), g.table_width = c.table_width;
+    g.batch = c.batch, g.kv_heads = c.kv_heads, g.group = d.heads / c.kv_heads, g.D = c.head_dim;
+    g.rows = d.rows, g.max_rows = d.max_rows, g.max_keys = d.max_keys, g.causal = d.causal;
+    if (c.pages == 0) g.max_keys = 0; // no page is there: no key
+    rr_scale(g, d.scale);
+    return launch_ragged(g, true, workspace, workspace_bytes, stream);
+}
+
+} // namespace rt
