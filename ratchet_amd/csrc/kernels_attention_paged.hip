@@ -1,0 +1,496 @@
+// Attention over a key/value cache held in pages, up to 32 rows per head of keys (ragged.h): a step of one or a few tokens of every sequence.
+//
+//   out[m] = sum_j p_j v_j,  p = softmax_j(scale * q[m] . k_j);  row m = query row * group + head of the group
+//
+// What has to be done is to read the pages once, so the kernel is laid out around the loads: each of a workgroup's four wavefronts takes 32 keys of 128 in turn, brings
+// them into a part of LDS of its own, straight from memory, and waits for nobody else.  There is one block of keys and one of values: a wavefront asks for its next keys as soon as
+// the scores are made, and for the values behind them when those are multiplied, so that 8 to 16 KB a wavefront are on their way at any time.
+//   S^T = K Q^T and O^T += V^T P^T by v_mfma_f32_16x16x32_f16, as in kernels_attention_ragged.hip: a lane has four keys of 16 for one row, its probabilities are an operand as
+//   they lie, and the values' comes transposed out of LDS.
+// The work is the line of all 128 keys of all sequences and heads of keys; a workgroup takes an equal part of it, whatever the sequences' lengths, and so ends within a sequence.
+// What it has of one that others share goes to the workspace, at most twice, and a second kernel joins the parts in a fixed order.  Lengths stay on the device.
+#include "ragged.h"
+
+#include <algorithm>
+
+namespace rt {
+
+constexpr int PS_KEYS = 128, PS_UNIT = 32; // of a workgroup's step, of a wavefront's
+constexpr int ps_pitch(int ks) { return ks <= 4 ? 64 : 128; }
+constexpr int ps_ring(int ks) { return 2 * PS_UNIT * ps_pitch(ks) * 2; } // bytes of a wavefront
+typedef __fp16 ps_fp16x4 __attribute__((ext_vector_type(4)));
+
+__device__ __forceinline__ constexpr int ps_waitcnt(int n) { return 0x0070 | (n & 0xF) | (((n >> 4) & 0x3) << 14); } // vmcnt(n) lgkmcnt(0)
+
+// As rr_swizzle of the tiled kernel: rows four apart differ in the low bits, neighbours in the high ones.
+template <int PITCH> __device__ __forceinline__ int ps_swizzle(int r) {
+    return PITCH == 128 ? ((r & 3) << 2) | ((r >> 2) & 3) : (((r >> 1) & 1) << 2) | ((r >> 2) & 3);
+}
+
+// Steps of a sequence (at least one where it has rows: they are NaN), and of all up to a sequence.
+__device__ __forceinline__ int ps_steps(const RaggedArgs &g, int b) {
+    int first;
+    if (b >= g.batch || rg_rows(g, b, first) == 0) return 0;
+    return max(1, (rg_keys<true>(g, b, first) + PS_KEYS - 1) / PS_KEYS);
+}
+
+// The place in the line at which workgroup i begins, and which workgroup has place c.
+// (No more workgroups than places.)
+__device__ __forceinline__ int ps_begin(int64_t i, int64_t total, int wgs) { return (int)(i * total / wgs); }
+__device__ __forceinline__ int ps_owner(int64_t c, int64_t total, int wgs) { return (int)(((c + 1) * wgs + total - 1) / total) - 1; }
+
+// KS: steps of 16 over head_dim (the last may be half).  NR: tiles of 16 rows
+template <int KS, int NR> __global__ __launch_bounds__(256, 2) void attention_paged_stream_kernel(RaggedArgs g, int whole) {
+    constexpr int P = ps_pitch(KS), CPR = P / 8, KK = (KS + 1) / 2, RPI = 64 / CPR, NI = PS_UNIT / RPI;
+    constexpr int BLK = PS_UNIT * P; // halves of a block of keys, of values
+    extern __shared__ __attribute__((aligned(16))) uint8_t smem[];
+    const int t = threadIdx.x, lane = t & 63, wave = __builtin_amdgcn_readfirstlane(t >> 6);
+    const int fr = lane & 15, fg = lane >> 4;
+    half_t *const mine = (half_t *)(smem + wave * ps_ring(KS));  // this wavefront's [keys | values][32][P]
+    float *const sums = (float *)(smem + 4 * ps_ring(KS));       // [wavefront][row][2]
+
+    // ---- where this workgroup begins and ends
+    int b = 0, kh = 0, step = 0, todo;
+    if (whole) { // a head of keys each
+        b = blockIdx.x / g.kv_heads, kh = blockIdx.x - b * g.kv_heads;
+        todo = __builtin_amdgcn_readfirstlane(ps_steps(g, b));
+    } else {
+        int64_t total = 0;
+        for (int c = 0; c < g.batch; c += 64) total += rg_sum(ps_steps(g, c + lane));
+        total *= g.kv_heads;
+        const int wgs = (int)min((int64_t)gridDim.x, total);
+        if (blockIdx.x >= wgs) return;
+        int at = ps_begin(blockIdx.x, total, wgs);
+        todo = ps_begin(blockIdx.x + 1, total, wgs) - at;
+        if (todo > 0)
+            for (int c = 0; c < g.batch; c += 64) {
+                const int s = ps_steps(g, c + lane), upto = rg_scan(s, lane), all = __builtin_amdgcn_readlane(upto, 63);
+                if (at >= all * g.kv_heads) { // (no step count passes 31 bits: host)
+                    at -= all * g.kv_heads;
+                    continue;
+                }
+                const int l = __builtin_ctzll(__builtin_amdgcn_ballot_w64(upto * g.kv_heads > at));
+                const int n = __builtin_amdgcn_readlane(s, l);
+                at -= (__builtin_amdgcn_readlane(upto, l) - n) * g.kv_heads;
+                b = c + l, kh = at / n, step = at - kh * n;
+                break;
+            }
+    }
+    b = __builtin_amdgcn_readfirstlane(b), kh = __builtin_amdgcn_readfirstlane(kh), step = __builtin_amdgcn_readfirstlane(step), todo = __builtin_amdgcn_readfirstlane(todo);
+    if (todo <= 0) return;
+
+    // columns behind head_dim are zeros: no load writes them
+    if (g.D < P) {
+        for (int i = lane; i < ps_ring(KS) / 16; i += 64) ((uint4_t *)mine)[i] = uint4_t{0, 0, 0, 0};
+        __builtin_amdgcn_s_waitcnt(ps_waitcnt(0));
+    }
+    const int lr = lane / CPR;
+    int chunk[NI];
+    uint64_t lanes[NI];
+#pragma unroll
+    for (int i = 0; i < NI; i++) {
+        chunk[i] = (lane % CPR) ^ ps_swizzle<P>(RPI * i + lr);
+        lanes[i] = __builtin_amdgcn_ballot_w64(8 * chunk[i] < g.D);
+    }
+    const uint32_t lds0 = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) uint8_t *)mine;
+    int koff[KK];
+#pragma unroll
+    for (int k = 0; k < KK; k++) koff[k] = fr * P + 8 * ((4 * k + fg) ^ ps_swizzle<P>(fr));
+    const int vrow = 4 * fg + (fr >> 2), vhalf = (fr & 3) >> 1;
+
+    bool begun = false; // whether this is not the first head of keys of the workgroup
+    while (todo > 0) {
+        int first, unused;
+        if (b >= g.batch) return;
+        const int n = __builtin_amdgcn_readfirstlane(rg_rows(g, b, first)), len = __builtin_amdgcn_readfirstlane(rg_keys<true>(g, b, unused));
+        first = __builtin_amdgcn_readfirstlane(first);
+        const int all = max(1, (len + PS_KEYS - 1) / PS_KEYS);
+        if (n == 0) { // (has no steps)
+            b++;
+            continue;
+        }
+        const int upto = min(all, step + todo), rows = n * g.group, off = len - n;
+        auto sees = [&](int m) { return g.causal ? max(0, min(len, m / g.group + off + 1)) : len; };
+        const int seen_all = sees(0), seen_any = sees(rows - 1);
+
+        half8_t fq[NR][KK];
+        int last[NR];
+#pragma unroll
+        for (int u = 0; u < NR; u++) {
+            const int m = min(16 * u + fr, rows - 1), qi = m / g.group;
+            last[u] = g.causal ? min(len - 1, qi + off) : len - 1;
+            const half_t *q = g.Q + (int64_t)(first + qi) * g.q_rs + (int64_t)(kh * g.group + (m - qi * g.group)) * g.q_hs;
+            const half_t sign = (half_t)g.sign;
+#pragma unroll
+            for (int k = 0; k < KK; k++) {
+                const int d = 32 * k + 8 * fg;
+                fq[u][k] = d < g.D ? *(const half8_t *)(q + d) * half8_t{sign, sign, sign, sign, sign, sign, sign, sign} : half8_t{};
+            }
+        }
+
+        typedef __attribute__((address_space(4))) const int32_t *scalar_t; // read through the scalar cache
+        const scalar_t table = (scalar_t)(uintptr_t)(g.table + b * g.table_stride);
+        const int last_entry = max(0, len - 1) >> g.page_shift;
+        const half_t *const K = g.K + (int64_t)kh * g.k_hs, *const V = g.V + (int64_t)kh * g.v_hs;
+        int pages[2], at_keys; // of the next unit's 16 keys each; its first key
+        auto look = [&](int j) __attribute__((always_inline)) {
+            at_keys = j;
+#pragma unroll
+            for (int i = 0; i < 2; i++) pages[i] = table[min((j + 16 * i) >> g.page_shift, last_entry)];
+        };
+        int64_t where[2]; // of them in a pool, halves from the head's
+        auto place = [&]() __attribute__((always_inline)) {
+            uint32_t there = 3u;
+#pragma unroll
+            for (int i = 0; i < 2; i++) {
+                const bool is = (uint32_t)pages[i] < (uint32_t)g.pages;
+                if (!is) there &= ~(1u << i);
+                where[i] = (int64_t)(is ? pages[i] : 0) * g.k_rs + (int64_t)((at_keys + 16 * i) & ((1 << g.page_shift) - 1)) * g.D;
+            }
+            return there;
+        };
+        auto issue = [&](const half_t *pool, uint32_t dst0) __attribute__((always_inline)) {
+#pragma unroll
+            for (int i = 0; i < NI; i++) {
+                const half_t *p = pool + where[RPI * i >> 4] + (RPI * i & 15) * g.D;
+                const uint32_t o = 2u * (uint32_t)(lr * g.D + 8 * chunk[i]), dst = __builtin_amdgcn_readfirstlane(dst0 + 2u * RPI * i * P);
+                // (every lane is active here, and is again)
+                asm volatile("s_mov_b64 exec, %3\n\ts_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2\n\ts_mov_b64 exec, -1" ::"s"(dst), "v"(o), "s"(p), "s"(lanes[i])
+                             : "m0", "memory");
+            }
+        };
+        auto wait = [&](auto keep) __attribute__((always_inline)) {
+            __builtin_amdgcn_sched_barrier(0);
+            asm volatile("" ::: "memory");
+            __builtin_amdgcn_s_waitcnt(ps_waitcnt(decltype(keep)::value));
+            asm volatile("" ::: "memory");
+            __builtin_amdgcn_sched_barrier(0);
+        };
+        using All = std::integral_constant<int, 0>;
+        using But = std::integral_constant<int, NI>;
+
+        float4_t acc[NR][KS];
+        float c_run[NR], l_run[NR];
+        bool coarse = false;
+#pragma unroll
+        for (int u = 0; u < NR; u++) {
+            c_run[u] = -INFINITY, l_run[u] = 0.f;
+#pragma unroll
+            for (int d = 0; d < KS; d++) acc[u][d] = float4_t{0.f, 0.f, 0.f, 0.f};
+        }
+        auto values = [&](int d) __attribute__((always_inline)) { // dimensions 16 d ..; keys 4 fg .. and 16 + 4 fg ..
+            typedef uint64_t u64x2_t __attribute__((ext_vector_type(2)));
+            typedef __attribute__((address_space(3))) ps_fp16x4 *lds4;
+            const half_t *p = mine + BLK + vrow * P + 8 * ((2 * d + vhalf) ^ ps_swizzle<P>(vrow)) + 4 * (fr & 1);
+            const uint64_t v0 = __builtin_bit_cast(uint64_t, __builtin_amdgcn_ds_read_tr16_b64_v4f16((lds4)p));
+            const uint64_t v1 = __builtin_bit_cast(uint64_t, __builtin_amdgcn_ds_read_tr16_b64_v4f16((lds4)(p + 16 * P)));
+            return __builtin_bit_cast(half8_t, u64x2_t{v0, v1});
+        };
+
+        int j = step * PS_KEYS + PS_UNIT * wave; // this wavefront's keys
+        const int j_end = min(upto * PS_KEYS, seen_any);
+        if (j < j_end) {
+            look(j);
+            uint32_t there = place();
+            issue(K, lds0), issue(V, lds0 + 2 * BLK);
+            bool more = j + PS_KEYS < j_end;
+            if (more) look(j + PS_KEYS);
+            wait(But{}); // (with the queries: the compiler waits for all)
+            while (true) {
+                // ---- scores
+                float4_t S[NR][2];
+#pragma unroll
+                for (int u = 0; u < NR; u++) S[u][0] = S[u][1] = float4_t{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                for (int h = 0; h < 2; h++)
+#pragma unroll
+                    for (int k = 0; k < KK; k++) {
+                        const half8_t fk = *(const half8_t *)(mine + koff[k] + 16 * h * P);
+#pragma unroll
+                        for (int u = 0; u < NR; u++) S[u][h] = __builtin_amdgcn_mfma_f32_16x16x32_f16(fk, fq[u][k], S[u][h], 0, 0, 0);
+                    }
+                const uint32_t now = there;
+                if (more) {
+                    wait(But{}); // (of LDS: the keys have been read.  The values are not awaited: they are NI loads)
+                    there = place();
+                    issue(K, lds0);
+                }
+                // ---- softmax
+                int left[NR];
+#pragma unroll
+                for (int u = 0; u < NR; u++) left[u] = last[u] - j - 4 * fg;
+                const bool lean = j + PS_UNIT <= seen_all && now == 3u;
+                auto sees_key = [&](int u, int e) { return 16 * (e >> 2) + (e & 3) <= left[u] && ((now >> (e >> 2)) & 1u); };
+                half8_t fp[NR];
+#pragma unroll
+                for (int u = 0; u < NR; u++) {
+                    if (!lean)
+#pragma unroll
+                        for (int e = 0; e < 8; e++) S[u][e >> 2][e & 3] = sees_key(u, e) ? S[u][e >> 2][e & 3] : -INFINITY;
+                    float top = -INFINITY;
+#pragma unroll
+                    for (int e = 0; e < 8; e++) top = fmaxf(top, S[u][e >> 2][e & 3]);
+                    top = rt_groups_max(top) * g.sc;
+                    if (__builtin_amdgcn_ballot_w64(top - c_run[u] > RG_ABOVE)) {
+                        const float c = fmaxf(c_run[u], top - RG_BELOW), alpha = c == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(c_run[u] - c);
+                        c_run[u] = c;
+                        l_run[u] *= alpha;
+#pragma unroll
+                        for (int d = 0; d < KS; d++) acc[u][d] *= alpha;
+                        // (scores past 4096 are rounded before the reference is taken away: kernels_attention_ragged.hip)
+                        coarse = coarse || __builtin_amdgcn_ballot_w64(c != -INFINITY && !(__builtin_fabsf(c) < 4096.f)) != 0;
+                    }
+                    const float sc = coarse ? 1.f : g.sc, c = c_run[u] == -INFINITY ? 0.f : c_run[u];
+                    if (coarse)
+#pragma unroll
+                        for (int h = 0; h < 2; h++) S[u][h] *= g.sc;
+                    float sum = 0.f;
+#pragma unroll
+                    for (int e = 0; e < 8; e += 2) {
+                        const half2_t p = {(half_t)__builtin_amdgcn_exp2f(fmaf(S[u][e >> 2][e & 3], sc, -c)), (half_t)__builtin_amdgcn_exp2f(fmaf(S[u][e >> 2][(e & 3) + 1], sc, -c))};
+                        sum = __builtin_amdgcn_fdot2(p, half2_t{(half_t)1, (half_t)1}, sum, false);
+                        fp[u][e] = p[0], fp[u][e + 1] = p[1];
+                    }
+                    l_run[u] += sum;
+                }
+                // ---- values
+                if (more) wait(But{});
+                else wait(All{});
+                bool odd = false;
+                if (!lean) { // a value that is not finite must not reach, as 0 * inf, the rows that do not see its key
+                    float x = 0.f;
+#pragma unroll
+                    for (int d = 0; d < KS; d++) x = rg_odd(values(d), x);
+                    odd = __builtin_amdgcn_ballot_w64(x != 0.f) != 0;
+                }
+                if (odd) {
+                    half8_t vis[NR];
+#pragma unroll
+                    for (int u = 0; u < NR; u++)
+#pragma unroll
+                        for (int e = 0; e < 8; e++) vis[u][e] = __builtin_bit_cast(half_t, (uint16_t)(sees_key(u, e) ? 0x3C00 : 0));
+                    asm volatile("" ::: "memory"); // (the values are read again)
+#pragma unroll
+                    for (int d = 0; d < KS; d++) {
+                        half8_t v = values(d);
+                        const half8_t code = rg_take_odd(v);
+#pragma unroll
+                        for (int u = 0; u < NR; u++) {
+                            acc[u][d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v, fp[u], acc[u][d], 0, 0, 0);
+                            const float4_t mark = __builtin_amdgcn_mfma_f32_16x16x32_f16(code, vis[u], float4_t{0.f, 0.f, 0.f, 0.f}, 0, 0, 0);
+#pragma unroll
+                            for (int i = 0; i < 4; i++) {
+                                acc[u][d][i] += (int)mark[i] & 255 ? INFINITY : 0.f;
+                                acc[u][d][i] += mark[i] >= 256.f ? -INFINITY : 0.f;
+                            }
+                        }
+                    }
+                } else {
+#pragma unroll
+                    for (int d = 0; d < KS; d++) {
+                        const half8_t v = values(d);
+#pragma unroll
+                        for (int u = 0; u < NR; u++) acc[u][d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v, fp[u], acc[u][d], 0, 0, 0);
+                    }
+                }
+                if (!more) break;
+                asm volatile("" ::: "memory");
+                __builtin_amdgcn_s_waitcnt(0xC07F); // lgkmcnt(0): the values have been read
+                asm volatile("" ::: "memory");
+                issue(V, lds0 + 2 * BLK);
+                j += PS_KEYS;
+                more = j + PS_KEYS < j_end;
+                if (more) look(j + PS_KEYS);
+                wait(But{}); // the keys
+            }
+        }
+        // ---- the four wavefronts' results: outputs where their blocks were, [tile][dimensions' tile][lane] four, references and sums
+        float4_t *const rest = (float4_t *)mine;
+#pragma unroll
+        for (int u = 0; u < NR; u++) {
+            const float l = rt_groups_sum(l_run[u]);
+            if (fg == 0) *(float2_t *)(sums + 2 * (wave * 16 * NR + 16 * u + fr)) = float2_t{c_run[u], l};
+#pragma unroll
+            for (int d = 0; d < KS; d++) rest[(u * KS + d) * 64 + lane] = acc[u][d];
+        }
+        __syncthreads();
+        const bool parted = step > 0 || upto < all; // others have the rest
+        const int64_t slot = 2 * (int64_t)blockIdx.x + (begun ? 1 : 0);
+        for (int e = t; e < NR * KS * 64; e += 256) {
+            const int l = e & 63, ud = e >> 6, u = ud / KS, d = ud - u * KS, m = 16 * u + (l & 15), x = 16 * d + 4 * (l >> 4);
+            if (m >= rows || x >= g.D) continue;
+            float2_t ml[4];
+            float4_t o[4];
+#pragma unroll
+            for (int w = 0; w < 4; w++) ml[w] = *(const float2_t *)(sums + 2 * (w * 16 * NR + m)), o[w] = *(const float4_t *)(smem + w * ps_ring(KS) + 16 * e);
+            const float top = fmaxf(fmaxf(ml[0][0], ml[1][0]), fmaxf(ml[2][0], ml[3][0])), base = top == -INFINITY ? 0.f : top;
+            float4_t y = {0.f, 0.f, 0.f, 0.f};
+            float s = 0.f;
+#pragma unroll
+            for (int w = 0; w < 4; w++) {
+                const float a = __builtin_amdgcn_exp2f(ml[w][0] - base);
+                s = fmaf(ml[w][1], a, s);
+#pragma unroll
+                for (int i = 0; i < 4; i++) y[i] = fmaf(o[w][i], a, y[i]);
+            }
+            if (parted) {
+                const int64_t at = slot * (g.max_rows * g.group) + m;
+                *(float4_t *)(g.part_o + at * g.D + x) = y;
+                if (x == 0) *(float2_t *)(g.part_ml + 2 * at) = float2_t{top, s};
+            } else {
+                const int qi = m / g.group;
+                half_t *const out = g.O + (int64_t)(first + qi) * g.o_rs + (int64_t)(kh * g.group + (m - qi * g.group)) * g.o_hs + x;
+                typedef half_t half4_u1 __attribute__((ext_vector_type(4), aligned(2)));
+                *(half4_u1 *)out = half4_u1{(half_t)(y[0] / s), (half_t)(y[1] / s), (half_t)(y[2] / s), (half_t)(y[3] / s)}; // no visible key: 0 / 0
+            }
+        }
+        __syncthreads();
+        if (g.D < P) { // the zeros again
+            for (int i = lane; i < ps_ring(KS) / 16; i += 64) ((uint4_t *)mine)[i] = uint4_t{0, 0, 0, 0};
+            __builtin_amdgcn_s_waitcnt(ps_waitcnt(0));
+        }
+        todo -= upto - step, step = 0, begun = true;
+        if (++kh == g.kv_heads) kh = 0, b++;
+    }
+}
+
+// Joins the parts of a row (blockIdx.x: sequence, head of keys, row) in a fixed order: 32 threads have four columns each, 8 groups of them the parts.
+__global__ __launch_bounds__(256) void attention_paged_join_kernel(RaggedArgs g, int wgs) {
+    __shared__ __attribute__((aligned(16))) float part[8][128], mls[8][2];
+    const int t = threadIdx.x, lane = t & 63, per = g.max_rows * g.group;
+    const int m = blockIdx.x % per, bk = blockIdx.x / per, b = bk / g.kv_heads, kh = bk - b * g.kv_heads;
+    int first;
+    const int n = rg_rows(g, b, first);
+    if (m >= n * g.group) return;
+    int64_t total = 0, before = 0;
+    for (int c = 0; c < g.batch; c += 64) {
+        const int s = ps_steps(g, c + lane);
+        total += rg_sum(s);
+        before += rg_sum(c + lane < b ? s : 0);
+    }
+    const int steps = ps_steps(g, b);
+    total *= g.kv_heads;
+    wgs = (int)min((int64_t)wgs, total);
+    const int64_t from = before * g.kv_heads + (int64_t)kh * steps;
+    const int i0 = ps_owner(from, total, wgs), i1 = ps_owner(from + steps - 1, total, wgs);
+    if (i0 == i1) return; // it is written
+    auto row_of = [&](int i) { return (2 * (int64_t)i + (ps_begin(i, total, wgs) >= from ? 0 : 1)) * per + m; }; // a workgroup that begins here has it first
+    const int c = t & 31, sg = t >> 5;
+    const bool live = 4 * c < g.D;
+    float top = -INFINITY, l = 0.f;
+    float4_t y = {0.f, 0.f, 0.f, 0.f};
+    for (int i = i0 + sg; i <= i1; i += 32) { // four parts at a time
+        float2_t ml[4];
+        float4_t v[4];
+#pragma unroll
+        for (int k = 0; k < 4; k++) {
+            const int64_t at = row_of(min(i + 8 * k, i1));
+            ml[k] = *(const float2_t *)(g.part_ml + 2 * at), v[k] = *(const float4_t *)(g.part_o + at * g.D + (live ? 4 * c : 0));
+            if (i + 8 * k > i1) ml[k] = float2_t{-INFINITY, 0.f}, v[k] = float4_t{0.f, 0.f, 0.f, 0.f};
+        }
+        const float now = fmaxf(fmaxf(top, fmaxf(ml[0][0], ml[1][0])), fmaxf(ml[2][0], ml[3][0])), base = now == -INFINITY ? 0.f : now;
+        const float old = __builtin_amdgcn_exp2f(top - base);
+        top = now, l *= old;
+#pragma unroll
+        for (int x = 0; x < 4; x++) y[x] *= old;
+#pragma unroll
+        for (int k = 0; k < 4; k++) {
+            const float a = __builtin_amdgcn_exp2f(ml[k][0] - base);
+            l = fmaf(a, ml[k][1], l);
+#pragma unroll
+            for (int x = 0; x < 4; x++) y[x] = fmaf(a, v[k][x], y[x]);
+        }
+    }
+    *(float4_t *)&part[sg][4 * c] = y;
+    if (c == 0) mls[sg][0] = top, mls[sg][1] = l;
+    __syncthreads();
+    if (t < g.D) {
+        float all = -INFINITY, sum = 0.f, s = 0.f;
+#pragma unroll
+        for (int k = 0; k < 8; k++) all = fmaxf(all, mls[k][0]);
+        const float ref = all == -INFINITY ? 0.f : all;
+#pragma unroll
+        for (int k = 0; k < 8; k++) {
+            const float a = __builtin_amdgcn_exp2f(mls[k][0] - ref);
+            sum = fmaf(part[k][t], a, sum), s = fmaf(mls[k][1], a, s);
+        }
+        const int qi = m / g.group;
+        g.O[(int64_t)(first + qi) * g.o_rs + (int64_t)(kh * g.group + (m - qi * g.group)) * g.o_hs + t] = (half_t)(sum / s);
+    }
+}
+
+// How a call is run: on the kernels above where a head of keys has up to 32 rows, and then a head of keys a workgroup, or all in equal parts.
+struct PagedPlan {
+    bool streams, whole;
+    int wgs;
+};
+static PagedPlan ps_plan(const rt_attention_paged_desc &d) {
+    const rt_paged_cache_desc &c = d.cache;
+    const int64_t per = (int64_t)d.max_rows * (d.heads / c.kv_heads), heads = (int64_t)c.batch * c.kv_heads, steps = std::max(1, (d.max_keys + PS_KEYS - 1) / PS_KEYS);
+    PagedPlan p{};
+    p.streams = per <= 32 && heads <= 0xffffff && heads * steps < (int64_t(1) << 31) && heads * per < (int64_t(1) << 24);
+    p.whole = steps <= 2 || heads >= 2048;
+    p.wgs = (int)std::min<int64_t>(512, heads * steps);
+    return p;
+}
+
+bool attention_paged_fits(const rt_attention_paged_desc &d) {
+    if (d.cache.batch == 0 || d.heads == 0 || d.rows == 0) return true;
+    return ragged_fits(d.cache.batch, d.cache.kv_heads, d.heads / d.cache.kv_heads, d.rows, d.max_rows);
+}
+uint64_t attention_paged_workspace_bytes(const rt_attention_paged_desc &d) {
+    if (d.cache.batch == 0 || d.heads == 0 || d.rows == 0 || d.max_rows == 0) return 0;
+    const PagedPlan p = ps_plan(d);
+    if (!p.streams) return ragged_workspace_bytes(d.cache.batch, d.heads, d.cache.kv_heads, d.rows, d.max_rows, d.max_keys, d.cache.head_dim);
+    return p.whole ? 0 : (uint64_t)2 * p.wgs * d.max_rows * (d.heads / d.cache.kv_heads) * (d.cache.head_dim + 2) * sizeof(float);
+}
+
+template <int KS, int NR> static hipError_t launch_ps(const RaggedArgs &g, int whole, unsigned wgs, hipStream_t st) {
+    constexpr size_t lds = 4 * ps_ring(KS) + 4 * 16 * NR * 2 * sizeof(float);
+    if (const hipError_t e = ensure_lds_limit<&attention_paged_stream_kernel<KS, NR>>(); e != hipSuccess) return e;
+    hipLaunchKernelGGL((attention_paged_stream_kernel<KS, NR>), dim3(wgs), dim3(256), lds, st, g, whole);
+    return hipGetLastError();
+}
+
+hipError_t launch_attention_paged(const rt_attention_paged_desc &d, const void *q, const void *k_pool, const void *v_pool, const int32_t *table, const int32_t *lens,
+                                  const int32_t *starts, void *out, void *workspace, uint64_t workspace_bytes, hipStream_t stream, const DeviceInfo &dev) {
+    RaggedArgs g{};
+    const rt_paged_cache_desc &c = d.cache;
+    g.Q = (const half_t *)q, g.K = (const half_t *)k_pool, g.V = (const half_t *)v_pool, g.O = (half_t *)out, g.starts = starts, g.table = table, g.lens = lens;
+    g.q_rs = d.q_strides[0], g.q_hs = d.q_strides[1], g.o_rs = d.o_strides[0], g.o_hs = d.o_strides[1];
+    g.k_hs = g.v_hs = (int64_t)c.page_size * c.head_dim, g.k_rs = g.v_rs = g.k_hs * c.kv_heads; // a head's part of a page, a page
+    g.table_stride = c.table_stride, g.pages = c.pages, g.page_shift = __builtin_ctz(c.page_size), g.table_width = c.table_width;
+    g.batch = c.batch, g.kv_heads = c.kv_heads, g.group = d.heads / c.kv_heads, g.D = c.head_dim;
+    g.rows = d.rows, g.max_rows = d.max_rows, g.max_keys = d.max_keys, g.causal = d.causal;
+    if (c.pages == 0) g.max_keys = 0; // no page is there: no key
+    ragged_scale(g, d.scale);
+    PagedPlan p = ps_plan(d);
+    if (!p.streams) return launch_ragged(g, true, workspace, workspace_bytes, stream);
+    const int per = g.max_rows * g.group;
+    const uint64_t need = attention_paged_workspace_bytes(d);
+    if (!p.whole && workspace && workspace_bytes >= need && !((uintptr_t)workspace & 15u))
+        g.part_o = (float *)workspace, g.part_ml = g.part_o + (uint64_t)2 * p.wgs * per * g.D;
+    else
+        p.whole = true;
+    const unsigned wgs = p.whole ? (unsigned)(c.batch * c.kv_heads) : (unsigned)p.wgs;
+    auto go = [&](auto ks) -> hipError_t {
+        constexpr int KS = decltype(ks)::value;
+        return per <= 16 ? launch_ps<KS, 1>(g, p.whole, wgs, stream) : launch_ps<KS, 2>(g, p.whole, wgs, stream);
+    };
+    hipError_t e;
+    switch ((g.D + 15) / 16) {
+    case 1: e = go(std::integral_constant<int, 1>{}); break;
+    case 2: e = go(std::integral_constant<int, 2>{}); break;
+    case 3: e = go(std::integral_constant<int, 3>{}); break;
+    case 4: e = go(std::integral_constant<int, 4>{}); break;
+    case 5: e = go(std::integral_constant<int, 5>{}); break;
+    case 6: e = go(std::integral_constant<int, 6>{}); break;
+    case 7: e = go(std::integral_constant<int, 7>{}); break;
+    default: e = go(std::integral_constant<int, 8>{}); break;
+    }
+    if (e != hipSuccess || p.whole) return e;
+    hipLaunchKernelGGL(attention_paged_join_kernel, dim3((unsigned)(c.batch * c.kv_heads * per)), dim3(256), 0, stream, g, p.wgs);
+    return hipGetLastError();
+}
+
+} // namespace rt

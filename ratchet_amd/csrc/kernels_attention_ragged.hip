@@ -376,10 +376,10 @@ static uint64_t rr_workspace(int heads, int rows, int head_dim, int splits) {
     return splits <= 1 ? 0 : (uint64_t)rows * heads * splits * (head_dim + 2) * sizeof(float);
 }
 
-static bool rr_fits(int batch, int kv_heads, int group, int rows, int max_rows) {
+bool ragged_fits(int batch, int kv_heads, int group, int rows, int max_rows) {
     return rr_tiles(batch, group, rows, max_rows) * kv_heads <= 0xffffff; // a grid's threads are fewer than 2^32; shares take no call past that
 }
-static uint64_t rr_workspace_bytes(int batch, int heads, int kv_heads, int rows, int max_rows, int max_keys, int head_dim) {
+uint64_t ragged_workspace_bytes(int batch, int heads, int kv_heads, int rows, int max_rows, int max_keys, int head_dim) {
     return rr_workspace(heads, rows, head_dim, rr_splits(rr_tiles(batch, heads / kv_heads, rows, max_rows) * kv_heads, max_keys));
 }
 
@@ -391,13 +391,13 @@ template <int KS, bool PAGED> static hipError_t launch_rr(const RaggedArgs &g, h
 }
 
 // exp(scale * s) as exp2(sc * s) with sc above 0, whatever the scale's sign; a scale of 0 leaves scores of 0
-static void rr_scale(RaggedArgs &g, float scale) {
+void ragged_scale(RaggedArgs &g, float scale) {
     g.sign = scale > 0.f ? 1.f : scale < 0.f ? -1.f : 0.f;
     g.sc = scale == 0.f ? 1.f : std::fabs(scale) * kLog2eR;
 }
 
 // `g` has the operands; the shares, and where partial results go, are chosen here.
-static hipError_t launch_ragged(RaggedArgs &g, bool paged, void *workspace, uint64_t workspace_bytes, hipStream_t stream) {
+hipError_t launch_ragged(RaggedArgs &g, bool paged, void *workspace, uint64_t workspace_bytes, hipStream_t stream) {
     g.tiles = (int)rr_tiles(g.batch, g.group, g.rows, g.max_rows);
     g.splits = rr_splits((int64_t)g.tiles * g.kv_heads, g.max_keys);
     const uint64_t need = rr_workspace(g.kv_heads * g.group, g.rows, g.D, g.splits);
@@ -427,11 +427,11 @@ static hipError_t launch_ragged(RaggedArgs &g, bool paged, void *workspace, uint
 
 bool attention_packed_fits(const rt_attention_packed_desc &d) {
     if (d.batch == 0 || d.heads == 0 || d.rows == 0) return true;
-    return rr_fits(d.batch, d.kv_heads, d.heads / d.kv_heads, d.rows, d.max_rows);
+    return ragged_fits(d.batch, d.kv_heads, d.heads / d.kv_heads, d.rows, d.max_rows);
 }
 uint64_t attention_packed_workspace_bytes(const rt_attention_packed_desc &d) {
     if (d.batch == 0 || d.heads == 0 || d.rows == 0) return 0;
-    return rr_workspace_bytes(d.batch, d.heads, d.kv_heads, d.rows, d.max_rows, d.max_keys, d.head_dim);
+    return ragged_workspace_bytes(d.batch, d.heads, d.kv_heads, d.rows, d.max_rows, d.max_keys, d.head_dim);
 }
 hipError_t launch_attention_packed(const rt_attention_packed_desc &d, const void *q, const void *k, const void *v, const int32_t *starts, const int32_t *kv_starts,
                                    void *out, void *workspace, uint64_t workspace_bytes, hipStream_t stream, const DeviceInfo &dev) {
@@ -441,31 +441,8 @@ hipError_t launch_attention_packed(const rt_attention_packed_desc &d, const void
     g.k_rs = d.k_strides[0], g.k_hs = d.k_strides[1], g.v_rs = d.v_strides[0], g.v_hs = d.v_strides[1];
     g.batch = d.batch, g.kv_heads = d.kv_heads, g.group = d.heads / d.kv_heads, g.D = d.head_dim;
     g.rows = d.rows, g.kv_rows = d.kv_rows, g.max_rows = d.max_rows, g.max_keys = d.max_keys, g.causal = d.causal;
-    rr_scale(g, d.scale);
+    ragged_scale(g, d.scale);
     return launch_ragged(g, false, workspace, workspace_bytes, stream);
-}
-
-bool attention_paged_fits(const rt_attention_paged_desc &d) {
-    if (d.cache.batch == 0 || d.heads == 0 || d.rows == 0) return true;
-    return rr_fits(d.cache.batch, d.cache.kv_heads, d.heads / d.cache.kv_heads, d.rows, d.max_rows);
-}
-uint64_t attention_paged_workspace_bytes(const rt_attention_paged_desc &d) {
-    if (d.cache.batch == 0 || d.heads == 0 || d.rows == 0) return 0;
-    return rr_workspace_bytes(d.cache.batch, d.heads, d.cache.kv_heads, d.rows, d.max_rows, d.max_keys, d.cache.head_dim);
-}
-hipError_t launch_attention_paged(const rt_attention_paged_desc &d, const void *q, const void *k_pool, const void *v_pool, const int32_t *table, const int32_t *lens,
-                                  const int32_t *starts, void *out, void *workspace, uint64_t workspace_bytes, hipStream_t stream, const DeviceInfo &dev) {
-    RaggedArgs g{};
-    const rt_paged_cache_desc &c = d.cache;
-    g.Q = (const half_t *)q, g.K = (const half_t *)k_pool, g.V = (const half_t *)v_pool, g.O = (half_t *)out, g.starts = starts, g.table = table, g.lens = lens;
-    g.q_rs = d.q_strides[0], g.q_hs = d.q_strides[1], g.o_rs = d.o_strides[0], g.o_hs = d.o_strides[1];
-    g.k_hs = g.v_hs = (int64_t)c.page_size * c.head_dim, g.k_rs = g.v_rs = g.k_hs * c.kv_heads; // a head's part of a page, a page
-    g.table_stride = c.table_stride, g.pages = c.pages, g.page_shift = __builtin_ctz(c.page_size), g.table_width = c.table_width;
-    g.batch = c.batch, g.kv_heads = c.kv_heads, g.group = d.heads / c.kv_heads, g.D = c.head_dim;
-    g.rows = d.rows, g.max_rows = d.max_rows, g.max_keys = d.max_keys, g.causal = d.causal;
-    if (c.pages == 0) g.max_keys = 0; // no page is there: no key
-    rr_scale(g, d.scale);
-    return launch_ragged(g, true, workspace, workspace_bytes, stream);
 }
 
 } // namespace rt
