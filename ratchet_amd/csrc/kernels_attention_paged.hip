@@ -22,16 +22,29 @@ typedef __fp16 ps_fp16x4 __attribute__((ext_vector_type(4)));
 
 __device__ __forceinline__ constexpr int ps_waitcnt(int n) { return 0x0070 | (n & 0xF) | (((n >> 4) & 0x3) << 14); } // vmcnt(n) lgkmcnt(0)
 
+// Everything of this wavefront's has arrived and been written, for the compiler too: loads into LDS behind this find nothing in their way.
+__device__ __forceinline__ void ps_settle() {
+    asm volatile("" ::: "memory");
+    __builtin_amdgcn_s_waitcnt(ps_waitcnt(0));
+    asm volatile("" ::: "memory");
+}
+
 // As rr_swizzle of the tiled kernel: rows four apart differ in the low bits, neighbours in the high ones.
 template <int PITCH> __device__ __forceinline__ int ps_swizzle(int r) {
     return PITCH == 128 ? ((r & 3) << 2) | ((r >> 2) & 3) : (((r >> 1) & 1) << 2) | ((r >> 2) & 3);
 }
 
 // Steps of a sequence (at least one where it has rows: they are NaN), and of all up to a sequence.
-__device__ __forceinline__ int ps_steps(const RaggedArgs &g, int b) {
-    int first;
-    if (b >= g.batch || rg_rows(g, b, first) == 0) return 0;
-    return max(1, (rg_keys<true>(g, b, first) + PS_KEYS - 1) / PS_KEYS);
+struct PagedSeq {
+    int first, rows, keys, steps;
+};
+__device__ __forceinline__ PagedSeq ps_seq(const RaggedArgs &g, int b) {
+    PagedSeq s;
+    int unused;
+    const int at = min(b, g.batch - 1);
+    s.rows = rg_rows(g, at, s.first), s.keys = rg_keys<true>(g, at, unused);
+    s.steps = b < g.batch && s.rows > 0 ? max(1, (s.keys + PS_KEYS - 1) / PS_KEYS) : 0;
+    return s;
 }
 
 // The place in the line at which workgroup i begins, and which workgroup has place c.
@@ -41,7 +54,7 @@ __device__ __forceinline__ int ps_owner(int64_t c, int64_t total, int wgs) { ret
 
 // KS: steps of 16 over head_dim (the last may be half).  NR: tiles of 16 rows
 template <int KS, int NR> __global__ __launch_bounds__(256, 2) void attention_paged_stream_kernel(RaggedArgs g, int whole) {
-    constexpr int P = ps_pitch(KS), CPR = P / 8, KK = (KS + 1) / 2, RPI = 64 / CPR, NI = PS_UNIT / RPI;
+    constexpr int P = ps_pitch(KS), CPR = P / 8, KK = KS / 2, ODD = KS & 1, RPI = 64 / CPR, NI = PS_UNIT / RPI;
     constexpr int BLK = PS_UNIT * P; // halves of a block of keys, of values
     extern __shared__ __attribute__((aligned(16))) uint8_t smem[];
     const int t = threadIdx.x, lane = t & 63, wave = __builtin_amdgcn_readfirstlane(t >> 6);
@@ -50,39 +63,51 @@ template <int KS, int NR> __global__ __launch_bounds__(256, 2) void attention_pa
     float *const sums = (float *)(smem + 4 * ps_ring(KS));       // [wavefront][row][2]
 
     // ---- where this workgroup begins and ends
-    int b = 0, kh = 0, step = 0, todo;
+    int b = 0, kh = 0, step = 0, todo, wgs = 0;
+    int64_t total = 0, from = 0; // places in the line; that of this head of keys' first step
+    PagedSeq seq;
+    auto of_lane = [&](PagedSeq s, int l) {
+        return PagedSeq{__builtin_amdgcn_readlane(s.first, l), __builtin_amdgcn_readlane(s.rows, l), __builtin_amdgcn_readlane(s.keys, l), __builtin_amdgcn_readlane(s.steps, l)};
+    };
     if (whole) { // a head of keys each
         b = blockIdx.x / g.kv_heads, kh = blockIdx.x - b * g.kv_heads;
-        todo = __builtin_amdgcn_readfirstlane(ps_steps(g, b));
+        seq = of_lane(ps_seq(g, b), 0);
+        todo = seq.steps;
     } else {
-        int64_t total = 0;
-        for (int c = 0; c < g.batch; c += 64) total += rg_sum(ps_steps(g, c + lane));
+        const PagedSeq s0 = ps_seq(g, lane);
+        total = rg_sum(s0.steps);
+        for (int c = 64; c < g.batch; c += 64) total += rg_sum(ps_seq(g, c + lane).steps);
         total *= g.kv_heads;
-        const int wgs = (int)min((int64_t)gridDim.x, total);
-        if (blockIdx.x >= wgs) return;
-        int at = ps_begin(blockIdx.x, total, wgs);
+        wgs = (int)min((int64_t)gridDim.x, total);
+        if ((int)blockIdx.x >= wgs) return;
+        const int begin = ps_begin(blockIdx.x, total, wgs);
+        int at = begin;
         todo = ps_begin(blockIdx.x + 1, total, wgs) - at;
-        if (todo > 0)
-            for (int c = 0; c < g.batch; c += 64) {
-                const int s = ps_steps(g, c + lane), upto = rg_scan(s, lane), all = __builtin_amdgcn_readlane(upto, 63);
-                if (at >= all * g.kv_heads) { // (no step count passes 31 bits: host)
-                    at -= all * g.kv_heads;
-                    continue;
-                }
+        PagedSeq s = s0;
+        for (int c = 0;;) {
+            const int upto = rg_scan(s.steps, lane), all = __builtin_amdgcn_readlane(upto, 63);
+            if (at < all * g.kv_heads) { // (no step count passes 31 bits: host)
                 const int l = __builtin_ctzll(__builtin_amdgcn_ballot_w64(upto * g.kv_heads > at));
-                const int n = __builtin_amdgcn_readlane(s, l);
-                at -= (__builtin_amdgcn_readlane(upto, l) - n) * g.kv_heads;
-                b = c + l, kh = at / n, step = at - kh * n;
+                seq = of_lane(s, l);
+                at -= (__builtin_amdgcn_readlane(upto, l) - seq.steps) * g.kv_heads;
+                b = c + l, kh = at / seq.steps, step = at - kh * seq.steps;
                 break;
             }
+            at -= all * g.kv_heads;
+            c += 64;
+            if (c >= g.batch) return; // (not reached: the place is in the line)
+            s = ps_seq(g, c + lane);
+        }
+        from = begin - step;
     }
     b = __builtin_amdgcn_readfirstlane(b), kh = __builtin_amdgcn_readfirstlane(kh), step = __builtin_amdgcn_readfirstlane(step), todo = __builtin_amdgcn_readfirstlane(todo);
     if (todo <= 0) return;
 
-    // columns behind head_dim are zeros: no load writes them
-    if (g.D < P) {
+    // Of the columns behind head_dim, which no load writes, the products read those of a last step that is half full: they are zeros.
+    const bool half_step = g.D < 16 * KS;
+    if (half_step) {
         for (int i = lane; i < ps_ring(KS) / 16; i += 64) ((uint4_t *)mine)[i] = uint4_t{0, 0, 0, 0};
-        __builtin_amdgcn_s_waitcnt(ps_waitcnt(0));
+        ps_settle();
     }
     const int lr = lane / CPR;
     int chunk[NI];
@@ -93,39 +118,30 @@ template <int KS, int NR> __global__ __launch_bounds__(256, 2) void attention_pa
         lanes[i] = __builtin_amdgcn_ballot_w64(8 * chunk[i] < g.D);
     }
     const uint32_t lds0 = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) uint8_t *)mine;
-    int koff[KK];
+    int koff[KK + ODD]; // the last of an odd number of steps by v_mfma_f32_16x16x16_f16: dimensions 16 KS - 16 + 4 fg ..
 #pragma unroll
     for (int k = 0; k < KK; k++) koff[k] = fr * P + 8 * ((4 * k + fg) ^ ps_swizzle<P>(fr));
+    if constexpr (ODD) koff[KK] = fr * P + 8 * ((4 * KK + (fg >> 1)) ^ ps_swizzle<P>(fr)) + 4 * (fg & 1);
     const int vrow = 4 * fg + (fr >> 2), vhalf = (fr & 3) >> 1;
 
     bool begun = false; // whether this is not the first head of keys of the workgroup
     while (todo > 0) {
-        int first, unused;
-        if (b >= g.batch) return;
-        const int n = __builtin_amdgcn_readfirstlane(rg_rows(g, b, first)), len = __builtin_amdgcn_readfirstlane(rg_keys<true>(g, b, unused));
-        first = __builtin_amdgcn_readfirstlane(first);
-        const int all = max(1, (len + PS_KEYS - 1) / PS_KEYS);
-        if (n == 0) { // (has no steps)
-            b++;
-            continue;
-        }
+        const int first = seq.first, n = seq.rows, len = seq.keys, all = seq.steps;
         const int upto = min(all, step + todo), rows = n * g.group, off = len - n;
-        auto sees = [&](int m) { return g.causal ? max(0, min(len, m / g.group + off + 1)) : len; };
+        auto sees = [&](int m) { return g.causal ? max(0, min(len, rg_query(g, m) + off + 1)) : len; };
         const int seen_all = sees(0), seen_any = sees(rows - 1);
 
-        half8_t fq[NR][KK];
+        half8_t fq[NR][KK + 1]; // (without KK)
+        half4_t ft[NR];
         int last[NR];
 #pragma unroll
         for (int u = 0; u < NR; u++) {
-            const int m = min(16 * u + fr, rows - 1), qi = m / g.group;
+            const int m = min(16 * u + fr, rows - 1), qi = rg_query(g, m);
             last[u] = g.causal ? min(len - 1, qi + off) : len - 1;
             const half_t *q = g.Q + (int64_t)(first + qi) * g.q_rs + (int64_t)(kh * g.group + (m - qi * g.group)) * g.q_hs;
-            const half_t sign = (half_t)g.sign;
 #pragma unroll
-            for (int k = 0; k < KK; k++) {
-                const int d = 32 * k + 8 * fg;
-                fq[u][k] = d < g.D ? *(const half8_t *)(q + d) * half8_t{sign, sign, sign, sign, sign, sign, sign, sign} : half8_t{};
-            }
+            for (int k = 0; k < KK; k++) fq[u][k] = 32 * k + 8 * fg < g.D ? *(const half8_t *)(q + 32 * k + 8 * fg) : half8_t{};
+            if constexpr (ODD) ft[u] = 32 * KK + 4 * fg < g.D ? *(const half4_t *)(q + 32 * KK + 4 * fg) : half4_t{};
         }
 
         typedef __attribute__((address_space(4))) const int32_t *scalar_t; // read through the scalar cache
@@ -195,20 +211,45 @@ template <int KS, int NR> __global__ __launch_bounds__(256, 2) void attention_pa
             issue(K, lds0), issue(V, lds0 + 2 * BLK);
             bool more = j + PS_KEYS < j_end;
             if (more) look(j + PS_KEYS);
-            wait(But{}); // (with the queries: the compiler waits for all)
+            if (g.sign != 1.f) {
+                const half_t sign = (half_t)g.sign;
+#pragma unroll
+                for (int u = 0; u < NR; u++) {
+#pragma unroll
+                    for (int k = 0; k < KK; k++) fq[u][k] *= half8_t{sign, sign, sign, sign, sign, sign, sign, sign};
+                    ft[u] *= half4_t{sign, sign, sign, sign};
+                }
+            }
+            // awaited here: a first use in the loop would wait there, for these and with them for every load into LDS
+#pragma unroll
+            for (int u = 0; u < NR; u++) {
+#pragma unroll
+                for (int k = 0; k < KK; k++) asm volatile("" : "+v"(fq[u][k]));
+                if constexpr (ODD) asm volatile("" : "+v"(ft[u]));
+            }
+            wait(But{});
             while (true) {
                 // ---- scores
-                float4_t S[NR][2];
+                float4_t S[NR][2], tail[NR][2]; // (tail: a sum of its own.  As the third operand of the shorter instruction right behind the longer one that makes it, S came out wrong)
 #pragma unroll
                 for (int u = 0; u < NR; u++) S[u][0] = S[u][1] = float4_t{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
                 for (int h = 0; h < 2; h++)
 #pragma unroll
-                    for (int k = 0; k < KK; k++) {
-                        const half8_t fk = *(const half8_t *)(mine + koff[k] + 16 * h * P);
+                    for (int k = 0; k < KK + ODD; k++) {
+                        if (k < KK) {
+                            const half8_t fk = *(const half8_t *)(mine + koff[k] + 16 * h * P);
 #pragma unroll
-                        for (int u = 0; u < NR; u++) S[u][h] = __builtin_amdgcn_mfma_f32_16x16x32_f16(fk, fq[u][k], S[u][h], 0, 0, 0);
+                            for (int u = 0; u < NR; u++) S[u][h] = __builtin_amdgcn_mfma_f32_16x16x32_f16(fk, fq[u][k], S[u][h], 0, 0, 0);
+                        } else {
+                            const half4_t fk = *(const half4_t *)(mine + koff[k] + 16 * h * P);
+#pragma unroll
+                            for (int u = 0; u < NR; u++) tail[u][h] = __builtin_amdgcn_mfma_f32_16x16x16f16(fk, ft[u], float4_t{0.f, 0.f, 0.f, 0.f}, 0, 0, 0);
+                        }
                     }
+                if constexpr (ODD)
+#pragma unroll
+                    for (int u = 0; u < NR; u++) S[u][0] += tail[u][0], S[u][1] += tail[u][1];
                 const uint32_t now = there;
                 if (more) {
                     wait(But{}); // (of LDS: the keys have been read.  The values are not awaited: they are NI loads)
@@ -338,43 +379,42 @@ template <int KS, int NR> __global__ __launch_bounds__(256, 2) void attention_pa
                 *(float4_t *)(g.part_o + at * g.D + x) = y;
                 if (x == 0) *(float2_t *)(g.part_ml + 2 * at) = float2_t{top, s};
             } else {
-                const int qi = m / g.group;
+                const int qi = rg_query(g, m);
                 half_t *const out = g.O + (int64_t)(first + qi) * g.o_rs + (int64_t)(kh * g.group + (m - qi * g.group)) * g.o_hs + x;
                 typedef half_t half4_u1 __attribute__((ext_vector_type(4), aligned(2)));
                 *(half4_u1 *)out = half4_u1{(half_t)(y[0] / s), (half_t)(y[1] / s), (half_t)(y[2] / s), (half_t)(y[3] / s)}; // no visible key: 0 / 0
             }
         }
         __syncthreads();
-        if (g.D < P) { // the zeros again
+        if (half_step) { // the zeros again
             for (int i = lane; i < ps_ring(KS) / 16; i += 64) ((uint4_t *)mine)[i] = uint4_t{0, 0, 0, 0};
-            __builtin_amdgcn_s_waitcnt(ps_waitcnt(0));
+            ps_settle();
         }
-        todo -= upto - step, step = 0, begun = true;
-        if (++kh == g.kv_heads) kh = 0, b++;
+        if (!whole && step == 0 && t == 0) { // for the join: who has parts of this head of keys
+            int32_t *const o = g.owners + 2 * (b * g.kv_heads + kh);
+            o[0] = 2 * (int)blockIdx.x + (begun ? 1 : 0), o[1] = ps_owner(from + all - 1, total, wgs);
+        }
+        todo -= upto - step, step = 0, begun = true, from += all;
+        if (++kh == g.kv_heads && todo > 0) {
+            kh = 0;
+            do { // (empty sequences have no steps)
+                if (++b >= g.batch) return; // (not reached: there are steps to do)
+                seq = of_lane(ps_seq(g, b), 0);
+            } while (seq.steps == 0);
+        }
     }
 }
 
 // Joins the parts of a row (blockIdx.x: sequence, head of keys, row) in a fixed order: 32 threads have four columns each, 8 groups of them the parts.
-__global__ __launch_bounds__(256) void attention_paged_join_kernel(RaggedArgs g, int wgs) {
+__global__ __launch_bounds__(256) void attention_paged_join_kernel(RaggedArgs g) {
     __shared__ __attribute__((aligned(16))) float part[8][128], mls[8][2];
-    const int t = threadIdx.x, lane = t & 63, per = g.max_rows * g.group;
+    const int t = threadIdx.x, per = g.max_rows * g.group;
     const int m = blockIdx.x % per, bk = blockIdx.x / per, b = bk / g.kv_heads, kh = bk - b * g.kv_heads;
+    const int slot = g.owners[2 * bk], i1 = g.owners[2 * bk + 1], i0 = slot >> 1; // (not written for a sequence without rows)
     int first;
     const int n = rg_rows(g, b, first);
-    if (m >= n * g.group) return;
-    int64_t total = 0, before = 0;
-    for (int c = 0; c < g.batch; c += 64) {
-        const int s = ps_steps(g, c + lane);
-        total += rg_sum(s);
-        before += rg_sum(c + lane < b ? s : 0);
-    }
-    const int steps = ps_steps(g, b);
-    total *= g.kv_heads;
-    wgs = (int)min((int64_t)wgs, total);
-    const int64_t from = before * g.kv_heads + (int64_t)kh * steps;
-    const int i0 = ps_owner(from, total, wgs), i1 = ps_owner(from + steps - 1, total, wgs);
-    if (i0 == i1) return; // it is written
-    auto row_of = [&](int i) { return (2 * (int64_t)i + (ps_begin(i, total, wgs) >= from ? 0 : 1)) * per + m; }; // a workgroup that begins here has it first
+    if (m >= n * g.group || i0 == i1) return; // or it is written
+    auto row_of = [&](int i) { return (int64_t)(i == i0 ? slot : 2 * i) * per + m; }; // workgroups behind the first begin with it
     const int c = t & 31, sg = t >> 5;
     const bool live = 4 * c < g.D;
     float top = -INFINITY, l = 0.f;
@@ -414,7 +454,7 @@ __global__ __launch_bounds__(256) void attention_paged_join_kernel(RaggedArgs g,
             const float a = __builtin_amdgcn_exp2f(mls[k][0] - ref);
             sum = fmaf(part[k][t], a, sum), s = fmaf(mls[k][1], a, s);
         }
-        const int qi = m / g.group;
+        const int qi = rg_query(g, m);
         g.O[(int64_t)(first + qi) * g.o_rs + (int64_t)(kh * g.group + (m - qi * g.group)) * g.o_hs + t] = (half_t)(sum / s);
     }
 }
@@ -442,7 +482,7 @@ uint64_t attention_paged_workspace_bytes(const rt_attention_paged_desc &d) {
     if (d.cache.batch == 0 || d.heads == 0 || d.rows == 0 || d.max_rows == 0) return 0;
     const PagedPlan p = ps_plan(d);
     if (!p.streams) return ragged_workspace_bytes(d.cache.batch, d.heads, d.cache.kv_heads, d.rows, d.max_rows, d.max_keys, d.cache.head_dim);
-    return p.whole ? 0 : (uint64_t)2 * p.wgs * d.max_rows * (d.heads / d.cache.kv_heads) * (d.cache.head_dim + 2) * sizeof(float);
+    return p.whole ? 0 : (uint64_t)2 * p.wgs * d.max_rows * (d.heads / d.cache.kv_heads) * (d.cache.head_dim + 2) * sizeof(float) + (uint64_t)2 * d.cache.batch * d.cache.kv_heads * sizeof(int32_t);
 }
 
 template <int KS, int NR> static hipError_t launch_ps(const RaggedArgs &g, int whole, unsigned wgs, hipStream_t st) {
@@ -469,7 +509,7 @@ hipError_t launch_attention_paged(const rt_attention_paged_desc &d, const void *
     const int per = g.max_rows * g.group;
     const uint64_t need = attention_paged_workspace_bytes(d);
     if (!p.whole && workspace && workspace_bytes >= need && !((uintptr_t)workspace & 15u))
-        g.part_o = (float *)workspace, g.part_ml = g.part_o + (uint64_t)2 * p.wgs * per * g.D;
+        g.part_o = (float *)workspace, g.part_ml = g.part_o + (uint64_t)2 * p.wgs * per * g.D, g.owners = (int32_t *)(g.part_ml + (uint64_t)4 * p.wgs * per);
     else
         p.whole = true;
     const unsigned wgs = p.whole ? (unsigned)(c.batch * c.kv_heads) : (unsigned)p.wgs;
@@ -489,7 +529,7 @@ hipError_t launch_attention_paged(const rt_attention_paged_desc &d, const void *
     default: e = go(std::integral_constant<int, 8>{}); break;
     }
     if (e != hipSuccess || p.whole) return e;
-    hipLaunchKernelGGL(attention_paged_join_kernel, dim3((unsigned)(c.batch * c.kv_heads * per)), dim3(256), 0, stream, g, p.wgs);
+    hipLaunchKernelGGL(attention_paged_join_kernel, dim3((unsigned)(c.batch * c.kv_heads * per)), dim3(256), 0, stream, g);
     return hipGetLastError();
 }
 

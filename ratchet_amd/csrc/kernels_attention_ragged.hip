@@ -394,6 +394,7 @@ template <int KS, bool PAGED> static hipError_t launch_rr(const RaggedArgs &g, h
 void ragged_scale(RaggedArgs &g, float scale) {
     g.sign = scale > 0.f ? 1.f : scale < 0.f ? -1.f : 0.f;
     g.sc = scale == 0.f ? 1.f : std::fabs(scale) * kLog2eR;
+    g.per_group = 1.f / g.group;
 }
 
 // `g` has the operands; the shares, and where partial results go, are chosen here.

@@ -15,9 +15,14 @@ struct RaggedArgs {
     int batch, kv_heads, group, D, rows, kv_rows, max_rows, max_keys;
     int pages, page_shift, table_width;
     int causal, splits, tiles;
+    int32_t *owners; // of the streaming kernel: for each sequence and head of keys the first workgroup that has a part (twice, and 1 where it is not its first) and the last
     float sc;  // |scale| log2(e), or 1 where the scale is 0
     float sign; // of the scale: the queries are multiplied by it (exactly)
+    float per_group; // 1 / group
 };
+
+// m / group for m below 2^22: a multiple of 1 / group plus a half of that is further from a whole number than the product's error
+__device__ __forceinline__ int rg_query(const RaggedArgs &g, int m) { return (int)(((float)m + 0.5f) * g.per_group); }
 
 constexpr float kLog2eR = 1.4426950408889634f;
 // The exponentials' reference is put this much, in base 2, below the maximum, and follows it where that is RG_ABOVE past it: outputs and sums are seldom rescaled, a probability
