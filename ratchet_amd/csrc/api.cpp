@@ -863,7 +863,7 @@ rt_status rt_attention_packed_validate(const rt_attention_packed_desc *d) {
     for (int i = 0; i < 2; i++)
         for (int j = 0; j < 2; j++) {
             if (strides[i][j] < 0) return RT_ERR_INVALID_SHAPE;
-            if (strides[i][j] % 8 || strides[i][j] > (int64_t(1) << 27)) return RT_ERR_UNSUPPORTED; // a few rows' offsets are 32 bits
+            if (strides[i][j] % 8 || strides[i][j] > (int64_t(1) << 24)) return RT_ERR_UNSUPPORTED; // offsets within 64 rows are 32 bits
         }
     return rt::attention_packed_fits(*d) ? RT_OK : RT_ERR_UNSUPPORTED;
 }

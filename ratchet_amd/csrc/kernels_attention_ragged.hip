@@ -92,8 +92,10 @@ template <int KS, bool PAGED> __global__ __launch_bounds__(256, 2) void attentio
         for (int i = t; i < STAGES * 2 * BLK / 8; i += 256) ((uint4_t *)smem)[i] = uint4_t{0, 0, 0, 0};
     __syncthreads();
 
-    // ---- loads: instruction i of this wavefront brings the rows RPI (wave + 4 i) .. of the block; lane l the chunk l % CPR of row l / CPR
-    const int lr = lane / CPR;
+    // ---- loads: instruction i of this wavefront brings the rows RPI (wave + 4 i) .. of the block; lane l the chunk l % CPR of row l / CPR.  All of its instructions are at the same
+    // row of 16, so that offsets, chunks and lanes are the same for all, and only the 16 rows' address differs
+    const int row16 = (RPI * wave) & 15, lrow = row16 + lane / CPR, c = 8 * ((lane % CPR) ^ rr_swizzle<P>(lrow));
+    const uint64_t lanes = __builtin_amdgcn_ballot_w64(c < g.D); // whose chunk is a part of the row
     const half_t *const K = g.K + (int64_t)kh * g.k_hs, *const V = g.V + (int64_t)kh * g.v_hs;
     typedef __attribute__((address_space(4))) const int32_t *scalar_t; // read through the scalar cache: no vector load is awaited for them
     const scalar_t table = PAGED ? (scalar_t)(uintptr_t)(g.table + b * g.table_stride) : (scalar_t)0;
@@ -105,37 +107,35 @@ template <int KS, bool PAGED> __global__ __launch_bounds__(256, 2) void attentio
             for (int i = 0; i < 4; i++) pages[i] = table[min((kb * RR_KEYS + 16 * i) >> g.page_shift, last_entry)];
         }
     };
-    int chunk[NI];      // this lane's chunk of its row
-    uint64_t lanes[NI]; // those whose chunk is a part of the row
-#pragma unroll
-    for (int i = 0; i < NI; i++) {
-        chunk[i] = (lane % CPR) ^ rr_swizzle<P>(RPI * (wave + 4 * i) + lr);
-        lanes[i] = __builtin_amdgcn_ballot_w64(8 * chunk[i] < g.D);
-    }
     const uint32_t lds0 = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) uint8_t *)smem;
+    const uint32_t k_off = 2u * ((uint32_t)lrow * (uint32_t)(PAGED ? g.D : g.k_rs) + (uint32_t)c), v_off = 2u * ((uint32_t)lrow * (uint32_t)(PAGED ? g.D : g.v_rs) + (uint32_t)c);
     // block kb into a stage, from the pages that `pages` has; -> whether its four sixteenths are there, as bits
     auto issue = [&](int stage, int kb) __attribute__((always_inline)) {
         uint32_t there = 15u;
+        const int j0 = kb * RR_KEYS;
+        const bool part = !PAGED && j0 + RR_KEYS > len; // of rows behind the last of packed keys the last is read again
+        const half_t *const k0 = K + (int64_t)(key0 + j0) * g.k_rs, *const v0 = V + (int64_t)(key0 + j0) * g.v_rs;
 #pragma unroll
         for (int i = 0; i < NI; i++) {
-            const int row = RPI * (wave + 4 * i), c = chunk[i]; // row of the block; this lane's chunk
+            const int row = RPI * (wave + 4 * i) - row16; // of the block: a multiple of 16
             const half_t *kp, *vp;
-            uint32_t ko, vo;
+            uint32_t ko = k_off, vo = v_off;
             if constexpr (PAGED) {
-                const int x = RPI == 4 ? pages[i] : wave < 2 ? pages[(2 * i) & 3] : pages[(2 * i + 1) & 3], page = (uint32_t)x < (uint32_t)g.pages ? x : 0; // (of row / 16)
-                const int64_t at = (int64_t)page * g.k_rs + (int64_t)((kb * RR_KEYS + row) & ((1 << g.page_shift) - 1)) * g.D;
+                const int x = RPI == 4 ? pages[i] : wave < 2 ? pages[(2 * i) & 3] : pages[(2 * i + 1) & 3], page = (uint32_t)x < (uint32_t)g.pages ? x : 0;
+                const int64_t at = (int64_t)page * g.k_rs + (int64_t)(((j0 + row) & ((1 << g.page_shift) - 1)) * g.D);
                 kp = K + at, vp = V + at;
-                ko = vo = 2u * (uint32_t)(lr * g.D + 8 * c);
+            } else if (part) {
+                const uint32_t j = (uint32_t)min(row + lrow, len - 1 - j0);
+                kp = k0, vp = v0;
+                ko = 2u * (j * (uint32_t)g.k_rs + (uint32_t)c), vo = 2u * (j * (uint32_t)g.v_rs + (uint32_t)c);
             } else {
-                const int j = min(kb * RR_KEYS + row, len - 1), more = min(lr, len - 1 - j); // rows behind the last: the last again
-                kp = K + (key0 + j) * g.k_rs, vp = V + (key0 + j) * g.v_rs;
-                ko = 2u * (uint32_t)(more * (int)g.k_rs + 8 * c), vo = 2u * (uint32_t)(more * (int)g.v_rs + 8 * c);
+                kp = k0 + row * g.k_rs, vp = v0 + row * g.v_rs;
             }
-            const uint32_t dst = __builtin_amdgcn_readfirstlane(lds0 + (uint32_t)(2 * (stage * 2 * BLK + row * P)));
+            const uint32_t dst = __builtin_amdgcn_readfirstlane(lds0 + (uint32_t)(2 * (stage * 2 * BLK + (row + row16) * P)));
             // (every lane is active here, and is again)
             asm volatile("s_mov_b64 exec, %6\n\ts_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %2, %3\n\t"
                          "s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %4, %5\n\ts_mov_b64 exec, -1" ::"s"(dst),
-                         "s"(dst + 2 * BLK), "v"(ko), "s"(kp), "v"(vo), "s"(vp), "s"(lanes[i])
+                         "s"(dst + 2 * BLK), "v"(ko), "s"(kp), "v"(vo), "s"(vp), "s"(lanes)
                          : "m0", "memory");
         }
         if constexpr (PAGED) {
@@ -185,16 +185,26 @@ template <int KS, bool PAGED> __global__ __launch_bounds__(256, 2) void attentio
     auto step = [&](int stage, int kb, uint32_t there, auto lean_c) __attribute__((always_inline)) {
         constexpr bool LEAN = decltype(lean_c)::value;
         const half_t *const st = ring + stage * 2 * BLK;
-        float16_t S[2];
+        // Operands are read four ahead of the products that take them: left to itself the compiler reads each right before its product, and waits
+        float16_t S[2] = {};
+        half8_t ahead[2][4];
+        auto keys = [&](int i) __attribute__((always_inline)) { return *(const half8_t *)(st + koff[(i / 2) % KS] + 32 * (i & 1) * P); }; // of products 0 .. 2 KS - 1: both tiles of 32 keys in turn
 #pragma unroll
-        for (int u = 0; u < 2; u++) {
-            S[u] = float16_t{};
+        for (int i = 0; i < 4 && i < 2 * KS; i++) ahead[0][i] = keys(i);
 #pragma unroll
-            for (int k = 0; k < KS; k++) {
-                const half8_t fk = *(const half8_t *)(st + koff[k] + 32 * u * P);
-                S[u] = __builtin_amdgcn_mfma_f32_32x32x16_f16(fk, fq[k], S[u], 0, 0, 0);
-            }
+        for (int q = 0; q < (2 * KS + 3) / 4; q++) {
+#pragma unroll
+            for (int i = 4 * q + 4; i < 4 * q + 8 && i < 2 * KS; i++) ahead[(q + 1) & 1][i & 3] = keys(i);
+            __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+            for (int i = 4 * q; i < 4 * q + 4 && i < 2 * KS; i++) S[i & 1] = __builtin_amdgcn_mfma_f32_32x32x16_f16(ahead[q & 1][i & 3], fq[i / 2], S[i & 1], 0, 0, 0);
+            __builtin_amdgcn_sched_barrier(0);
         }
+        half8_t next[2][DT];
+        if constexpr (LEAN)
+#pragma unroll
+            for (int d = 0; d < DT; d++) next[0][d] = values(st, d, 0);
+        __builtin_amdgcn_sched_barrier(0);
         // register i of S[u]: key 32 u + 8 (i / 4) + 4 hi + i % 4 of the block
         int left = last - kb * RR_KEYS - 4 * hi;
         auto sees_key = [&](int u, int i) { return 32 * u + 8 * (i >> 2) + (i & 3) <= left && ((there >> (2 * u + (i >> 3))) & 1u); };
@@ -273,10 +283,19 @@ template <int KS, bool PAGED> __global__ __launch_bounds__(256, 2) void attentio
                 __builtin_amdgcn_sched_barrier(0);
             }
         } else {
+            if constexpr (!LEAN)
 #pragma unroll
-            for (int s = 0; s < 4; s++)
+                for (int d = 0; d < DT; d++) next[0][d] = values(st, d, 0);
 #pragma unroll
-                for (int d = 0; d < DT; d++) acc[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(values(st, d, s), fp[s], acc[d], 0, 0, 0);
+            for (int s = 0; s < 4; s++) {
+                if (s < 3)
+#pragma unroll
+                    for (int d = 0; d < DT; d++) next[(s + 1) & 1][d] = values(st, d, s + 1);
+                __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+                for (int d = 0; d < DT; d++) acc[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(next[s & 1][d], fp[s], acc[d], 0, 0, 0);
+                __builtin_amdgcn_sched_barrier(0);
+            }
         }
     };
 
