@@ -76,9 +76,9 @@ class Device:
         self._torch_device = None
 
     def torch_device(self):
-        """The torch.device of a GPU device (its name is parsed once, not per allocation)."""
+        """The torch.device (its name is parsed once, not per allocation)."""
         if self._torch_device is None:
-            self._torch_device = _torch().device(f"cuda:{self.ordinal}")
+            self._torch_device = _torch().device(f"cuda:{self.ordinal}" if self.kind == "gpu" else "cpu")
         return self._torch_device
 
     @staticmethod
@@ -430,6 +430,168 @@ class AttentionQ4:
         return [self.q, self.k, self.v] + ([self.mask] if self.mask is not None else [])
 
 
+def _i32(*sizes):
+    """Sizes that go into 32-bit fields (ctypes would take them modulo 2^32)."""
+    if any(not 0 <= int(s) <= 0x7fffffff for s in sizes):
+        raise OperationError(_ffi.RT_ERR_INVALID_SHAPE, f"sizes {sizes}")
+    return [int(s) for s in sizes]
+
+
+class Sequences:
+    """Whose rows a packed tensor holds, for the operators on sequences of different lengths: int32 GPU tensors of torch, read when a call runs, so that a
+    captured graph takes what they hold then.
+
+      batch     sequences
+      starts    [batch + 1]: sequence b has the rows starts[b] .. starts[b + 1] - 1 (None: max_rows each)
+      max_rows  no sequence has more rows
+      lens      [batch]: keys of each sequence, the rows' own among them (a cache in pages)
+      table     [batch, width]: the page of each page_size positions; another number than a page's where there is none
+      max_keys  no sequence has more keys (default: what the table holds; without a table max_rows)"""
+
+    def __init__(self, batch: int, starts=None, max_rows: int = 1, lens=None, table=None, max_keys: Optional[int] = None):
+        self.batch, self.max_rows = _i32(batch, max_rows)
+        self.starts, self.lens, self.table = starts, lens, table
+        self.max_keys = None if max_keys is None else _i32(max_keys)[0]
+
+    def check(self, device: "Device", paged: bool):
+        _lengths(self.starts, self.batch + 1, device, "starts")
+        if not paged:
+            return
+        if self.lens is None or self.table is None:
+            raise OperationError(_ffi.RT_ERR_INVALID_ARG, "a cache in pages needs lens and a table")
+        _lengths(self.lens, self.batch, device, "lens")
+        t, torch = self.table, _torch()
+        if t.dtype != torch.int32 or t.dim() != 2 or t.shape[0] != self.batch or t.device != device.torch_device() or (t.numel() and t.stride(1) != 1):
+            raise OperationError(_ffi.RT_ERR_INVALID_ARG, f"table: an int32 tensor [{self.batch}, width] on the cache's device, entries side by side")
+
+    def cache_desc(self, pool: "Tensor"):
+        c = _ffi.PagedCacheDesc()
+        c.pages, c.kv_heads, c.page_size, c.head_dim = _i32(*pool.shape)
+        c.batch, c.table_width = self.batch, _i32(self.table.shape[1])[0]
+        c.table_stride = max(int(self.table.stride(0)), c.table_width) if self.batch > 1 else c.table_width
+        return c
+
+
+def _rows_of(t: "Tensor", width: int, what: str):
+    """Rows of a packed tensor [.., heads * head_dim]."""
+    if not t.shape or (t.shape[-1] != width):
+        raise OperationError(_ffi.RT_ERR_INVALID_SHAPE, f"{what}: {t.shape}, rows of {width}")
+    return _i32(math.prod(t.shape[:-1]))[0]
+
+
+class CachePaged:
+    """The write of packed rows [.., kv_heads * head_dim], F16 or F32, into a pool [pages, kv_heads, page_size, head_dim] (Tensor.empty_cache), in place: the
+    last rows of each sequence's positions (rt_cache_write_paged_enqueue)."""
+
+    def __init__(self, pool: "Tensor", source: "Tensor", seqs: Sequences):
+        if len(pool.shape) != 4:
+            raise InvariantError(_ffi.RT_ERR_INVALID_SHAPE, "cache: rank 4 expected")
+        self.cache, self.source, self.seqs, self.fresh = pool, source, seqs, False
+        self.width = pool.shape[1] * pool.shape[3]
+        self.rows = _rows_of(source, self.width, "cache: source")
+        seqs.check(pool.device, True)
+        if seqs.starts is None and self.rows != seqs.batch * seqs.max_rows:
+            raise OperationError(_ffi.RT_ERR_INVALID_SHAPE, f"cache: {self.rows} rows of {seqs.batch} sequences with {seqs.max_rows}")
+        self.desc = seqs.cache_desc(pool)
+        self.out_shape = pool.shape
+
+    def check_invariants(self):
+        if self.cache.dt != DType.F16 or self.source.dt not in (DType.F16, DType.F32):
+            raise InvariantError(_ffi.RT_ERR_DTYPE_MISMATCH, "cache: pools are F16, the source is F16 or F32")
+        c = self.desc
+        if c.page_size < 16 or c.page_size > 65536 or c.page_size & (c.page_size - 1) or c.head_dim < 8 or c.head_dim > 128 or c.head_dim % 8:
+            raise InvariantError(_ffi.RT_ERR_INVALID_SHAPE, f"cache: pages of {c.page_size}, heads of {c.head_dim}")
+
+    def srcs(self):
+        return [self.cache, self.source]
+
+    def _enqueue(self, device, stream, k, ks, v=None, vs=None):
+        q = self.seqs
+        st = _ffi.lib().rt_cache_write_paged_enqueue(device.ctx, self.desc, int(self.source.dt), k, ks, v, vs, _strides2(self.width, self.cache.shape[3]), q.table.data_ptr(),
+                                                     q.lens.data_ptr(), None if q.starts is None else q.starts.data_ptr(), self.rows, stream)
+        _check(st, device)
+
+
+class AttentionPaged:
+    """Attention of packed rows q [.., heads * head_dim] over pools of keys and values (rt_attention_paged_enqueue); the result has q's shape."""
+
+    def __init__(self, q: "Tensor", k: "Tensor", v: "Tensor", seqs: Sequences, scale: Optional[float], causal: bool):
+        if len(k.shape) != 4 or k.shape != v.shape:
+            raise OperationError(_ffi.RT_ERR_INVALID_SHAPE, f"attention: k {k.shape}, v {v.shape}")
+        self.q, self.k, self.v, self.seqs, self.use_workspace = q, k, v, seqs, True
+        D = k.shape[3]
+        width = q.shape[-1] if q.shape else 0
+        if D == 0 or width % D:
+            raise OperationError(_ffi.RT_ERR_INVALID_SHAPE, f"attention: q {q.shape}, pools {k.shape}")
+        seqs.check(k.device, True)
+        d = _ffi.AttentionPagedDesc()
+        d.cache = seqs.cache_desc(k)
+        d.heads, d.rows = width // D, _rows_of(q, width, "attention: q")
+        if seqs.starts is None and d.rows != seqs.batch * seqs.max_rows:
+            raise OperationError(_ffi.RT_ERR_INVALID_SHAPE, f"attention: {d.rows} rows of {seqs.batch} sequences with {seqs.max_rows}")
+        d.max_rows, d.max_keys = seqs.max_rows, _i32(d.cache.table_width * d.cache.page_size if seqs.max_keys is None else seqs.max_keys)[0]
+        d.causal, d.scale = int(bool(causal)), 1.0 / math.sqrt(D) if scale is None else float(scale)
+        d.q_strides[:] = d.o_strides[:] = [width, D]
+        self.desc, self.out_shape = d, q.shape
+
+    def check_invariants(self):
+        if self.q.dt != DType.F16 or self.k.dt != DType.F16 or self.v.dt != DType.F16:
+            raise InvariantError(_ffi.RT_ERR_DTYPE_MISMATCH, "attention: q and the pools are F16")
+        st = _ffi.lib().rt_attention_paged_validate(self.desc)
+        _check(st, panic=st == _ffi.RT_ERR_INVALID_SHAPE)
+
+    def srcs(self):
+        return [self.q, self.k, self.v]
+
+    def _enqueue(self, device, stream, out, ws, ws_bytes):
+        q = self.seqs
+        return _ffi.lib().rt_attention_paged_enqueue(device.ctx, self.desc, self.q._ptr(), self.k._ptr(), self.v._ptr(), q.table.data_ptr(), q.lens.data_ptr(),
+                                                     None if q.starts is None else q.starts.data_ptr(), out, ws, ws_bytes, stream)
+
+    def _workspace(self, need):
+        return _ffi.lib().rt_attention_paged_workspace_bytes(self.desc, need)
+
+
+class AttentionPacked:
+    """Attention of packed prompts that see themselves: q [.., heads * head_dim], k and v [.., kv_heads * head_dim] with the same rows
+    (rt_attention_packed_enqueue); the result has q's shape."""
+
+    def __init__(self, q: "Tensor", k: "Tensor", v: "Tensor", seqs: Sequences, heads: int, scale: Optional[float], causal: bool):
+        self.q, self.k, self.v, self.seqs, self.use_workspace = q, k, v, seqs, True
+        width, kv_width = q.shape[-1] if q.shape else 0, k.shape[-1] if k.shape else 0
+        D = width // heads if heads > 0 else 0
+        if D == 0 or D * heads != width or kv_width % D or k.shape != v.shape:
+            raise OperationError(_ffi.RT_ERR_INVALID_SHAPE, f"attention: q {q.shape}, k {k.shape}, v {v.shape}, {heads} heads")
+        seqs.check(q.device, False)
+        d = _ffi.AttentionPackedDesc()
+        d.batch, d.heads, d.kv_heads, d.head_dim = _i32(seqs.batch, heads, kv_width // D, D)
+        d.rows, d.kv_rows = _rows_of(q, width, "attention: q"), _rows_of(k, kv_width, "attention: k")
+        if d.rows != d.kv_rows or (seqs.starts is None and d.rows != seqs.batch * seqs.max_rows):
+            raise OperationError(_ffi.RT_ERR_INVALID_SHAPE, f"attention: {d.rows} rows of q, {d.kv_rows} of k, {seqs.batch} sequences with {seqs.max_rows}")
+        d.max_rows, d.max_keys = seqs.max_rows, seqs.max_rows if seqs.max_keys is None else seqs.max_keys
+        d.causal, d.scale = int(bool(causal)), 1.0 / math.sqrt(D) if scale is None else float(scale)
+        d.q_strides[:] = d.o_strides[:] = [width, D]
+        d.k_strides[:] = d.v_strides[:] = [kv_width, D]
+        self.desc, self.out_shape = d, q.shape
+
+    def check_invariants(self):
+        if self.q.dt != DType.F16 or self.k.dt != DType.F16 or self.v.dt != DType.F16:
+            raise InvariantError(_ffi.RT_ERR_DTYPE_MISMATCH, "attention: q, k and v are F16")
+        st = _ffi.lib().rt_attention_packed_validate(self.desc)
+        _check(st, panic=st == _ffi.RT_ERR_INVALID_SHAPE)
+
+    def srcs(self):
+        return [self.q, self.k, self.v]
+
+    def _enqueue(self, device, stream, out, ws, ws_bytes):
+        s = self.seqs.starts
+        return _ffi.lib().rt_attention_packed_enqueue(device.ctx, self.desc, self.q._ptr(), self.k._ptr(), self.v._ptr(), None if s is None else s.data_ptr(), None, out, ws,
+                                                      ws_bytes, stream)
+
+    def _workspace(self, need):
+        return _ffi.lib().rt_attention_packed_workspace_bytes(self.desc, need)
+
+
 # An activation whose input is a Matmul node nobody has resolved yet runs in that product's
 # epilogue (one kernel, one rounding) instead of as a second pass over the output.
 FUSE_ACTIVATIONS = True
@@ -445,6 +607,7 @@ POISON_OUTPUTS = False
 
 
 _strides3 = ctypes.c_int64 * 3
+_strides2 = ctypes.c_int64 * 2
 
 
 def _touches(storage, lo: int, hi: int) -> bool:
@@ -459,13 +622,15 @@ def _write_key_and_value(k: "Tensor", v: "Tensor", stream: int):
     source, the values' write.  The launch runs both sources first and has no order between the two writes, so it is taken only where
     the values' source neither reads what the keys' write changes nor writes a cache, and no write touches what the other reads or writes."""
     a, b = k.op, v.op
-    q4 = type(a) is CacheQ4 and type(b) is CacheQ4
-    if k.storage is not None or v.storage is not None or not (q4 or (type(a) is Cache and type(b) is Cache)) or a.fresh or b.fresh:
+    q4, paged = type(a) is CacheQ4 and type(b) is CacheQ4, type(a) is CachePaged and type(b) is CachePaged
+    if k.storage is not None or v.storage is not None or not (q4 or paged or (type(a) is Cache and type(b) is Cache)) or a.fresh or b.fresh:
         return
     if q4 and (a.source.dt != b.source.dt or a.offsets is not b.offsets):
         return
+    if paged and (a.source.dt != b.source.dt or a.seqs is not b.seqs or a.rows != b.rows):
+        return
     if (a.cache.storage is None or b.cache.storage is None or k.dt != v.dt or k.shape != v.shape
-            or (a.offset, a.len, a.src_strides) != (b.offset, b.len, b.src_strides) or k.device is not v.device or k.device.kind != "gpu"):
+            or (not paged and (a.offset, a.len, a.src_strides) != (b.offset, b.len, b.src_strides)) or k.device is not v.device or k.device.kind != "gpu"):
         return
     keys, vals, ks, vs = a.cache.storage, b.cache.storage, a.source, b.source
     kc, vc = keys.data_ptr(), vals.data_ptr()
@@ -473,7 +638,7 @@ def _write_key_and_value(k: "Tensor", v: "Tensor", stream: int):
     if ks.device.kind != "gpu" or vs.device.kind != "gpu" or (kc < vc_end and vc < kc_end):
         return
     if vs.storage is None:
-        if type(vs.op) in (Cache, CacheQ4):
+        if type(vs.op) in (Cache, CacheQ4, CachePaged):
             return
         for s in vs.op.srcs():
             if s.storage is None or s.device.kind != "gpu" or _touches(s.storage, kc, kc_end):
@@ -486,7 +651,7 @@ def _write_key_and_value(k: "Tensor", v: "Tensor", stream: int):
         vs._execute(stream)
     if _touches(vs.storage, kc, kc_end):
         return
-    if q4:
+    if q4 or paged:
         a._enqueue(k.device, stream, kc, ks.storage.data_ptr(), vc, vs.storage.data_ptr())
         k.storage, v.storage = a.cache.storage, b.cache.storage
         return
@@ -650,6 +815,24 @@ class Tensor:
         op.check_invariants()
         return Tensor(op.out_shape, self.dt, self.device, None, op)
 
+    def cache_write_paged(self, source: "Tensor", seqs: Sequences) -> "Tensor":
+        """The write of packed new rows into this pool of pages, in place; see CachePaged.  The result is the pool itself (same storage)."""
+        op = CachePaged(self, source, seqs)
+        op.check_invariants()
+        return Tensor(op.out_shape, self.dt, self.device, None, op)
+
+    def attention_paged(self, k: "Tensor", v: "Tensor", seqs: Sequences, scale: Optional[float] = None, causal: bool = True) -> "Tensor":
+        """softmax(scale * self k^T) v over a cache in pages, of sequences of different lengths; see AttentionPaged."""
+        op = AttentionPaged(self, k, v, seqs, scale, causal)
+        op.check_invariants()
+        return Tensor(op.out_shape, self.dt, self.device, None, op)
+
+    def attention_packed(self, k: "Tensor", v: "Tensor", seqs: Sequences, heads: int, scale: Optional[float] = None, causal: bool = True) -> "Tensor":
+        """softmax(scale * self k^T) v of packed prompts of different lengths, each of which sees itself; see AttentionPacked."""
+        op = AttentionPacked(self, k, v, seqs, heads, scale, causal)
+        op.check_invariants()
+        return Tensor(op.out_shape, self.dt, self.device, None, op)
+
     def gelu(self) -> "Tensor":
         """tensor.rs `gelu()` (impl_unary_op): the lazy Unary node; same shape and dtype."""
         return self._unary("gelu")
@@ -709,7 +892,7 @@ class Tensor:
                 and op.input.consumers <= 1):
             act, op = op.act, op.input.op
             kind = Matmul
-        if kind is Attention or kind is AttentionQ4:
+        if kind is Attention or kind is AttentionQ4 or kind is AttentionPaged:
             if op.q.storage is None:
                 op.q._execute(stream)   # first, as in srcs(): it may read the caches as they were
             _write_key_and_value(op.k, op.v, stream)
@@ -730,7 +913,7 @@ class Tensor:
                                             op.offset, op.len, D, stream), dev)
             self.storage = op.cache.storage
             return
-        if kind is CacheQ4:
+        if kind is CacheQ4 or kind is CachePaged:
             op._enqueue(dev, stream, op.cache._ptr(), op.source._ptr())
             self.storage = op.cache.storage
             return
@@ -762,6 +945,11 @@ class Tensor:
             _check(L.rt_attention_q4_enqueue(dev.ctx, op.desc, op.q._ptr(), op.k._ptr(), op.v._ptr(), op.mask._ptr() if op.mask is not None else None,
                                              None if op.kv_lens is None else op.kv_lens.data_ptr(), ptr, ws.data_ptr() if ws is not None else None,
                                              need.value if ws is not None else 0, stream), dev)
+        elif kind is AttentionPaged or kind is AttentionPacked:
+            need = ctypes.c_uint64()
+            _check(op._workspace(need), dev)
+            ws = self._empty(need.value) if need.value and op.use_workspace else None
+            _check(op._enqueue(dev, stream, ptr, ws.data_ptr() if ws is not None else None, need.value if ws is not None else 0), dev)
         elif kind is Cache:
             B, H, cap, D = op.cache.shape
             _check(L.rt_cache_write_enqueue(dev.ctx, int(self.dt), op.cache._ptr(), op.source._ptr(), _strides3(*op.src_strides), ptr, B, H, cap,
