@@ -483,7 +483,7 @@ bool attention_paged_fits(const rt_attention_paged_desc &d) {
 uint64_t attention_paged_workspace_bytes(const rt_attention_paged_desc &d) {
     if (d.cache.batch == 0 || d.heads == 0 || d.rows == 0 || d.max_rows == 0) return 0;
     const PagedPlan p = ps_plan(d);
-    if (!p.streams) return ragged_workspace_bytes(d.cache.batch, d.heads, d.cache.kv_heads, d.rows, d.max_rows, d.max_keys, d.cache.head_dim);
+    if (!p.streams) return ragged_workspace_bytes(d.cache.batch, d.heads, d.cache.kv_heads, d.rows, d.max_rows, d.max_keys, d.cache.head_dim, d.causal);
     return p.whole ? 0 : (uint64_t)2 * p.wgs * d.max_rows * (d.heads / d.cache.kv_heads) * (d.cache.head_dim + 2) * sizeof(float) + (uint64_t)2 * d.cache.batch * d.cache.kv_heads * sizeof(int32_t);
 }
 

@@ -3,8 +3,9 @@
 //   out[r, h] = sum_j p_j v_j,  p = softmax_j(scale * q[r, h] . k_j) over the keys j that row r sees
 //
 // The rows of the heads that share a head of keys are one matrix, row m = query row * group + head of the group, so that a block of keys and values is read
-// once for all of them.  A workgroup of four wavefronts has 128 such rows of a sequence, a wavefront 32, against blocks of 64 keys that go from memory straight into LDS
-// (no registers; two stages of the ring at head_dim above 64, four below), rows of 64 or 128 halves, 16-byte chunks XOR-swizzled by the row.
+// once for all of them.  A workgroup has 128 such rows of a sequence, a wavefront 32, against blocks of 64 keys that go from memory straight into LDS (no registers; two stages of the
+// ring at head_dim above 64, four below), rows of 64 or 128 halves, 16-byte chunks XOR-swizzled by the row.  Four wavefronts and two workgroups on a compute unit where there are
+// enough of them, else eight wavefronts, of which four have the other 64 of 128 keys, and the halves meet at the end (rr_plan).
 //   S^T = K Q^T, v_mfma_f32_32x32x16_f16 with the keys as first operand: a lane has 16 of a tile's 32 keys of one row, and its neighbour 32 lanes on the others.
 //   softmax: scores stay as the product has them; p = exp2(s * sc - c) with the row's running reference c (RG_BELOW).  Sums and references are f32; probabilities enter the
 //     second product as f16 and the sum is that of the rounded ones.
@@ -18,7 +19,7 @@
 
 namespace rt {
 
-constexpr int RR_ROWS = 128, RR_KEYS = 64;
+constexpr int RR_ROWS = 128, RR_KEYS = 64; // rows of a workgroup; keys of a wavefront's block
 constexpr int RR_MAX_SPLITS = 64;
 constexpr int rr_pitch(int ks) { return ks <= 4 ? 64 : 128; } // halves of a row in LDS
 constexpr int rr_stages(int ks) { return ks <= 4 ? 4 : 2; }
@@ -45,16 +46,17 @@ __device__ __forceinline__ float rr_pair_sum(float v) {
     return __builtin_bit_cast(float, (uint32_t)a[0]) + __builtin_bit_cast(float, (uint32_t)a[1]);
 }
 
-// KS: steps of 16 over head_dim (the last one may be half)
-template <int KS, bool PAGED> __global__ __launch_bounds__(256, 2) void attention_ragged_kernel(RaggedArgs g) {
+// KS: steps of 16 over head_dim (the last one may be half).  NH: groups of four wavefronts, each with its 64 keys of a step
+template <int KS, bool PAGED, int NH> __global__ __launch_bounds__(256 * NH, 2) void attention_ragged_kernel(RaggedArgs g) {
+    constexpr int RR_STEP = RR_KEYS * NH, WAVES = 4 * NH;
     constexpr int P = rr_pitch(KS), CPR = P / 8, DT = (KS + 1) / 2, STAGES = rr_stages(KS);
-    constexpr int BLK = RR_KEYS * P;              // halves of a block of keys (or of values)
+    constexpr int BLK = RR_STEP * P;              // halves of a step's keys (or values)
     constexpr int RPI = 64 / CPR;                 // rows of a load instruction
-    constexpr int NI = RR_KEYS / RPI / 4;         // of them a wavefront issues per block and tensor
+    constexpr int NI = RR_STEP / RPI / WAVES;         // of them a wavefront issues per step and tensor
     extern __shared__ __attribute__((aligned(16))) uint8_t smem[];
-    const half_t *const ring = (const half_t *)smem; // [STAGES][keys | values][64][P]
+    const half_t *const ring = (const half_t *)smem; // [STAGES][keys | values][RR_STEP][P]
     const int t = threadIdx.x, lane = t & 63, wave = __builtin_amdgcn_readfirstlane(t >> 6);
-    const int r = lane & 31, hi = lane >> 5;
+    const int r = lane & 31, hi = lane >> 5, rg = wave & 3, half = wave >> 2; // group of rows, of wavefronts
 
     int b, tile, first, key0;
     const int line = blockIdx.x / g.kv_heads, kh = blockIdx.x - line * g.kv_heads, place = line / g.splits, share = line - place * g.splits;
@@ -63,10 +65,10 @@ template <int KS, bool PAGED> __global__ __launch_bounds__(256, 2) void attentio
     const int n = __builtin_amdgcn_readfirstlane(rg_rows(g, b, first)), len = __builtin_amdgcn_readfirstlane(rg_keys<PAGED>(g, b, key0));
     first = __builtin_amdgcn_readfirstlane(first), key0 = __builtin_amdgcn_readfirstlane(key0);
     const int rows = n * g.group, off = len - n; // causal: query row i sees keys up to i + off
-    const int row0 = tile * RR_ROWS, rw = row0 + 32 * wave;
+    const int row0 = tile * RR_ROWS, rw = row0 + 32 * rg;
     auto sees = [&](int m) { return g.causal ? max(0, min(len, min(m, rows - 1) / g.group + off + 1)) : len; }; // keys that row m sees: the first so many
-    // this share's blocks of those that a row of the tile sees
-    const int nkb = (sees(row0 + RR_ROWS - 1) + RR_KEYS - 1) / RR_KEYS;
+    // this share's steps of those that a row of the tile sees
+    const int nkb = (sees(row0 + RR_ROWS - 1) + RR_STEP - 1) / RR_STEP;
     const int kb0 = __builtin_amdgcn_readfirstlane((int)((int64_t)nkb * share / g.splits)), kb1 = __builtin_amdgcn_readfirstlane((int)((int64_t)nkb * (share + 1) / g.splits));
     const int seen_all = __builtin_amdgcn_readfirstlane(rw < rows ? sees(rw) : 0), seen_any = __builtin_amdgcn_readfirstlane(rw < rows ? sees(rw + 31) : 0); // by each, by any of the wavefront's rows
 
@@ -89,10 +91,10 @@ template <int KS, bool PAGED> __global__ __launch_bounds__(256, 2) void attentio
 
     // columns behind head_dim are zeros: no load writes them
     if (g.D < P)
-        for (int i = t; i < STAGES * 2 * BLK / 8; i += 256) ((uint4_t *)smem)[i] = uint4_t{0, 0, 0, 0};
+        for (int i = t; i < STAGES * 2 * BLK / 8; i += 64 * WAVES) ((uint4_t *)smem)[i] = uint4_t{0, 0, 0, 0};
     __syncthreads();
 
-    // ---- loads: instruction i of this wavefront brings the rows RPI (wave + 4 i) .. of the block; lane l the chunk l % CPR of row l / CPR.  All of its instructions are at the same
+    // ---- loads: instruction i of this wavefront brings the rows RPI (wave + WAVES i) .. of the step's; lane l the chunk l % CPR of row l / CPR.  All of its instructions are at the same
     // row of 16, so that offsets, chunks and lanes are the same for all, and only the 16 rows' address differs
     const int row16 = (RPI * wave) & 15, lrow = row16 + lane / CPR, c = 8 * ((lane % CPR) ^ rr_swizzle<P>(lrow));
     const uint64_t lanes = __builtin_amdgcn_ballot_w64(c < g.D); // whose chunk is a part of the row
@@ -100,28 +102,30 @@ template <int KS, bool PAGED> __global__ __launch_bounds__(256, 2) void attentio
     typedef __attribute__((address_space(4))) const int32_t *scalar_t; // read through the scalar cache: no vector load is awaited for them
     const scalar_t table = PAGED ? (scalar_t)(uintptr_t)(g.table + b * g.table_stride) : (scalar_t)0;
     const int last_entry = PAGED ? max(0, len - 1) >> g.page_shift : 0;
-    int pages[4]; // of the 16 keys each of a block
+    int pages[NI], own[4]; // of the 16 rows each that this wavefront brings, and of those that it multiplies
     auto look = [&](int kb) __attribute__((always_inline)) {
         if constexpr (PAGED) {
 #pragma unroll
-            for (int i = 0; i < 4; i++) pages[i] = table[min((kb * RR_KEYS + 16 * i) >> g.page_shift, last_entry)];
+            for (int i = 0; i < NI; i++) pages[i] = table[min((kb * RR_STEP + RPI * (wave + WAVES * i)) >> g.page_shift, last_entry)];
+#pragma unroll
+            for (int i = 0; i < 4; i++) own[i] = table[min((kb * RR_STEP + RR_KEYS * half + 16 * i) >> g.page_shift, last_entry)];
         }
     };
     const uint32_t lds0 = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) uint8_t *)smem;
     const uint32_t k_off = 2u * ((uint32_t)lrow * (uint32_t)(PAGED ? g.D : g.k_rs) + (uint32_t)c), v_off = 2u * ((uint32_t)lrow * (uint32_t)(PAGED ? g.D : g.v_rs) + (uint32_t)c);
-    // block kb into a stage, from the pages that `pages` has; -> whether its four sixteenths are there, as bits
+    // step kb into a stage, from the pages that `pages` has; -> whether this wavefront's four times 16 keys are there, as bits
     auto issue = [&](int stage, int kb) __attribute__((always_inline)) {
         uint32_t there = 15u;
-        const int j0 = kb * RR_KEYS;
-        const bool part = !PAGED && j0 + RR_KEYS > len; // of rows behind the last of packed keys the last is read again
+        const int j0 = kb * RR_STEP;
+        const bool part = !PAGED && j0 + RR_STEP > len; // of rows behind the last of packed keys the last is read again
         const half_t *const k0 = K + (int64_t)(key0 + j0) * g.k_rs, *const v0 = V + (int64_t)(key0 + j0) * g.v_rs;
 #pragma unroll
         for (int i = 0; i < NI; i++) {
-            const int row = RPI * (wave + 4 * i) - row16; // of the block: a multiple of 16
+            const int row = RPI * (wave + WAVES * i) - row16; // of the step: a multiple of 16
             const half_t *kp, *vp;
             uint32_t ko = k_off, vo = v_off;
             if constexpr (PAGED) {
-                const int x = RPI == 4 ? pages[i] : wave < 2 ? pages[(2 * i) & 3] : pages[(2 * i + 1) & 3], page = (uint32_t)x < (uint32_t)g.pages ? x : 0;
+                const int page = (uint32_t)pages[i] < (uint32_t)g.pages ? pages[i] : 0;
                 const int64_t at = (int64_t)page * g.k_rs + (int64_t)(((j0 + row) & ((1 << g.page_shift) - 1)) * g.D);
                 kp = K + at, vp = V + at;
             } else if (part) {
@@ -141,7 +145,7 @@ template <int KS, bool PAGED> __global__ __launch_bounds__(256, 2) void attentio
         if constexpr (PAGED) {
 #pragma unroll
             for (int i = 0; i < 4; i++)
-                if ((uint32_t)pages[i] >= (uint32_t)g.pages) there &= ~(1u << i);
+                if ((uint32_t)own[i] >= (uint32_t)g.pages) there &= ~(1u << i);
         }
         return there;
     };
@@ -184,7 +188,8 @@ template <int KS, bool PAGED> __global__ __launch_bounds__(256, 2) void attentio
 
     auto step = [&](int stage, int kb, uint32_t there, auto lean_c) __attribute__((always_inline)) {
         constexpr bool LEAN = decltype(lean_c)::value;
-        const half_t *const st = ring + stage * 2 * BLK;
+        const half_t *const st = ring + stage * 2 * BLK + half * RR_KEYS * P;
+        const int j0 = kb * RR_STEP + half * RR_KEYS; // this wavefront's first key
         // Operands are read four ahead of the products that take them: left to itself the compiler reads each right before its product, and waits
         float16_t S[2] = {};
         half8_t ahead[2][4];
@@ -206,7 +211,7 @@ template <int KS, bool PAGED> __global__ __launch_bounds__(256, 2) void attentio
             for (int d = 0; d < DT; d++) next[0][d] = values(st, d, 0);
         __builtin_amdgcn_sched_barrier(0);
         // register i of S[u]: key 32 u + 8 (i / 4) + 4 hi + i % 4 of the block
-        int left = last - kb * RR_KEYS - 4 * hi;
+        int left = last - j0 - 4 * hi;
         auto sees_key = [&](int u, int i) { return 32 * u + 8 * (i >> 2) + (i & 3) <= left && ((there >> (2 * u + (i >> 3))) & 1u); };
         float top = -INFINITY;
 #pragma unroll
@@ -320,13 +325,34 @@ template <int KS, bool PAGED> __global__ __launch_bounds__(256, 2) void attentio
             cur = cur + 1 == STAGES ? 0 : cur + 1, fill = fill + 1 == STAGES ? 0 : fill + 1;
             kb++;
         };
-        const int lean = min(kb1, seen_all / RR_KEYS), any = min(kb1, (seen_any + RR_KEYS - 1) / RR_KEYS);
+        // steps of which each of the wavefront's rows sees all of its keys, of which any sees one
+        const int lean = min(kb1, (seen_all / RR_KEYS + NH - 1 - half) / NH), any = min(kb1, ((seen_any + RR_KEYS - 1) / RR_KEYS + NH - 1 - half) / NH);
         while (kb < lean && there[0] == 15u) turn([&](uint32_t) { step(cur, kb, 15u, std::true_type{}); });
         while (kb < any) turn([&](uint32_t now) { step(cur, kb, now, std::false_type{}); });
         while (kb < kb1) turn([](uint32_t) {}); // blocks that only other wavefronts need
     }
     __builtin_amdgcn_s_waitcnt(rr_waitcnt(0)); // nothing lands after the workgroup has ended
-    const float l = rr_pair_sum(l_run);
+    float l = rr_pair_sum(l_run);
+    if constexpr (NH == 2) { // the two halves of the keys through LDS: [group of rows][reference, sum, outputs][lane]
+        __syncthreads();
+        float *const other = (float *)smem + rg * (2 + 16 * DT) * 64 + lane;
+        if (half) {
+            other[0] = c_run, other[64] = l;
+#pragma unroll
+            for (int d = 0; d < DT; d++)
+#pragma unroll
+                for (int i = 0; i < 16; i++) other[(2 + 16 * d + i) * 64] = acc[d][i];
+        }
+        __syncthreads();
+        if (half) return;
+        const float c1 = other[0], top = fmaxf(c_run, c1), base = top == -INFINITY ? 0.f : top;
+        const float a0 = __builtin_amdgcn_exp2f(c_run - base), a1 = __builtin_amdgcn_exp2f(c1 - base);
+        l = l * a0 + other[64] * a1, c_run = top;
+#pragma unroll
+        for (int d = 0; d < DT; d++)
+#pragma unroll
+            for (int i = 0; i < 16; i++) acc[d][i] = fmaf(acc[d][i], a0, other[(2 + 16 * d + i) * 64] * a1);
+    }
     if (rw + r >= rows) return;
     const int64_t row = first + qi;
     if (g.splits > 1) {
@@ -355,57 +381,99 @@ template <int KS, bool PAGED> __global__ __launch_bounds__(256, 2) void attentio
     }
 }
 
-// Joins the shares of a row in a fixed order.  A workgroup has 16 of a tile's 128 rows (blockIdx.y), 16 threads each, four columns a thread at a time.
-__global__ __launch_bounds__(256) void attention_ragged_join_kernel(RaggedArgs g) {
+// Joins the shares of a row in a fixed order: 32 lanes a row, which have a share's weight each (two past 32 shares) and then four columns, eight shares' loads at a time.  A workgroup has
+// RJ_ROWS of a tile's rows (blockIdx.y).
+constexpr int RJ_ROWS = 8;
+__global__ __launch_bounds__(32 * RJ_ROWS) void attention_ragged_join_kernel(RaggedArgs g) {
     int b, tile, first;
     const int place = blockIdx.x / g.kv_heads, kh = blockIdx.x - place * g.kv_heads;
     if (!rg_locate<RR_ROWS>(g, place, b, tile)) return;
-    const int n = rg_rows(g, b, first), m = tile * RR_ROWS + blockIdx.y * 16 + (threadIdx.x >> 4);
-    if (m >= n * g.group) return;
+    const int rows = rg_rows(g, b, first) * g.group, m0 = tile * RR_ROWS + blockIdx.y * RJ_ROWS;
+    if (m0 >= rows) return;
+    const int c = threadIdx.x & 31, m = min(m0 + (int)(threadIdx.x >> 5), rows - 1); // (all lanes stay: they exchange)
     const int qi = m / g.group, h = kh * g.group + (m - qi * g.group);
     const int64_t row = first + qi, at = (row * g.kv_heads * g.group + h) * g.splits;
-    float top = -INFINITY;
-    for (int s = 0; s < g.splits; s++) top = fmaxf(top, g.part_ml[2 * (at + s)]);
-    const float base = top == -INFINITY ? 0.f : top;
-    float l = 0.f;
-    for (int s = 0; s < g.splits; s++) l = fmaf(__builtin_amdgcn_exp2f(g.part_ml[2 * (at + s)] - base), g.part_ml[2 * (at + s) + 1], l);
-    for (int d = 4 * (threadIdx.x & 15); d < g.D; d += 64) {
-        float4_t y = {0.f, 0.f, 0.f, 0.f};
-        for (int s = 0; s < g.splits; s++) {
-            const float2_t ml = *(const float2_t *)(g.part_ml + 2 * (at + s));
-            if (ml[1] == 0.f) continue; // no key, and no outputs were written
-            const float a = __builtin_amdgcn_exp2f(ml[0] - base);
-            const float4_t v = *(const float4_t *)(g.part_o + (at + s) * g.D + d);
+    float2_t ml[2];
 #pragma unroll
-            for (int k = 0; k < 4; k++) y[k] = fmaf(a, v[k], y[k]);
-        }
-        *(half4_ru *)(g.O + row * g.o_rs + (int64_t)h * g.o_hs + d) = half4_ru{(half_t)(y[0] / l), (half_t)(y[1] / l), (half_t)(y[2] / l), (half_t)(y[3] / l)};
+    for (int i = 0; i < 2; i++) {
+        ml[i] = *(const float2_t *)(g.part_ml + 2 * (at + min(c + 32 * i, g.splits - 1)));
+        if (c + 32 * i >= g.splits) ml[i] = float2_t{-INFINITY, 0.f};
     }
+    float top = fmaxf(ml[0][0], ml[1][0]);
+#pragma unroll
+    for (int x = 16; x; x >>= 1) top = fmaxf(top, __shfl_xor(top, x));
+    const float base = top == -INFINITY ? 0.f : top;
+    float w[2], l;
+#pragma unroll
+    for (int i = 0; i < 2; i++) w[i] = __builtin_amdgcn_exp2f(ml[i][0] - base);
+    l = w[0] * ml[0][1] + w[1] * ml[1][1];
+#pragma unroll
+    for (int x = 16; x; x >>= 1) l += __shfl_xor(l, x);
+    const float *const po = g.part_o + at * g.D + (4 * c < g.D ? 4 * c : 0);
+    float4_t y = {0.f, 0.f, 0.f, 0.f};
+    for (int s0 = 0; s0 < g.splits; s0 += 8) {
+        float4_t v[8];
+        float a[8];
+#pragma unroll
+        for (int i = 0; i < 8; i++) {
+            const int s = min(s0 + i, g.splits - 1), from = (threadIdx.x & 32) + (s & 31);
+            v[i] = *(const float4_t *)(po + (int64_t)s * g.D);
+            const float sum = s < 32 ? __shfl(ml[0][1], from) : __shfl(ml[1][1], from); // (s is the same in all lanes)
+            a[i] = s < 32 ? __shfl(w[0], from) : __shfl(w[1], from);
+            if (s0 + i >= g.splits || sum == 0.f) a[i] = 0.f, v[i] = float4_t{0.f, 0.f, 0.f, 0.f}; // (no key: no outputs were written)
+        }
+#pragma unroll
+        for (int i = 0; i < 8; i++)
+#pragma unroll
+            for (int k = 0; k < 4; k++) y[k] = fmaf(a[i], v[i][k], y[k]);
+    }
+    if (m0 + (int)(threadIdx.x >> 5) >= rows || 4 * c >= g.D) return;
+    const float inv = 1.f / l; // no visible key: 0 * inf, NaN
+    *(half4_ru *)(g.O + row * g.o_rs + (int64_t)h * g.o_hs + 4 * c) = half4_ru{(half_t)(y[0] * inv), (half_t)(y[1] * inv), (half_t)(y[2] * inv), (half_t)(y[3] * inv)};
 }
 
 // Tiles of a call, at most: sequences have `rows` rows in all, and each may leave one tile begun.
 static int64_t rr_tiles(int batch, int group, int rows, int max_rows) {
     return std::min<int64_t>((int64_t)batch * (((int64_t)max_rows * group + RR_ROWS - 1) / RR_ROWS), (int64_t)rows * group / RR_ROWS + batch);
 }
-static int rr_splits(int64_t wgs, int max_keys) {
-    const int64_t steps = (max_keys + RR_KEYS - 1) / RR_KEYS;
-    return (int)std::max<int64_t>(1, std::min<int64_t>({(int64_t)RR_MAX_SPLITS, steps / 4, 512 / std::max<int64_t>(wgs, 1)}));
+// Groups of wavefronts of a workgroup, and shares of a row's keys.
+struct RaggedPlan {
+    int groups, splits;
+};
+// From 512 workgroups on two of four wavefronts fill each compute unit; where the causal flag makes tiles of unlike lengths the longest of fewer of them end last, alone, and eight wavefronts
+// on each are faster (us, four and eight: 2048 rows of 24 heads of 96, 384 tiles, 48.8 and 41.7; without the flag, 4 x 1500 rows of six heads of 64, 288 tiles, 36.7 and 43.8), as
+// they are where there is no second workgroup (512 rows on 4096 keys, 32 heads on 8 of 128, 208 tiles, 88.4 and 81.5).  Short ones do not pay for the join of the halves (24 prompts of up to
+// 100 rows 8.6 and 9.6).
+// Shares: the least of what rounds of workgroups, the partial results and the second launch take.  A step of 128 keys is some 0.5 + 0.016 head_dim us, partial results are written and read at 2.5 TB/s.
+static RaggedPlan rr_plan(int64_t wgs, int heads, int rows, int max_keys, int head_dim, int causal) {
+    RaggedPlan p{1, 1};
+    const int64_t steps = (max_keys + 2 * RR_KEYS - 1) / (2 * RR_KEYS);
+    if (steps > 2 && (wgs <= 256 || (causal && wgs < 512))) p.groups = 2;
+    if (p.groups == 2 && wgs <= 256) {
+        const double step = 0.5 + 0.016 * head_dim, part = (double)rows * heads * (head_dim + 2) * 8 / 2.5e6;
+        double best = 0;
+        for (int n = 1; n <= std::min<int64_t>(steps, RR_MAX_SPLITS); n++) {
+            const double t = (double)((wgs * n + 255) / 256) * ((steps + n - 1) / n) * step + (n > 1 ? 6 + n * part : 0);
+            if (n == 1 || t < best) best = t, p.splits = n;
+        }
+    }
+    return p;
 }
 static uint64_t rr_workspace(int heads, int rows, int head_dim, int splits) {
     return splits <= 1 ? 0 : (uint64_t)rows * heads * splits * (head_dim + 2) * sizeof(float);
 }
 
 bool ragged_fits(int batch, int kv_heads, int group, int rows, int max_rows) {
-    return rr_tiles(batch, group, rows, max_rows) * kv_heads <= 0xffffff; // a grid's threads are fewer than 2^32; shares take no call past that
+    return rr_tiles(batch, group, rows, max_rows) * kv_heads <= 0x7fffff; // a grid's threads are fewer than 2^32; shares take no call past that
 }
-uint64_t ragged_workspace_bytes(int batch, int heads, int kv_heads, int rows, int max_rows, int max_keys, int head_dim) {
-    return rr_workspace(heads, rows, head_dim, rr_splits(rr_tiles(batch, heads / kv_heads, rows, max_rows) * kv_heads, max_keys));
+uint64_t ragged_workspace_bytes(int batch, int heads, int kv_heads, int rows, int max_rows, int max_keys, int head_dim, int causal) {
+    return rr_workspace(heads, rows, head_dim, rr_plan(rr_tiles(batch, heads / kv_heads, rows, max_rows) * kv_heads, heads, rows, max_keys, head_dim, causal).splits);
 }
 
-template <int KS, bool PAGED> static hipError_t launch_rr(const RaggedArgs &g, hipStream_t st) {
-    constexpr size_t lds = (size_t)rr_stages(KS) * 2 * RR_KEYS * rr_pitch(KS) * sizeof(half_t);
-    if (const hipError_t e = ensure_lds_limit<&attention_ragged_kernel<KS, PAGED>>(); e != hipSuccess) return e;
-    hipLaunchKernelGGL((attention_ragged_kernel<KS, PAGED>), dim3((unsigned)((int64_t)g.tiles * g.kv_heads * g.splits)), dim3(256), lds, st, g);
+template <int KS, bool PAGED, int NH> static hipError_t launch_rr(const RaggedArgs &g, hipStream_t st) {
+    constexpr size_t lds = (size_t)rr_stages(KS) * 2 * NH * RR_KEYS * rr_pitch(KS) * sizeof(half_t);
+    if (const hipError_t e = ensure_lds_limit<&attention_ragged_kernel<KS, PAGED, NH>>(); e != hipSuccess) return e;
+    hipLaunchKernelGGL((attention_ragged_kernel<KS, PAGED, NH>), dim3((unsigned)((int64_t)g.tiles * g.kv_heads * g.splits)), dim3(256 * NH), lds, st, g);
     return hipGetLastError();
 }
 
@@ -419,7 +487,8 @@ void ragged_scale(RaggedArgs &g, float scale) {
 // `g` has the operands; the shares, and where partial results go, are chosen here.
 hipError_t launch_ragged(RaggedArgs &g, bool paged, void *workspace, uint64_t workspace_bytes, hipStream_t stream) {
     g.tiles = (int)rr_tiles(g.batch, g.group, g.rows, g.max_rows);
-    g.splits = rr_splits((int64_t)g.tiles * g.kv_heads, g.max_keys);
+    const RaggedPlan plan = rr_plan((int64_t)g.tiles * g.kv_heads, g.kv_heads * g.group, g.rows, g.max_keys, g.D, g.causal);
+    g.splits = plan.splits;
     const uint64_t need = rr_workspace(g.kv_heads * g.group, g.rows, g.D, g.splits);
     if (need && workspace && workspace_bytes >= need && !((uintptr_t)workspace & 15u))
         g.part_o = (float *)workspace, g.part_ml = g.part_o + (uint64_t)g.rows * g.kv_heads * g.group * g.splits * g.D;
@@ -427,7 +496,8 @@ hipError_t launch_ragged(RaggedArgs &g, bool paged, void *workspace, uint64_t wo
         g.splits = 1;
     auto go = [&](auto ks) -> hipError_t {
         constexpr int KS = decltype(ks)::value;
-        return paged ? launch_rr<KS, true>(g, stream) : launch_rr<KS, false>(g, stream);
+        if (plan.groups == 2) return paged ? launch_rr<KS, true, 2>(g, stream) : launch_rr<KS, false, 2>(g, stream);
+        return paged ? launch_rr<KS, true, 1>(g, stream) : launch_rr<KS, false, 1>(g, stream);
     };
     hipError_t e;
     switch ((g.D + 15) / 16) {
@@ -441,7 +511,7 @@ hipError_t launch_ragged(RaggedArgs &g, bool paged, void *workspace, uint64_t wo
     default: e = go(std::integral_constant<int, 8>{}); break;
     }
     if (e != hipSuccess || g.splits <= 1) return e;
-    hipLaunchKernelGGL(attention_ragged_join_kernel, dim3((unsigned)((int64_t)g.tiles * g.kv_heads), RR_ROWS / 16), dim3(256), 0, stream, g);
+    hipLaunchKernelGGL(attention_ragged_join_kernel, dim3((unsigned)((int64_t)g.tiles * g.kv_heads), RR_ROWS / RJ_ROWS), dim3(32 * RJ_ROWS), 0, stream, g);
     return hipGetLastError();
 }
 
@@ -451,7 +521,7 @@ bool attention_packed_fits(const rt_attention_packed_desc &d) {
 }
 uint64_t attention_packed_workspace_bytes(const rt_attention_packed_desc &d) {
     if (d.batch == 0 || d.heads == 0 || d.rows == 0) return 0;
-    return ragged_workspace_bytes(d.batch, d.heads, d.kv_heads, d.rows, d.max_rows, d.max_keys, d.head_dim);
+    return ragged_workspace_bytes(d.batch, d.heads, d.kv_heads, d.rows, d.max_rows, d.max_keys, d.head_dim, d.causal);
 }
 hipError_t launch_attention_packed(const rt_attention_packed_desc &d, const void *q, const void *k, const void *v, const int32_t *starts, const int32_t *kv_starts,
                                    void *out, void *workspace, uint64_t workspace_bytes, hipStream_t stream, const DeviceInfo &dev) {

@@ -135,7 +135,7 @@ template <int TILE> __device__ __forceinline__ bool rg_locate(const RaggedArgs &
 // The tiled kernel, for any number of rows (kernels_attention_ragged.hip): whether its grid holds a call, what workspace it asks for, the scale's part of
 // the arguments, and the launch.
 bool ragged_fits(int batch, int kv_heads, int group, int rows, int max_rows);
-uint64_t ragged_workspace_bytes(int batch, int heads, int kv_heads, int rows, int max_rows, int max_keys, int head_dim);
+uint64_t ragged_workspace_bytes(int batch, int heads, int kv_heads, int rows, int max_rows, int max_keys, int head_dim, int causal);
 void ragged_scale(RaggedArgs &g, float scale);
 hipError_t launch_ragged(RaggedArgs &g, bool paged, void *workspace, uint64_t workspace_bytes, hipStream_t stream);
 
