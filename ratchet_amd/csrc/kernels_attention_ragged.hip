@@ -4,7 +4,7 @@
 //
 // The rows of the heads that share a head of keys are one matrix, row m = query row * group + head of the group, so that a block of keys and values is read
 // once for all of them.  A workgroup has 128 such rows of a sequence, a wavefront 32, against blocks of 64 keys that go from memory straight into LDS (no registers; two stages of the
-// ring at head_dim above 64, four below), rows of 64 or 128 halves, 16-byte chunks XOR-swizzled by the row.  Four wavefronts and two workgroups on a compute unit where there are
+// ring at head_dim above 64, three below), rows of 64 or 128 halves, 16-byte chunks XOR-swizzled by the row.  Four wavefronts and two workgroups on a compute unit where there are
 // enough of them, else eight wavefronts, of which four have the other 64 of 128 keys, and the halves meet at the end (rr_plan).
 //   S^T = K Q^T, v_mfma_f32_32x32x16_f16 with the keys as first operand: a lane has 16 of a tile's 32 keys of one row, and its neighbour 32 lanes on the others.
 //   softmax: scores stay as the product has them; p = exp2(s * sc - c) with the row's running reference c (RG_BELOW).  Sums and references are f32; probabilities enter the
@@ -22,7 +22,7 @@ namespace rt {
 constexpr int RR_ROWS = 128, RR_KEYS = 64; // rows of a workgroup; keys of a wavefront's block
 constexpr int RR_MAX_SPLITS = 64;
 constexpr int rr_pitch(int ks) { return ks <= 4 ? 64 : 128; } // halves of a row in LDS
-constexpr int rr_stages(int ks) { return ks <= 4 ? 4 : 2; }
+constexpr int rr_stages(int ks) { return ks <= 4 ? 3 : 2; } // (with three of 16 KB, and registers for three wavefronts of a SIMD, three workgroups share a compute unit: prompts of up to 4096 rows, 32 heads on 8 of 64, 235 -> 216 us)
 typedef __fp16 rr_fp16x4 __attribute__((ext_vector_type(4)));
 typedef half_t half4_ru __attribute__((ext_vector_type(4), aligned(2)));
 
@@ -47,7 +47,7 @@ __device__ __forceinline__ float rr_pair_sum(float v) {
 }
 
 // KS: steps of 16 over head_dim (the last one may be half).  NH: groups of four wavefronts, each with its 64 keys of a step
-template <int KS, bool PAGED, int NH> __global__ __launch_bounds__(256 * NH, 2) void attention_ragged_kernel(RaggedArgs g) {
+template <int KS, bool PAGED, int NH> __global__ __launch_bounds__(256 * NH, KS <= 4 && NH == 1 ? 3 : 2) void attention_ragged_kernel(RaggedArgs g) {
     constexpr int RR_STEP = RR_KEYS * NH, WAVES = 4 * NH;
     constexpr int P = rr_pitch(KS), CPR = P / 8, DT = (KS + 1) / 2, STAGES = rr_stages(KS);
     constexpr int BLK = RR_STEP * P;              // halves of a step's keys (or values)
