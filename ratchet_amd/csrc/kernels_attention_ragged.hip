@@ -444,8 +444,10 @@ struct RaggedPlan {
 // on each are faster (us, four and eight: 2048 rows of 24 heads of 96, 384 tiles, 48.8 and 41.7; without the flag, 4 x 1500 rows of six heads of 64, 288 tiles, 36.7 and 43.8), as
 // they are where there is no second workgroup (512 rows on 4096 keys, 32 heads on 8 of 128, 208 tiles, 88.4 and 81.5).  Short ones do not pay for the join of the halves (24 prompts of up to
 // 100 rows 8.6 and 9.6).
-// Shares: the least of what rounds of workgroups, the partial results and the second launch take.  A step of 128 keys is some 0.5 + 0.016 head_dim us, partial results are written and read at 2.5 TB/s.
-static RaggedPlan rr_plan(int64_t wgs, int heads, int rows, int max_keys, int head_dim, int causal) {
+// Shares: the least of what the steps, the partial results and the second launch take.  A step of 128 keys is some 0.5 + 0.016 head_dim us, partial results are written and read at 2.5 TB/s.  Tiles of one
+// length take rounds of workgroups; with the causal flag they are of unlike lengths, and take what the longest takes, or all of them on 256 compute units (5088 rows of four heads on one of
+// 96, 160 tiles: 70 us in one share, 58 in three).
+static RaggedPlan rr_plan(int64_t wgs, int heads, int rows, int max_rows, int max_keys, int head_dim, int causal) {
     RaggedPlan p{1, 1};
     const int64_t steps = (max_keys + 2 * RR_KEYS - 1) / (2 * RR_KEYS);
     if (steps > 2 && (wgs <= 256 || (causal && wgs < 512))) p.groups = 2;
@@ -453,7 +455,8 @@ static RaggedPlan rr_plan(int64_t wgs, int heads, int rows, int max_keys, int he
         const double step = 0.5 + 0.016 * head_dim, part = (double)rows * heads * (head_dim + 2) * 8 / 2.5e6;
         double best = 0;
         for (int n = 1; n <= std::min<int64_t>(steps, RR_MAX_SPLITS); n++) {
-            const double t = (double)((wgs * n + 255) / 256) * ((steps + n - 1) / n) * step + (n > 1 ? 6 + n * part : 0);
+            const double per = (double)((steps + n - 1) / n), all = (double)wgs * steps / 256 * (1 - 0.5 * std::min(max_rows, max_keys) / max_keys);
+            const double t = (causal ? std::max(per, all) : (double)((wgs * n + 255) / 256) * per) * step + (n > 1 ? 6 + n * part : 0);
             if (n == 1 || t < best) best = t, p.splits = n;
         }
     }
@@ -467,7 +470,7 @@ bool ragged_fits(int batch, int kv_heads, int group, int rows, int max_rows) {
     return rr_tiles(batch, group, rows, max_rows) * kv_heads <= 0x7fffff; // a grid's threads are fewer than 2^32; shares take no call past that
 }
 uint64_t ragged_workspace_bytes(int batch, int heads, int kv_heads, int rows, int max_rows, int max_keys, int head_dim, int causal) {
-    return rr_workspace(heads, rows, head_dim, rr_plan(rr_tiles(batch, heads / kv_heads, rows, max_rows) * kv_heads, heads, rows, max_keys, head_dim, causal).splits);
+    return rr_workspace(heads, rows, head_dim, rr_plan(rr_tiles(batch, heads / kv_heads, rows, max_rows) * kv_heads, heads, rows, max_rows, max_keys, head_dim, causal).splits);
 }
 
 template <int KS, bool PAGED, int NH> static hipError_t launch_rr(const RaggedArgs &g, hipStream_t st) {
@@ -487,7 +490,7 @@ void ragged_scale(RaggedArgs &g, float scale) {
 // `g` has the operands; the shares, and where partial results go, are chosen here.
 hipError_t launch_ragged(RaggedArgs &g, bool paged, void *workspace, uint64_t workspace_bytes, hipStream_t stream) {
     g.tiles = (int)rr_tiles(g.batch, g.group, g.rows, g.max_rows);
-    const RaggedPlan plan = rr_plan((int64_t)g.tiles * g.kv_heads, g.kv_heads * g.group, g.rows, g.max_keys, g.D, g.causal);
+    const RaggedPlan plan = rr_plan((int64_t)g.tiles * g.kv_heads, g.kv_heads * g.group, g.rows, g.max_rows, g.max_keys, g.D, g.causal);
     g.splits = plan.splits;
     const uint64_t need = rr_workspace(g.kv_heads * g.group, g.rows, g.D, g.splits);
     if (need && workspace && workspace_bytes >= need && !((uintptr_t)workspace & 15u))

@@ -138,6 +138,30 @@ def test_parts_of_a_fused_projection_and_strided_outputs(device):
 
 
 @gpu
+def test_rows_far_apart(device):
+    """The largest strides of keys and values: rows 32 MiB apart, offsets past 2^32 within a sequence."""
+    rows, d, far = 200, 64, 1 << 24
+    q, k, v = inputs(14, rows, rows, 2, 1, d)
+    room = torch.empty((rows - 1) * far + 2 * d, dtype=torch.float16, device="cuda")
+    kv = torch.as_strided(room, (rows, 2, d), (far, d, 1))
+    kv[:, 0], kv[:, 1] = k[:, 0].cuda(), v[:, 0].cuda()
+    n = [rows - 65, 65]
+    want, tol = reference(q, split(k, n), split(v, n), n, n, 0.125, True)
+    for most in (rows, 400):     # one group of wavefronts, two
+        out = torch.empty(q.shape, dtype=torch.float16, device="cuda")
+        desc = packed_desc(2, 2, 1, d, rows, rows, most, most, True, 0.125, None, [far, 0], [far, 0])
+        attend_packed(device, desc, q.cuda(), kv, kv[:, 1:], starts_of(n).cuda(), None, out)
+        close(out, want, tol, most)
+
+
+@gpu
+@pytest.mark.parametrize("heads,kv_heads,d,causal,n", [(32, 8, 128, True, [700, 300, 1000]), (6, 6, 64, False, [600, 500]), (4, 1, 96, True, [1500]), (40, 40, 40, True, [300, 10]), (2, 2, 128, False, [900])])
+def test_longer_prompts(device, heads, kv_heads, d, causal, n):
+    """One and two groups of wavefronts, one and several shares."""
+    run(device, heads, n, heads, kv_heads, d, causal)
+
+
+@gpu
 def test_without_starts_every_sequence_has_as_many_rows(device):
     b, n, heads, d = 3, 77, 2, 64
     q, k, v = inputs(11, b * n, b * n, heads, heads, d)

@@ -182,6 +182,34 @@ def test_bounds_far_above_the_lengths(device, rows):
 
 
 @gpu
+@pytest.mark.parametrize("batch,kv,d,most,rows", [(150, 2, 64, 2000, 2), (300, 1, 40, 1500, 1), (300, 8, 16, 700, 1), (65, 3, 96, 900, 5), (64, 1, 128, 3000, 8)])
+def test_many_sequences_share_workgroups(device, batch, kv, d, most, rows):
+    """Parts of one workgroup end and begin within sequences of any length, empty ones and ones without rows among them; from 2048 heads of keys on each has a workgroup."""
+    gen = torch.Generator().manual_seed(batch)
+    lens = torch.randint(0, most, (batch,), generator=gen).tolist()
+    n = torch.randint(0, rows + 1, (batch,), generator=gen).tolist()
+    n[0], lens[0], n[1], n[-1] = rows, most, 0, rows
+    attend(device, batch, n, lens, 2 * kv, kv, d, 16, max_rows=rows)
+
+
+@gpu
+def test_more_rows_than_promised(device):
+    """Sequences are cut to max_rows rows: what lies past them is left as it was, and the others are right."""
+    c = Paged(3, [700, 90], 2, 64, 16)
+    q = torch.randn((12, 4, 64), generator=torch.Generator().manual_seed(2)).half()
+    k_pool, v_pool, table, lens = c.on_gpu()
+    want, tol = reference(q[9:], [c.k[1]], [c.v[1]], [3], [90], 0.125, True)
+    for rows in (3, 40):     # on both kernels
+        x = torch.cat([q[:9].repeat_interleave(rows // 3, 0), q[9:].repeat_interleave(1, 0)])
+        first = 9 * (rows // 3)
+        out = torch.full(x.shape, 7.0, dtype=torch.float16, device="cuda")
+        starts = torch.tensor([0, first, first + 3], dtype=torch.int32).cuda()
+        attend_paged(device, paged_desc(c.cache, 4, first + 3, rows, c.width * 16, True, 0.125), x.cuda(), k_pool, v_pool, table, lens, starts, out)
+        assert bool((out[rows:first] == 7.0).all()) and bool(torch.isfinite(out[:rows]).all())
+        close(out[first:], want, tol, rows)
+
+
+@gpu
 @pytest.mark.parametrize("rows", [1, 9, 60])
 def test_pages_that_are_not_there(device, rows):
     """Entries outside the pool, at the beginning (what has left a window), in the middle, at the end, and all of a sequence's."""
