@@ -585,7 +585,7 @@ typedef struct rt_paged_cache_desc {
  *   src     packed [rows, kv_heads, head_dim], F16, or F32 (rounded to f16); src_strides: row, head, in elements, both tensors'
  *   starts  as above; NULL: rows / batch each
  * Row i of the n rows of sequence b goes to position lens[b] - n + i; one below 0, past the table or without a page is not
- * written.  Everything else in the pools keeps its bytes.  v_pool and v_src may both be NULL: one tensor.  Two rows of a call that
+ * written.  At most 2^25 rows (RT_ERR_UNSUPPORTED beyond).  Everything else in the pools keeps its bytes.  v_pool and v_src may both be NULL: one tensor.  Two rows of a call that
  * name the same place of a page (sequences that share one): one of the two is there afterwards. */
 RT_API rt_status rt_cache_write_paged_enqueue(rt_ctx *ctx, const rt_paged_cache_desc *desc, int32_t src_dtype, void *k_pool, const void *k_src,
                                               void *v_pool, const void *v_src, const int64_t *src_strides, const int32_t *table,
@@ -600,7 +600,9 @@ RT_API rt_status rt_cache_write_paged_enqueue(rt_ctx *ctx, const rt_paged_cache_
  * A row that sees no key is NaN, as in rt_attention_enqueue.  Keys that a row does not see, and what lies in pages behind a sequence's keys, have no effect on
  * it, whatever they hold; a row that sees a value that is not finite is not finite in that dimension.
  * Sums, references and scores are f32; the probabilities enter the second product as f16.
- * Limits (RT_ERR_UNSUPPORTED beyond): 2^25 rows, 2^30 keys of a sequence, rows times heads below 2^31, 65535 sequences. */
+ * Limits (RT_ERR_UNSUPPORTED beyond): 2^25 rows, 2^30 keys of a sequence, rows times heads below 2^31, 65535 sequences, 2^23 - 1 tiles of 128 rows of
+ * the heads that share a head of keys (a sequence may begin one) times kv_heads.  Up to 32 such rows a sequence run on a kernel that reads the pages at the rate of
+ * memory, and more on tiles: a step of one token for some and a prompt for others is faster in two calls. */
 typedef struct rt_attention_paged_desc {
     rt_paged_cache_desc cache;
     int32_t heads;              /* a multiple of cache.kv_heads */
@@ -621,7 +623,8 @@ RT_API rt_status rt_attention_paged_enqueue(rt_ctx *ctx, const rt_attention_page
 
 /* Attention of packed prompts: keys and values are packed rows too, [kv_rows, kv_heads, head_dim], those of sequence b at kv_starts[b] ..
  * kv_starts[b + 1] - 1; kv_starts == NULL: where its query rows are (kv_rows == rows), each prompt seeing itself.  q, k and v may be parts of one fused
- * projection's output.  All else as rt_attention_paged_enqueue; with the causal flag row i of n sees the first (keys - n + i + 1) keys. */
+ * projection's output.  All else as rt_attention_paged_enqueue; with the causal flag row i of n sees the first (keys - n + i + 1) keys.
+ * Strides of keys and values are at most 2^24 elements (RT_ERR_UNSUPPORTED beyond). */
 typedef struct rt_attention_packed_desc {
     int32_t batch, heads, kv_heads;
     int32_t head_dim;           /* a multiple of 8, 8 .. 128 */

@@ -9,6 +9,9 @@
 //   they lie, and the values' comes transposed out of LDS.
 // The work is the line of all 128 keys of all sequences and heads of keys; a workgroup takes an equal part of it, whatever the sequences' lengths, and so ends within a sequence.
 // What it has of one that others share goes to the workspace, at most twice, and a second kernel joins the parts in a fixed order.  Lengths stay on the device.
+//
+// 32 sequences of up to 8192 keys, 8 heads of 128, one row of 32 heads, 684 MB: 110 us, 6.2 TB/s, as a copy of this kernel that only loads takes, and 4.7 in the join.  Small ones wait: 100 keys of
+// 32 heads of 80 6.2 us, in a launch, three trips to memory one after another (lengths, pages, keys) and one step; 1024 keys 6.8 and 3.4 in the join.
 #include "ragged.h"
 
 #include <algorithm>
