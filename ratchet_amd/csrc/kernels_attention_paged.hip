@@ -473,9 +473,12 @@ static PagedPlan ps_plan(const rt_attention_paged_desc &d) {
     const int64_t per = (int64_t)d.max_rows * (d.heads / c.kv_heads), heads = (int64_t)c.batch * c.kv_heads, steps = std::max(1, (d.max_keys + PS_KEYS - 1) / PS_KEYS);
     PagedPlan p{};
     p.streams = per <= 32 && heads <= 0xffffff && heads * steps < (int64_t(1) << 31) && heads * per < (int64_t(1) << 24);
-    // Up to four steps a workgroup takes less time over all of a head than the second launch does: 32 heads of 80, 100 and 250 keys 6.2 and 7.3 us, a step 1.1 more; a launch for the join 3.3
-    p.whole = steps <= 4 || heads >= 2048;
-    p.wgs = (int)std::min<int64_t>(512, heads * steps);
+    // A workgroup takes 6.2 us over a head of 100 keys and 1.1 more for each step, the join's launch 3.3 and more: few steps, or many heads, which keep the memory busy by themselves, are faster
+    // without equal parts (us, in equal parts and a head each: 32 heads of 80, 8 steps 9.6 and 12.2; 96 of 96, 8 / 16 steps 15.6 / 19.2 and 13.3 / 21.9; 128 of 128 17.7 / 25.0 and 16.8 / 28.6; 256 of
+    // 128, 16 / 32 steps 39.6 / 66.2 and 36.1 / 67.6; 1024, 8 steps 71 and 60).
+    p.whole = steps <= std::max<int64_t>(4, heads / 12);
+    // Two workgroups to a compute unit where there is work for them: 32 x 8 heads, 16 steps; below, one, and half as many parts to join (96 heads of 96, 16 steps, 21.0 us with 512, 19.2 with 256).
+    p.wgs = (int)std::min<int64_t>(heads * steps < 2048 ? 256 : 512, heads * steps);
     return p;
 }
 

@@ -182,7 +182,7 @@ def test_bounds_far_above_the_lengths(device, rows):
 
 
 @gpu
-@pytest.mark.parametrize("batch,kv,d,most,rows", [(150, 2, 64, 2000, 2), (300, 1, 40, 1500, 1), (300, 8, 16, 700, 1), (65, 3, 96, 900, 5), (64, 1, 128, 3000, 8)])
+@pytest.mark.parametrize("batch,kv,d,most,rows", [(150, 2, 64, 2000, 2), (300, 1, 40, 1500, 1), (300, 8, 16, 700, 1), (65, 3, 96, 900, 5), (64, 1, 128, 3000, 8), (100, 1, 64, 2500, 2), (130, 1, 96, 3000, 1), (70, 2, 128, 2500, 3)])
 def test_many_sequences_share_workgroups(device, batch, kv, d, most, rows):
     """Parts of one workgroup end and begin within sequences of any length, empty ones and ones without rows among them; from 2048 heads of keys on each has a workgroup."""
     gen = torch.Generator().manual_seed(batch)
