@@ -240,6 +240,14 @@ def test_refusals(field, value, status):
     assert L.rt_attention_packed_workspace_bytes(d, need) == status
 
 
+def test_rows_times_heads():
+    """Tiles of 128 rows past the last one still have numbers of 31 bits."""
+    for rows, status in (((1 << 25) - 1, _ffi.RT_ERR_UNSUPPORTED), ((1 << 25) - 4, _ffi.RT_OK)):
+        d = packed_desc(1, 64, 64, 8, rows, rows, 1, 1, True, 0.1)
+        d.max_rows = 128
+        assert _ffi.lib().rt_attention_packed_validate(d) == status, rows
+
+
 @pytest.mark.parametrize("name", ["q_strides", "k_strides", "v_strides", "o_strides"])
 def test_refused_strides(name):
     for i in range(2):
