@@ -783,7 +783,7 @@ static rt_status ragged_validate(int32_t batch, int32_t heads, int32_t kv_heads,
     }
     if (causal != 0 && causal != 1) return RT_ERR_INVALID_ARG;
     if (!(std::fabs(scale) <= 3.4e38f)) return RT_ERR_INVALID_ARG;
-    if (batch > 65535 || rows > (1 << 25) || max_keys > (1 << 30) || (int64_t)rows * heads > (int64_t(1) << 31) - 256) return RT_ERR_UNSUPPORTED; // (rounded up to tiles they are 31 bits)
+    if (batch > 65535 || heads > (1 << 20) || rows > (1 << 25) || max_keys > (1 << 30) || (int64_t)rows * heads > (int64_t(1) << 31) - 256) return RT_ERR_UNSUPPORTED; // (rounded up to tiles they are 31 bits)
     return RT_OK;
 }
 

@@ -63,25 +63,27 @@ template <int KS, bool PAGED, int NH> __global__ __launch_bounds__(256 * NH, KS 
     const int t = threadIdx.x, lane = t & 63, wave = __builtin_amdgcn_readfirstlane(t >> 6);
     const int r = lane & 31, hi = lane >> 5, rg = wave & 3, half = wave >> 2; // group of rows, of wavefronts
 
-    int b, tile, first, key0;
+    int b, tile, first, n, key0;
     const int line = blockIdx.x / g.kv_heads, kh = blockIdx.x - line * g.kv_heads, place = line / g.splits, share = line - place * g.splits;
-    if (!rg_locate<RR_ROWS>(g, place, b, tile)) return;
-    b = __builtin_amdgcn_readfirstlane(b), tile = __builtin_amdgcn_readfirstlane(tile);
-    const int n = __builtin_amdgcn_readfirstlane(rg_rows(g, b, first)), len = __builtin_amdgcn_readfirstlane(rg_keys<PAGED>(g, b, key0));
+    if (!rg_locate<RR_ROWS>(g, place, b, tile, first, n)) return;
+    b = __builtin_amdgcn_readfirstlane(b), tile = __builtin_amdgcn_readfirstlane(tile), n = __builtin_amdgcn_readfirstlane(n);
+    const int len = __builtin_amdgcn_readfirstlane(rg_keys<PAGED>(g, b, key0));
     first = __builtin_amdgcn_readfirstlane(first), key0 = __builtin_amdgcn_readfirstlane(key0);
     const int rows = n * g.group, off = len - n; // causal: query row i sees keys up to i + off
     const int row0 = tile * RR_ROWS, rw = row0 + 32 * rg;
-    auto sees = [&](int m) { return g.causal ? max(0, min(len, min(m, rows - 1) / g.group + off + 1)) : len; }; // keys that row m sees: the first so many
+    const int q0 = row0 / g.group, over = row0 - q0 * g.group; // (the tile's other query rows are found from its first without a division)
+    auto query = [&](int m) { return q0 + rg_query(g, m - row0 + over); };
+    auto sees = [&](int m) { return g.causal ? max(0, min(len, query(min(m, rows - 1)) + off + 1)) : len; }; // keys that row m sees: the first so many
     // this share's steps of those that a row of the tile sees
     const int nkb = (sees(row0 + RR_ROWS - 1) + RR_STEP - 1) / RR_STEP;
     const int kb0 = __builtin_amdgcn_readfirstlane((int)((int64_t)nkb * share / g.splits)), kb1 = __builtin_amdgcn_readfirstlane((int)((int64_t)nkb * (share + 1) / g.splits));
     const int seen_all = __builtin_amdgcn_readfirstlane(rw < rows ? sees(rw) : 0), seen_any = __builtin_amdgcn_readfirstlane(rw < rows ? sees(rw + 31) : 0); // by each, by any of the wavefront's rows
 
     // queries: row rw + r, dimensions 16 k + 8 hi .. + 7
-    const int m = min(rw + r, rows - 1), qi = m / g.group, qh = kh * g.group + (m - qi * g.group);
+    const int m = min(rw + r, rows - 1), qi = query(m), qh = kh * g.group + (m - qi * g.group);
     const int last = min(len - 1, g.causal ? qi + off : len - 1);
     half8_t fq[KS];
-    {
+    auto queries = [&]() __attribute__((always_inline)) {
         const half_t *q = g.Q + (int64_t)(first + qi) * g.q_rs + (int64_t)qh * g.q_hs;
         const half_t sign = (half_t)g.sign;
 #pragma unroll
@@ -89,15 +91,16 @@ template <int KS, bool PAGED, int NH> __global__ __launch_bounds__(256 * NH, KS 
             const int d = 16 * k + 8 * hi;
             fq[k] = d < g.D ? *(const half8_t *)(q + d) * half8_t{sign, sign, sign, sign, sign, sign, sign, sign} : half8_t{};
         }
-    }
-    // awaited here: a first use in the loop would wait there, for these and with them for every load into LDS
+        // awaited here: a first use in the loop would wait there, for these and with them for every load into LDS
 #pragma unroll
-    for (int k = 0; k < KS; k++) asm volatile("" : "+v"(fq[k]));
+        for (int k = 0; k < KS; k++) asm volatile("" : "+v"(fq[k]));
+    };
 
-    // columns behind head_dim are zeros: no load writes them
-    if (g.D < P)
+    // Of the columns behind head_dim, which no load writes, the products read those up to the next 32: they are zeros
+    if (g.D < 32 * DT) {
         for (int i = t; i < STAGES * 2 * BLK / 8; i += 64 * WAVES) ((uint4_t *)smem)[i] = uint4_t{0, 0, 0, 0};
-    __syncthreads();
+        __syncthreads();
+    }
 
     // ---- loads: instruction i of this wavefront brings the rows RPI (wave + WAVES i) .. of the step's; lane l the chunk l % CPR of row l / CPR.  All of its instructions are at the same
     // row of 16, so that offsets, chunks and lanes are the same for all, and only the 16 rows' address differs
@@ -317,6 +320,7 @@ template <int KS, bool PAGED, int NH> __global__ __launch_bounds__(256 * NH, KS 
             there[s] = issue(s, min(kb0 + s, kb1 - 1)); // past the end: the last block again, into a stage that nobody reads
             look(min(kb0 + s + 1, kb1 - 1));
         }
+        queries(); // behind the first blocks' loads: the trips to memory are one
         publish(std::integral_constant<int, STAGES - 2>{});
         int cur = 0, fill = STAGES - 1, kb = kb0;
         auto turn = [&](auto body) __attribute__((always_inline)) {
@@ -390,10 +394,10 @@ template <int KS, bool PAGED, int NH> __global__ __launch_bounds__(256 * NH, KS 
 // RJ_ROWS of a tile's rows (blockIdx.y).
 constexpr int RJ_ROWS = 8;
 __global__ __launch_bounds__(32 * RJ_ROWS) void attention_ragged_join_kernel(RaggedArgs g) {
-    int b, tile, first;
+    int b, tile, first, n;
     const int place = blockIdx.x / g.kv_heads, kh = blockIdx.x - place * g.kv_heads;
-    if (!rg_locate<RR_ROWS>(g, place, b, tile)) return;
-    const int rows = rg_rows(g, b, first) * g.group, m0 = tile * RR_ROWS + blockIdx.y * RJ_ROWS;
+    if (!rg_locate<RR_ROWS>(g, place, b, tile, first, n)) return;
+    const int rows = n * g.group, m0 = tile * RR_ROWS + blockIdx.y * RJ_ROWS;
     if (m0 >= rows) return;
     const int c = threadIdx.x & 31, m = min(m0 + (int)(threadIdx.x >> 5), rows - 1); // (all lanes stay: they exchange)
     const int qi = m / g.group, h = kh * g.group + (m - qi * g.group);

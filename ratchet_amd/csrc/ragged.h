@@ -21,7 +21,7 @@ struct RaggedArgs {
     float per_group; // 1 / group
 };
 
-// m / group for m below 2^22: a multiple of 1 / group plus a half of that is further from a whole number than the product's error
+// m / group for m below 2^22 (group is at most 2^20): a multiple of 1 / group plus a half of that is further from a whole number than the product's error
 __device__ __forceinline__ int rg_query(const RaggedArgs &g, int m) { return (int)(((float)m + 0.5f) * g.per_group); }
 
 constexpr float kLog2eR = 1.4426950408889634f;
@@ -81,16 +81,21 @@ __device__ __forceinline__ int rg_nth(uint64_t mask, int place, int lane) {
 
 // Every tile of TILE rows (query rows times heads that share a head of keys) of every sequence has a place in a line.  Tile t of a sequence comes before all tiles below t,
 // so that with the causal flag the long ones come first; past 256 sequences the line goes by sequence instead.  -> whether there is such a place.
-template <int TILE> __device__ __forceinline__ bool rg_locate(const RaggedArgs &g, int place, int &b, int &tile) {
+// `first`, `rows`: that sequence's.
+template <int TILE> __device__ __forceinline__ bool rg_locate(const RaggedArgs &g, int place, int &b, int &tile, int &first, int &rows) {
     const int lane = threadIdx.x & 63;
-    auto tiles_of = [&](int i) {
-        int first;
-        return i < g.batch ? (rg_rows(g, i, first) * g.group + TILE - 1) / TILE : 0;
+    auto look = [&](int i, int &at, int &count) { // -> tiles
+        count = rg_rows(g, min(i, g.batch - 1), at);
+        return i < g.batch ? (count * g.group + TILE - 1) / TILE : 0;
     };
     if (g.batch <= 256) {
-        int n[4], most = 0;
+        int n[4], at[4], count[4], most = 0;
 #pragma unroll
-        for (int c = 0; c < 4; c++) n[c] = 64 * c < g.batch ? tiles_of(64 * c + lane) : 0, most = max(most, n[c]);
+        for (int c = 0; c < 4; c++) {
+            n[c] = at[c] = count[c] = 0;
+            if (64 * c < g.batch) n[c] = look(64 * c + lane, at[c], count[c]);
+            most = max(most, n[c]);
+        }
         most = rg_reduce(most, [](int x, int y) { return max(x, y); });
         auto above = [&](int level) { // tiles of that number and up
             int s = 0;
@@ -110,21 +115,24 @@ template <int TILE> __device__ __forceinline__ bool rg_locate(const RaggedArgs &
 #pragma unroll
         for (int c = 0; c < 4; c++) {
             const uint64_t mask = __builtin_amdgcn_ballot_w64(n[c] > lo);
-            const int count = __builtin_popcountll(mask);
-            if (place < count) {
-                b = 64 * c + rg_nth(mask, place, lane);
+            const int here = __builtin_popcountll(mask);
+            if (place < here) {
+                const int l = rg_nth(mask, place, lane);
+                b = 64 * c + l, first = __builtin_amdgcn_readlane(at[c], l), rows = __builtin_amdgcn_readlane(count[c], l);
                 return true;
             }
-            place -= count;
+            place -= here;
         }
         return false;
     }
     for (int c = 0; c < g.batch; c += 64) {
-        const int n = tiles_of(c + lane), upto = rg_scan(n, lane), all = __builtin_amdgcn_readlane(upto, 63);
+        int from, count;
+        const int n = look(c + lane, from, count), upto = rg_scan(n, lane), all = __builtin_amdgcn_readlane(upto, 63);
         if (place < all) {
             const int at = __builtin_ctzll(__builtin_amdgcn_ballot_w64(upto > place));
             b = c + at;
             tile = __builtin_amdgcn_readlane(upto, at) - 1 - place;
+            first = __builtin_amdgcn_readlane(from, at), rows = __builtin_amdgcn_readlane(count, at);
             return true;
         }
         place -= all;

@@ -230,7 +230,7 @@ def fine():
     ("rows", -1, _ffi.RT_ERR_INVALID_SHAPE), ("kv_rows", -1, _ffi.RT_ERR_INVALID_SHAPE), ("max_rows", -1, _ffi.RT_ERR_INVALID_SHAPE), ("max_keys", -1, _ffi.RT_ERR_INVALID_SHAPE),
     ("causal", 2, _ffi.RT_ERR_INVALID_ARG), ("scale", float("nan"), _ffi.RT_ERR_INVALID_ARG), ("scale", float("inf"), _ffi.RT_ERR_INVALID_ARG),
     ("rows", (1 << 25) + 1, _ffi.RT_ERR_UNSUPPORTED), ("max_keys", (1 << 30) + 1, _ffi.RT_ERR_UNSUPPORTED), ("batch", 65536, _ffi.RT_ERR_UNSUPPORTED),
-    ("heads", 1 << 29, _ffi.RT_ERR_UNSUPPORTED),
+    ("heads", 1 << 29, _ffi.RT_ERR_UNSUPPORTED), ("heads", (1 << 20) + 2, _ffi.RT_ERR_UNSUPPORTED),
 ])
 def test_refusals(field, value, status):
     L, d, need = _ffi.lib(), fine(), ctypes.c_uint64()
