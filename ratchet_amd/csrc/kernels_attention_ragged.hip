@@ -13,7 +13,7 @@
 //     LDS (ds_read_b64_tr_b16).
 // Which tile of which sequence a workgroup has it finds out by itself (rg_locate): the host knows no lengths.
 //
-// Prompts of 4096 to 1792 rows, 32 heads on 8 of 128, causal, 308 GFLOP: 360 us, 856 TFLOP/s, at 1.9 GHz, which is what the package's power leaves (the library's product of 8192^3 1140).  Matrix
+// Prompts of 4096 to 1792 rows, 32 heads on 8 of 128, causal, 308 GFLOP: 365 us, 843 TFLOP/s, at 1.9 GHz, which is what the package's power leaves (the library's product of 8192^3 1140).  Matrix
 // instructions run 41 % of the cycles, vector ones 36 %; the rest are waits for LDS and of two wavefronts for one unit.  Without its loads the kernel takes 16 % less, which is
 // not their latency (with half a step more for the values, and a second barrier, it took 2 % more), without its exponentials 4 %.
 // Scores of the next block beside this block's probabilities, so that both units work for one wavefront, need 64 registers more, and with them in scratch or remade took 6 to 20 % longer.
