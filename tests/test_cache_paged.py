@@ -278,6 +278,23 @@ def test_hidden_keys_have_no_effect(device, rows, d):
 
 
 @gpu
+@pytest.mark.parametrize("rows", [1, 7, 50])
+def test_pages_that_sequences_share(device, rows):
+    """A prefix that two sequences have in common, and a page twice in one sequence: each sees what its own row of the table names."""
+    c = Paged(11, [200, 150], 2, 64, 16)
+    c.table[1, :5] = c.table[0, :5]
+    c.table[1, 7] = c.table[1, 6]
+    pages = [c.table[i, : (n + 15) // 16].long() for i, n in enumerate(c.lens)]
+    k, v = ([pool[p].transpose(1, 2).reshape(-1, 2, 64)[:n] for p, n in zip(pages, c.lens)] for pool in (c.k_pool, c.v_pool))
+    q = torch.randn((2 * rows, 4, 64), generator=torch.Generator().manual_seed(1)).half()
+    want, tol = reference(q, k, v, [rows, rows], c.lens, 0.125, True)
+    k_pool, v_pool, table, lens = c.on_gpu()
+    out = torch.empty(q.shape, dtype=torch.float16, device="cuda")
+    attend_paged(device, paged_desc(c.cache, 4, 2 * rows, rows, c.width * 16, True, 0.125), q.cuda(), k_pool, v_pool, table, lens, None, out)
+    close(out, want, tol)
+
+
+@gpu
 def test_no_pages_and_no_table(device):
     q = torch.randn((3, 2, 64)).half().cuda()
     for pages, width in ((0, 4), (4, 0)):
