@@ -2,7 +2,7 @@
 //
 //   out[m] = sum_j p_j v_j,  p = softmax_j(scale * q[m] . k_j);  row m = query row * group + head of the group
 //
-// What has to be done is to read the pages once, so the kernel is laid out around the loads: each of a workgroup's four wavefronts takes 32 keys of 128 in turn, brings
+// What has to be done is to read the pages once, so the kernel is laid out around the loads: each of a workgroup's four (or eight) wavefronts takes 32 keys of 128 in turn, brings
 // them into a part of LDS of its own, straight from memory, and waits for nobody else.  There is one block of keys and one of values: a wavefront asks for its next keys as soon as
 // the scores are made, and for the values behind them when those are multiplied, so that 8 to 16 KB a wavefront are on their way at any time.
 //   S^T = K Q^T and O^T += V^T P^T by v_mfma_f32_16x16x32_f16, as in kernels_attention_ragged.hip: a lane has four keys of 16 for one row, its probabilities are an operand as
@@ -11,7 +11,7 @@
 // What it has of one that others share goes to the workspace, at most twice, and a second kernel joins the parts in a fixed order.  Lengths stay on the device.
 //
 // 32 sequences of up to 8192 keys, 8 heads of 128, one row of 32 heads, 684 MB: 110 us, 6.2 TB/s, as a copy of this kernel that only loads takes, and 4.7 in the join.  Small ones wait: 100 keys of
-// 32 heads of 80 6.2 us, in a launch, three trips to memory one after another (lengths, pages, keys) and one step; 1024 keys 6.8 and 3.4 in the join.
+// 32 heads of 80 5.8 us, in a launch, three trips to memory one after another (lengths, pages, keys) and one step; 1024 keys 6.8 and 3.4 in the join.
 #include "ragged.h"
 
 #include <algorithm>
@@ -55,15 +55,15 @@ __device__ __forceinline__ PagedSeq ps_seq(const RaggedArgs &g, int b) {
 __device__ __forceinline__ int ps_begin(int64_t i, int64_t total, int wgs) { return (int)(i * total / wgs); }
 __device__ __forceinline__ int ps_owner(int64_t c, int64_t total, int wgs) { return (int)(((c + 1) * wgs + total - 1) / total) - 1; }
 
-// KS: steps of 16 over head_dim (the last may be half).  NR: tiles of 16 rows
-template <int KS, int NR> __global__ __launch_bounds__(256, 2) void attention_paged_stream_kernel(RaggedArgs g, int whole) {
+// KS: steps of 16 over head_dim (the last may be half).  NR: tiles of 16 rows.  NW: wavefronts; eight only with a head of keys each
+template <int KS, int NR, int NW> __global__ __launch_bounds__(64 * NW, 2) void attention_paged_stream_kernel(RaggedArgs g, int whole) {
     constexpr int P = ps_pitch(KS), CPR = P / 8, KK = KS / 2, ODD = KS & 1, RPI = 64 / CPR, NI = PS_UNIT / RPI, NC = NI / 2; // (rows of a load instruction; instructions of a block, of 16 rows)
     constexpr int BLK = PS_UNIT * P; // halves of a block of keys, of values
     extern __shared__ __attribute__((aligned(16))) uint8_t smem[];
     const int t = threadIdx.x, lane = t & 63, wave = __builtin_amdgcn_readfirstlane(t >> 6);
     const int fr = lane & 15, fg = lane >> 4;
     half_t *const mine = (half_t *)(smem + wave * ps_ring(KS));  // this wavefront's [keys | values][32][P]
-    float *const sums = (float *)(smem + 4 * ps_ring(KS));       // [wavefront][row][2]
+    float *const sums = (float *)(smem + NW * ps_ring(KS));       // [wavefront][row][2]
 
     // ---- where this workgroup begins and ends
     int b = 0, kh = 0, step = 0, todo, wgs = 0;
@@ -212,8 +212,9 @@ template <int KS, int NR> __global__ __launch_bounds__(256, 2) void attention_pa
                 for (int k = 0; k < KK; k++) fq[u][k] = 32 * k + 8 * fg < g.D ? *(const half8_t *)(q + 32 * k + 8 * fg) : half8_t{};
                 if constexpr (ODD) ft[u] = 32 * KK + 4 * fg < g.D ? *(const half4_t *)(q + 32 * KK + 4 * fg) : half4_t{};
             }
-            bool more = j + PS_KEYS < j_end;
-            if (more) look(j + PS_KEYS);
+            constexpr int NEXT = NW * PS_UNIT; // keys to this wavefront's next
+            bool more = j + NEXT < j_end;
+            if (more) look(j + NEXT);
             if (g.sign != 1.f) {
                 const half_t sign = (half_t)g.sign;
 #pragma unroll
@@ -342,13 +343,13 @@ template <int KS, int NR> __global__ __launch_bounds__(256, 2) void attention_pa
                 __builtin_amdgcn_s_waitcnt(0xC07F); // lgkmcnt(0): the values have been read
                 asm volatile("" ::: "memory");
                 issue(V, lds0 + 2 * BLK);
-                j += PS_KEYS;
-                more = j + PS_KEYS < j_end;
-                if (more) look(j + PS_KEYS);
+                j += NEXT;
+                more = j + NEXT < j_end;
+                if (more) look(j + NEXT);
                 wait(But{}); // the keys
             }
         }
-        // ---- the four wavefronts' results: outputs where their blocks were, [tile][dimensions' tile][lane] four, references and sums
+        // ---- the wavefronts' results: outputs where their blocks were, [tile][dimensions' tile][lane] four, references and sums
         float4_t *const rest = (float4_t *)mine;
 #pragma unroll
         for (int u = 0; u < NR; u++) {
@@ -360,18 +361,21 @@ template <int KS, int NR> __global__ __launch_bounds__(256, 2) void attention_pa
         __syncthreads();
         const bool parted = step > 0 || upto < all; // others have the rest
         const int64_t slot = 2 * (int64_t)blockIdx.x + (begun ? 1 : 0);
-        for (int e = t; e < NR * KS * 64; e += 256) {
+        for (int e = t; e < NR * KS * 64; e += 64 * NW) {
             const int l = e & 63, ud = e >> 6, u = ud / KS, d = ud - u * KS, m = 16 * u + (l & 15), x = 16 * d + 4 * (l >> 4);
             if (m >= rows || x >= g.D) continue;
-            float2_t ml[4];
-            float4_t o[4];
+            float2_t ml[NW];
+            float4_t o[NW];
 #pragma unroll
-            for (int w = 0; w < 4; w++) ml[w] = *(const float2_t *)(sums + 2 * (w * 16 * NR + m)), o[w] = *(const float4_t *)(smem + w * ps_ring(KS) + 16 * e);
-            const float top = fmaxf(fmaxf(ml[0][0], ml[1][0]), fmaxf(ml[2][0], ml[3][0])), base = top == -INFINITY ? 0.f : top;
+            for (int w = 0; w < NW; w++) ml[w] = *(const float2_t *)(sums + 2 * (w * 16 * NR + m)), o[w] = *(const float4_t *)(smem + w * ps_ring(KS) + 16 * e);
+            float top = ml[0][0];
+#pragma unroll
+            for (int w = 1; w < NW; w++) top = fmaxf(top, ml[w][0]);
+            const float base = top == -INFINITY ? 0.f : top;
             float4_t y = {0.f, 0.f, 0.f, 0.f};
             float s = 0.f;
 #pragma unroll
-            for (int w = 0; w < 4; w++) {
+            for (int w = 0; w < NW; w++) {
                 const float a = __builtin_amdgcn_exp2f(ml[w][0] - base);
                 s = fmaf(ml[w][1], a, s);
 #pragma unroll
@@ -473,9 +477,9 @@ static PagedPlan ps_plan(const rt_attention_paged_desc &d) {
     const int64_t per = (int64_t)d.max_rows * (d.heads / c.kv_heads), heads = (int64_t)c.batch * c.kv_heads, steps = std::max(1, (d.max_keys + PS_KEYS - 1) / PS_KEYS);
     PagedPlan p{};
     p.streams = per <= 32 && heads <= 0xffffff && heads * steps < (int64_t(1) << 31) && heads * per < (int64_t(1) << 24);
-    // A workgroup takes 6.2 us over a head of 100 keys and 1.1 more for each step, the join's launch 3.3 and more: few steps, or many heads, which keep the memory busy by themselves, are faster
-    // without equal parts (us, in equal parts and a head each: 32 heads of 80, 8 steps 9.6 and 12.2; 96 of 96, 8 / 16 steps 15.6 / 19.2 and 13.3 / 21.9; 128 of 128 17.7 / 25.0 and 16.8 / 28.6; 256 of
-    // 128, 16 / 32 steps 39.6 / 66.2 and 36.1 / 67.6; 1024, 8 steps 71 and 60).
+    // A workgroup takes 5.8 us over a head of 100 keys and 0.8 more for each step, the join's launch 3.3 and more: few steps, or many heads, which keep the memory busy by themselves, are faster
+    // without equal parts (us, in equal parts and a head each: 32 heads of 80, 8 steps 10.0 and 11.4; 96 of 96, 8 steps 15.6 and 13.1; 96 of 128, 12 steps 18.5 and 20.1; 128 of 128, 16 steps 24.1 and
+    // 26.5; 256 of 128, 16 / 32 steps 39.6 / 67.7 and 35.0 / 66.6; 1024, 8 steps 71 and 60).
     p.whole = steps <= std::max<int64_t>(4, heads / 12);
     // Two workgroups to a compute unit where there is work for them: 32 x 8 heads, 16 steps; below, one, and half as many parts to join (96 heads of 96, 16 steps, 21.0 us with 512, 19.2 with 256).
     p.wgs = (int)std::min<int64_t>(heads * steps < 2048 ? 256 : 512, heads * steps);
@@ -493,10 +497,10 @@ uint64_t attention_paged_workspace_bytes(const rt_attention_paged_desc &d) {
     return p.whole ? 0 : (uint64_t)2 * p.wgs * d.max_rows * (d.heads / d.cache.kv_heads) * (d.cache.head_dim + 2) * sizeof(float) + (uint64_t)2 * d.cache.batch * d.cache.kv_heads * sizeof(int32_t);
 }
 
-template <int KS, int NR> static hipError_t launch_ps(const RaggedArgs &g, int whole, unsigned wgs, hipStream_t st) {
-    constexpr size_t lds = 4 * ps_ring(KS) + 4 * 16 * NR * 2 * sizeof(float);
-    if (const hipError_t e = ensure_lds_limit<&attention_paged_stream_kernel<KS, NR>>(); e != hipSuccess) return e;
-    hipLaunchKernelGGL((attention_paged_stream_kernel<KS, NR>), dim3(wgs), dim3(256), lds, st, g, whole);
+template <int KS, int NR, int NW> static hipError_t launch_ps(const RaggedArgs &g, int whole, unsigned wgs, hipStream_t st) {
+    constexpr size_t lds = NW * ps_ring(KS) + NW * 16 * NR * 2 * sizeof(float);
+    if (const hipError_t e = ensure_lds_limit<&attention_paged_stream_kernel<KS, NR, NW>>(); e != hipSuccess) return e;
+    hipLaunchKernelGGL((attention_paged_stream_kernel<KS, NR, NW>), dim3(wgs), dim3(64 * NW), lds, st, g, whole);
     return hipGetLastError();
 }
 
@@ -523,7 +527,11 @@ hipError_t launch_attention_paged(const rt_attention_paged_desc &d, const void *
     const unsigned wgs = p.whole ? (unsigned)(c.batch * c.kv_heads) : (unsigned)p.wgs;
     auto go = [&](auto ks) -> hipError_t {
         constexpr int KS = decltype(ks)::value;
-        return per <= 16 ? launch_ps<KS, 1>(g, p.whole, wgs, stream) : launch_ps<KS, 2>(g, p.whole, wgs, stream);
+        // Eight wavefronts, 133 KB of LDS, where a head of keys is a workgroup's, each has a compute unit and more than one step: half as many steps follow each other (us, with four and with eight:
+        // 32 heads of 80, 512 keys 9.0 and 8.4; 96 of 96, 7 rows, 300 keys 8.2 and 7.5, 1000 keys 13.5 and 13.1; 256 of 128, 1024 keys 19.5 and 19.0).  One step leaves four of them idle (5.8 and 6.0),
+        // and more heads than compute units do better with two workgroups of four to each (512 heads of 128, 300 keys 14.1 and 16.5; 1024, 1000 keys 62.1 and 67.3).
+        if (p.whole && wgs <= 256 && g.max_keys > PS_KEYS) return per <= 16 ? launch_ps<KS, 1, 8>(g, 1, wgs, stream) : launch_ps<KS, 2, 8>(g, 1, wgs, stream);
+        return per <= 16 ? launch_ps<KS, 1, 4>(g, p.whole, wgs, stream) : launch_ps<KS, 2, 4>(g, p.whole, wgs, stream);
     };
     hipError_t e;
     switch ((g.D + 15) / 16) {

@@ -167,6 +167,16 @@ def test_more_rows_than_keys(device, rows):
 
 
 @gpu
+@pytest.mark.parametrize("d", [8, 24, 40, 64, 72, 88, 104, 128])
+@pytest.mark.parametrize("rows", [1, 5])
+@pytest.mark.parametrize("lens", [[129, 255, 256, 257, 0, 1, 500, 512], [160, 288, 511] * 40], ids=["few", "many"])
+def test_a_few_steps(device, rows, d, lens):
+    """Heads of keys of two to four steps, fewer and more of them than there are compute units."""
+    attend(device, rows + d, [min(rows, x) for x in lens], lens, 12, 3, d, 16)
+    attend(device, rows + d, [min(rows, x) for x in lens], lens, 12, 3, d, 16, causal=False, hidden={(0, 3), (2, 15), (3, 2)})
+
+
+@gpu
 @pytest.mark.parametrize("rows,lens", [(1, [9000]), (1, [20000, 5, 3000]), (6, [9001]), (40, [9000, 100]), (200, [3000])])
 @pytest.mark.parametrize("workspace", [True, False])
 def test_long_sequences(device, rows, lens, workspace):
