@@ -445,7 +445,7 @@ class Sequences:
       starts    [batch + 1]: sequence b has the rows starts[b] .. starts[b + 1] - 1 (None: max_rows each)
       max_rows  no sequence has more rows
       lens      [batch]: keys of each sequence, the rows' own among them (a cache in pages)
-      table     [batch, width]: the page of each page_size positions; another number than a page's where there is none
+      table     [batch, width]: the page of each page_size positions; another number than a page's where there is none.  Rows may lie further apart than width, not closer
       max_keys  no sequence has more keys (default: what the table holds; without a table max_rows)"""
 
     def __init__(self, batch: int, starts=None, max_rows: int = 1, lens=None, table=None, max_keys: Optional[int] = None):
@@ -463,12 +463,14 @@ class Sequences:
         t, torch = self.table, _torch()
         if t.dtype != torch.int32 or t.dim() != 2 or t.shape[0] != self.batch or t.device != device.torch_device() or (t.numel() and t.stride(1) != 1):
             raise OperationError(_ffi.RT_ERR_INVALID_ARG, f"table: an int32 tensor [{self.batch}, width] on the cache's device, entries side by side")
+        if self.batch > 1 and t.stride(0) < t.shape[1]:   # expanded, or windows of one line
+            raise OperationError(_ffi.RT_ERR_INVALID_ARG, f"table: rows that do not overlap, {t.shape[1]} entries each, got rows {t.stride(0)} apart (contiguous() makes a copy)")
 
     def cache_desc(self, pool: "Tensor"):
         c = _ffi.PagedCacheDesc()
         c.pages, c.kv_heads, c.page_size, c.head_dim = _i32(*pool.shape)
         c.batch, c.table_width = self.batch, _i32(self.table.shape[1])[0]
-        c.table_stride = max(int(self.table.stride(0)), c.table_width) if self.batch > 1 else c.table_width
+        c.table_stride = int(self.table.stride(0)) if self.batch > 1 else c.table_width
         return c
 
 
