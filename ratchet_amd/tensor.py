@@ -453,6 +453,12 @@ class Sequences:
         self.starts, self.lens, self.table = starts, lens, table
         self.max_keys = None if max_keys is None else _i32(max_keys)[0]
 
+    def __setattr__(self, name, value):
+        """Once: an operator checks the tensors when it is made and reads them when it runs."""
+        if name in self.__dict__:
+            raise AttributeError(f"{name}: sequences stay as they were made (what their tensors hold may change)")
+        object.__setattr__(self, name, value)
+
     def check(self, device: "Device", paged: bool):
         _lengths(self.starts, self.batch + 1, device, "starts")
         if not paged:

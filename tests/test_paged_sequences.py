@@ -56,3 +56,15 @@ def test_one_sequence_has_a_row_of_any_stride():
     for table in (ints(0, 1, 2, 3)[None].expand(1, 4), torch.zeros((1, 4), dtype=torch.int32).as_strided((1, 4), (1, 1))):
         desc = zeros(4, 512).attention_paged(pool, pool, Sequences(1, ints(0, 4), 4, ints(5), table)).op.desc.cache
         assert (desc.table_width, desc.table_stride) == (4, 4)
+
+
+@pytest.mark.parametrize("name,value", [("lens", ints(5)), ("starts", ints(0)), ("table", torch.zeros((1, 1), dtype=torch.int32)), ("batch", 9), ("max_rows", 4), ("max_keys", 64)])
+def test_sequences_stay_as_they_were_made(name, value):
+    """An operator checks the tensors when it is made and reads them when it runs: another, shorter one in between would be read past its end."""
+    seqs = Sequences(2, ints(0, 3, 4), 3, ints(5, 6), torch.zeros((2, 4), dtype=torch.int32))
+    kept = getattr(seqs, name)
+    with pytest.raises(AttributeError):
+        setattr(seqs, name, value)
+    assert getattr(seqs, name) is kept
+    seqs.lens.copy_(ints(7, 8))      # what they hold may change
+    assert seqs.lens.tolist() == [7, 8]
