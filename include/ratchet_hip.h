@@ -593,10 +593,10 @@ RT_API rt_status rt_cache_write_paged_enqueue(rt_ctx *ctx, const rt_paged_cache_
 
 /* Attention over the pages: out = softmax(scale * q k^T) v for the packed query rows, F16, of every sequence.  Head h reads the pools'
  * head h / (heads / kv_heads).
- *   lens      keys of each sequence, taken between 0 and max_keys
+ *   lens      keys of each sequence; none where it is below 0
  *   causal    row i of the n rows of a sequence sees the keys up to position lens[b] - n + i; without it all of the sequence's
- *   max_rows  no sequence has more rows than this: rows past it are left as they were.  starts == NULL: each has so many
- *   max_keys  likewise for the keys; at most table_width * page_size
+ *   max_rows  a sequence's rows past this many are left as they were; those before them see what they see without the bound.  starts == NULL: each has so many
+ *   max_keys  a sequence's keys past this many are seen by no row; at most table_width * page_size
  * A row that sees no key is NaN, as in rt_attention_enqueue.  Keys that a row does not see, and what lies in pages behind a sequence's keys, have no effect on
  * it, whatever they hold; a row that sees a value that is not finite is not finite in that dimension.
  * Sums, references and scores are f32; the probabilities enter the second product as f16.
@@ -623,7 +623,8 @@ RT_API rt_status rt_attention_paged_enqueue(rt_ctx *ctx, const rt_attention_page
 
 /* Attention of packed prompts: keys and values are packed rows too, [kv_rows, kv_heads, head_dim], those of sequence b at kv_starts[b] ..
  * kv_starts[b + 1] - 1; kv_starts == NULL: where its query rows are (kv_rows == rows), each prompt seeing itself.  q, k and v may be parts of one fused
- * projection's output.  All else as rt_attention_paged_enqueue; with the causal flag row i of n sees the first (keys - n + i + 1) keys.
+ * projection's output.  All else as rt_attention_paged_enqueue; with the causal flag row i of n sees the first (keys - n + i + 1) keys, n and keys as starts and kv_starts
+ * have them, of which those past max_keys and behind the tensor are not there.
  * Strides of keys and values are at most 2^24 elements (RT_ERR_UNSUPPORTED beyond). */
 typedef struct rt_attention_packed_desc {
     int32_t batch, heads, kv_heads;

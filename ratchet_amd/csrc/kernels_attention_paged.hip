@@ -40,12 +40,14 @@ template <int PITCH> __device__ __forceinline__ int ps_swizzle(int r) {
 // Steps of a sequence (at least one where it has rows: they are NaN), and of all up to a sequence.
 struct PagedSeq {
     int first, rows, keys, steps;
+    int off; // causal: row i sees keys up to i + off
 };
 __device__ __forceinline__ PagedSeq ps_seq(const RaggedArgs &g, int b) {
     PagedSeq s;
-    int unused;
+    int unused, all;
     const int at = min(b, g.batch - 1);
-    s.rows = rg_rows(g, at, s.first), s.keys = rg_keys<true>(g, at, unused);
+    s.rows = rg_rows(g, at, s.first), s.keys = rg_keys<true>(g, at, unused, all);
+    s.off = all - rg_all_rows(g, at, s.first);
     s.steps = b < g.batch && s.rows > 0 ? max(1, (s.keys + PS_KEYS - 1) / PS_KEYS) : 0;
     return s;
 }
@@ -70,7 +72,8 @@ template <int KS, int NR, int NW> __global__ __launch_bounds__(64 * NW, 2) void 
     int64_t total = 0, from = 0; // places in the line; that of this head of keys' first step
     PagedSeq seq;
     auto of_lane = [&](PagedSeq s, int l) {
-        return PagedSeq{__builtin_amdgcn_readlane(s.first, l), __builtin_amdgcn_readlane(s.rows, l), __builtin_amdgcn_readlane(s.keys, l), __builtin_amdgcn_readlane(s.steps, l)};
+        return PagedSeq{__builtin_amdgcn_readlane(s.first, l), __builtin_amdgcn_readlane(s.rows, l), __builtin_amdgcn_readlane(s.keys, l), __builtin_amdgcn_readlane(s.steps, l),
+                        __builtin_amdgcn_readlane(s.off, l)};
     };
     if (whole) { // a head of keys each
         b = blockIdx.x / g.kv_heads, kh = blockIdx.x - b * g.kv_heads;
@@ -130,7 +133,7 @@ template <int KS, int NR, int NW> __global__ __launch_bounds__(64 * NW, 2) void 
     bool begun = false; // whether this is not the first head of keys of the workgroup
     while (todo > 0) {
         const int first = seq.first, n = seq.rows, len = seq.keys, all = seq.steps;
-        const int upto = min(all, step + todo), rows = n * g.group, off = len - n;
+        const int upto = min(all, step + todo), rows = n * g.group, off = seq.off;
         auto sees = [&](int m) { return g.causal ? max(0, min(len, rg_query(g, m) + off + 1)) : len; };
         const int seen_all = sees(0), seen_any = sees(rows - 1);
 

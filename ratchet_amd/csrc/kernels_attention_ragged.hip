@@ -67,9 +67,10 @@ template <int KS, bool PAGED, int NH> __global__ __launch_bounds__(256 * NH, KS 
     const int line = blockIdx.x / g.kv_heads, kh = blockIdx.x - line * g.kv_heads, place = line / g.splits, share = line - place * g.splits;
     if (!rg_locate<RR_ROWS>(g, place, b, tile, first, n)) return;
     b = __builtin_amdgcn_readfirstlane(b), tile = __builtin_amdgcn_readfirstlane(tile), n = __builtin_amdgcn_readfirstlane(n);
-    const int len = __builtin_amdgcn_readfirstlane(rg_keys<PAGED>(g, b, key0));
+    int all_keys;
+    const int len = __builtin_amdgcn_readfirstlane(rg_keys<PAGED>(g, b, key0, all_keys));
     first = __builtin_amdgcn_readfirstlane(first), key0 = __builtin_amdgcn_readfirstlane(key0);
-    const int rows = n * g.group, off = len - n; // causal: query row i sees keys up to i + off
+    const int rows = n * g.group, off = __builtin_amdgcn_readfirstlane(all_keys - rg_all_rows(g, b, first)); // causal: query row i sees keys up to i + off
     const int row0 = tile * RR_ROWS, rw = row0 + 32 * rg;
     const int q0 = row0 / g.group, over = row0 - q0 * g.group; // (the tile's other query rows are found from its first without a division)
     auto query = [&](int m) { return q0 + rg_query(g, m - row0 + over); };

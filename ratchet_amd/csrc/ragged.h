@@ -39,17 +39,20 @@ __device__ __forceinline__ int rg_rows(const RaggedArgs &g, int b, int &first) {
     first = a;
     return min(e - a, g.max_rows);
 }
-template <bool PAGED> __device__ __forceinline__ int rg_keys(const RaggedArgs &g, int b, int &first) {
+// Rows from `first` (rg_rows) to the sequence's end, those past max_rows or behind the tensor too: by them goes which keys a row sees.
+__device__ __forceinline__ int rg_all_rows(const RaggedArgs &g, int b, int first) { return g.starts ? max(g.starts[b + 1], first) - first : g.max_rows; }
+// First key and number of keys.  `all`: with those past max_keys or behind the tensor.  (all - rg_all_rows + a row + 1 is `all` at most: it fits 31 bits.)
+template <bool PAGED> __device__ __forceinline__ int rg_keys(const RaggedArgs &g, int b, int &first, int &all) {
     if constexpr (PAGED) {
-        first = 0;
-        return min(max(g.lens[b], 0), g.max_keys);
+        first = 0, all = max(g.lens[b], 0);
+        return min(all, g.max_keys);
     } else {
         const int32_t *s = g.kv_starts ? g.kv_starts : g.starts;
         int a = b * g.max_rows, e = a + g.max_rows;
         if (s) a = s[b], e = s[b + 1];
-        a = min(max(a, 0), g.kv_rows), e = min(max(e, a), g.kv_rows);
-        first = a;
-        return min(e - a, g.max_keys);
+        a = min(max(a, 0), g.kv_rows), e = max(e, a);
+        first = a, all = e - a;
+        return min(min(e, g.kv_rows) - a, g.max_keys);
     }
 }
 
