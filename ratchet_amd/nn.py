@@ -73,8 +73,10 @@ class PagedKVCache:
     """A key/value cache whose memory goes to sequences a page at a time (no counterpart in the reference, whose KVEntry reserves the whole capacity,
     kv_cache.rs:3-19): pools [pages, kv_heads, page_size, head_dim] for each layer, and one table for all of them.  `batch` sequences of up to `max_pages` pages.
 
-    A pass over the model: extend(rows) with the new rows of each sequence (a prompt's length, 1 for a step, 0 for none), then the layers with the packed rows.  What
-    the GPU reads (table, lens, starts) stays in the same memory, so that a pass captured into a graph runs on what the last extend() left there."""
+    A pass over the model: extend(rows) with the new rows of each sequence (a prompt's length, 1 for a step, 0 for none), then the layers with the packed rows, resolved
+    before the next extend() or release(): operators of an earlier pass are refused.  What the GPU reads (table, lens, starts) stays in the same memory, so that a pass captured
+    into a graph (resolve(wait=False)) runs on what the last extend() left there: on sequences that have grown to any length, in all of no more rows than the
+    captured tensors have, and none of a sequence more than the longest had there."""
 
     def __init__(self, n_layers: int, shape, device: Device, batch: int, max_pages: int):
         import torch
@@ -84,6 +86,7 @@ class PagedKVCache:
         self.free = list(range(self.pages))[::-1]
         self.owned: List[List[int]] = [[] for _ in range(self.batch)]
         self.entries = [0] * self.batch
+        self.passes = 0   # what has changed the tensors below, so many times
         where = device.torch_device()
         self.table = torch.full((self.batch, self.max_pages), -1, dtype=torch.int32, device=where)
         self.lens = torch.zeros(self.batch, dtype=torch.int32, device=where)
@@ -101,6 +104,7 @@ class PagedKVCache:
         needs = [-(-(n + r) // self.page_size) - len(own) for n, r, own in zip(self.entries, rows, self.owned)]
         if any(len(own) + n > self.max_pages for own, n in zip(self.owned, needs)) or sum(needs) > len(self.free):
             raise OperationError(_ffi.RT_ERR_OOM, f"cache: {sum(needs)} pages wanted, {len(self.free)} free, {self.max_pages} a sequence")
+        self.passes += 1
         for i, (r, n) in enumerate(zip(rows, needs)):
             self.owned[i] += [self.free.pop() for _ in range(n)]
             self.entries[i] += r
@@ -111,10 +115,11 @@ class PagedKVCache:
             at.append(at[-1] + r)
         self.starts.copy_(torch.tensor(at, dtype=torch.int32))
         self.lens.copy_(torch.tensor(self.entries, dtype=torch.int32))
-        return Sequences(self.batch, self.starts, max(rows + [0]), self.lens, self.table, max(self.entries + [0]))
+        return Sequences(self.batch, self.starts, max(rows + [0]), self.lens, self.table, max(self.entries + [0]), self)
 
     def release(self, i: int):
         """Sequence i has ended: its pages are free."""
+        self.passes += 1
         self.free += self.owned[i][::-1]
         self.owned[i], self.entries[i] = [], 0
         self.table[i].fill_(-1)
@@ -138,6 +143,8 @@ class SelfAttention:
         if isinstance(cache, PagedKVEntry):
             if sequences is None:
                 raise OperationError(_ffi.RT_ERR_INVALID_ARG, "attention: a cache in pages needs the pass's sequences")
+            if sequences.cache is not None and sequences.cache is not cache.owner:
+                raise OperationError(_ffi.RT_ERR_INVALID_ARG, "attention: sequences of another cache")
             keys, values = cache.k_pool.cache_write_paged(k, sequences), cache.v_pool.cache_write_paged(v, sequences)
             return self.o.schedule(q.attention_paged(keys, values, sequences))
         if sequences is not None:

@@ -439,19 +439,21 @@ def _i32(*sizes):
 
 class Sequences:
     """Whose rows a packed tensor holds, for the operators on sequences of different lengths: int32 GPU tensors of torch, read when a call runs, so that a
-    captured graph takes what they hold then.
+    captured graph takes what they hold then.  max_rows and max_keys are fixed by then: they have to hold for all of its replays.
 
       batch     sequences
       starts    [batch + 1]: sequence b has the rows starts[b] .. starts[b + 1] - 1 (None: max_rows each)
       max_rows  no sequence has more rows
       lens      [batch]: keys of each sequence, the rows' own among them (a cache in pages)
       table     [batch, width]: the page of each page_size positions; another number than a page's where there is none.  Rows may lie further apart than width, not closer
-      max_keys  no sequence has more keys (default: what the table holds; without a table max_rows)"""
+      max_keys  no sequence has more keys (default: what the table holds; without a table max_rows)
+      cache     the nn.PagedKVCache whose extend() made them: its next pass overwrites the tensors, and operators of this one are refused from then on"""
 
-    def __init__(self, batch: int, starts=None, max_rows: int = 1, lens=None, table=None, max_keys: Optional[int] = None):
+    def __init__(self, batch: int, starts=None, max_rows: int = 1, lens=None, table=None, max_keys: Optional[int] = None, cache=None):
         self.batch, self.max_rows = _i32(batch, max_rows)
         self.starts, self.lens, self.table = starts, lens, table
         self.max_keys = None if max_keys is None else _i32(max_keys)[0]
+        self.cache, self.passes = cache, cache.passes if cache is not None else 0
 
     def __setattr__(self, name, value):
         """Once: an operator checks the tensors when it is made and reads them when it runs."""
@@ -459,7 +461,12 @@ class Sequences:
             raise AttributeError(f"{name}: sequences stay as they were made (what their tensors hold may change)")
         object.__setattr__(self, name, value)
 
+    def check_pass(self):
+        if self.cache is not None and self.cache.passes != self.passes:
+            raise OperationError(_ffi.RT_ERR_INVALID_ARG, "sequences of an earlier pass: extend() or release() of their cache has changed what they hold")
+
     def check(self, device: "Device", paged: bool):
+        self.check_pass()
         _lengths(self.starts, self.batch + 1, device, "starts")
         if not paged:
             return
@@ -515,6 +522,7 @@ class CachePaged:
 
     def _enqueue(self, device, stream, k, ks, v=None, vs=None):
         q = self.seqs
+        q.check_pass()
         st = _ffi.lib().rt_cache_write_paged_enqueue(device.ctx, self.desc, int(self.source.dt), k, ks, v, vs, _strides2(self.width, self.cache.shape[3]), q.table.data_ptr(),
                                                      q.lens.data_ptr(), None if q.starts is None else q.starts.data_ptr(), self.rows, stream)
         _check(st, device)
@@ -557,6 +565,11 @@ class AttentionPaged:
                                                      None if q.starts is None else q.starts.data_ptr(), out, ws, ws_bytes, stream)
 
     def _workspace(self, need):
+        self.seqs.check_pass()
+        if self.seqs.cache is not None and _torch().cuda.is_current_stream_capturing():
+            # a replay runs on what a later extend() leaves: the bound is what a sequence may come to hold
+            self.desc.max_keys = _i32(self.desc.cache.table_width * self.desc.cache.page_size)[0]
+            self.check_invariants()
         return _ffi.lib().rt_attention_paged_workspace_bytes(self.desc, need)
 
 
@@ -597,6 +610,7 @@ class AttentionPacked:
                                                       ws_bytes, stream)
 
     def _workspace(self, need):
+        self.seqs.check_pass()
         return _ffi.lib().rt_attention_packed_workspace_bytes(self.desc, need)
 
 
@@ -870,8 +884,9 @@ class Tensor:
         """tensor.rs `half()`: cast to F16."""
         return self.cast(DType.F16)
 
-    def resolve(self) -> "Tensor":
-        """tensor.rs:738-787: run every unresolved node below this one, then wait."""
+    def resolve(self, wait: bool = True) -> "Tensor":
+        """tensor.rs:738-787: run every unresolved node below this one, then wait.  wait=False leaves the wait out: what torch's current stream does next comes behind, and a
+        stream that is being captured, which cannot be waited for, records the nodes."""
         if self.resolved():
             return self
         dev = self.device
@@ -879,7 +894,8 @@ class Tensor:
             raise OperationError(_ffi.RT_ERR_NO_DEVICE, "resolve() needs a GPU tensor (try_gpu)")
         stream = _stream_ptr()
         self._execute(stream)
-        _check(_ffi.lib().rt_sync(dev.ctx, stream), dev)
+        if wait:
+            _check(_ffi.lib().rt_sync(dev.ctx, stream), dev)
         return self
 
     def _empty(self, nbytes: int):
