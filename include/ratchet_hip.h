@@ -600,6 +600,7 @@ RT_API rt_status rt_cache_write_paged_enqueue(rt_ctx *ctx, const rt_paged_cache_
  * A row that sees no key is NaN, as in rt_attention_enqueue.  Keys that a row does not see, and what lies in pages behind a sequence's keys, have no effect on
  * it, whatever they hold; a row that sees a value that is not finite is not finite in that dimension.
  * Sums, references and scores are f32; the probabilities enter the second product as f16.
+ * |scale| log2(e) is an f32: |scale| up to 2.358e38 (RT_ERR_INVALID_ARG beyond).
  * Limits (RT_ERR_UNSUPPORTED beyond): 2^25 rows, 2^30 keys of a sequence, rows times heads of 2^31 - 256, 2^20 heads, 65535 sequences, 2^23 - 1 tiles of 128 rows of
  * the heads that share a head of keys (a sequence may begin one) times kv_heads.  Up to 32 such rows a sequence run on a kernel that reads the pages at the rate of
  * memory, and more on tiles: a step of one token for some and a prompt for others is faster in two calls. */

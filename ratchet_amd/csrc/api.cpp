@@ -782,7 +782,7 @@ static rt_status ragged_validate(int32_t batch, int32_t heads, int32_t kv_heads,
         if (q_strides[j] > (int64_t(1) << 31) || o_strides[j] > (int64_t(1) << 31)) return RT_ERR_UNSUPPORTED;
     }
     if (causal != 0 && causal != 1) return RT_ERR_INVALID_ARG;
-    if (!(std::fabs(scale) <= 3.4e38f)) return RT_ERR_INVALID_ARG;
+    if (!std::isfinite(std::fabs(scale) * 1.4426950408889634f)) return RT_ERR_INVALID_ARG; // (the kernels' scale: that and log2(e) in f32)
     if (batch > 65535 || heads > (1 << 20) || rows > (1 << 25) || max_keys > (1 << 30) || (int64_t)rows * heads > (int64_t(1) << 31) - 256) return RT_ERR_UNSUPPORTED; // (rounded up to tiles they are 31 bits)
     return RT_OK;
 }
