@@ -180,3 +180,31 @@ def test_a_pass_run_too_late_is_refused(device, then):
     torch.cuda.synchronize()
     assert not bool(c[0].k_pool.storage.any()) and not bool(c[0].v_pool.storage.any())
     assert q0.shape[0] == 4
+
+
+@gpu
+@pytest.mark.parametrize("k_type,v_type", [(np.float32, np.float32), (np.float32, np.float16), (np.float16, np.float32)])
+def test_writes_of_f32_rows(device, k_type, v_type):
+    """Keys and values of either type, in one launch where they are of one: the rows rounded to f16, bit for bit, and what the attention then reads."""
+    kv, d, ps = 2, 64, 16
+    c = nn.PagedKVCache(1, (6, kv, ps, d), device, 2, 4)
+    rng = np.random.default_rng(3)
+    for n in ([20, 3], [1, 14]):
+        seqs = c.extend(n)
+        k, v = ((rng.standard_normal((sum(n), kv * d)) * 3).astype(t) for t in (k_type, v_type))
+        q = rng.standard_normal((sum(n), kv * d)).astype(np.float16)
+        K, V, Q = (Tensor.from_data(x).to(device) for x in (k, v, q))
+        before = [p.to(CPU).storage.copy() for p in (c[0].k_pool, c[0].v_pool)]
+        out = Q.attention_paged(c[0].k_pool.cache_write_paged(K, seqs), c[0].v_pool.cache_write_paged(V, seqs), seqs).resolve()
+        table, want, at = c.table.cpu().numpy(), before, 0
+        for i, r in enumerate(n):
+            for j in range(r):
+                p = c.entries[i] - r + j
+                for pool, x in zip(want, (k, v)):
+                    pool[table[i, p // ps], :, p % ps] = x[at + j].astype(np.float16).reshape(kv, d)
+            at += r
+        for pool, x in zip((c[0].k_pool, c[0].v_pool), want):
+            assert np.array_equal(pool.to(CPU).storage.view(np.uint16), x.view(np.uint16))
+        held = [[torch.from_numpy(x[table[i, : -(-m // ps)]].transpose(0, 2, 1, 3).reshape(-1, kv, d)[:m].copy()) for i, m in enumerate(c.entries)] for x in want]
+        exact = reference(torch.from_numpy(q).view(-1, kv, d), *held, n, c.entries, d ** -0.5, True)
+        close(values_of(out, (sum(n), kv, d)), *exact)

@@ -69,3 +69,18 @@ def test_packed(device, n, lens, max_rows, max_keys, rows, kv_rows, causal):
     kv_starts = None if lens is None and rows == kv_rows else starts_of(keys).cuda()
     attend_packed(device, packed_desc(len(n), 4, 2, 64, rows, kv_rows, max_rows, max_keys, causal, 0.125), q[:rows].cuda(), k[:kv_rows].cuda(), v[:kv_rows].cuda(), starts_of(n).cuda(), kv_starts, out)
     compare(out, want, tol, kept_rows(n, max_rows, rows), (n, keys))
+
+
+@gpu
+@pytest.mark.parametrize("heads,kv", [(32, 1), (33, 1), (40, 1), (64, 1), (71, 1), (130, 2), (129, 1)])
+@pytest.mark.parametrize("lens", [[1], [37, 128, 0, 129], [3000, 5], [600] * 30], ids=lambda x: f"{len(x)}x{max(x)}")
+def test_one_row_of_many_heads_on_one(device, heads, kv, lens):
+    """A token of more than 32 heads that share their keys: on both sides of the border between the kernels, and of a tile's."""
+    c = Paged(heads, lens, kv, 64, 16)
+    q = torch.randn((len(lens), heads, 64), generator=torch.Generator().manual_seed(2)).half()
+    want, tol = reference(q, c.k, c.v, [1] * len(lens), lens, 0.125, True)
+    k_pool, v_pool, table, on_lens = c.on_gpu()
+    for starts in (None, starts_of([1] * len(lens)).cuda()):
+        out = torch.full(q.shape, 7.0, dtype=torch.float16, device="cuda")
+        attend_paged(device, paged_desc(c.cache, heads, len(lens), 1, c.width * 16, True, 0.125), q.cuda(), k_pool, v_pool, table, on_lens, starts, out)
+        close(out, want, tol, (heads, kv, lens))
