@@ -848,7 +848,7 @@ rt_status rt_attention_paged_enqueue(rt_ctx *ctx, const rt_attention_paged_desc 
         return fail(ctx, RT_ERR_INVALID_ARG, "attention: out, table, lens and starts must be aligned to their types");
     DeviceGuard dg(ctx->dev.ordinal);
     if (!dg.ok) return fail(ctx, RT_ERR_NO_DEVICE, "hipSetDevice failed");
-    hipError_t e = rt::launch_attention_paged(*desc, q, k_pool, v_pool, table, lens, starts, out, workspace, workspace_bytes, (hipStream_t)stream, ctx->dev);
+    hipError_t e = rt::launch_attention_paged(*desc, q, k_pool, v_pool, table, lens, starts, out, workspace, workspace_bytes, (hipStream_t)stream);
     if (e != hipSuccess) return hip_fail(ctx, "attention launch", e);
     return RT_OK;
     RT_GUARD_END(ctx)
@@ -863,7 +863,7 @@ rt_status rt_attention_packed_validate(const rt_attention_packed_desc *d) {
     for (int i = 0; i < 2; i++)
         for (int j = 0; j < 2; j++) {
             if (strides[i][j] < 0) return RT_ERR_INVALID_SHAPE;
-            if (strides[i][j] % 8 || strides[i][j] > (int64_t(1) << 24)) return RT_ERR_UNSUPPORTED; // offsets within 64 rows are 32 bits
+            if (strides[i][j] % 8 || strides[i][j] > (int64_t(1) << 24)) return RT_ERR_UNSUPPORTED; // offsets within the 128 rows of a step are 32 bits
         }
     return rt::attention_packed_fits(*d) ? RT_OK : RT_ERR_UNSUPPORTED;
 }
@@ -892,7 +892,7 @@ rt_status rt_attention_packed_enqueue(rt_ctx *ctx, const rt_attention_packed_des
         return fail(ctx, RT_ERR_INVALID_ARG, "attention: out, starts and kv_starts must be aligned to their types");
     DeviceGuard dg(ctx->dev.ordinal);
     if (!dg.ok) return fail(ctx, RT_ERR_NO_DEVICE, "hipSetDevice failed");
-    hipError_t e = rt::launch_attention_packed(*desc, q, k, v, starts, kv_starts, out, workspace, workspace_bytes, (hipStream_t)stream, ctx->dev);
+    hipError_t e = rt::launch_attention_packed(*desc, q, k, v, starts, kv_starts, out, workspace, workspace_bytes, (hipStream_t)stream);
     if (e != hipSuccess) return hip_fail(ctx, "attention launch", e);
     return RT_OK;
     RT_GUARD_END(ctx)

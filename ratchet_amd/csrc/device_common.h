@@ -286,11 +286,11 @@ hipError_t launch_cache_write_paged(const rt_paged_cache_desc &d, int src_dtype,
 bool attention_paged_fits(const rt_attention_paged_desc &d);
 uint64_t attention_paged_workspace_bytes(const rt_attention_paged_desc &d);
 hipError_t launch_attention_paged(const rt_attention_paged_desc &d, const void *q, const void *k_pool, const void *v_pool, const int32_t *table, const int32_t *lens,
-                                  const int32_t *starts, void *out, void *workspace, uint64_t workspace_bytes, hipStream_t stream, const DeviceInfo &dev);
+                                  const int32_t *starts, void *out, void *workspace, uint64_t workspace_bytes, hipStream_t stream);
 bool attention_packed_fits(const rt_attention_packed_desc &d);
 uint64_t attention_packed_workspace_bytes(const rt_attention_packed_desc &d);
 hipError_t launch_attention_packed(const rt_attention_packed_desc &d, const void *q, const void *k, const void *v, const int32_t *starts, const int32_t *kv_starts,
-                                   void *out, void *workspace, uint64_t workspace_bytes, hipStream_t stream, const DeviceInfo &dev);
+                                   void *out, void *workspace, uint64_t workspace_bytes, hipStream_t stream);
 hipError_t launch_softmax(int dtype, void *x, int64_t rows, int64_t n, hipStream_t stream);
 hipError_t launch_attention(const rt_attention_desc &d, const void *q, const void *k, const void *v, const void *mask,
                             void *out, void *workspace, uint64_t workspace_bytes, hipStream_t stream, const DeviceInfo &dev);

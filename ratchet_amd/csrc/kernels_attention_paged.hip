@@ -237,7 +237,9 @@ template <int KS, int NR, int NW> __global__ __launch_bounds__(64 * NW, 2) void 
             wait(But{});
             while (true) {
                 // ---- scores
-                float4_t S[NR][2], tail[NR][2]; // (tail: a sum of its own.  As the third operand of the shorter instruction right behind the longer one that makes it, S came out wrong)
+                // tail: a sum of its own.  With S as the third operand of the shorter instruction, heads of 72, 80 and 112 gave wrong scores: the compiler puts the two behind each other without a
+                // wait, as it does (rightly) for two of one kind, and v_mfma_f32_16x16x32 seems not to hand its result on to an instruction of another length.  No other kernel here chains two kinds.
+                float4_t S[NR][2], tail[NR][2];
 #pragma unroll
                 for (int u = 0; u < NR; u++) S[u][0] = S[u][1] = float4_t{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
@@ -470,7 +472,8 @@ __global__ __launch_bounds__(256) void attention_paged_join_kernel(RaggedArgs g)
     }
 }
 
-// How a call is run: on the kernels above where a head of keys has up to 32 rows, and then a head of keys a workgroup, or all in equal parts.
+// How a call is run: on the kernels above where a head of keys has up to 32 rows, and then a head of keys a workgroup, or all in equal parts.  (8 sequences of 4096 keys, heads of 128, 32 and
+// 33 of such rows: one row of as many heads on one of keys 13.9 and 18.2 us, and of 32 heads on 8, 8 and 9 rows, 33.5 and 33.3.)
 struct PagedPlan {
     bool streams, whole;
     int wgs;
@@ -508,7 +511,7 @@ template <int KS, int NR, int NW> static hipError_t launch_ps(const RaggedArgs &
 }
 
 hipError_t launch_attention_paged(const rt_attention_paged_desc &d, const void *q, const void *k_pool, const void *v_pool, const int32_t *table, const int32_t *lens,
-                                  const int32_t *starts, void *out, void *workspace, uint64_t workspace_bytes, hipStream_t stream, const DeviceInfo &dev) {
+                                  const int32_t *starts, void *out, void *workspace, uint64_t workspace_bytes, hipStream_t stream) {
     RaggedArgs g{};
     const rt_paged_cache_desc &c = d.cache;
     g.Q = (const half_t *)q, g.K = (const half_t *)k_pool, g.V = (const half_t *)v_pool, g.O = (half_t *)out, g.starts = starts, g.table = table, g.lens = lens;

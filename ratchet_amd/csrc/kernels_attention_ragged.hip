@@ -454,6 +454,7 @@ struct RaggedPlan {
 // on each are faster (us, four and eight: 2048 rows of 24 heads of 96, 384 tiles, 48.8 and 41.7; without the flag, 4 x 1500 rows of six heads of 64, 288 tiles, 36.7 and 43.8), as
 // they are where there is no second workgroup (512 rows on 4096 keys, 32 heads on 8 of 128, 208 tiles, 88.4 and 81.5).  Short ones do not pay for the join of the halves (24 prompts of up to
 // 100 rows 8.6 and 9.6).
+// (256 compute units are the card's; the workspace is asked for without a device to look at.)
 // Shares: the least of what the steps, the partial results and the second launch take.  A step of 128 keys is some 0.5 + 0.016 head_dim us, partial results are written and read at 2.5 TB/s.  Tiles of one
 // length take rounds of workgroups; with the causal flag they are of unlike lengths, and take what the longest takes, or all of them on 256 compute units (5088 rows of four heads on one of
 // 96, 160 tiles: 70 us in one share, 58 in three).
@@ -537,7 +538,7 @@ uint64_t attention_packed_workspace_bytes(const rt_attention_packed_desc &d) {
     return ragged_workspace_bytes(d.batch, d.heads, d.kv_heads, d.rows, d.max_rows, d.max_keys, d.head_dim, d.causal);
 }
 hipError_t launch_attention_packed(const rt_attention_packed_desc &d, const void *q, const void *k, const void *v, const int32_t *starts, const int32_t *kv_starts,
-                                   void *out, void *workspace, uint64_t workspace_bytes, hipStream_t stream, const DeviceInfo &dev) {
+                                   void *out, void *workspace, uint64_t workspace_bytes, hipStream_t stream) {
     RaggedArgs g{};
     g.Q = (const half_t *)q, g.K = (const half_t *)k, g.V = (const half_t *)v, g.O = (half_t *)out, g.starts = starts, g.kv_starts = kv_starts;
     g.q_rs = d.q_strides[0], g.q_hs = d.q_strides[1], g.o_rs = d.o_strides[0], g.o_hs = d.o_strides[1];
